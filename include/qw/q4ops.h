@@ -12,6 +12,9 @@
  *   qw_moe_experts_w4a8   gpu::moe_experts_w4a8     src/kernels/moe_tiling.hpp:14-20
  *   qw_quant_rows_i8      quant_rows_kernel         src/kernels/moe_w4a8.hip:17-36
  *   qw_moe_combine        gpu::moe_combine_B/T      src/kernels/moe.hpp:42-46
+ *   qw_w8a8_gemm, qw_w8a8_linear, qw_moe_experts_w8a8, qw_moe_sort, qw_moe_permute,
+ *   qw_moe_unpermute and its gradient have no counterpart there: products of
+ *   checkpoints quantised to 8 bits, and expert rows held in memory.
  *   qw_w16_gemv           gpu::gemv_rows (fp16 W)   src/kernels/gemv.hpp:13-14
  *   qw_w16_gemv_tiled     gpu::gemv_rows (fp16 W)   src/kernels/gemv.hpp:13-14 (weights tiled at load)
  *   qw_w16_swiglu_gemv_tiled  gpu::swiglu_T + gemv_rows  src/kernels/moe_route.hip:187-197, gemv.hpp:13-14
@@ -314,6 +317,108 @@ int qw_quant_rows_i8(const uint16_t *x, int x_f16, int rows, int K, int ldx, int
  * Sums in fp32: the shared value, then the selections in order. */
 int qw_moe_combine(const void *yp, int yp_f16, const int32_t *tok_slot, const float *tok_w, const void *shared,
                    int shared_f16, int T, int topk, int H, void *out, int out_type, void *stream);
+
+/* ---- W8A8: int8 rows with a scale per token times int8 weights with a scale
+ * per output row (checkpoints quantised to 8 bits; the engine's own int8 copy
+ * of its dense weights keeps 16-bit rows: qw_i8_gemv).
+ *
+ * The rows' quantiser (the recipe of quant_rows_kernel,
+ * src/kernels/moe_w4a8.hip:17-36, over whole rows), in fp32:
+ *   scale[t] = max_k |x[t][k]| / 127  (at least 2^-126; 1 for a row of zeros)
+ *   q[t][k]  = rint(x[t][k] * (1 / scale[t]))   (round half to even)
+ * A row that holds an infinity or a NaN gets scale NaN and zeros: its outputs
+ * are NaN, and no other row's. x of x_type QW_T_F32, QW_T_BF16 or QW_T_F16,
+ * rows of stride ldx (elements, any); q int8 rows of stride ldq (a multiple
+ * of 16, 16-byte aligned); K a multiple of 16, T >= 1. */
+int qw_quant_tokens_i8(const void *x, int x_type, int ldx, int T, int K, int8_t *q, int ldq, float *scale,
+                       void *stream);
+
+/* Y[t][n] = float(sum_k q[t][k] * W[n][k]) * sw[n] * sx[t],  t < T, n < N
+ * The sum in int32, exact; then rounded to fp32, multiplied by the weight
+ * row's scale and by the token's, and rounded to y_type (QW_T_F32, QW_T_BF16:
+ * nearest even, QW_T_F16: nearest even, finite values beyond +-65504
+ * saturate). A row's result does not depend on the batch it is in. W int8
+ * row-major [N][K] with stride ldw as the checkpoint holds it, sw fp32 [N], q
+ * and sx as qw_quant_tokens_i8 writes them (any int8 values). K a multiple of
+ * 16 up to 131056 (the int32 sum cannot overflow), ldw and ldq multiples of 16
+ * from K, W and q 16-byte aligned; any T from one token (decode) to chunks,
+ * any N; ldy >= N. */
+int qw_w8a8_gemm(const int8_t *W, int ldw, const float *sw, const int8_t *q, int ldq, const float *sx, int T, void *Y,
+                 int ldy, int y_type, int N, int K, void *stream);
+
+/* qw_quant_tokens_i8 followed by qw_w8a8_gemm, bit for bit, from rows x of
+ * x_type. workspace: qw_w8a8_workspace_size(T, K) bytes, 256-byte aligned,
+ * scratch (it holds nothing between calls; calls that share it must not
+ * overlap). */
+size_t qw_w8a8_workspace_size(int T, int K);
+int qw_w8a8_linear(const int8_t *W, int ldw, const float *sw, const void *x, int x_type, int ldx, int T, void *Y,
+                   int ldy, int y_type, int N, int K, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Routed experts in W8A8, any batch from one token (the arguments of
+ * qw_moe_experts_w4a8 with int8 weights, a scale per output row): for every
+ * slot p of expert e
+ *   h[p]  = fp16(silu(g) * u), g and u the products of x[pair_tok[p]]
+ *           (quantised per token) with e's gate and up rows   fp16 [T*k][F]
+ *   yp[p] = the product of h[p] (quantised per slot) with e's down rows
+ *                                                     yp_type [T*k][H]
+ * each product as qw_w8a8_gemm. Weights of the stacked experts: gw, uw int8
+ * [E][F][H] with gs, us fp32 [E][F]; dw int8 [E][H][F] with ds fp32 [E][H].
+ * Tile list of qw_moe_route or qw_moe_sort with tile_m =
+ * qw_moe_w8a8_tile_m(). x [T][H] of x_type. Slots that no choice has (rows
+ * behind offsets[E]) are left as they were. Finite h and fp16 yp beyond
+ * +-65504 saturate. H and F multiples of 16 up to 131056; gw, uw, dw 16-byte
+ * aligned. workspace: qw_moe_w8a8_workspace_size(T, topk, H, F) bytes,
+ * 256-byte aligned, scratch (calls that share it must not overlap). */
+int qw_moe_w8a8_tile_m(void);
+size_t qw_moe_w8a8_workspace_size(int T, int topk, int H, int F);
+int qw_moe_experts_w8a8(const int8_t *gw, const float *gs, const int8_t *uw, const float *us, const int8_t *dw,
+                        const float *ds, int E, int H, int F, const int32_t *offsets, const int32_t *pair_tok,
+                        const int32_t *tile_e, const int32_t *tile_m0, const int32_t *n_tiles, const void *x,
+                        int x_type, int T, int topk, uint16_t *h, void *yp, int yp_type, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
+/* ---- Tokens sorted by expert and back, with the gradients.
+ * The slots of given choices top_e [T][k] (another router's, or qw_moe_route's
+ * top_e with some of them removed; qw_moe_route gives its own choices' slots):
+ * experts ascending, within one the choices in order (t, i). A choice outside
+ * 0 .. E - 1 (an expert another rank holds) has slot -1, and qw_moe_combine and
+ * the calls below skip it; a token may name an expert twice. Outputs and tile
+ * list as qw_moe_route's, with offsets[E] the number of slots; pair_tok of the
+ * T*k - offsets[E] places behind them is -1. Limits: 1 <= E <= 1024,
+ * 1 <= k <= 64, T * k < 2^30. */
+int qw_moe_sort(const int32_t *top_e, int T, int E, int topk, int tile_m, int32_t *counts, int32_t *offsets,
+                int32_t *tok_slot, int32_t *pair_tok, int32_t *active, int32_t *n_active, int32_t *tile_e,
+                int32_t *tile_m0, int32_t *n_tiles, void *stream);
+
+/* The rows in slot order: xs[tok_slot[t][i]][j] = x[t][j], j < H, for every
+ * choice with a slot (0 <= slot < T*k; others are skipped, and rows no choice
+ * has are left as they were). Elements of elem_bytes 1, 2 or 4 are moved as
+ * they are (int8 rows, their fp32 scales with H = 1, 16- and 32-bit rows);
+ * strides ldx, ldxs >= H in elements, any alignment of the element. xs must
+ * not overlap x. T <= 2^23. Its gradient is qw_moe_unpermute without weights. */
+int qw_moe_permute(const void *x, int ldx, int elem_bytes, int T, int topk, int H, const int32_t *tok_slot, void *xs,
+                   int ldxs, void *stream);
+
+/* The rows back at their tokens:
+ *   out[t][j] = sum_i tok_w[t][i] * yp[tok_slot[t][i]][j]
+ * over the choices with a slot, in order, in fp32, rounded once to out_type
+ * (fp16: finite values beyond +-65504 saturate). tok_w fp32 [T][k], or NULL:
+ * all 1 (the gradient of qw_moe_permute). A token without slots gets zeros.
+ * yp_type and out_type QW_T_F32, QW_T_BF16 or QW_T_F16; strides ldyp, ldo >= H
+ * in elements. qw_moe_combine is the form with a shared expert's rows. */
+int qw_moe_unpermute(const void *yp, int yp_type, int ldyp, const int32_t *tok_slot, const float *tok_w, int T,
+                     int topk, int H, void *out, int out_type, int ldo, void *stream);
+
+/* The gradients of qw_moe_unpermute, from dout [T][H] of dout_type:
+ *   dyp[tok_slot[t][i]][j] = tok_w[t][i] * dout[t][j]   (of yp_type, one rounding;
+ *                            rows no choice has are left as they were)
+ *   dw[t][i] = sum_j yp[tok_slot[t][i]][j] * dout[t][j] (fp32; 0 without a slot)
+ * Either of dyp and dw may be NULL (not wanted); yp is read for dw only. tok_w
+ * NULL: all 1. Every sum has a fixed order. Where a slot is named twice, by a
+ * tok_slot that qw_moe_sort did not write, its dyp row is one of the two. */
+int qw_moe_unpermute_backward(const void *dout, int dout_type, int ldd, const void *yp, int yp_type, int ldyp,
+                              const int32_t *tok_slot, const float *tok_w, int T, int topk, int H, void *dyp,
+                              int lddyp, float *dw, void *stream);
 
 /* Format surface (bit-exact): nibbles as bytes [N][K]; dequantised fp32
  * weights [N][K]; reference-engine word order -> checkpoint word order. */

@@ -1,0 +1,156 @@
+"""What the W8A8 products and the expert-row calls refuse, each with a message
+and nothing launched (host-side checks: no GPU needed)."""
+import ctypes
+
+import pytest
+
+import qwq4
+
+P = ctypes.c_void_p(4096)      # aligned, never read: every call below is refused first
+ODD = ctypes.c_void_p(4096 + 1)
+EIGHT = ctypes.c_void_p(4096 + 8)
+BIG = 1 << 40
+
+
+def quant(x=P, t=1, ldx=64, T=4, K=64, q=P, ldq=64, s=P):
+    return "qw_quant_tokens_i8", (x, t, ldx, T, K, q, ldq, s, None)
+
+
+def gemm(W=P, ldw=64, sw=P, q=P, ldq=64, sx=P, T=4, Y=P, ldy=32, yt=1, N=32, K=64):
+    return "qw_w8a8_gemm", (W, ldw, sw, q, ldq, sx, T, Y, ldy, yt, N, K, None)
+
+
+def linear(W=P, ldw=64, sw=P, x=P, xt=1, ldx=64, T=4, Y=P, ldy=32, yt=1, N=32, K=64, ws=P, wb=BIG):
+    return "qw_w8a8_linear", (W, ldw, sw, x, xt, ldx, T, Y, ldy, yt, N, K, ws, wb, None)
+
+
+def experts(w=(P,) * 6, E=8, H=64, F=32, lists=(P,) * 5, x=P, xt=1, T=4, k=2, h=P, yp=P, yt=2, ws=P, wb=BIG):
+    return "qw_moe_experts_w8a8", (*w, E, H, F, *lists, x, xt, T, k, h, yp, yt, ws, wb, None)
+
+
+def sort(e=P, T=4, E=8, k=2, tile_m=0, outs=(P,) * 6, tiles=(None,) * 3):
+    return "qw_moe_sort", (e, T, E, k, tile_m, *outs, *tiles, None)
+
+
+def permute(x=P, ldx=64, b=2, T=4, k=2, H=64, slot=P, xs=P, ldxs=64):
+    return "qw_moe_permute", (x, ldx, b, T, k, H, slot, xs, ldxs, None)
+
+
+def unpermute(yp=P, yt=1, ldyp=64, slot=P, w=P, T=4, k=2, H=64, out=P, ot=1, ldo=64):
+    return "qw_moe_unpermute", (yp, yt, ldyp, slot, w, T, k, H, out, ot, ldo, None)
+
+
+def grad(dout=P, dt=1, ldd=64, yp=P, yt=1, ldyp=64, slot=P, w=P, T=4, k=2, H=64, dyp=P, lddyp=64, dw=P):
+    return "qw_moe_unpermute_backward", (dout, dt, ldd, yp, yt, ldyp, slot, w, T, k, H, dyp, lddyp, dw, None)
+
+
+CALLS = {
+    "quant null x": quant(x=None), "quant null q": quant(q=None), "quant null scale": quant(s=None),
+    "quant type": quant(t=3), "quant K 40": quant(K=40, ldx=40, ldq=48), "quant K 0": quant(K=0),
+    "quant K past the limit": quant(K=131072, ldx=131072, ldq=131072), "quant no rows": quant(T=0),
+    "quant negative rows": quant(T=-1), "quant ldx": quant(ldx=63), "quant ldq": quant(ldq=72),
+    "quant ldq short": quant(ldq=48), "quant q at 8": quant(q=EIGHT), "quant x odd": quant(x=ODD),
+    "quant fp32 x at 2": quant(t=0, x=ctypes.c_void_p(4098)), "quant too many rows": quant(T=(1 << 23) + 1),
+    "gemm null W": gemm(W=None), "gemm null sw": gemm(sw=None), "gemm null q": gemm(q=None), "gemm null sx": gemm(sx=None),
+    "gemm null Y": gemm(Y=None), "gemm K 24": gemm(K=24), "gemm ldw": gemm(ldw=72), "gemm ldw short": gemm(ldw=48),
+    "gemm W at 8": gemm(W=EIGHT), "gemm ldq": gemm(ldq=56), "gemm y type": gemm(yt=4), "gemm ldy": gemm(ldy=31),
+    "gemm no rows": gemm(T=0), "gemm no columns": gemm(N=0), "gemm Y odd": gemm(Y=ODD),
+    "gemm fp32 Y at 2": gemm(yt=0, Y=ctypes.c_void_p(4098)),
+    "gemm too many outputs": gemm(T=1 << 20, N=1 << 20, ldy=1 << 20),
+    "linear null x": linear(x=None), "linear x type": linear(xt=-1), "linear no workspace": linear(ws=None),
+    "linear small workspace": linear(wb=256), "linear workspace at 8": linear(ws=EIGHT), "linear ldx": linear(ldx=60),
+    "linear null W": linear(W=None),
+    **{f"experts null weights {i}": experts(w=tuple(None if j == i else P for j in range(6))) for i in range(6)},
+    **{f"experts null list {i}": experts(lists=tuple(None if j == i else P for j in range(5))) for i in range(5)},
+    "experts E": experts(E=1025), "experts no expert": experts(E=0), "experts H": experts(H=72), "experts F": experts(F=40),
+    "experts F 0": experts(F=0), "experts topk": experts(k=65), "experts topk 0": experts(k=0), "experts no token": experts(T=0),
+    "experts slots": experts(T=1 << 22, k=4), "experts grid": experts(T=1 << 20, k=8, H=16384),
+    "experts weights at 8": experts(w=(P, P, P, P, EIGHT, P)), "experts null h": experts(h=None),
+    "experts null yp": experts(yp=None), "experts yp type": experts(yt=3), "experts small workspace": experts(wb=1023),
+    "experts no workspace": experts(ws=None), "experts x type": experts(xt=7), "experts yp odd": experts(yp=ODD),
+    "sort null": sort(e=None), "sort null output": sort(outs=(P, P, None, P, P, P)), "sort E": sort(E=1025),
+    "sort E 0": sort(E=0), "sort T": sort(T=0), "sort topk": sort(k=65), "sort topk 0": sort(k=0),
+    "sort pairs": sort(T=1 << 25, k=64), "sort tiles": sort(tile_m=-32), "sort tile_m": sort(tile_m=4096, tiles=(P,) * 3),
+    "permute null x": permute(x=None), "permute null slot": permute(slot=None), "permute null xs": permute(xs=None),
+    "permute 8 bytes": permute(b=8), "permute 3 bytes": permute(b=3), "permute ldx": permute(ldx=63),
+    "permute ldxs": permute(ldxs=63), "permute H": permute(H=0), "permute T": permute(T=0),
+    "permute odd 16-bit rows": permute(x=ODD), "permute many": permute(T=(1 << 23) + 1), "permute topk": permute(k=65),
+    "unpermute null yp": unpermute(yp=None), "unpermute null out": unpermute(out=None), "unpermute null slot": unpermute(slot=None),
+    "unpermute yp type": unpermute(yt=5), "unpermute out type": unpermute(ot=-1), "unpermute ldyp": unpermute(ldyp=63),
+    "unpermute ldo": unpermute(ldo=63), "unpermute T": unpermute(T=0), "unpermute weights at 1": unpermute(w=ODD),
+    "grad null dout": grad(dout=None), "grad nothing wanted": grad(dyp=None, dw=None), "grad dw without yp": grad(yp=None),
+    "grad dout type": grad(dt=3), "grad yp type": grad(yt=3), "grad ldd": grad(ldd=63), "grad ldyp": grad(ldyp=63),
+    "grad lddyp": grad(lddyp=63), "grad topk": grad(k=0), "grad null slot": grad(slot=None), "grad H": grad(H=-1),
+}
+
+
+@pytest.mark.parametrize("name", sorted(CALLS))
+def test_refused(lib, name):
+    fn, args = CALLS[name]
+    assert getattr(lib, fn)(*args) == -1
+    message = lib.qw_q4_last_error().decode()
+    assert message.startswith(fn + ":"), message
+
+
+def test_sizes(lib):
+    assert lib.qw_w8a8_workspace_size(0, 64) == 0 and lib.qw_w8a8_workspace_size(4, 0) == 0
+    assert lib.qw_w8a8_workspace_size(4096, 4096) >= 4096 * 4096 + 4096 * 4
+    assert lib.qw_moe_w8a8_workspace_size(0, 8, 64, 64) == 0
+    assert lib.qw_moe_w8a8_workspace_size(4096, 8, 4096, 1536) >= 4096 * 4096 + 4096 * 8 * 1536
+    # sizes whose products pass 32 bits
+    assert lib.qw_w8a8_workspace_size(1 << 20, 131056) >= (1 << 20) * 131056
+
+
+def test_binding_refusals():
+    """Shapes, types and tensors off the GPU, before any library call."""
+    import torch
+    W, sw = torch.zeros(8, 32, dtype=torch.int8), torch.zeros(8)
+    x, slot = torch.zeros(3, 32), torch.zeros(3, 2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        qwq4.linear_w8a8(W, sw, x)
+    with pytest.raises(ValueError, match="W is"):
+        qwq4.linear_w8a8(W, sw, torch.zeros(3, 48))
+    with pytest.raises(TypeError, match="W is"):
+        qwq4.linear_w8a8(W.float(), sw, x)
+    with pytest.raises(ValueError, match="sw is"):
+        qwq4.linear_w8a8(W, sw[:7], x)
+    with pytest.raises(ValueError, match="contiguous"):
+        qwq4.linear_w8a8(W, sw, torch.zeros(32, 3).t())
+    with pytest.raises(ValueError, match="contiguous"):
+        qwq4.linear_w8a8(W, torch.zeros(16)[::2], x)
+    with pytest.raises(TypeError, match="element type"):
+        qwq4.linear_w8a8(W, sw, x.double())
+    with pytest.raises(TypeError, match="the output is"):
+        qwq4.linear_w8a8(W, sw, x, Y=torch.zeros(3, 8), y_dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="the output is"):
+        qwq4.linear_w8a8(W, sw, x, Y=torch.zeros(3, 9))
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        qwq4.quant_tokens_i8(x)
+    with pytest.raises(TypeError, match="q is"):
+        qwq4.gemm_w8a8(W, sw, x, torch.zeros(3))
+    with pytest.raises(ValueError, match="sx is"):
+        qwq4.gemm_w8a8(W, sw, torch.zeros(3, 32, dtype=torch.int8), torch.zeros(4))
+    with pytest.raises(TypeError, match="top_e is"):
+        qwq4.moe_sort(slot.long(), 4)
+    with pytest.raises(ValueError, match="top_e is"):
+        qwq4.moe_sort(slot.flatten(), 4)
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        qwq4.moe_sort(slot, 4)
+    with pytest.raises(ValueError, match="x is"):
+        qwq4.moe_permute(torch.zeros(4, 32), slot)
+    with pytest.raises(ValueError, match="xs is"):
+        qwq4.moe_permute(x, slot, xs=torch.zeros(5, 32))
+    with pytest.raises(TypeError, match="xs is"):
+        qwq4.moe_permute(x, slot, xs=torch.zeros(6, 32).half())
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        qwq4.moe_permute(x, slot)
+    with pytest.raises(ValueError, match="yp is"):
+        qwq4.moe_unpermute(torch.zeros(5, 32), slot)
+    with pytest.raises(TypeError, match="tok_w is"):
+        qwq4.moe_unpermute(torch.zeros(6, 32), slot, torch.zeros(3, 2).half())
+    with pytest.raises(ValueError, match="dout is"):
+        qwq4.moe_unpermute_backward(torch.zeros(3, 31), torch.zeros(6, 32), slot)
+    with pytest.raises(TypeError, match="dyp is"):
+        qwq4.moe_unpermute_backward(x, torch.zeros(6, 32), slot, dyp=torch.zeros(6, 32).half())
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        qwq4.moe_unpermute_backward(x, torch.zeros(6, 32), slot)

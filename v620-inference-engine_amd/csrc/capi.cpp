@@ -375,6 +375,183 @@ int qw_moe_combine(const void *yp, int yp_f16, const int32_t *tok_slot, const fl
     return launched("qw_moe_combine");
 }
 
+// ---- W8A8
+static bool is_type(int t) { return t == QW_T_F32 || t == QW_T_BF16 || t == QW_T_F16; }
+static size_t type_bytes(int t) { return t == QW_T_F32 ? 4 : 2; }
+
+constexpr int kW8MaxK = 131056;    // 128 * 128 * K < 2^31: an int32 sum of any int8 values
+constexpr int kMaxRows = 1 << 23;  // rows of a launch (a block or less each, blocks of at most 512 threads)
+
+static int check_w8_rows(const char *fn, const void *x, int x_type, int ldx, int T, int K) {
+    REQUIRE(x, "%s: null x", fn);
+    REQUIRE(is_type(x_type), "%s: x_type = %d (0 fp32, 1 bf16, 2 fp16)", fn, x_type);
+    REQUIRE(K >= 16 && K % 16 == 0 && K <= kW8MaxK, "%s: K = %d must be a multiple of 16 from 16 to %d", fn, K, kW8MaxK);
+    REQUIRE(T >= 1 && T <= kMaxRows, "%s: T = %d outside 1..%d", fn, T, kMaxRows);
+    REQUIRE(T == 1 || ldx >= K, "%s: x stride %d < K = %d", fn, ldx, K);
+    REQUIRE(aligned(x, type_bytes(x_type)), "%s: x misaligned", fn);
+    return 0;
+}
+
+static int check_w8_product(const char *fn, const int8_t *W, int ldw, const float *sw, int T, const void *Y, int ldy,
+                            int y_type, int N, int K) {
+    REQUIRE(W && sw && Y, "%s: null W, sw or Y", fn);
+    REQUIRE(K >= 16 && K % 16 == 0 && K <= kW8MaxK, "%s: K = %d must be a multiple of 16 from 16 to %d", fn, K, kW8MaxK);
+    REQUIRE(T >= 1 && T <= kMaxRows && N >= 1 && N <= kMaxRows && int64_t(T) * N <= (int64_t(1) << 38),
+            "%s: T = %d, N = %d (need 1..%d each, at most 2^38 outputs)", fn, T, N, kMaxRows);
+    REQUIRE(ldw >= K && ldw % 16 == 0 && aligned(W, 16),
+            "%s: ldw %d must be >= K, a multiple of 16, W 16-byte aligned", fn, ldw);
+    REQUIRE(is_type(y_type), "%s: y_type = %d (0 fp32, 1 bf16, 2 fp16)", fn, y_type);
+    REQUIRE((T == 1 || ldy >= N) && aligned(Y, type_bytes(y_type)), "%s: y stride %d < N = %d, or Y misaligned", fn,
+            ldy, N);
+    REQUIRE(aligned(sw, 4), "%s: sw misaligned", fn);
+    return 0;
+}
+
+int qw_quant_tokens_i8(const void *x, int x_type, int ldx, int T, int K, int8_t *q, int ldq, float *scale,
+                       void *stream) {
+    const char *fn = "qw_quant_tokens_i8";
+    if (int r = check_w8_rows(fn, x, x_type, ldx, T, K)) return r;
+    REQUIRE(q && scale, "%s: null q or scale", fn);
+    REQUIRE(ldq >= K && ldq % 16 == 0 && aligned(q, 16) && aligned(scale, 4),
+            "%s: ldq %d must be >= K, a multiple of 16, q 16-byte aligned", fn, ldq);
+    qwq4::launch_quant_tokens(x, x_type, ldx, T, K, q, ldq, scale, st(stream));
+    return launched(fn);
+}
+
+int qw_w8a8_gemm(const int8_t *W, int ldw, const float *sw, const int8_t *q, int ldq, const float *sx, int T, void *Y,
+                 int ldy, int y_type, int N, int K, void *stream) {
+    const char *fn = "qw_w8a8_gemm";
+    if (int r = check_w8_product(fn, W, ldw, sw, T, Y, ldy, y_type, N, K)) return r;
+    REQUIRE(q && sx, "%s: null q or sx", fn);
+    REQUIRE(ldq >= K && ldq % 16 == 0 && aligned(q, 16) && aligned(sx, 4),
+            "%s: ldq %d must be >= K, a multiple of 16, q 16-byte aligned", fn, ldq);
+    qwq4::launch_w8a8_gemm(qwq4::W8GemmArgs{W, ldw, sw, q, ldq, sx, T, Y, ldy, y_type, N, K}, st(stream));
+    return launched(fn);
+}
+
+size_t qw_w8a8_workspace_size(int T, int K) { return T < 1 || K < 16 ? 0 : qwq4::w8a8_workspace_bytes(T, K); }
+
+int qw_w8a8_linear(const int8_t *W, int ldw, const float *sw, const void *x, int x_type, int ldx, int T, void *Y,
+                   int ldy, int y_type, int N, int K, void *workspace, size_t workspace_bytes, void *stream) {
+    const char *fn = "qw_w8a8_linear";
+    if (int r = check_w8_product(fn, W, ldw, sw, T, Y, ldy, y_type, N, K)) return r;
+    if (int r = check_w8_rows(fn, x, x_type, ldx, T, K)) return r;
+    const size_t need = qwq4::w8a8_workspace_bytes(T, K);
+    REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 256),
+            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", fn, need, workspace_bytes);
+    qwq4::launch_w8a8_linear(qwq4::W8GemmArgs{W, ldw, sw, nullptr, 0, nullptr, T, Y, ldy, y_type, N, K}, x, x_type, ldx,
+                             workspace, st(stream));
+    return launched(fn);
+}
+
+int qw_moe_w8a8_tile_m(void) { return qwq4::moe_w8a8_tile_m(); }
+
+size_t qw_moe_w8a8_workspace_size(int T, int topk, int H, int F) {
+    if (T < 1 || topk < 1 || H < 16 || F < 16) return 0;
+    return qwq4::moe_w8a8_workspace_bytes(T, topk, H, F);
+}
+
+int qw_moe_experts_w8a8(const int8_t *gw, const float *gs, const int8_t *uw, const float *us, const int8_t *dw,
+                        const float *ds, int E, int H, int F, const int32_t *offsets, const int32_t *pair_tok,
+                        const int32_t *tile_e, const int32_t *tile_m0, const int32_t *n_tiles, const void *x,
+                        int x_type, int T, int topk, uint16_t *h, void *yp, int yp_type, void *workspace,
+                        size_t workspace_bytes, void *stream) {
+    const char *fn = "qw_moe_experts_w8a8";
+    REQUIRE(gw && gs && uw && us && dw && ds, "%s: null weight or scale pointer", fn);
+    REQUIRE(offsets && pair_tok && tile_e && tile_m0 && n_tiles && h && yp, "%s: null pointer", fn);
+    REQUIRE(E >= 1 && E <= 1024, "%s: E = %d outside 1..1024", fn, E);
+    if (int r = check_w8_rows(fn, x, x_type, H, T, H)) return r;
+    REQUIRE(F >= 16 && F % 16 == 0 && F <= kW8MaxK, "%s: F = %d must be a multiple of 16 from 16 to %d", fn, F, kW8MaxK);
+    REQUIRE(topk >= 1 && topk <= 64 && int64_t(T) * topk <= kMaxRows, "%s: topk = %d (1..64), T * topk at most %d", fn,
+            topk, kMaxRows);
+    // (blocks of the widest grid: list entries times 32-row tiles of F or H)
+    REQUIRE((int64_t(T) * topk / 32 + E) * ((H > F ? H : F) / 32 + 1) <= (1 << 23),
+            "%s: T * topk = %lld slots with H = %d, F = %d are too many for one call", fn, (long long)T * topk, H, F);
+    REQUIRE(aligned(gw, 16) && aligned(uw, 16) && aligned(dw, 16), "%s: weights must be 16-byte aligned", fn);
+    REQUIRE(is_type(yp_type), "%s: yp_type = %d (0 fp32, 1 bf16, 2 fp16)", fn, yp_type);
+    REQUIRE(aligned(h, 2) && aligned(yp, type_bytes(yp_type)), "%s: misaligned h or yp", fn);
+    const size_t need = qwq4::moe_w8a8_workspace_bytes(T, topk, H, F);
+    REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 256),
+            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", fn, need, workspace_bytes);
+    qwq4::MoeW8A8Args a{gw, uw, dw, gs, us, ds, E, H, F, offsets, pair_tok, tile_e, tile_m0, n_tiles, h, yp, yp_type,
+                        nullptr, nullptr, nullptr, nullptr};
+    qwq4::launch_moe_w8a8(a, x, x_type, T, topk, workspace, st(stream));
+    return launched(fn);
+}
+
+// ---- tokens sorted by expert and back
+int qw_moe_sort(const int32_t *top_e, int T, int E, int topk, int tile_m, int32_t *counts, int32_t *offsets,
+                int32_t *tok_slot, int32_t *pair_tok, int32_t *active, int32_t *n_active, int32_t *tile_e,
+                int32_t *tile_m0, int32_t *n_tiles, void *stream) {
+    const char *fn = "qw_moe_sort";
+    REQUIRE(top_e && counts && offsets && tok_slot && pair_tok && active && n_active, "%s: null pointer", fn);
+    REQUIRE(T >= 1 && E >= 1 && E <= 1024, "%s: T = %d, E = %d (need T >= 1, 1 <= E <= 1024)", fn, T, E);
+    REQUIRE(topk >= 1 && topk <= 64 && int64_t(T) * topk < (1 << 30), "%s: topk = %d (1..64), T * topk below 2^30", fn,
+            topk);
+    REQUIRE(tile_m > -4096 && tile_m < 4096, "%s: |tile_m| >= 4096", fn);
+    REQUIRE(tile_m == 0 || (tile_e && tile_m0 && n_tiles), "%s: tile_m != 0 needs the tile outputs", fn);
+    qwq4::launch_sort(qwq4::SortArgs{top_e, T, E, topk, tile_m, counts, offsets, tok_slot, pair_tok, active, n_active,
+                                     tile_e, tile_m0, n_tiles},
+                      st(stream));
+    return launched(fn);
+}
+
+static int check_rows(const char *fn, int T, int topk, int H) {
+    REQUIRE(T >= 1 && T <= kMaxRows && topk >= 1 && topk <= 64 && int64_t(T) * topk < (1 << 30) && H >= 1,
+            "%s: T = %d (1..%d), topk = %d (1..64), H = %d (from 1), T * topk below 2^30", fn, T, kMaxRows, topk, H);
+    return 0;
+}
+
+int qw_moe_permute(const void *x, int ldx, int elem_bytes, int T, int topk, int H, const int32_t *tok_slot, void *xs,
+                   int ldxs, void *stream) {
+    const char *fn = "qw_moe_permute";
+    REQUIRE(x && tok_slot && xs, "%s: null pointer", fn);
+    if (int r = check_rows(fn, T, topk, H)) return r;
+    REQUIRE(elem_bytes == 1 || elem_bytes == 2 || elem_bytes == 4, "%s: elem_bytes = %d (1, 2 or 4)", fn, elem_bytes);
+    REQUIRE((T == 1 || ldx >= H) && (int64_t(T) * topk == 1 || ldxs >= H), "%s: stride %d or %d < H = %d", fn, ldx, ldxs,
+            H);
+    REQUIRE(aligned(x, elem_bytes) && aligned(xs, elem_bytes) && aligned(tok_slot, 4), "%s: misaligned buffer", fn);
+    qwq4::launch_permute(x, ldx, elem_bytes, T, topk, H, tok_slot, xs, ldxs, st(stream));
+    return launched(fn);
+}
+
+int qw_moe_unpermute(const void *yp, int yp_type, int ldyp, const int32_t *tok_slot, const float *tok_w, int T,
+                     int topk, int H, void *out, int out_type, int ldo, void *stream) {
+    const char *fn = "qw_moe_unpermute";
+    REQUIRE(yp && tok_slot && out, "%s: null pointer", fn);
+    if (int r = check_rows(fn, T, topk, H)) return r;
+    REQUIRE(is_type(yp_type) && is_type(out_type), "%s: yp_type = %d, out_type = %d (0 fp32, 1 bf16, 2 fp16)", fn,
+            yp_type, out_type);
+    REQUIRE((int64_t(T) * topk == 1 || ldyp >= H) && (T == 1 || ldo >= H), "%s: stride %d or %d < H = %d", fn, ldyp, ldo,
+            H);
+    REQUIRE(aligned(yp, type_bytes(yp_type)) && aligned(out, type_bytes(out_type)) && aligned(tok_slot, 4) &&
+                aligned(tok_w, 4),
+            "%s: misaligned buffer", fn);
+    qwq4::launch_unpermute(yp, yp_type, ldyp, tok_slot, tok_w, T, topk, H, out, out_type, ldo, st(stream));
+    return launched(fn);
+}
+
+int qw_moe_unpermute_backward(const void *dout, int dout_type, int ldd, const void *yp, int yp_type, int ldyp,
+                              const int32_t *tok_slot, const float *tok_w, int T, int topk, int H, void *dyp,
+                              int lddyp, float *dw, void *stream) {
+    const char *fn = "qw_moe_unpermute_backward";
+    REQUIRE(dout && tok_slot && (dyp || dw) && (yp || !dw), "%s: null pointer (dout, tok_slot; dyp or dw; yp with dw)",
+            fn);
+    if (int r = check_rows(fn, T, topk, H)) return r;
+    REQUIRE(is_type(dout_type) && is_type(yp_type), "%s: dout_type = %d, yp_type = %d (0 fp32, 1 bf16, 2 fp16)", fn,
+            dout_type, yp_type);
+    const bool one = int64_t(T) * topk == 1;
+    REQUIRE((T == 1 || ldd >= H) && (one || !dw || ldyp >= H) && (one || !dyp || lddyp >= H),
+            "%s: stride %d, %d or %d < H = %d", fn, ldd, ldyp, lddyp, H);
+    REQUIRE(aligned(dout, type_bytes(dout_type)) && aligned(yp, type_bytes(yp_type)) &&
+                aligned(dyp, type_bytes(yp_type)) && aligned(tok_slot, 4) && aligned(tok_w, 4) && aligned(dw, 4),
+            "%s: misaligned buffer", fn);
+    qwq4::launch_unpermute_backward(
+        qwq4::UnpermuteGradArgs{dout, dout_type, ldd, yp, yp_type, ldyp, tok_slot, tok_w, T, topk, H, dyp, lddyp, dw},
+        st(stream));
+    return launched(fn);
+}
+
 void qw_q4_tiled_size(int64_t N, int64_t K, size_t *wt_bytes, size_t *st_bytes, size_t *zt_bytes) {
     const int64_t G = K / 128, GC = (G + 3) / 4;
     if (wt_bytes) *wt_bytes = size_t(N) * size_t(K) / 2;

@@ -264,6 +264,71 @@ void launch_moe_w4a8(W8Args a, const uint16_t *x, int x_f16, int T, int topk, hi
 void launch_quant_rows(const uint16_t *x, int x_f16, int64_t ldx, int rows, int K, int8_t *q, float *scale,
                        hipStream_t s);
 
+// Dense W8A8 (w8a8.hip): int8 rows with a scale per token times int8 weights
+// with a scale per row; K and the leading dimensions multiples of 16.
+struct W8GemmArgs {
+    const int8_t *W;
+    int64_t ldw;
+    const float *sw;
+    const int8_t *q;
+    int64_t ldq;
+    const float *sx;
+    int T;
+    void *Y;
+    int64_t ldy;
+    int y_type, N, K;
+};
+void launch_quant_tokens(const void *x, int x_type, int64_t ldx, int T, int K, int8_t *q, int64_t ldq, float *scale,
+                         hipStream_t s);
+void launch_w8a8_gemm(const W8GemmArgs &a, hipStream_t s);
+size_t w8a8_workspace_bytes(int T, int K);
+// a.q, a.ldq and a.sx are set to the workspace's quantised rows
+void launch_w8a8_linear(W8GemmArgs a, const void *x, int x_type, int64_t ldx, void *ws, hipStream_t s);
+
+// W8A8 grouped experts (moe_w8a8.hip): gate / up [E*F][H], down [E*H][F].
+// qx / sx / qh / sh point into the workspace (set by launch_moe_w8a8).
+struct MoeW8A8Args {
+    const int8_t *gw, *uw, *dw;
+    const float *gs, *us, *ds;
+    int E, H, F;
+    const int32_t *offsets, *pair_tok, *tile_e, *tile_m0, *n_tiles;
+    uint16_t *h;
+    void *yp;
+    int yp_type;
+    const int8_t *qx, *qh;
+    const float *sx, *sh;
+};
+int moe_w8a8_tile_m();
+size_t moe_w8a8_workspace_bytes(int T, int topk, int H, int F);
+void launch_moe_w8a8(MoeW8A8Args a, const void *x, int x_type, int T, int topk, void *ws, hipStream_t s);
+
+// Tokens sorted by expert and back (moe_rows.hip).
+struct SortArgs {
+    const int32_t *top_e;
+    int T, E, topk, tile_m;
+    int32_t *counts, *offsets, *tok_slot, *pair_tok, *active, *n_active, *tile_e, *tile_m0, *n_tiles;
+};
+void launch_sort(const SortArgs &a, hipStream_t s);
+void launch_permute(const void *x, int64_t ldx, int elem_bytes, int T, int topk, int H, const int32_t *tok_slot,
+                    void *xs, int64_t ldxs, hipStream_t s);
+void launch_unpermute(const void *yp, int yp_type, int64_t ldy, const int32_t *tok_slot, const float *tok_w, int T,
+                      int topk, int H, void *out, int out_type, int64_t ldo, hipStream_t s);
+struct UnpermuteGradArgs {
+    const void *dout;
+    int dout_type;
+    int64_t ldd;
+    const void *yp;
+    int yp_type;  // of dyp too
+    int64_t ldy;
+    const int32_t *tok_slot;
+    const float *tok_w;  // or null: all 1
+    int T, topk, H;
+    void *dyp;  // or null
+    int64_t lddy;
+    float *dw;  // or null
+};
+void launch_unpermute_backward(const UnpermuteGradArgs &a, hipStream_t s);
+
 struct GemmArgs {
     const uint32_t *W;
     const uint16_t *S;

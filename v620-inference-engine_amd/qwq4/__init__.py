@@ -23,6 +23,9 @@ SYMBOLS = (
     "qw_moe_decode_static_reset", "qw_moe_decode_with_shared_workspace_size", "qw_moe_decode_with_shared",
     "qw_w16_gemv", "qw_w16_tiled_size", "qw_w16_tile", "qw_w16_gemv_tiled", "qw_w16_swiglu_gemv_tiled", "qw_i8_gemv", "qw_i8_tiled_size", "qw_i8_tile",
     "qw_moe_w4a8_tile_m", "qw_moe_w4a8_workspace_size", "qw_moe_experts_w4a8", "qw_quant_rows_i8", "qw_swiglu_gate",
+    "qw_quant_tokens_i8", "qw_w8a8_gemm", "qw_w8a8_workspace_size", "qw_w8a8_linear", "qw_moe_w8a8_tile_m",
+    "qw_moe_w8a8_workspace_size", "qw_moe_experts_w8a8", "qw_moe_sort", "qw_moe_permute", "qw_moe_unpermute",
+    "qw_moe_unpermute_backward",
     "qw_wcache_open", "qw_wcache_put", "qw_wcache_get", "qw_wcache_finish", "qw_wcache_close",
 )
 
@@ -67,6 +70,17 @@ _SIGS = {
     "qw_moe_experts_w4a8": ([_P] * 9 + [_I, _I, _I] + [_P] * 6 + [_I, _I, _I, _P, _P, _P, _SZ, _P], _I),
     "qw_quant_rows_i8": ([_P, _I, _I, _I, _I, _P, _P, _P], _I),
     "qw_swiglu_gate": ([_P, _I, _I, _I, _P, _P], _I),
+    "qw_quant_tokens_i8": ([_P, _I, _I, _I, _I, _P, _I, _P, _P], _I),
+    "qw_w8a8_gemm": ([_P, _I, _P, _P, _I, _P, _I, _P, _I, _I, _I, _I, _P], _I),
+    "qw_w8a8_workspace_size": ([_I, _I], _SZ),
+    "qw_w8a8_linear": ([_P, _I, _P, _P, _I, _I, _I, _P, _I, _I, _I, _I, _P, _SZ, _P], _I),
+    "qw_moe_w8a8_tile_m": ([], _I),
+    "qw_moe_w8a8_workspace_size": ([_I, _I, _I, _I], _SZ),
+    "qw_moe_experts_w8a8": ([_P] * 6 + [_I, _I, _I] + [_P] * 6 + [_I, _I, _I, _P, _P, _I, _P, _SZ, _P], _I),
+    "qw_moe_sort": ([_P, _I, _I, _I, _I] + [_P] * 10, _I),
+    "qw_moe_permute": ([_P, _I, _I, _I, _I, _I, _P, _P, _I, _P], _I),
+    "qw_moe_unpermute": ([_P, _I, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P], _I),
+    "qw_moe_unpermute_backward": ([_P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _P, _I, _P, _P], _I),
     "qw_moe_decode_static": ([_P, _I, _P, _I, _I, _I, _I] + [_P] * 9 + [_I, _I, _P, _P, _I] + [_P] * 6 + [_I, _P], _I),
     "qw_moe_decode_with_shared_workspace_size": ([_I, _I, _I, _I, _I, _I], _SZ),
     "qw_moe_decode_with_shared": ([_P, _I, _P, _I, _I, _I, _I] + [_P] * 9 + [_I, _I, _P, _P, _I, _P, _P, _P, _I]
@@ -476,6 +490,271 @@ def moe_combine(yp, route, H, shared=None, out=None, out_bf16=True, out_dtype=No
                               _ptr(out), _tcode(out), _stream())
     _check(rc, "qw_moe_combine")
     return out
+
+
+# ------------------------------------------------------------------- W8A8
+def _here(fn, *ts):
+    """Every tensor on the current GPU: the call goes to its current stream."""
+    import torch
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError(f"{fn}: all tensors must be on the GPU")
+        if dev is None:
+            dev = torch.cuda.current_device()
+        if t.get_device() != dev:
+            raise RuntimeError(f"{fn}: a tensor is on GPU {t.get_device()}, the current one is {dev}")
+
+
+def _matrix(fn, name, t, shape, dtype=None):
+    """The row stride of a [rows][cols] tensor whose rows are contiguous (a dimension of None is any size)."""
+    if t.dim() != 2 or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise ValueError(f"{fn}: {name} is {tuple(t.shape)}, not {shape}")
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError(f"{fn}: {name} is {t.dtype}, not {dtype}")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{fn}: the rows of {name} must be contiguous")
+    return t.stride(0) if rows > 1 else cols
+
+
+def _whole(fn, name, t, shape, dtype):
+    """A contiguous tensor of this shape and type."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{fn}: {name} is {tuple(t.shape)}, not {shape}")
+    if t.dtype != dtype:
+        raise TypeError(f"{fn}: {name} is {t.dtype}, not {dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{fn}: {name} must be contiguous")
+
+
+def quant_tokens_i8(x, q=None, scale=None):
+    """Rows x [T][K] (float32, bfloat16 or float16) -> (q int8 [T][K], scale fp32 [T]), a scale per row:
+    q = rint(x (1 / scale)), scale = max |x| / 127."""
+    import torch
+    fn = "quant_tokens_i8"
+    ldx = _matrix(fn, "x", x, (None, None))
+    T, K = x.shape
+    if q is None:
+        q = torch.empty((T, K), dtype=torch.int8, device=x.device)
+    if scale is None:
+        scale = torch.empty(T, dtype=torch.float32, device=x.device)
+    ldq = _matrix(fn, "q", q, (T, K), torch.int8)
+    _whole(fn, "scale", scale, (T,), torch.float32)
+    code = _tcode(x)
+    _here(fn, x, q, scale)
+    _check(lib().qw_quant_tokens_i8(_ptr(x), code, ldx, T, K, _ptr(q), ldq, _ptr(scale), _stream()),
+           "qw_quant_tokens_i8")
+    return q, scale
+
+
+def _w8_out(fn, Y, y_dtype, T, N, default, device):
+    """The output rows, their stride and their QW_T_* code."""
+    import torch
+    if Y is None:
+        Y = torch.empty((T, N), dtype=y_dtype if y_dtype is not None else default, device=device)
+    elif y_dtype is not None and Y.dtype != y_dtype:
+        raise TypeError(f"{fn}: the output is {Y.dtype}, not {y_dtype}")
+    return Y, _matrix(fn, "the output", Y, (T, N)), _tcode(Y)
+
+
+def gemm_w8a8(W, sw, q, sx, Y=None, y_dtype=None):
+    """Y[t][n] = (sum_k q[t][k] W[n][k]) sw[n] sx[t], the sum in whole numbers. W int8 [N][K] and sw fp32 [N] as the
+    checkpoint holds them, (q, sx) from quant_tokens_i8; any T. Y bfloat16, or y_dtype / the dtype of a given Y."""
+    import torch
+    fn = "gemm_w8a8"
+    ldq, ldw = _matrix(fn, "q", q, (None, None), torch.int8), _matrix(fn, "W", W, (None, q.shape[-1]), torch.int8)
+    (T, K), N = q.shape, W.shape[0]
+    _whole(fn, "sw", sw, (N,), torch.float32)
+    _whole(fn, "sx", sx, (T,), torch.float32)
+    Y, ldy, code = _w8_out(fn, Y, y_dtype, T, N, torch.bfloat16, q.device)
+    _here(fn, W, sw, q, sx, Y)
+    _check(lib().qw_w8a8_gemm(_ptr(W), ldw, _ptr(sw), _ptr(q), ldq, _ptr(sx), T, _ptr(Y), ldy, code, N, K, _stream()),
+           "qw_w8a8_gemm")
+    return Y
+
+
+def w8a8_workspace_size(T, K):
+    return lib().qw_w8a8_workspace_size(T, K)
+
+
+def linear_w8a8(W, sw, x, Y=None, y_dtype=None, workspace=None):
+    """gemm_w8a8(W, sw, *quant_tokens_i8(x)) in one call, bit for bit; x [T][K] float32, bfloat16 or float16. Y of
+    x's type, or y_dtype / the dtype of a given Y."""
+    import torch
+    fn = "linear_w8a8"
+    ldx, ldw = _matrix(fn, "x", x, (None, None)), _matrix(fn, "W", W, (None, x.shape[-1]), torch.int8)
+    (T, K), N = x.shape, W.shape[0]
+    _whole(fn, "sw", sw, (N,), torch.float32)
+    code = _tcode(x)
+    Y, ldy, ycode = _w8_out(fn, Y, y_dtype, T, N, x.dtype, x.device)
+    if workspace is None:
+        workspace = torch.empty(w8a8_workspace_size(T, K), dtype=torch.uint8, device=x.device)
+    _here(fn, W, sw, x, Y, workspace)
+    _check(lib().qw_w8a8_linear(_ptr(W), ldw, _ptr(sw), _ptr(x), code, ldx, T, _ptr(Y), ldy, ycode, N, K,
+                                _ptr(workspace), workspace.numel() * workspace.element_size(), _stream()),
+           "qw_w8a8_linear")
+    return Y
+
+
+def moe_w8a8_tile_m():
+    return lib().qw_moe_w8a8_tile_m()
+
+
+def moe_w8a8_workspace_size(T, topk, H, F):
+    return lib().qw_moe_w8a8_workspace_size(T, topk, H, F)
+
+
+def moe_experts_w8a8(gate, up, down, route, x, h=None, yp=None, yp_dtype=None, workspace=None):
+    """The routed experts in W8A8 (route from moe_route or moe_sort with tile_m = moe_w8a8_tile_m()): gate and up
+    (int8 [E][F][H], fp32 [E][F]), down (int8 [E][H][F], fp32 [E][H]), x [T][H] float32, bfloat16 or float16. Returns
+    (h fp16 [T*k][F], yp [T*k][H]); yp float16, or yp_dtype / the dtype of a given yp."""
+    import torch
+    fn = "moe_experts_w8a8"
+    T, topk, E = route.T, route.topk, route.E
+    if gate[0].dim() != 3:
+        raise ValueError(f"{fn}: gate is {tuple(gate[0].shape)}, not [E][F][H]")
+    F, H = gate[0].shape[1:]
+    for name, (w, s), n, k in (("gate", gate, F, H), ("up", up, F, H), ("down", down, H, F)):
+        _whole(fn, name, w, (E, n, k), torch.int8)
+        _whole(fn, name + " scales", s, (E, n), torch.float32)
+    if route.tile_m != moe_w8a8_tile_m():
+        raise ValueError(f"{fn}: route has the tile list of tile_m = {route.tile_m}, not moe_w8a8_tile_m()")
+    code = _tcode(x)
+    _whole(fn, "x", x, (T, H), x.dtype)
+    if h is None:
+        h = torch.empty((T * topk, F), dtype=torch.float16, device=x.device)
+    if yp is None:
+        yp = torch.empty((T * topk, H), dtype=yp_dtype if yp_dtype is not None else torch.float16, device=x.device)
+    elif yp_dtype is not None and yp.dtype != yp_dtype:
+        raise TypeError(f"{fn}: yp is {yp.dtype}, not {yp_dtype}")
+    _whole(fn, "h", h, (T * topk, F), torch.float16)
+    _whole(fn, "yp", yp, (T * topk, H), yp.dtype)
+    ycode = _tcode(yp)
+    if workspace is None:
+        workspace = torch.empty(moe_w8a8_workspace_size(T, topk, H, F), dtype=torch.uint8, device=x.device)
+    _here(fn, x, h, yp, workspace, route.offsets, *gate, *up, *down)
+    rc = lib().qw_moe_experts_w8a8(*[_ptr(t) for t in (*gate, *up, *down)], E, H, F, _ptr(route.offsets),
+                                   _ptr(route.pair_tok), _ptr(route.tile_e), _ptr(route.tile_m0), _ptr(route.n_tiles),
+                                   _ptr(x), code, T, topk, _ptr(h), _ptr(yp), ycode, _ptr(workspace),
+                                   workspace.numel() * workspace.element_size(), _stream())
+    _check(rc, "qw_moe_experts_w8a8")
+    return h, yp
+
+
+# ----------------------------------------- tokens sorted by expert and back
+def moe_sort(top_e, E, tile_m=0, out=None):
+    """The slots of given choices top_e int32 [T][k], as a Route (top_w is not set): experts ascending, within one
+    the choices in order; a choice outside 0 .. E - 1 has slot -1, a place behind the last slot token -1."""
+    import torch
+    fn = "moe_sort"
+    if top_e.dim() != 2:
+        raise ValueError(f"{fn}: top_e is {tuple(top_e.shape)}, not [T][k]")
+    T, k = top_e.shape
+    _whole(fn, "top_e", top_e, (T, k), torch.int32)
+    if out is None:
+        r = Route.__new__(Route)
+        r.T, r.E, r.topk, r.tile_m, r.top_w = T, E, k, tile_m, None
+        P = T * k
+        nt = P // abs(tile_m) + E if tile_m else 0
+        # (one buffer for all of the lists: an allocation each would cost more than the sort)
+        own = torch.empty(2 * P + 3 * E + 3 + 2 * nt, dtype=torch.int32, device=top_e.device)
+        slot, r.pair_tok, r.counts, r.offsets, r.active, r.n_active, tile_e, tile_m0, n_tiles = own.split(
+            (P, P, E, E + 1, E, 1, nt, nt, 1))
+        r.tok_slot = slot.view(T, k)
+        r.tile_e, r.tile_m0, r.n_tiles = (tile_e, tile_m0, n_tiles) if tile_m else (None, None, None)
+    else:
+        r = out
+        if (r.T, r.E, r.topk, r.tile_m) != (T, E, k, tile_m):
+            raise ValueError(f"{fn}: out was made for T, E, k, tile_m = {r.T, r.E, r.topk, r.tile_m}")
+        r.top_w = None
+    r.top_e = top_e
+    _here(fn, top_e, r.pair_tok)
+    rc = lib().qw_moe_sort(_ptr(top_e), T, E, k, tile_m, _ptr(r.counts), _ptr(r.offsets), _ptr(r.tok_slot),
+                           _ptr(r.pair_tok), _ptr(r.active), _ptr(r.n_active), _ptr(r.tile_e), _ptr(r.tile_m0),
+                           _ptr(r.n_tiles), _stream())
+    _check(rc, "qw_moe_sort")
+    return r
+
+
+def _slots(fn, tok_slot):
+    import torch
+    if tok_slot.dim() != 2:
+        raise ValueError(f"{fn}: tok_slot is {tuple(tok_slot.shape)}, not [T][k]")
+    _whole(fn, "tok_slot", tok_slot, tuple(tok_slot.shape), torch.int32)
+    return tok_slot.shape
+
+
+def moe_permute(x, tok_slot, xs=None):
+    """The rows in slot order: xs[tok_slot[t][i]] = x[t] (x [T][H] of 1, 2 or 4 bytes an element). Rows of xs
+    [T*k][H] that no choice has are left as they were (a new xs: not set). Its gradient is moe_permute_backward."""
+    import torch
+    fn = "moe_permute"
+    T, k = _slots(fn, tok_slot)
+    ldx = _matrix(fn, "x", x, (T, None))
+    H = x.shape[1]
+    if xs is None:
+        xs = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
+    ldxs = _matrix(fn, "xs", xs, (T * k, H), x.dtype)
+    _here(fn, x, tok_slot, xs)
+    _check(lib().qw_moe_permute(_ptr(x), ldx, x.element_size(), T, k, H, _ptr(tok_slot), _ptr(xs), ldxs, _stream()),
+           "qw_moe_permute")
+    return xs
+
+
+def moe_unpermute(yp, tok_slot, tok_w=None, out=None, out_dtype=None):
+    """out[t] = sum_i tok_w[t][i] yp[tok_slot[t][i]] over the choices with a slot, in order, in fp32 (tok_w None: all
+    1); yp [T*k][H]. out of yp's type, or out_dtype / the dtype of a given out. moe_combine is the form with a shared
+    expert's rows."""
+    import torch
+    fn = "moe_unpermute"
+    T, k = _slots(fn, tok_slot)
+    ldyp = _matrix(fn, "yp", yp, (T * k, None))
+    H = yp.shape[1]
+    if tok_w is not None:
+        _whole(fn, "tok_w", tok_w, (T, k), torch.float32)
+    code = _tcode(yp)
+    out, ldo, ocode = _w8_out(fn, out, out_dtype, T, H, yp.dtype, yp.device)
+    _here(fn, yp, tok_slot, tok_w, out)
+    _check(lib().qw_moe_unpermute(_ptr(yp), code, ldyp, _ptr(tok_slot), _ptr(tok_w), T, k, H, _ptr(out), ocode, ldo,
+                                  _stream()), "qw_moe_unpermute")
+    return out
+
+
+def moe_permute_backward(dxs, tok_slot, dx=None, dx_dtype=None):
+    """The gradient of moe_permute: dx[t] = sum_i dxs[tok_slot[t][i]]."""
+    return moe_unpermute(dxs, tok_slot, None, dx, dx_dtype)
+
+
+def moe_unpermute_backward(dout, yp, tok_slot, tok_w=None, dyp=None, dw=None, need_dyp=True, need_dw=True):
+    """The gradients of moe_unpermute from dout [T][H]: (dyp [T*k][H] of yp's type, dw fp32 [T][k]), either None
+    where it is not needed. Rows of dyp that no choice has are left as they were (a new dyp: not set)."""
+    import torch
+    fn = "moe_unpermute_backward"
+    T, k = _slots(fn, tok_slot)
+    ldyp = _matrix(fn, "yp", yp, (T * k, None))
+    H = yp.shape[1]
+    ldd = _matrix(fn, "dout", dout, (T, H))
+    dcode, code = _tcode(dout), _tcode(yp)
+    if tok_w is not None:
+        _whole(fn, "tok_w", tok_w, (T, k), torch.float32)
+    if not need_dyp:
+        dyp = None
+    elif dyp is None:
+        dyp = torch.empty((T * k, H), dtype=yp.dtype, device=yp.device)
+    if not need_dw:
+        dw = None
+    elif dw is None:
+        dw = torch.empty((T, k), dtype=torch.float32, device=yp.device)
+    lddyp = _matrix(fn, "dyp", dyp, (T * k, H), yp.dtype) if dyp is not None else H
+    if dw is not None:
+        _whole(fn, "dw", dw, (T, k), torch.float32)
+    _here(fn, dout, yp, tok_slot, tok_w, dyp, dw)
+    _check(lib().qw_moe_unpermute_backward(_ptr(dout), dcode, ldd, _ptr(yp), code, ldyp, _ptr(tok_slot), _ptr(tok_w), T,
+                                           k, H, _ptr(dyp), lddyp, _ptr(dw), _stream()), "qw_moe_unpermute_backward")
+    return dyp, dw
 
 
 def unpack(W, N, K):
