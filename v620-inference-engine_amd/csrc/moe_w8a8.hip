@@ -53,23 +53,27 @@ __global__ __launch_bounds__(S::THREADS) void moe_gate_up_w8a8_kernel(MoeW8A8Arg
         for (int j = 0; j < S::AJ; ++j) ap[j] = a.qx + int64_t(pt[min(m0 + S::load_row(j), t.M - 1)]) * a.H;
         i32x16 acc[S::MT][S::NT];
         w8_clear<S>(acc);
-        if (!w8_tile<S, 1>(ap, bp, a.H, acc)) continue;
+        unsigned char *spare;
+        if (!w8_tile<S, 1>(ap, bp, a.H, acc, spare)) continue;
+        const int m_first = m0 + S::m_base(), col = j0 + S::n_base() / 2, l32 = int(threadIdx.x) % 32;
+        float sx[S::MT], sg[S::NT / 2][16], su[S::NT / 2][16];
 #pragma unroll
-        for (int j = 0; j < S::NT; j += 2) {
-            const int col = j0 + S::n_of(j) / 64 * 32 + S::n_of(j) % 32;
-            if (col >= a.F) continue;
-            const float sg = a.gs[eF + col], su = a.us[eF + col];
+        for (int i = 0; i < S::MT; ++i) sx[i] = a.sx[pt[min(m_first + 32 * i + l32, t.M - 1)]];
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i)
+        for (int c = 0; c < S::NT / 2; ++c)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int m = m0 + S::m_of(i, r);
-                    if (m >= t.M) continue;
-                    const float sx = a.sx[pt[m]];
-                    const float g = w8_value(acc[i][j][r], sg, sx), u = w8_value(acc[i][j + 1][r], su, sx);
-                    w8_store(a.h, 2, int64_t(t.base + m) * a.F + col, silu_ref(g) * u);
-                }
-        }
+            for (int r = 0; r < 16; ++r) {
+                const int64_t n = eF + min(col + 32 * c + S::n_of(r), a.F - 1);
+                sg[c][r] = a.gs[n];
+                su[c][r] = a.us[n];
+            }
+        auto value = [&](int i, int c, int r) {
+            const float g = w8_value(acc[i][2 * c][r], sg[c][r], sx[i]);
+            return silu_ref(g) * w8_value(acc[i][2 * c + 1][r], su[c][r], sx[i]);
+        };
+        w8_output<S, S::NT / 2>(spare, a.h, 2, a.F - col, value, [&](int m) -> int64_t {
+            return m_first + m < t.M ? int64_t(t.base + m_first + m) * a.F + col : -1;
+        });
     }
 }
 
@@ -89,22 +93,20 @@ __global__ __launch_bounds__(S::THREADS) void moe_down_w8a8_kernel(MoeW8A8Args a
         for (int j = 0; j < S::AJ; ++j) ap[j] = a.qh + int64_t(t.base + min(m0 + S::load_row(j), t.M - 1)) * a.F;
         i32x16 acc[S::MT][S::NT];
         w8_clear<S>(acc);
-        if (!w8_tile<S, 2>(ap, bp, a.F, acc)) continue;
+        unsigned char *spare;
+        if (!w8_tile<S, 2>(ap, bp, a.F, acc, spare)) continue;
+        const int m_first = m0 + S::m_base(), n_first = n0 + S::n_base(), l32 = int(threadIdx.x) % 32;
+        float sx[S::MT], sw[S::NT][16];
 #pragma unroll
-        for (int j = 0; j < S::NT; ++j) {
-            const int n = n0 + S::n_of(j);
-            if (n >= a.H) continue;
-            const float sw = a.ds[eH + n];
+        for (int i = 0; i < S::MT; ++i) sx[i] = a.sh[t.base + min(m_first + 32 * i + l32, t.M - 1)];
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i)
+        for (int j = 0; j < S::NT; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int m = m0 + S::m_of(i, r);
-                    if (m < t.M)
-                        w8_store(a.yp, a.yp_type, int64_t(t.base + m) * a.H + n,
-                                 w8_value(acc[i][j][r], sw, a.sh[t.base + m]));
-                }
-        }
+            for (int r = 0; r < 16; ++r) sw[j][r] = a.ds[eH + min(n_first + 32 * j + S::n_of(r), a.H - 1)];
+        auto value = [&](int i, int j, int r) { return w8_value(acc[i][j][r], sw[j][r], sx[i]); };
+        w8_output<S, S::NT>(spare, a.yp, a.yp_type, a.H - n_first, value, [&](int m) -> int64_t {
+            return m_first + m < t.M ? int64_t(t.base + m_first + m) * a.H + n_first : -1;
+        });
     }
 }
 
@@ -132,7 +134,7 @@ void launch_moe_w8a8(MoeW8A8Args a, const void *x, int x_type, int T, int topk, 
     a.sh = sh;
     const unsigned tiles = unsigned(P / size_t(-MW8_TILE_M)) + unsigned(a.E);
     launch_quant_tokens(x, x_type, a.H, T, a.H, qx, a.H, sx, s);
-    using S = W8Shape<64, 128, 2, 2, 1, 2>;
+    using S = W8Shape<64, 128, 2, 2, 1, 128, 2>;
     moe_gate_up_w8a8_kernel<S><<<tiles * unsigned((a.F + S::BN / 2 - 1) / (S::BN / 2)), S::THREADS, 0, s>>>(a);
     launch_quant_tokens(a.h, 2, a.F, int(P), a.F, qh, a.F, sh, s);
     moe_down_w8a8_kernel<S><<<tiles * unsigned((a.H + S::BN - 1) / S::BN), S::THREADS, 0, s>>>(a);

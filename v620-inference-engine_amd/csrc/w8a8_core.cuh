@@ -7,7 +7,7 @@
 // stages and waves, nor the batch changes a result: every shape of this loop
 // gives the same bits, and a variant is chosen by speed alone.
 //
-// Schedule. K runs in stages of 128 bytes through NS buffers of LDS, filled by
+// Schedule. K runs in stages of KB (64 or 128) bytes through NS buffers of LDS, filled by
 // direct global -> LDS loads (a wave instruction moves 8 rows of 128 bytes,
 // whole cache lines, from any row addresses: gathered rows cost the same as
 // neighbours) NS - 1 stages ahead. One barrier per stage: a wave waits for its
@@ -26,54 +26,54 @@ namespace qwq4 {
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int W8_KB = 128;  // K bytes per stage
-
 // What a lane loads for K columns past the row's end (K need not be a
 // multiple of 128): zeros, from memory that is always there.
 static __device__ const uint4 w8_zeros = {0u, 0u, 0u, 0u};
-
-// Byte offset of 16-byte chunk c (0..7) of row r in a [rows][128] stage. A
-// fragment read takes 32 consecutive rows at chunk c (lanes 0-31) and c + 1
-// (lanes 32-63); under this XOR its 16-lane parts fall on distinct banks.
-__device__ __forceinline__ int w8_swz_x(int r) { return (r & 7) ^ ((r >> 3) & 1); }
-__device__ __forceinline__ int w8_swz(int r, int c) { return r * W8_KB + ((c ^ w8_swz_x(r)) << 4); }
 
 __device__ __forceinline__ i32x16 w8_mfma(const uint4 &a, const uint4 &b, const i32x16 &c) {
     return __builtin_amdgcn_mfma_i32_32x32x32_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0,
                                                  0);
 }
 
-template <int BM_, int BN_, int WM_, int WN_, int KW_, int NS_>
+template <int BM_, int BN_, int WM_, int WN_, int KW_, int KB_, int NS_>
 struct W8Shape {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KW = KW_, NS = NS_;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KW = KW_, KB = KB_, NS = NS_;
     static constexpr int NW = WM * WN * KW, THREADS = NW * WAVE;
     static constexpr int MT = BM / 32 / WM, NT = BN / 32 / WN;  // 32 x 32 tiles per wave
-    static constexpr int AJ = BM / 8 / NW, BJ = BN / 8 / NW;    // load instructions per wave and stage
-    static constexpr int STAGE = (BM + BN) * W8_KB;             // bytes of one buffer
-    static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && BM % (32 * WM) == 0 && BN % (32 * WN) == 0, "tile");
-    static_assert(KW == 1 || KW == 2 || KW == 4, "a stage has 4 slabs");
-    static_assert(NS >= 2 && NS <= 4 && (KW == 1 || KW <= NS + 1), "one buffer per partial sum");
+    static constexpr int CH = KB / 16, RPL = 1024 / KB;         // chunks per row, rows per load instruction
+    static constexpr int AJ = BM / RPL / NW, BJ = BN / RPL / NW;  // load instructions per wave and stage
+    static constexpr int NQ = KB / 32 / KW;                     // slabs per wave and stage
+    static_assert(KB == 64 || KB == 128, "a stage's row is half a cache line or one");
+    static_assert(BM % (RPL * NW) == 0 && BN % (RPL * NW) == 0 && BM % (32 * WM) == 0 && BN % (32 * WN) == 0, "tile");
+    static_assert(NQ >= 1 && NQ * 32 * KW == KB, "whole slabs per wave");
+    static_assert(NS >= 2 && NS <= 5 && (KW == 1 || KW <= NS + 1), "one buffer per partial sum");
+    static_assert(NS * NQ % 2 == 0, "the fragments alternate between two sets of registers");
     static_assert(KW == 1 || WM * WN == 1, "partial sums are exchanged per wave tile");
-    static_assert(KW == 1 || BM * BN * 4 <= STAGE, "a partial sum fits a buffer");
+    static_assert(KW == 1 || BM * 4 <= KB, "a partial sum fits a buffer of weight rows");
 
+    // Byte offset of 16-byte chunk c of row r in a [rows][KB] buffer. A
+    // fragment read takes 32 consecutive rows at chunk c (lanes 0-31) and
+    // c + 1 (lanes 32-63); under this XOR each 16 lanes of it fall on the 64
+    // banks once.
+    __device__ static __forceinline__ int swz_x(int r) { return KB == 128 ? (r & 7) ^ ((r >> 3) & 1) : (r >> 2) & 3; }
+    __device__ static __forceinline__ int swz(int r, int c) { return r * KB + ((c ^ swz_x(r)) << 4); }
     // The tile row that part j of this lane's loads belongs to: A rows for
     // j < AJ, weight rows likewise for j < BJ.
     __device__ static __forceinline__ int load_row(int j) {
-        return (j * NW + int(threadIdx.x) / WAVE) * 8 + int(threadIdx.x) % WAVE / 8;
+        return (j * NW + int(threadIdx.x) / WAVE) * RPL + int(threadIdx.x) % WAVE / CH;
     }
-    // The chunk of that row it loads (the LDS slot is lane % 8).
-    __device__ static __forceinline__ int load_chunk(int j) {
-        return (int(threadIdx.x) % 8) ^ w8_swz_x(load_row(j));
-    }
-    // Wave coordinates, and the tile row / column of a lane's accumulator
-    // element: row 32 i + ..(r), column 32 j + lane % 32 of the wave's part.
+    // The chunk of that row it loads (its place in the row is lane % CH).
+    __device__ static __forceinline__ int load_chunk(int j) { return (int(threadIdx.x) % CH) ^ swz_x(load_row(j)); }
+    // The wave's place over the tile: its first row of Q and of W. Element r
+    // of accumulator (i, j) is row m_base() + 32 i + lane % 32 of Q and row
+    // n_base() + 32 j + n_of(r) of W.
     __device__ static __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE); }
-    __device__ static __forceinline__ int m_of(int i, int r) {
-        return (wave() / KW / WN * MT + i) * 32 + 8 * (r / 4) + 4 * (int(threadIdx.x) % WAVE / 32) + r % 4;
-    }
-    __device__ static __forceinline__ int n_of(int j) {
-        return (wave() / KW % WN * NT + j) * 32 + int(threadIdx.x) % 32;
-    }
+    __device__ static __forceinline__ int m_base() { return wave() / KW / WN * MT * 32; }
+    __device__ static __forceinline__ int n_base() { return wave() / KW % WN * NT * 32; }
+    __device__ static __forceinline__ int n_of(int r) { return 8 * (r / 4) + 4 * (int(threadIdx.x) % WAVE / 32) + r % 4; }
+    // LDS that a wave has to itself after the sums
+    static constexpr int PARTS = NS >= 4 ? 8 : 4;  // buffers it comes from
+    static constexpr int SPARE = (BM < BN ? BM : BN) * KB / ((NW + PARTS - 1) / PARTS);
 };
 
 // Waits until at most N vector-memory operations of this wave are in flight
@@ -91,102 +91,144 @@ __device__ __forceinline__ void w8_stage_barrier() {
 // start of the int8 row load_row(j) of Q / W (any valid row where the tile
 // passes the matrix). With KW > 1 the sums end in the waves with wave % KW
 // == 0 (acc of the others is void); returns whether this wave holds sums.
-// The LDS is not free for reuse until the block's next barrier. (USE tags the
-// caller: each call site instantiates its own specialization; the host
-// compilation pass rejects a second call site of a shared one.)
+// spare: S::SPARE bytes of LDS for this wave until the block's next barrier,
+// which has to come before another tile. (USE tags the caller: each call site
+// instantiates its own specialization; the host compilation pass rejects a
+// second call site of a shared one.)
 template <class S, int USE>
 __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t *(&bp)[S::BJ], int K,
-                                        i32x16 (&acc)[S::MT][S::NT]) {
+                                        i32x16 (&acc)[S::MT][S::NT], unsigned char *&spare) {
     constexpr int NS = S::NS, LPW = S::AJ + S::BJ;
-    __shared__ __align__(16) unsigned char s0[S::STAGE], s1[S::STAGE];
-    __shared__ __align__(16) unsigned char s2[NS > 2 ? S::STAGE : 16], s3[NS > 3 ? S::STAGE : 16];
+    constexpr int AB = S::BM * S::KB, BB = S::BN * S::KB;
+    __shared__ __align__(16) unsigned char sa0[AB], sa1[AB], sa2[NS > 2 ? AB : 16], sa3[NS > 3 ? AB : 16],
+        sa4[NS > 4 ? AB : 16];
+    __shared__ __align__(16) unsigned char sb0[BB], sb1[BB], sb2[NS > 2 ? BB : 16], sb3[NS > 3 ? BB : 16],
+        sb4[NS > 4 ? BB : 16];
     const int wave = S::wave(), lane = int(threadIdx.x) % WAVE, l32 = lane % 32, lh = lane / 32;
-    const int nk = (K + W8_KB - 1) / W8_KB;
+    const int nk = (K + S::KB - 1) / S::KB;
     // (distinct arrays picked at compile time: the compiler then sees that the
     // loads in flight into one do not touch the buffer being read)
-    auto buf = [&](auto i) -> unsigned char * {
-        if constexpr (decltype(i)::value == 0) return s0;
-        else if constexpr (decltype(i)::value == 1) return s1;
-        else if constexpr (decltype(i)::value == 2) return s2;
-        else return s3;
+    auto buf_a = [&](auto i) -> unsigned char * {
+        if constexpr (decltype(i)::value == 0) return sa0;
+        else if constexpr (decltype(i)::value == 1) return sa1;
+        else if constexpr (decltype(i)::value == 2) return sa2;
+        else if constexpr (decltype(i)::value == 3) return sa3;
+        else return sa4;
     };
-    auto issue = [&](int ks, unsigned char *dst) {
-        const int k0 = ks * W8_KB;
-        if (k0 + W8_KB <= K) {
+    auto buf_b = [&](auto i) -> unsigned char * {
+        if constexpr (decltype(i)::value == 0) return sb0;
+        else if constexpr (decltype(i)::value == 1) return sb1;
+        else if constexpr (decltype(i)::value == 2) return sb2;
+        else if constexpr (decltype(i)::value == 3) return sb3;
+        else return sb4;
+    };
+    // (a select per load rather than a branch on the row's end: the branch's
+    // two sides would share their last load, whose buffer the compiler then
+    // no longer knows)
+    const int8_t *zeros = reinterpret_cast<const int8_t *>(&w8_zeros);
+    auto issue = [&](int ks, unsigned char *da, unsigned char *db) {
 #pragma unroll
-            for (int j = 0; j < S::AJ; ++j)
-                __builtin_amdgcn_global_load_lds(ap[j] + k0 + S::load_chunk(j) * 16, dst + (j * S::NW + wave) * 1024, 16,
-                                                 0, 0);
+        for (int j = 0; j < S::AJ; ++j) {
+            const int k = ks * S::KB + S::load_chunk(j) * 16;
+            __builtin_amdgcn_global_load_lds(k < K ? ap[j] + k : zeros, da + (j * S::NW + wave) * 1024, 16, 0, 0);
+        }
 #pragma unroll
-            for (int j = 0; j < S::BJ; ++j)
-                __builtin_amdgcn_global_load_lds(bp[j] + k0 + S::load_chunk(j) * 16,
-                                                 dst + S::BM * W8_KB + (j * S::NW + wave) * 1024, 16, 0, 0);
-        } else {
-            const int8_t *z = reinterpret_cast<const int8_t *>(&w8_zeros);
-#pragma unroll
-            for (int j = 0; j < S::AJ; ++j) {
-                const int k = k0 + S::load_chunk(j) * 16;
-                __builtin_amdgcn_global_load_lds(k < K ? ap[j] + k : z, dst + (j * S::NW + wave) * 1024, 16, 0, 0);
-            }
-#pragma unroll
-            for (int j = 0; j < S::BJ; ++j) {
-                const int k = k0 + S::load_chunk(j) * 16;
-                __builtin_amdgcn_global_load_lds(k < K ? bp[j] + k : z, dst + S::BM * W8_KB + (j * S::NW + wave) * 1024,
-                                                 16, 0, 0);
-            }
+        for (int j = 0; j < S::BJ; ++j) {
+            const int k = ks * S::KB + S::load_chunk(j) * 16;
+            __builtin_amdgcn_global_load_lds(k < K ? bp[j] + k : zeros, db + (j * S::NW + wave) * 1024, 16, 0, 0);
         }
     };
     const int wm = wave / S::KW / S::WN, wn = wave / S::KW % S::WN, kw = wave % S::KW;
-    auto compute = [&](const unsigned char *a) {
-        const unsigned char *b = a + S::BM * W8_KB;
+    // Fragments of slab n of a stage (of this wave's NQ), read while the slab
+    // before is multiplied. (The scheduling barrier keeps the reads in front:
+    // left to itself the compiler moves them behind the products, and every
+    // slab then waits for its own.)
+    constexpr int NQ = S::NQ;
+    uint4 af[2][S::MT], bf[2][S::NT];
+    auto read = [&](int p, const unsigned char *a, const unsigned char *b, int n) {
+        const int c = 2 * (n * S::KW + kw) + lh;
 #pragma unroll
-        for (int q0 = 0; q0 < 4; q0 += S::KW) {
-            const int q = q0 + kw;
-            uint4 af[S::MT], bf[S::NT];
+        for (int i = 0; i < S::MT; ++i)
+            af[p][i] = *reinterpret_cast<const uint4 *>(a + S::swz((wm * S::MT + i) * 32 + l32, c));
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i)
-                af[i] = *reinterpret_cast<const uint4 *>(a + w8_swz((wm * S::MT + i) * 32 + l32, 2 * q + lh));
+        for (int j = 0; j < S::NT; ++j)
+            bf[p][j] = *reinterpret_cast<const uint4 *>(b + S::swz((wn * S::NT + j) * 32 + l32, c));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&](int p) {
 #pragma unroll
-            for (int j = 0; j < S::NT; ++j)
-                bf[j] = *reinterpret_cast<const uint4 *>(b + w8_swz((wn * S::NT + j) * 32 + l32, 2 * q + lh));
+        for (int i = 0; i < S::MT; ++i)
 #pragma unroll
-            for (int i = 0; i < S::MT; ++i)
+            for (int j = 0; j < S::NT; ++j) acc[i][j] = w8_mfma(bf[p][j], af[p][i], acc[i][j]);
+    };
+    // Stage ks in buffer I up to its last slab, whose fragments are then held.
+    auto inner = [&](auto i) {
+        constexpr int I = decltype(i)::value;
 #pragma unroll
-                for (int j = 0; j < S::NT; ++j) acc[i][j] = w8_mfma(af[i], bf[j], acc[i][j]);
+        for (int n = 0; n + 1 < NQ; ++n) {
+            read((I * NQ + n + 1) % 2, buf_a(i), buf_b(i), n + 1);
+            multiply((I * NQ + n) % 2);
         }
     };
+    // From stage ks in buffer I to the next. Before the last slab of ks is
+    // multiplied, the block meets: the next stage has landed and this one's
+    // buffer is read, so the next stage's first fragments and the loads of
+    // stage ks + NS go out, and the products behind them cover the wait. (The
+    // loop starts here, behind a wait that the compiler sees: entered at a
+    // read, it would wait for all loads in flight at every turn.)
     auto step = [&](auto i, int ks) {
         constexpr int I = decltype(i)::value;
-        if (ks + NS - 2 < nk) w8_stage_barrier<(NS - 2) * LPW>();
+        constexpr std::integral_constant<int, (I + 1) % NS> next{};
+        if (ks + NS <= nk) w8_stage_barrier<(NS - 2) * LPW>();
         else w8_stage_barrier<0>();
-        if (ks + NS - 1 < nk) issue(ks + NS - 1, buf(std::integral_constant<int, (I + NS - 1) % NS>{}));
-        compute(buf(i));
+        read((I * NQ + NQ) % 2, buf_a(next), buf_b(next), 0);
+        if (ks + NS < nk) issue(ks + NS, buf_a(i), buf_b(i));
+        multiply((I * NQ + NQ - 1) % 2);
+        inner(next);
     };
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
     using I3 = std::integral_constant<int, 3>;
-    issue(0, s0);
+    using I4 = std::integral_constant<int, 4>;
+    issue(0, sa0, sb0);
+    if (nk > 1) issue(1, sa1, sb1);
     if constexpr (NS > 2) {
-        if (nk > 1) issue(1, s1);
+        if (nk > 2) issue(2, sa2, sb2);
     }
     if constexpr (NS > 3) {
-        if (nk > 2) issue(2, s2);
+        if (nk > 3) issue(3, sa3, sb3);
     }
-    for (int ks = 0; ks < nk; ks += NS) {
+    if constexpr (NS > 4) {
+        if (nk > 4) issue(4, sa4, sb4);
+    }
+    if (nk >= NS) w8_stage_barrier<(NS - 1) * LPW>();
+    else w8_stage_barrier<0>();
+    read(0, sa0, sb0, 0);
+    inner(I0{});
+    for (int ks = 0; ks < nk - 1; ks += NS) {
         step(I0{}, ks);
-        if (ks + 1 < nk) step(I1{}, ks + 1);
+        if (ks + 1 < nk - 1) step(I1{}, ks + 1);
         if constexpr (NS > 2) {
-            if (ks + 2 < nk) step(I2{}, ks + 2);
+            if (ks + 2 < nk - 1) step(I2{}, ks + 2);
         }
         if constexpr (NS > 3) {
-            if (ks + 3 < nk) step(I3{}, ks + 3);
+            if (ks + 3 < nk - 1) step(I3{}, ks + 3);
+        }
+        if constexpr (NS > 4) {
+            if (ks + 4 < nk - 1) step(I4{}, ks + 4);
         }
     }
+    // the last slab of stage nk - 1 (NQ even: always in the second registers)
+    if (NQ % 2 == 0 || (nk - 1) % 2 == 1) multiply(1);
+    else multiply(0);
+    __syncthreads();  // the last stage is read
+    const int w = wave % S::PARTS;
+    spare = (w == 0 ? sa0 : w == 1 ? sb0 : w == 2 ? sa1 : w == 3 ? sb1 : w == 4 ? sa2 : w == 5 ? sb2 : w == 6 ? sa3 : sb3) +
+            wave / S::PARTS * S::SPARE;
     if constexpr (S::KW > 1) {
-        __syncthreads();  // the last stage is read
         auto part = [&](int w) -> int * {
-            return reinterpret_cast<int *>(w == 1 ? s0 : w == 2 ? s1 : s2);
+            return reinterpret_cast<int *>(w == 1 ? sb0 : w == 2 ? sb1 : sb2);
         };
         if (kw > 0) {
             int *p = part(kw);
@@ -227,10 +269,94 @@ __device__ __forceinline__ float w8_value(int sum, float sw, float sx) { return 
 
 // One element of an output of type QW_T_F32 (0), QW_T_BF16 (1) or QW_T_F16
 // (2; finite values beyond +-65504 saturate).
+__device__ __forceinline__ uint16_t w8_bits16(int type, float v) {
+    return type == 1 ? __builtin_bit_cast(uint16_t, __bf16(v)) : __builtin_bit_cast(uint16_t, f32_to_f16_satfinite(v));
+}
 __device__ __forceinline__ void w8_store(void *y, int type, int64_t at, float v) {
     if (type == 0) static_cast<float *>(y)[at] = v;
-    else if (type == 1) static_cast<uint16_t *>(y)[at] = f32_to_bf16_rne(v);
-    else static_cast<_Float16 *>(y)[at] = f32_to_f16_satfinite(v);
+    else static_cast<uint16_t *>(y)[at] = w8_bits16(type, v);
+}
+
+// The wave's values to rows of Y: value(i, c, r) is that of row 32 i +
+// lane % 32 of the wave's, column 32 c + S::n_of(r) of its NC * 32; row(m)
+// gives where row m of them starts in Y (in elements; negative: no such row)
+// and columns from `cols` on are left out. Through the wave's spare LDS, 32
+// rows at a time, so that a row goes out in 16-byte pieces next to each other
+// (stored as the accumulators hold them, 32 rows of 8 bytes an instruction,
+// a 4096 x 12288 product took 20 us longer).
+template <class S, int NC, int BYTES, class ValueF, class RowF>
+__device__ __forceinline__ void w8_store_rows(unsigned char *spare, void *Y, int type, int cols, ValueF value, RowF row) {
+    constexpr int FIT = (S::SPARE / 32 - 16) / (32 * BYTES);
+    constexpr int CG = FIT >= NC ? NC : FIT >= 2 && NC % 2 == 0 ? 2 : 1;  // 32-column groups at a time
+    static_assert(FIT >= 1, "32 columns fit");
+    constexpr int LD = CG * 32 * BYTES + 16, PIECES = CG * 32 * BYTES / 16, PER = 16 / BYTES;
+    const int lane = int(threadIdx.x) % WAVE, l32 = lane % 32, lh = lane / 32;
+    unsigned char *y8 = static_cast<unsigned char *>(Y);
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+        for (int c0 = 0; c0 < NC; c0 += CG) {
+#pragma unroll
+            for (int c = 0; c < CG; ++c)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = value(i, c0 + c, 4 * u + e);
+                    unsigned char *at = spare + l32 * LD + (c * 32 + 8 * u + 4 * lh) * BYTES;
+                    if constexpr (BYTES == 4) {
+                        *reinterpret_cast<float4 *>(at) = make_float4(v[0], v[1], v[2], v[3]);
+                    } else {
+                        *reinterpret_cast<uint2 *>(at) =
+                            make_uint2(w8_bits16(type, v[0]) | uint32_t(w8_bits16(type, v[1])) << 16,
+                                       w8_bits16(type, v[2]) | uint32_t(w8_bits16(type, v[3])) << 16);
+                    }
+                }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int p = 0; p < PIECES / 2; ++p) {
+                const int m = (p * WAVE + lane) / PIECES, piece = (p * WAVE + lane) % PIECES;
+                const uint4 w = *reinterpret_cast<const uint4 *>(spare + m * LD + piece * 16);
+                const int n = c0 * 32 + piece * PER;
+                const int64_t at = row(32 * i + m);
+                if (at < 0 || n >= cols) continue;
+                unsigned char *dst = y8 + (at + n) * BYTES;
+                if (n + PER <= cols && reinterpret_cast<uintptr_t>(dst) % 16 == 0) {
+                    *reinterpret_cast<uint4 *>(dst) = w;
+                } else {
+                    const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) {
+                        if (n + e >= cols) break;
+                        if constexpr (BYTES == 4) reinterpret_cast<uint32_t *>(dst)[e] = words[e];
+                        else reinterpret_cast<uint16_t *>(dst)[e] = uint16_t(words[e / 2] >> (16 * (e % 2)));
+                    }
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+}
+
+// w8_store_rows for either width of the output's type; the tiles whose waves
+// split K have little to store and do it as they hold it.
+template <class S, int NC, class ValueF, class RowF>
+__device__ __forceinline__ void w8_output(unsigned char *spare, void *Y, int type, int cols, ValueF value, RowF row) {
+    if constexpr (S::KW > 1) {
+#pragma unroll
+        for (int i = 0; i < S::MT; ++i) {
+            const int64_t at = row(32 * i + int(threadIdx.x) % 32);
+            if (at < 0) continue;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (32 * c + S::n_of(r) < cols) w8_store(Y, type, at + 32 * c + S::n_of(r), value(i, c, r));
+        }
+    } else if (type == 0) {
+        w8_store_rows<S, NC, 4>(spare, Y, type, cols, value, row);
+    } else {
+        w8_store_rows<S, NC, 2>(spare, Y, type, cols, value, row);
+    }
 }
 
 }  // namespace qwq4
