@@ -6,10 +6,18 @@
 //
 //   h[p]  = fp16(silu(g) * u),  g, u = W8A8 products of x[pair_tok[p]]
 //   yp[p] = W8A8 product of h[p], quantised per slot
+//
+// Work is the routing's tile list (an entry: an expert and 32 to 160 of its
+// slots) times blocks of weight rows. Above 8 tokens a block runs its entry in
+// tiles of 128 or 64 slots on the int8 MFMA (w8a8_core.cuh); up to 8 it streams
+// the weights past the slots' rows in LDS (w8a8_gemv.cuh). The sums being
+// whole numbers, both give a slot the same bits.
+#include <algorithm>
 #include <type_traits>
 
 #include "q4_kernels.hpp"
 #include "w8a8_core.cuh"
+#include "w8a8_gemv.cuh"
 
 namespace qwq4 {
 
@@ -30,86 +38,184 @@ __device__ __forceinline__ bool mw8_entry(const MoeW8A8Args &a, int tile, MW8Ent
     return true;
 }
 
-// gate/up: of every 64 weight rows of the tile the first 32 are gate rows, the
-// others the up rows of the same 32 columns of h: a wave holds both.
-template <class S>
-__global__ __launch_bounds__(S::THREADS) void moe_gate_up_w8a8_kernel(MoeW8A8Args a) {
+// ------------------------------------------------------------ tiles
+// Entry and block of weight rows of block b, nt of them per entry: an entry's
+// blocks go to one XCD (blocks go to the 8 in turn), whose L2 then holds the
+// entry's rows once.
+__device__ __forceinline__ int mw8_place(int b, int nt, int &col) {
+    col = b / 8 % nt;
+    return b / 8 / nt * 8 + b % 8;
+}
+
+using MW8Large = W8Shape<128, 128, 2, 2, 1, 128, 2>;
+using MW8Small = W8Shape<64, 128, 2, 2, 1, 128, 2>;
+
+// gate/up of slots m0 .. of the entry: of every 64 weight rows of the tile the
+// first 32 are gate rows, the others the up rows of the same 32 columns of h: a
+// wave holds both.
+template <class S, class L>
+__device__ __forceinline__ void gate_up_tile(const MoeW8A8Args &a, const MW8Entry &t, int m0, int j0) {
     static_assert(S::NT % 2 == 0, "a wave holds gate and up of a column");
-    const int nt = (a.F + S::BN / 2 - 1) / (S::BN / 2);
-    MW8Entry t;
-    if (!mw8_entry(a, int(blockIdx.x) / nt, t)) return;
-    const int j0 = int(blockIdx.x) % nt * (S::BN / 2);
     const int64_t eF = int64_t(t.e) * a.F;
+    const int32_t *pt = a.pair_tok + t.base;
     const int8_t *ap[S::AJ], *bp[S::BJ];
 #pragma unroll
     for (int j = 0; j < S::BJ; ++j) {
         const int r = S::load_row(j);
         bp[j] = ((r / 32) % 2 ? a.uw : a.gw) + (eF + min(j0 + r / 64 * 32 + r % 32, a.F - 1)) * a.H;
     }
-    const int32_t *pt = a.pair_tok + t.base;
-    for (int m0 = 0; m0 < t.M; m0 += S::BM) {
-        if (m0 > 0) __syncthreads();  // the tile before is read
 #pragma unroll
-        for (int j = 0; j < S::AJ; ++j) ap[j] = a.qx + int64_t(pt[min(m0 + S::load_row(j), t.M - 1)]) * a.H;
-        i32x16 acc[S::MT][S::NT];
-        w8_clear<S>(acc);
-        unsigned char *spare;
-        if (!w8_tile<S, 1>(ap, bp, a.H, acc, spare)) continue;
-        const int m_first = m0 + S::m_base(), col = j0 + S::n_base() / 2, l32 = int(threadIdx.x) % 32;
-        float sx[S::MT], sg[S::NT / 2][16], su[S::NT / 2][16];
+    for (int j = 0; j < S::AJ; ++j) ap[j] = a.qx + int64_t(pt[min(m0 + S::load_row(j), t.M - 1)]) * a.H;
+    i32x16 acc[S::MT][S::NT];
+    w8_clear<S>(acc);
+    unsigned char *spare;
+    w8_tile<S, 1, L>(ap, bp, a.H, acc, spare);
+    const int m_first = m0 + S::m_base(), col = j0 + S::n_base() / 2, l32 = int(threadIdx.x) % 32;
+    float sx[S::MT], sg[S::NT / 2][16], su[S::NT / 2][16];
 #pragma unroll
-        for (int i = 0; i < S::MT; ++i) sx[i] = a.sx[pt[min(m_first + 32 * i + l32, t.M - 1)]];
+    for (int i = 0; i < S::MT; ++i) sx[i] = a.sx[pt[min(m_first + 32 * i + l32, t.M - 1)]];
 #pragma unroll
-        for (int c = 0; c < S::NT / 2; ++c)
+    for (int c = 0; c < S::NT / 2; ++c)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t n = eF + min(col + 32 * c + S::n_of(r), a.F - 1);
-                sg[c][r] = a.gs[n];
-                su[c][r] = a.us[n];
-            }
-        auto value = [&](int i, int c, int r) {
-            const float g = w8_value(acc[i][2 * c][r], sg[c][r], sx[i]);
-            return silu_ref(g) * w8_value(acc[i][2 * c + 1][r], su[c][r], sx[i]);
-        };
-        w8_output<S, S::NT / 2>(spare, a.h, 2, a.F - col, value, [&](int m) -> int64_t {
-            return m_first + m < t.M ? int64_t(t.base + m_first + m) * a.F + col : -1;
-        });
-    }
+        for (int r = 0; r < 16; ++r) {
+            const int64_t n = eF + min(col + 32 * c + S::n_of(r), a.F - 1);
+            sg[c][r] = a.gs[n];
+            su[c][r] = a.us[n];
+        }
+    auto value = [&](int i, int c, int r) {
+        const float g = w8_value(acc[i][2 * c][r], sg[c][r], sx[i]);
+        return silu_ref(g) * w8_value(acc[i][2 * c + 1][r], su[c][r], sx[i]);
+    };
+    w8_output<S, S::NT / 2>(spare, a.h, 2, a.F - col, value, [&](int m) -> int64_t {
+        return m_first + m < t.M ? int64_t(t.base + m_first + m) * a.F + col : -1;
+    });
 }
 
-template <class S>
-__global__ __launch_bounds__(S::THREADS) void moe_down_w8a8_kernel(MoeW8A8Args a) {
-    const int nt = (a.H + S::BN - 1) / S::BN;
-    MW8Entry t;
-    if (!mw8_entry(a, int(blockIdx.x) / nt, t)) return;
-    const int n0 = int(blockIdx.x) % nt * S::BN;
+template <class S, class L>
+__device__ __forceinline__ void down_tile(const MoeW8A8Args &a, const MW8Entry &t, int m0, int n0) {
     const int64_t eH = int64_t(t.e) * a.H;
     const int8_t *ap[S::AJ], *bp[S::BJ];
 #pragma unroll
     for (int j = 0; j < S::BJ; ++j) bp[j] = a.dw + (eH + min(n0 + S::load_row(j), a.H - 1)) * a.F;
-    for (int m0 = 0; m0 < t.M; m0 += S::BM) {
+#pragma unroll
+    for (int j = 0; j < S::AJ; ++j) ap[j] = a.qh + int64_t(t.base + min(m0 + S::load_row(j), t.M - 1)) * a.F;
+    i32x16 acc[S::MT][S::NT];
+    w8_clear<S>(acc);
+    unsigned char *spare;
+    w8_tile<S, 2, L>(ap, bp, a.F, acc, spare);
+    const int m_first = m0 + S::m_base(), n_first = n0 + S::n_base(), l32 = int(threadIdx.x) % 32;
+    float sx[S::MT], sw[S::NT][16];
+#pragma unroll
+    for (int i = 0; i < S::MT; ++i) sx[i] = a.sh[t.base + min(m_first + 32 * i + l32, t.M - 1)];
+#pragma unroll
+    for (int j = 0; j < S::NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sw[j][r] = a.ds[eH + min(n_first + 32 * j + S::n_of(r), a.H - 1)];
+    auto value = [&](int i, int j, int r) { return w8_value(acc[i][j][r], sw[j][r], sx[i]); };
+    w8_output<S, S::NT>(spare, a.yp, a.yp_type, a.H - n_first, value, [&](int m) -> int64_t {
+        return m_first + m < t.M ? int64_t(t.base + m_first + m) * a.H + n_first : -1;
+    });
+}
+
+// DOWN: the down projection, else gate/up. LARGE: tiles of 128 slots while
+// more than 64 are left; without, 64 alone, in less LDS.
+template <bool DOWN, bool LARGE>
+__global__ __launch_bounds__(256, 2) void moe_w8a8_kernel(MoeW8A8Args a) {
+    static_assert(MW8Large::THREADS == 256 && MW8Small::THREADS == 256, "one launch shape");
+    using L = W8Lds<std::conditional_t<LARGE, MW8Large, MW8Small>, DOWN ? 2 : 1>;
+    constexpr int COLS = DOWN ? MW8Large::BN : MW8Large::BN / 2;
+    int col;
+    MW8Entry t;
+    if (!mw8_entry(a, mw8_place(int(blockIdx.x), ((DOWN ? a.H : a.F) + COLS - 1) / COLS, col), t)) return;
+    for (int m0 = 0; m0 < t.M;) {
         if (m0 > 0) __syncthreads();  // the tile before is read
-#pragma unroll
-        for (int j = 0; j < S::AJ; ++j) ap[j] = a.qh + int64_t(t.base + min(m0 + S::load_row(j), t.M - 1)) * a.F;
-        i32x16 acc[S::MT][S::NT];
-        w8_clear<S>(acc);
-        unsigned char *spare;
-        if (!w8_tile<S, 2>(ap, bp, a.F, acc, spare)) continue;
-        const int m_first = m0 + S::m_base(), n_first = n0 + S::n_base(), l32 = int(threadIdx.x) % 32;
-        float sx[S::MT], sw[S::NT][16];
-#pragma unroll
-        for (int i = 0; i < S::MT; ++i) sx[i] = a.sh[t.base + min(m_first + 32 * i + l32, t.M - 1)];
-#pragma unroll
-        for (int j = 0; j < S::NT; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sw[j][r] = a.ds[eH + min(n_first + 32 * j + S::n_of(r), a.H - 1)];
-        auto value = [&](int i, int j, int r) { return w8_value(acc[i][j][r], sw[j][r], sx[i]); };
-        w8_output<S, S::NT>(spare, a.yp, a.yp_type, a.H - n_first, value, [&](int m) -> int64_t {
-            return m_first + m < t.M ? int64_t(t.base + m_first + m) * a.H + n_first : -1;
-        });
+        if (LARGE && t.M - m0 > 64) {
+            if constexpr (DOWN) down_tile<MW8Large, L>(a, t, m0, col * COLS);
+            else gate_up_tile<MW8Large, L>(a, t, m0, col * COLS);
+            m0 += 128;
+        } else {
+            if constexpr (DOWN) down_tile<MW8Small, L>(a, t, m0, col * COLS);
+            else gate_up_tile<MW8Small, L>(a, t, m0, col * COLS);
+            m0 += 64;
+        }
     }
 }
 
+// ------------------------------------------------------------ few tokens
+// f with the number of slots to stage together as a constant: 1, 2 or (rows
+// that come quantised) 4 or 8.
+template <int XT, class F>
+__device__ __forceinline__ void mw8_by_slots(int M, F f) {
+    if (M <= 1) f(std::integral_constant<int, 1>{});
+    else if (XT != 3 || M <= 2) f(std::integral_constant<int, 2>{});
+    else if (M <= 4) f(std::integral_constant<int, 4>{});
+    else f(std::integral_constant<int, 8>{});
+}
+
+// gate/up of an entry: 8 columns of h per block, from rows x of type XT (3:
+// a.qx, a.sx).
+template <int XT, bool VEC>
+__global__ __launch_bounds__(256) void moe_gate_up_gemv_kernel(MoeW8A8Args a, const void *x) {
+    extern __shared__ __align__(16) unsigned char s_q[];
+    const int nt = (a.F + 7) / 8, j0 = int(blockIdx.x) % nt * 8;
+    MW8Entry t;
+    if (!mw8_entry(a, int(blockIdx.x) / nt, t)) return;
+    const int64_t eF = int64_t(t.e) * a.F, row = eF + min(j0 + gemv_row(), a.F - 1);
+    const int8_t *w[2] = {a.gw + row * a.H, a.uw + row * a.H};
+    const int32_t *pt = a.pair_tok + t.base;
+    mw8_by_slots<XT>(t.M, [&](auto tm) {
+        constexpr int TM = decltype(tm)::value;
+        for (int m0 = 0; m0 < t.M; m0 += TM) {
+            W8Stream<2> v;
+            v.load(w, a.H, gemv_wave());
+            auto token = [&](int m) { return int64_t(pt[min(m0 + m, t.M - 1)]); };
+            float sx[TM];
+            if (m0 > 0) __syncthreads();
+            if constexpr (XT == 3) gemv_stage_i8<TM>(a.qx, a.H, a.sx, a.H, s_q, sx, token);
+            else gemv_stage<XT, VEC, TM>(x, a.H, a.H, s_q, sx, token);
+            gemv_sums<TM, 2>(v, w, a.H, s_q, [&](auto sum) {
+                const int m = int(threadIdx.x) / 8, j = j0 + int(threadIdx.x) % 8;
+                if (m >= TM || m0 + m >= t.M || j >= a.F) return;
+                const float s = gemv_pick(sx, m);
+                const float g = w8_value(sum(m, int(threadIdx.x) % 8), a.gs[eF + j], s);
+                const float u = w8_value(sum(m, 8 + int(threadIdx.x) % 8), a.us[eF + j], s);
+                w8_store(a.h, 2, int64_t(t.base + m0 + m) * a.F + j, silu_ref(g) * u);
+            });
+        }
+    });
+}
+
+// down of an entry: 16 rows per block, from h (XT 2) or a.qh, a.sh (3).
+template <int XT, bool VEC>
+__global__ __launch_bounds__(256) void moe_down_gemv_kernel(MoeW8A8Args a) {
+    extern __shared__ __align__(16) unsigned char s_q[];
+    const int nt = (a.H + 15) / 16, n0 = int(blockIdx.x) % nt * 16;
+    MW8Entry t;
+    if (!mw8_entry(a, int(blockIdx.x) / nt, t)) return;
+    const int64_t eH = int64_t(t.e) * a.H;
+    const int8_t *w[2] = {a.dw + (eH + min(n0 + gemv_row(), a.H - 1)) * a.F,
+                          a.dw + (eH + min(n0 + 8 + gemv_row(), a.H - 1)) * a.F};
+    mw8_by_slots<XT>(t.M, [&](auto tm) {
+        constexpr int TM = decltype(tm)::value;
+        for (int m0 = 0; m0 < t.M; m0 += TM) {
+            W8Stream<2> v;
+            v.load(w, a.F, gemv_wave());
+            auto slot = [&](int m) { return int64_t(t.base + min(m0 + m, t.M - 1)); };
+            float sx[TM];
+            if (m0 > 0) __syncthreads();
+            if constexpr (XT == 3) gemv_stage_i8<TM>(a.qh, a.F, a.sh, a.F, s_q, sx, slot);
+            else gemv_stage<XT, VEC, TM>(a.h, a.F, a.F, s_q, sx, slot);
+            gemv_sums<TM, 2>(v, w, a.F, s_q, [&](auto sum) {
+                const int m = int(threadIdx.x) / 16, n = n0 + int(threadIdx.x) % 16;
+                if (m < TM && m0 + m < t.M && n < a.H)
+                    w8_store(a.yp, a.yp_type, int64_t(t.base + m0 + m) * a.H + n,
+                             w8_value(sum(m, int(threadIdx.x) % 16), a.ds[eH + n], gemv_pick(sx, m)));
+            });
+        }
+    });
+}
+
+// ------------------------------------------------------------ launches
 static size_t up256(size_t b) { return (b + 255) & ~size_t(255); }
 
 size_t moe_w8a8_workspace_bytes(int T, int topk, int H, int F) {
@@ -117,7 +223,6 @@ size_t moe_w8a8_workspace_bytes(int T, int topk, int H, int F) {
     return up256(size_t(T) * size_t(H)) + up256(size_t(T) * 4) + up256(P * size_t(F)) + up256(P * 4);
 }
 
-// x quantised, gate/up, h quantised, down: four launches on one stream.
 void launch_moe_w8a8(MoeW8A8Args a, const void *x, int x_type, int T, int topk, void *ws, hipStream_t s) {
     const size_t P = size_t(T) * size_t(topk);
     int8_t *w = static_cast<int8_t *>(ws);
@@ -132,12 +237,36 @@ void launch_moe_w8a8(MoeW8A8Args a, const void *x, int x_type, int T, int topk, 
     a.sx = sx;
     a.qh = qh;
     a.sh = sh;
-    const unsigned tiles = unsigned(P / size_t(-MW8_TILE_M)) + unsigned(a.E);
-    launch_quant_tokens(x, x_type, a.H, T, a.H, qx, a.H, sx, s);
-    using S = W8Shape<64, 128, 2, 2, 1, 128, 2>;
-    moe_gate_up_w8a8_kernel<S><<<tiles * unsigned((a.F + S::BN / 2 - 1) / (S::BN / 2)), S::THREADS, 0, s>>>(a);
-    launch_quant_tokens(a.h, 2, a.F, int(P), a.F, qh, a.F, sh, s);
-    moe_down_w8a8_kernel<S><<<tiles * unsigned((a.H + S::BN - 1) / S::BN), S::THREADS, 0, s>>>(a);
+    // entries of the list at most (each has a slot)
+    const unsigned tiles = unsigned(std::min(P, P / size_t(-MW8_TILE_M) + size_t(a.E)));
+    auto blocks = [](int rows, int per) { return unsigned((rows + per - 1) / per); };
+    const bool stream = T <= 8 && gemv_lds(8, std::max(a.H, a.F)) <= W8_GEMV_LDS;
+    if (stream && T <= 2) {
+        // one or two tokens: the blocks quantise the rows they stage
+        const unsigned gu = tiles * blocks(a.F, 8), dn = tiles * blocks(a.H, 16);
+        w8_by_rows(x, x_type, a.H, T, [&](auto xt, auto vec) {
+            moe_gate_up_gemv_kernel<decltype(xt)::value, decltype(vec)::value>
+                <<<gu, 256, gemv_lds(2, a.H), s>>>(a, x);
+        });
+        w8_by_rows(a.h, 2, a.F, int(P), [&](auto, auto vec) {
+            moe_down_gemv_kernel<2, decltype(vec)::value><<<dn, 256, gemv_lds(2, a.F), s>>>(a);
+        });
+    } else if (stream) {
+        launch_quant_tokens(x, x_type, a.H, T, a.H, qx, a.H, sx, s);
+        moe_gate_up_gemv_kernel<3, true><<<tiles * blocks(a.F, 8), 256, gemv_lds(8, a.H), s>>>(a, nullptr);
+        launch_quant_tokens(a.h, 2, a.F, int(P), a.F, qh, a.F, sh, s);
+        moe_down_gemv_kernel<3, true><<<tiles * blocks(a.H, 16), 256, gemv_lds(8, a.F), s>>>(a);
+    } else {
+        const unsigned rows = (tiles + 7) / 8 * 8;  // (whole turns of the 8 XCDs)
+        const unsigned gu = rows * blocks(a.F, MW8Large::BN / 2), dn = rows * blocks(a.H, MW8Large::BN);
+        const bool large = P > size_t(32) * size_t(a.E);
+        launch_quant_tokens(x, x_type, a.H, T, a.H, qx, a.H, sx, s);
+        if (large) moe_w8a8_kernel<false, true><<<gu, 256, 0, s>>>(a);
+        else moe_w8a8_kernel<false, false><<<gu, 256, 0, s>>>(a);
+        launch_quant_tokens(a.h, 2, a.F, int(P), a.F, qh, a.F, sh, s);
+        if (large) moe_w8a8_kernel<true, true><<<dn, 256, 0, s>>>(a);
+        else moe_w8a8_kernel<true, false><<<dn, 256, 0, s>>>(a);
+    }
 }
 
 }  // namespace qwq4

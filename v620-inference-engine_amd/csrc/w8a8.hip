@@ -13,80 +13,11 @@
 
 #include "q4_kernels.hpp"
 #include "w8a8_core.cuh"
+#include "w8a8_gemv.cuh"
 
 namespace qwq4 {
 
 // ------------------------------------------------------------ quantiser
-// The row scale of a maximum, and whether a row's values are all finite: a
-// row that is not gets scale NaN and zeros. (The maximum is taken over the
-// magnitudes' bit patterns: an infinity or NaN then has the largest.)
-__device__ __forceinline__ float w8_scale(uint32_t top, bool &finite) {
-    finite = top < 0x7f800000u;
-    const float mx = __builtin_bit_cast(float, top);
-    return !finite ? __builtin_nanf("") : top ? fmaxf(mx / 127.f, 1.17549435e-38f) : 1.f;
-}
-
-// 16 consecutive elements of a row of type XT as loaded, and their values.
-// VEC: the row is 16-byte aligned.
-template <int XT, bool VEC>
-struct W8Raw {
-    static constexpr int W = XT == 0 ? 16 : 8;
-    uint32_t w[W];
-    __device__ __forceinline__ void load(const void *x, int64_t at) {
-        if constexpr (VEC) {
-            const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const uint32_t *>(x) + (XT == 0 ? at : at / 2));
-#pragma unroll
-            for (int i = 0; i < W / 4; ++i) {
-                const uint4 v = p[i];
-                w[4 * i] = v.x;
-                w[4 * i + 1] = v.y;
-                w[4 * i + 2] = v.z;
-                w[4 * i + 3] = v.w;
-            }
-        } else if constexpr (XT == 0) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = static_cast<const uint32_t *>(x)[at + i];
-        } else {
-            const uint16_t *p = static_cast<const uint16_t *>(x) + at;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = uint32_t(p[2 * i]) | uint32_t(p[2 * i + 1]) << 16;
-        }
-    }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = 0u;
-    }
-    __device__ __forceinline__ float value(int i) const {
-        if constexpr (XT == 0) return __builtin_bit_cast(float, w[i]);
-        const uint16_t b = uint16_t(w[i / 2] >> (16 * (i % 2)));
-        return XT == 1 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
-    }
-    // (the words are taken anew afterwards: the values would otherwise stay
-    // in registers, two to a word)
-    __device__ __forceinline__ uint32_t top(uint32_t t) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) t = max(t, __builtin_bit_cast(uint32_t, value(i)) & 0x7fffffffu);
-#pragma unroll
-        for (int i = 0; i < W; ++i) asm volatile("" : "+v"(w[i]));
-        return t;
-    }
-    __device__ __forceinline__ uint4 quantised(float inv, bool finite) const {
-        uint32_t q[4] = {0u, 0u, 0u, 0u};
-        if (finite) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                q[i / 4] |= uint32_t(int(__builtin_rintf(value(i) * inv)) & 0xff) << (8 * (i % 4));
-        }
-        return make_uint4(q[0], q[1], q[2], q[3]);
-    }
-};
-
-__device__ __forceinline__ uint32_t wave_top(uint32_t t) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) t = max(t, uint32_t(__shfl_xor(int(t), o)));
-    return t;
-}
-
 // A row by G threads (64: a wave, four rows a block; 256: the block), 16
 // elements per thread and turn. C > 0: the row is held in C turns' registers
 // and read once; C = 0: any length, read twice (the second time from the
@@ -152,22 +83,9 @@ static void launch_quant_x(const void *x, int64_t ldx, int T, int K, int8_t *q, 
     else quant_tokens_kernel<XT, VEC, 256, 0><<<unsigned(T), 256, 0, s>>>(x, ldx, T, K, q, ldq, scale);
 }
 
-// f with the rows' type and whether each is 16-byte aligned, as constants
-template <class F>
-static void by_rows(const void *x, int x_type, int64_t ldx, int T, F f) {
-    const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (T == 1 || ldx * (x_type == 0 ? 4 : 2) % 16 == 0);
-    auto run = [&](auto xt) {
-        if (vec) f(xt, std::true_type{});
-        else f(xt, std::false_type{});
-    };
-    if (x_type == 0) run(std::integral_constant<int, 0>{});
-    else if (x_type == 1) run(std::integral_constant<int, 1>{});
-    else run(std::integral_constant<int, 2>{});
-}
-
 void launch_quant_tokens(const void *x, int x_type, int64_t ldx, int T, int K, int8_t *q, int64_t ldq, float *scale,
                          hipStream_t s) {
-    by_rows(x, x_type, ldx, T, [&](auto xt, auto vec) {
+    w8_by_rows(x, x_type, ldx, T, [&](auto xt, auto vec) {
         launch_quant_x<decltype(xt)::value, decltype(vec)::value>(x, ldx, T, K, q, ldq, scale, s);
     });
 }
@@ -224,143 +142,39 @@ static void launch_shape(const W8GemmArgs &a, hipStream_t s) {
 }
 
 // ------------------------------------------------------------ few tokens
-// Up to 8 tokens the product is a stream of the weights. A block takes 8 G
-// weight rows, its 4 waves the 128-byte steps of K in turn: a wave instruction
-// reads 128 bytes of each of 8 rows (whole cache lines of the row-major
-// matrix), lane (row, chunk) multiplies its 16 bytes by the tokens' in LDS
-// with v_dot4, and the 8 chunks and 4 waves are added at the end. For one or
-// two tokens the block quantises their rows itself (XT 0 to 2; 3: int8 rows
-// with their scales): that hides behind the first weights, which are requested
-// before, and saves the quantiser's launch (one token, 4096 -> 12288 from bf16:
-// 12.6 us against 15.2 in two launches).
+// Up to 8 tokens the product is a stream of the weights (w8a8_gemv.cuh), 8 G
+// rows of them per block. For one or two tokens the block quantises their rows
+// itself, which saves the quantiser's launch (one token, 4096 -> 12288 from
+// bf16: 12.6 us against 15.2 in two launches).
 template <int XT, bool VEC, int TM, int G>
 __global__ __launch_bounds__(256) void w8a8_gemv_kernel(W8GemmArgs a, const void *x, int64_t ldx) {
-    extern __shared__ __align__(16) unsigned char s_q[];  // [TM][kp]: the rows' 8 bits, zeros from K on
-    __shared__ uint32_t s_top[TM][4];
-    __shared__ int s_sum[4][TM][8 * G];
-    const int tid = int(threadIdx.x), wave = __builtin_amdgcn_readfirstlane(tid / WAVE), lane = tid % WAVE;
-    const int K = a.K, n16 = K / 16, steps = (K + 127) / 128, kp = steps * 128;
+    extern __shared__ __align__(16) unsigned char s_q[];
     const int n0 = int(blockIdx.x) * 8 * G;
-    constexpr int U = 8;  // steps a wave has on their way per row
     const int8_t *w[G];
 #pragma unroll
-    for (int g = 0; g < G; ++g) w[g] = a.W + int64_t(min(n0 + 8 * g + lane / 8, a.N - 1)) * a.ldw;
-    i32x4 v[U][G];
-    // steps s0 + 4 u of the wave; past the row's end any of its bytes (the
-    // tokens' are zeros there)
-    auto load = [&](int s0) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-                v[u][g] = __builtin_nontemporal_load(reinterpret_cast<const i32x4 *>(
-                    w[g] + 16 * int64_t(min((s0 + 4 * u) * 8 + lane % 8, n16 - 1))));
-    };
-    load(wave);
+    for (int g = 0; g < G; ++g) w[g] = a.W + int64_t(min(n0 + 8 * g + gemv_row(), a.N - 1)) * a.ldw;
+    W8Stream<G> v;
+    v.load(w, a.K, gemv_wave());
+    auto token = [&](int t) { return int64_t(min(t, a.T - 1)); };
     float sx[TM];
-    if constexpr (XT == 3) {
-#pragma unroll
-        for (int t = 0; t < TM; ++t) {
-            const uint4 *q = reinterpret_cast<const uint4 *>(a.q + int64_t(min(t, a.T - 1)) * a.ldq);
-            for (int i = tid; i < kp / 16; i += 256)
-                *reinterpret_cast<uint4 *>(s_q + t * kp + 16 * i) = i < n16 ? q[i] : make_uint4(0u, 0u, 0u, 0u);
-            sx[t] = a.sx[min(t, a.T - 1)];
+    if constexpr (XT == 3) gemv_stage_i8<TM>(a.q, a.ldq, a.sx, a.K, s_q, sx, token);
+    else gemv_stage<XT, VEC, TM>(x, ldx, a.K, s_q, sx, token);
+    gemv_sums<TM, G>(v, w, a.K, s_q, [&](auto sum) {
+        for (int i = int(threadIdx.x); i < TM * 8 * G; i += 256) {
+            const int t = i / (8 * G), r = i % (8 * G), n = n0 + r;
+            if (t < a.T && n < a.N)
+                w8_store(a.Y, a.y_type, int64_t(t) * a.ldy + n, w8_value(sum(t, r), a.sw[n], gemv_pick(sx, t)));
         }
-    } else {
-        constexpr int C = 2;  // the first C turns' elements are kept (rows up to 8192), the rest read again
-        W8Raw<XT, VEC> raw[TM][C];
-#pragma unroll
-        for (int t = 0; t < TM; ++t) {
-            const int64_t at = min(t, a.T - 1) * ldx;
-            uint32_t top = 0u;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                if (tid + 256 * c < n16) raw[t][c].load(x, at + (tid + 256 * c) * 16);
-                else raw[t][c].clear();
-            }
-#pragma unroll
-            for (int c = 0; c < C; ++c) top = raw[t][c].top(top);
-            for (int i = tid + 256 * C; i < n16; i += 256) {
-                W8Raw<XT, VEC> r;
-                r.load(x, at + i * 16);
-                top = r.top(top);
-            }
-            top = wave_top(top);
-            if (lane == 0) s_top[t][wave] = top;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int t = 0; t < TM; ++t) {
-            bool finite;
-            sx[t] = w8_scale(max(max(s_top[t][0], s_top[t][1]), max(s_top[t][2], s_top[t][3])), finite);
-            const float inv = 1.f / sx[t];
-            auto put = [&](int i, const W8Raw<XT, VEC> &r) {
-                *reinterpret_cast<uint4 *>(s_q + t * kp + 16 * i) = r.quantised(inv, finite);
-            };
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-                if (tid + 256 * c < kp / 16) put(tid + 256 * c, raw[t][c]);  // (zeros from K on)
-            for (int i = tid + 256 * C; i < kp / 16; i += 256) {
-                W8Raw<XT, VEC> r;
-                if (i < n16) r.load(x, min(t, a.T - 1) * ldx + i * 16);
-                else r.clear();
-                put(i, r);
-            }
-        }
-    }
-    __syncthreads();
-    int acc[TM][G];
-#pragma unroll
-    for (int t = 0; t < TM; ++t)
-#pragma unroll
-        for (int g = 0; g < G; ++g) acc[t][g] = 0;
-    for (int s0 = wave; s0 < steps; s0 += 4 * U) {
-        if (s0 != wave) load(s0);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (s0 + 4 * u >= steps) break;
-#pragma unroll
-            for (int t = 0; t < TM; ++t) {
-                const i32x4 q = *reinterpret_cast<const i32x4 *>(s_q + t * kp + (s0 + 4 * u) * 128 + lane % 8 * 16);
-#pragma unroll
-                for (int g = 0; g < G; ++g)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[t][g] = __builtin_amdgcn_sdot4(v[u][g][e], q[e], acc[t][g], false);
-            }
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < TM; ++t)
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-#pragma unroll
-            for (int o = 1; o < 8; o <<= 1) acc[t][g] += __shfl_xor(acc[t][g], o);
-            if (lane % 8 == 0) s_sum[wave][t][8 * g + lane / 8] = acc[t][g];
-        }
-    __syncthreads();
-    for (int i = tid; i < TM * 8 * G; i += 256) {
-        const int t = i / (8 * G), r = i % (8 * G), n = n0 + r;
-        if (t >= a.T || n >= a.N) continue;
-        float s = sx[0];
-#pragma unroll
-        for (int u = 1; u < TM; ++u) s = t == u ? sx[u] : s;
-        w8_store(a.Y, a.y_type, int64_t(t) * a.ldy + n,
-                 w8_value(s_sum[0][t][r] + s_sum[1][t][r] + s_sum[2][t][r] + s_sum[3][t][r], a.sw[n], s));
-    }
+    });
 }
 
-constexpr int W8_GEMV_LDS = 64 << 10;  // what a block stages of the tokens' rows at most
-
-static bool gemv_takes(int T, int K) {
-    const int tm = T <= 1 ? 1 : T <= 2 ? 2 : T <= 4 ? 4 : 8;
-    return T <= 8 && int64_t(tm) * ((K + 127) / 128 * 128) <= W8_GEMV_LDS;
-}
+static bool gemv_takes(int T, int K) { return T <= 8 && gemv_lds(T, K) <= W8_GEMV_LDS; }
 
 template <int XT, bool VEC>
 static void launch_gemv(const W8GemmArgs &a, const void *x, int64_t ldx, hipStream_t s) {
     auto run = [&](auto tm) {
         constexpr int TM = decltype(tm)::value;
-        const size_t lds = size_t(TM) * size_t((a.K + 127) / 128 * 128);
+        const size_t lds = gemv_lds(TM, a.K);
         if (a.N >= 8192)
             w8a8_gemv_kernel<XT, VEC, TM, 2><<<unsigned((a.N + 15) / 16), 256, lds, s>>>(a, x, ldx);
         else w8a8_gemv_kernel<XT, VEC, TM, 1><<<unsigned((a.N + 7) / 8), 256, lds, s>>>(a, x, ldx);
@@ -390,7 +204,7 @@ size_t w8a8_workspace_bytes(int T, int K) { return up256(size_t(T) * size_t(K)) 
 
 void launch_w8a8_linear(W8GemmArgs a, const void *x, int x_type, int64_t ldx, void *ws, hipStream_t s) {
     if (a.T <= 2 && gemv_takes(a.T, a.K)) {
-        by_rows(x, x_type, ldx, a.T, [&](auto xt, auto vec) {
+        w8_by_rows(x, x_type, ldx, a.T, [&](auto xt, auto vec) {
             launch_gemv<decltype(xt)::value, decltype(vec)::value>(a, x, ldx, s);
         });
         return;

@@ -76,6 +76,22 @@ struct W8Shape {
     static constexpr int SPARE = (BM < BN ? BM : BN) * KB / ((NW + PARTS - 1) / PARTS);
 };
 
+// The stage buffers of shape S; a kernel that runs several shapes takes those
+// of its largest for all of them.
+template <class S, int USE>
+struct W8Lds {
+    template <int I>
+    __device__ static __forceinline__ unsigned char *a() {
+        __shared__ __align__(16) unsigned char s[I < S::NS ? S::BM * S::KB : 16];
+        return s;
+    }
+    template <int I>
+    __device__ static __forceinline__ unsigned char *b() {
+        __shared__ __align__(16) unsigned char s[I < S::NS ? S::BN * S::KB : 16];
+        return s;
+    }
+};
+
 // Waits until at most N vector-memory operations of this wave are in flight
 // and its LDS reads are done, then the block's barrier. Nothing that touches
 // memory moves across.
@@ -95,19 +111,18 @@ __device__ __forceinline__ void w8_stage_barrier() {
 // which has to come before another tile. (USE tags the caller: each call site
 // instantiates its own specialization; the host compilation pass rejects a
 // second call site of a shared one.)
-template <class S, int USE>
+template <class S, int USE, class L = W8Lds<S, USE>>
 __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t *(&bp)[S::BJ], int K,
                                         i32x16 (&acc)[S::MT][S::NT], unsigned char *&spare) {
     constexpr int NS = S::NS, LPW = S::AJ + S::BJ;
-    constexpr int AB = S::BM * S::KB, BB = S::BN * S::KB;
-    __shared__ __align__(16) unsigned char sa0[AB], sa1[AB], sa2[NS > 2 ? AB : 16], sa3[NS > 3 ? AB : 16],
-        sa4[NS > 4 ? AB : 16];
-    __shared__ __align__(16) unsigned char sb0[BB], sb1[BB], sb2[NS > 2 ? BB : 16], sb3[NS > 3 ? BB : 16],
-        sb4[NS > 4 ? BB : 16];
-    const int wave = S::wave(), lane = int(threadIdx.x) % WAVE, l32 = lane % 32, lh = lane / 32;
-    const int nk = (K + S::KB - 1) / S::KB;
     // (distinct arrays picked at compile time: the compiler then sees that the
     // loads in flight into one do not touch the buffer being read)
+    unsigned char *const sa0 = L::template a<0>(), *const sa1 = L::template a<1>(), *const sa2 = L::template a<2>(),
+                  *const sa3 = L::template a<3>(), *const sa4 = L::template a<4>();
+    unsigned char *const sb0 = L::template b<0>(), *const sb1 = L::template b<1>(), *const sb2 = L::template b<2>(),
+                  *const sb3 = L::template b<3>(), *const sb4 = L::template b<4>();
+    const int wave = S::wave(), lane = int(threadIdx.x) % WAVE, l32 = lane % 32, lh = lane / 32;
+    const int nk = (K + S::KB - 1) / S::KB;
     auto buf_a = [&](auto i) -> unsigned char * {
         if constexpr (decltype(i)::value == 0) return sa0;
         else if constexpr (decltype(i)::value == 1) return sa1;
