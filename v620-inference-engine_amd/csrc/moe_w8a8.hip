@@ -47,8 +47,17 @@ __device__ __forceinline__ int mw8_place(int b, int nt, int &col) {
     return b / 8 / nt * 8 + b % 8;
 }
 
-using MW8Large = W8Shape<128, 128, 2, 2, 1, 128, 2>;
-using MW8Small = W8Shape<64, 128, 2, 2, 1, 128, 2>;
+// The tile heights of a launch, and what its buffers are made for.
+template <bool LARGE>
+struct MW8Tiles {
+    using H1 = W8Shape<128, 256, 2, 4, 1, 128, 3>;
+    using H0 = W8Shape<64, 256, 2, 4, 1, 128, 3>;
+};
+template <>
+struct MW8Tiles<false> {
+    using H1 = W8Shape<64, 128, 2, 2, 1, 128, 2>;
+    using H0 = H1;
+};
 
 // gate/up of slots m0 .. of the entry: of every 64 weight rows of the tile the
 // first 32 are gate rows, the others the up rows of the same 32 columns of h: a
@@ -117,28 +126,36 @@ __device__ __forceinline__ void down_tile(const MoeW8A8Args &a, const MW8Entry &
     });
 }
 
-// DOWN: the down projection, else gate/up. LARGE: tiles of 128 slots while
-// more than 64 are left; without, 64 alone, in less LDS.
+// DOWN: the down projection, else gate/up.
 template <bool DOWN, bool LARGE>
-__global__ __launch_bounds__(256, 2) void moe_w8a8_kernel(MoeW8A8Args a) {
-    static_assert(MW8Large::THREADS == 256 && MW8Small::THREADS == 256, "one launch shape");
-    using L = W8Lds<std::conditional_t<LARGE, MW8Large, MW8Small>, DOWN ? 2 : 1>;
-    constexpr int COLS = DOWN ? MW8Large::BN : MW8Large::BN / 2;
+__global__ __launch_bounds__(MW8Tiles<LARGE>::H1::THREADS, 2) void moe_w8a8_kernel(MoeW8A8Args a) {
+    using T = MW8Tiles<LARGE>;
+    using L = W8Lds<typename T::H1, DOWN ? 2 : 1>;
+    constexpr int COLS = DOWN ? T::H1::BN : T::H1::BN / 2;
     int col;
     MW8Entry t;
     if (!mw8_entry(a, mw8_place(int(blockIdx.x), ((DOWN ? a.H : a.F) + COLS - 1) / COLS, col), t)) return;
+    auto tile = [&](auto shape, int m0) {
+        using S = decltype(shape);
+        if constexpr (DOWN) down_tile<S, L>(a, t, m0, col * COLS);
+        else gate_up_tile<S, L>(a, t, m0, col * COLS);
+        return S::BM;
+    };
     for (int m0 = 0; m0 < t.M;) {
         if (m0 > 0) __syncthreads();  // the tile before is read
-        if (LARGE && t.M - m0 > 64) {
-            if constexpr (DOWN) down_tile<MW8Large, L>(a, t, m0, col * COLS);
-            else gate_up_tile<MW8Large, L>(a, t, m0, col * COLS);
-            m0 += 128;
-        } else {
-            if constexpr (DOWN) down_tile<MW8Small, L>(a, t, m0, col * COLS);
-            else gate_up_tile<MW8Small, L>(a, t, m0, col * COLS);
-            m0 += 64;
-        }
+        if constexpr (!LARGE) m0 += tile(typename T::H0{}, m0);
+        else if (t.M - m0 > T::H0::BM) m0 += tile(typename T::H1{}, m0);
+        else m0 += tile(typename T::H0{}, m0);
     }
+}
+
+template <bool LARGE>
+static void launch_moe_tiles(MoeW8A8Args a, unsigned tiles, size_t P, int8_t *qh, float *sh, hipStream_t s) {
+    constexpr int BN = MW8Tiles<LARGE>::H1::BN, THREADS = MW8Tiles<LARGE>::H1::THREADS;
+    const unsigned rows = (tiles + 7) / 8 * 8;  // (whole turns of the 8 XCDs)
+    moe_w8a8_kernel<false, LARGE><<<rows * unsigned((a.F + BN / 2 - 1) / (BN / 2)), THREADS, 0, s>>>(a);
+    launch_quant_tokens(a.h, 2, a.F, int(P), a.F, qh, a.F, sh, s);
+    moe_w8a8_kernel<true, LARGE><<<rows * unsigned((a.H + BN - 1) / BN), THREADS, 0, s>>>(a);
 }
 
 // ------------------------------------------------------------ few tokens
@@ -257,15 +274,9 @@ void launch_moe_w8a8(MoeW8A8Args a, const void *x, int x_type, int T, int topk, 
         launch_quant_tokens(a.h, 2, a.F, int(P), a.F, qh, a.F, sh, s);
         moe_down_gemv_kernel<3, true><<<tiles * blocks(a.H, 16), 256, gemv_lds(8, a.F), s>>>(a);
     } else {
-        const unsigned rows = (tiles + 7) / 8 * 8;  // (whole turns of the 8 XCDs)
-        const unsigned gu = rows * blocks(a.F, MW8Large::BN / 2), dn = rows * blocks(a.H, MW8Large::BN);
-        const bool large = P > size_t(32) * size_t(a.E);
         launch_quant_tokens(x, x_type, a.H, T, a.H, qx, a.H, sx, s);
-        if (large) moe_w8a8_kernel<false, true><<<gu, 256, 0, s>>>(a);
-        else moe_w8a8_kernel<false, false><<<gu, 256, 0, s>>>(a);
-        launch_quant_tokens(a.h, 2, a.F, int(P), a.F, qh, a.F, sh, s);
-        if (large) moe_w8a8_kernel<true, true><<<dn, 256, 0, s>>>(a);
-        else moe_w8a8_kernel<true, false><<<dn, 256, 0, s>>>(a);
+        if (P > size_t(32) * size_t(a.E)) launch_moe_tiles<true>(a, tiles, P, qh, sh, s);
+        else launch_moe_tiles<false>(a, tiles, P, qh, sh, s);
     }
 }
 

@@ -72,8 +72,7 @@ struct W8Shape {
     __device__ static __forceinline__ int n_base() { return wave() / KW % WN * NT * 32; }
     __device__ static __forceinline__ int n_of(int r) { return 8 * (r / 4) + 4 * (int(threadIdx.x) % WAVE / 32) + r % 4; }
     // LDS that a wave has to itself after the sums
-    static constexpr int PARTS = NS >= 4 ? 8 : 4;  // buffers it comes from
-    static constexpr int SPARE = (BM < BN ? BM : BN) * KB / ((NW + PARTS - 1) / PARTS);
+    static constexpr int SPARE = BN * KB / ((NW + NS - 1) / NS);  // (of the weights' buffers)
 };
 
 // The stage buffers of shape S; a kernel that runs several shapes takes those
@@ -137,21 +136,24 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
         else if constexpr (decltype(i)::value == 3) return sb3;
         else return sb4;
     };
-    // (a select per load rather than a branch on the row's end: the branch's
-    // two sides would share their last load, whose buffer the compiler then
-    // no longer knows)
+    // Load n of a stage's LPW. Past the end of the rows (the last stage of a K
+    // that is no multiple of KB) Q's chunks are zeros and W's any of the row's:
+    // a select rather than a branch, whose two sides would share their last
+    // load, whose buffer the compiler then no longer knows. All of a lane's
+    // loads are of one chunk.
+    static_assert(S::NW % 2 == 0, "load_chunk(j) is load_chunk(0)");
     const int8_t *zeros = reinterpret_cast<const int8_t *>(&w8_zeros);
+    auto issue_one = [&](int ks, int n, unsigned char *da, unsigned char *db) {
+        const int k = ks * S::KB + S::load_chunk(0) * 16;
+        if (n < S::AJ)
+            __builtin_amdgcn_global_load_lds(k < K ? ap[n] + k : zeros, da + (n * S::NW + wave) * 1024, 16, 0, 0);
+        else
+            __builtin_amdgcn_global_load_lds(bp[n - S::AJ] + min(k, K - 16),
+                                             db + ((n - S::AJ) * S::NW + wave) * 1024, 16, 0, 0);
+    };
     auto issue = [&](int ks, unsigned char *da, unsigned char *db) {
 #pragma unroll
-        for (int j = 0; j < S::AJ; ++j) {
-            const int k = ks * S::KB + S::load_chunk(j) * 16;
-            __builtin_amdgcn_global_load_lds(k < K ? ap[j] + k : zeros, da + (j * S::NW + wave) * 1024, 16, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < S::BJ; ++j) {
-            const int k = ks * S::KB + S::load_chunk(j) * 16;
-            __builtin_amdgcn_global_load_lds(k < K ? bp[j] + k : zeros, db + (j * S::NW + wave) * 1024, 16, 0, 0);
-        }
+        for (int n = 0; n < LPW; ++n) issue_one(ks, n, da, db);
     };
     const int wm = wave / S::KW / S::WN, wn = wave / S::KW % S::WN, kw = wave % S::KW;
     // Fragments of slab n of a stage (of this wave's NQ), read while the slab
@@ -176,71 +178,96 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
 #pragma unroll
             for (int j = 0; j < S::NT; ++j) acc[i][j] = w8_mfma(bf[p][j], af[p][i], acc[i][j]);
     };
-    // Stage ks in buffer I up to its last slab, whose fragments are then held.
-    auto inner = [&](auto i) {
-        constexpr int I = decltype(i)::value;
+    // The same with the loads of stage ks between the products: in front of
+    // them they would hold up all waves at once, behind the barrier.
+    auto multiply_and_issue = [&](int p, int ks, unsigned char *da, unsigned char *db) {
+        constexpr int TILES = S::MT * S::NT, PER = (LPW + TILES - 1) / TILES;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const int i = t / S::NT, j = t % S::NT;
+            acc[i][j] = w8_mfma(bf[p][j], af[p][i], acc[i][j]);
+#pragma unroll
+            for (int n = t * PER; n < (t + 1) * PER && n < LPW; ++n) issue_one(ks, n, da, db);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // A stage up to its last slab, whose fragments are then held; the first
+    // slab's are in set p0.
+    auto inner = [&](int p0, const unsigned char *a, const unsigned char *b) {
 #pragma unroll
         for (int n = 0; n + 1 < NQ; ++n) {
-            read((I * NQ + n + 1) % 2, buf_a(i), buf_b(i), n + 1);
-            multiply((I * NQ + n) % 2);
+            read((p0 + n + 1) % 2, a, b, n + 1);
+            multiply((p0 + n) % 2);
         }
     };
     // From stage ks in buffer I to the next. Before the last slab of ks is
     // multiplied, the block meets: the next stage has landed and this one's
     // buffer is read, so the next stage's first fragments and the loads of
-    // stage ks + NS go out, and the products behind them cover the wait. (The
-    // loop starts here, behind a wait that the compiler sees: entered at a
-    // read, it would wait for all loads in flight at every turn.)
+    // stage ks + NS go out, and the products behind them cover the wait. (There
+    // is a stage ks + NS: these steps have no branch. Around one the compiler
+    // moves the sums, or waits for all loads.)
     auto step = [&](auto i, int ks) {
         constexpr int I = decltype(i)::value;
         constexpr std::integral_constant<int, (I + 1) % NS> next{};
-        if (ks + NS <= nk) w8_stage_barrier<(NS - 2) * LPW>();
-        else w8_stage_barrier<0>();
+        w8_stage_barrier<(NS - 2) * LPW>();
         read((I * NQ + NQ) % 2, buf_a(next), buf_b(next), 0);
-        if (ks + NS < nk) issue(ks + NS, buf_a(i), buf_b(i));
-        multiply((I * NQ + NQ - 1) % 2);
-        inner(next);
+        multiply_and_issue((I * NQ + NQ - 1) % 2, ks + NS, buf_a(i), buf_b(i));
+        inner((I * NQ + NQ) % 2, buf_a(next), buf_b(next));
     };
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
     using I3 = std::integral_constant<int, 3>;
     using I4 = std::integral_constant<int, 4>;
+    // (a K of fewer stages loads its last one again, where nobody reads it)
     issue(0, sa0, sb0);
-    if (nk > 1) issue(1, sa1, sb1);
-    if constexpr (NS > 2) {
-        if (nk > 2) issue(2, sa2, sb2);
-    }
-    if constexpr (NS > 3) {
-        if (nk > 3) issue(3, sa3, sb3);
-    }
-    if constexpr (NS > 4) {
-        if (nk > 4) issue(4, sa4, sb4);
-    }
-    if (nk >= NS) w8_stage_barrier<(NS - 1) * LPW>();
-    else w8_stage_barrier<0>();
+    issue(min(1, nk - 1), sa1, sb1);
+    if constexpr (NS > 2) issue(min(2, nk - 1), sa2, sb2);
+    if constexpr (NS > 3) issue(min(3, nk - 1), sa3, sb3);
+    if constexpr (NS > 4) issue(min(4, nk - 1), sa4, sb4);
+    w8_stage_barrier<(NS - 1) * LPW>();
     read(0, sa0, sb0, 0);
-    inner(I0{});
-    for (int ks = 0; ks < nk - 1; ks += NS) {
+    inner(0, sa0, sb0);
+    int ks = 0;
+    for (; ks + 2 * NS - 1 < nk; ks += NS) {
         step(I0{}, ks);
-        if (ks + 1 < nk - 1) step(I1{}, ks + 1);
-        if constexpr (NS > 2) {
-            if (ks + 2 < nk - 1) step(I2{}, ks + 2);
+        step(I1{}, ks + 1);
+        if constexpr (NS > 2) step(I2{}, ks + 2);
+        if constexpr (NS > 3) step(I3{}, ks + 3);
+        if constexpr (NS > 4) step(I4{}, ks + 4);
+    }
+    // The last stages (up to 2 NS - 1; ks is at buffer 0 again), in one piece
+    // of code for every buffer.
+    constexpr int TWO = NQ % 2 ? 2 : 1;  // (with one slab a stage the sets change places every stage)
+    auto pick_a = [&](int i) { return i == 0 ? sa0 : i == 1 ? sa1 : i == 2 ? sa2 : i == 3 ? sa3 : sa4; };
+    auto pick_b = [&](int i) { return i == 0 ? sb0 : i == 1 ? sb1 : i == 2 ? sb2 : i == 3 ? sb3 : sb4; };
+    auto last = [&](int s, int p0) {
+        const int cur = s % NS, next = (s + 1) % NS;
+        if (s + NS <= nk) w8_stage_barrier<(NS - 2) * LPW>();
+        else w8_stage_barrier<0>();
+        read(p0, pick_a(next), pick_b(next), 0);
+        if (s + NS < nk) issue(s + NS, pick_a(cur), pick_b(cur));
+        multiply(1 - p0);
+        inner(p0, pick_a(next), pick_b(next));
+    };
+    if constexpr (TWO == 1) {
+        for (; ks < nk - 1; ++ks) last(ks, 0);
+        multiply(1);
+    } else {
+        for (; ks < nk - 2; ks += 2) {
+            last(ks, 1);
+            last(ks + 1, 0);
         }
-        if constexpr (NS > 3) {
-            if (ks + 3 < nk - 1) step(I3{}, ks + 3);
-        }
-        if constexpr (NS > 4) {
-            if (ks + 4 < nk - 1) step(I4{}, ks + 4);
+        if (ks < nk - 1) {
+            last(ks, 1);
+            multiply(1);
+        } else {
+            multiply(0);
         }
     }
-    // the last slab of stage nk - 1 (NQ even: always in the second registers)
-    if (NQ % 2 == 0 || (nk - 1) % 2 == 1) multiply(1);
-    else multiply(0);
     __syncthreads();  // the last stage is read
-    const int w = wave % S::PARTS;
-    spare = (w == 0 ? sa0 : w == 1 ? sb0 : w == 2 ? sa1 : w == 3 ? sb1 : w == 4 ? sa2 : w == 5 ? sb2 : w == 6 ? sa3 : sb3) +
-            wave / S::PARTS * S::SPARE;
+    const int w = wave % NS;
+    spare = (w == 0 ? sb0 : w == 1 ? sb1 : w == 2 ? sb2 : w == 3 ? sb3 : sb4) + wave / NS * S::SPARE;
     if constexpr (S::KW > 1) {
         auto part = [&](int w) -> int * {
             return reinterpret_cast<int *>(w == 1 ? sb0 : w == 2 ? sb1 : sb2);
