@@ -20,26 +20,33 @@
 namespace qwq4 {
 
 // ------------------------------------------------------------ sort
-// Exclusive scan over the values of the first E threads (1024-thread block);
-// the total is returned in every thread.
-__device__ __forceinline__ int rows_scan_excl(int v, int *s_w, int &total) {
+// Exclusive scans of three values per thread over the 1024-thread block: v
+// becomes the sums before the thread's, total the sums of all.
+__device__ __forceinline__ void rows_scan_excl(int (&v)[3], int (*s_w)[16], int (&total)[3]) {
     const int lane = int(threadIdx.x) % WAVE, wave = int(threadIdx.x) / WAVE;
-    int inc = v;
+    int inc[3];
 #pragma unroll
-    for (int o = 1; o < WAVE; o <<= 1) {
-        const int u = __shfl_up(inc, o);
-        if (lane >= o) inc += u;
-    }
-    if (lane == WAVE - 1) s_w[wave] = inc;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int w = 0; w < int(blockDim.x) / WAVE; ++w) {
-        before += w < wave ? s_w[w] : 0;
-        all += s_w[w];
+    for (int c = 0; c < 3; ++c) {
+        inc[c] = v[c];
+#pragma unroll
+        for (int o = 1; o < WAVE; o <<= 1) {
+            const int u = __shfl_up(inc[c], o);
+            if (lane >= o) inc[c] += u;
+        }
+        if (lane == WAVE - 1) s_w[c][wave] = inc[c];
     }
     __syncthreads();
-    total = all;
-    return before + inc - v;
+#pragma unroll
+    for (int c = 0; c < 3; ++c) {
+        int before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            before += w < wave ? s_w[c][w] : 0;
+            all += s_w[c][w];
+        }
+        total[c] = all;
+        v[c] = before + inc[c] - v[c];
+    }
 }
 
 // Every block counts the choices of all pairs and of the pairs before its own
@@ -49,7 +56,7 @@ __device__ __forceinline__ int rows_scan_excl(int v, int *s_w, int &total) {
 // its bit in the lanes that hold that expert. No block reads what another
 // writes, so one launch needs no hand-off.
 __global__ __launch_bounds__(1024) void sort_kernel(SortArgs a, int per) {
-    __shared__ int s_rest[1024], s_at[1024], s_w[16];
+    __shared__ int s_rest[1024], s_at[1024], s_w[3][16];
     const int tid = int(threadIdx.x), E = a.E, P = a.T * a.topk;
     const int p0 = int(blockIdx.x) * per, p1 = min(p0 + per, P);
     s_rest[tid] = 0;
@@ -69,27 +76,25 @@ __global__ __launch_bounds__(1024) void sort_kernel(SortArgs a, int per) {
     }
     __syncthreads();
     const int c = s_at[tid] + s_rest[tid];
-    int total;
-    const int off = rows_scan_excl(c, s_w, total);
+    const int ntl = a.tile_m != 0 ? tile_count(c, a.tile_m) : 0;
+    int at[3] = {c, c > 0, ntl}, all[3];  // slots, experts with any, list entries
+    rows_scan_excl(at, s_w, all);
+    const int off = at[0], total = all[0];
     s_at[tid] += off;
     if (blockIdx.x == 0) {
-        int n_act, n_tiles = 0;
-        const int act = rows_scan_excl(c > 0, s_w, n_act);
-        const int ntl = a.tile_m != 0 ? tile_count(c, a.tile_m) : 0;
-        const int tile0 = a.tile_m != 0 ? rows_scan_excl(ntl, s_w, n_tiles) : 0;
         if (tid < E) {
             a.offsets[tid] = off;
             a.counts[tid] = c;
-            if (c > 0) a.active[act] = tid;
+            if (c > 0) a.active[at[1]] = tid;
             for (int j = 0, m0 = 0; j < ntl; ++j, m0 += tile_rows(c - m0, a.tile_m)) {
-                a.tile_e[tile0 + j] = tid;
-                a.tile_m0[tile0 + j] = m0;
+                a.tile_e[at[2] + j] = tid;
+                a.tile_m0[at[2] + j] = m0;
             }
         }
         if (tid == 0) {
             a.offsets[E] = total;
-            *a.n_active = n_act;
-            if (a.tile_m != 0) *a.n_tiles = n_tiles;
+            *a.n_active = all[1];
+            if (a.tile_m != 0) *a.n_tiles = all[2];
         }
         for (int i = total + tid; i < P; i += 1024) a.pair_tok[i] = -1;
     }

@@ -49,7 +49,7 @@ struct W8Shape {
     static_assert(NS >= 2 && NS <= 5 && (KW == 1 || KW <= NS + 1), "one buffer per partial sum");
     static_assert(NS * NQ % 2 == 0, "the fragments alternate between two sets of registers");
     static_assert(KW == 1 || WM * WN == 1, "partial sums are exchanged per wave tile");
-    static_assert(KW == 1 || BM * 4 <= KB, "a partial sum fits a buffer of weight rows");
+    static_assert(KW == 1 || BN * 4 <= KB, "a partial sum fits a buffer of rows");
 
     // Byte offset of 16-byte chunk c of row r in a [rows][KB] buffer. A
     // fragment read takes 32 consecutive rows at chunk c (lanes 0-31) and
@@ -270,7 +270,7 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
     spare = (w == 0 ? sb0 : w == 1 ? sb1 : w == 2 ? sb2 : w == 3 ? sb3 : sb4) + wave / NS * S::SPARE;
     if constexpr (S::KW > 1) {
         auto part = [&](int w) -> int * {
-            return reinterpret_cast<int *>(w == 1 ? sb0 : w == 2 ? sb1 : sb2);
+            return reinterpret_cast<int *>(w == 1 ? sa0 : w == 2 ? sa1 : sa2);
         };
         if (kw > 0) {
             int *p = part(kw);

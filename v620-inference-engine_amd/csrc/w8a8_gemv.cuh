@@ -115,15 +115,17 @@ __device__ __forceinline__ int gemv_row() { return int(threadIdx.x) % WAVE / 8; 
 template <int G>
 struct W8Stream {
     i32x4 v[GEMV_U][G];
-    // steps s0, s0 + 4, .. of the rows; past a row's end any of its bytes (the
-    // tokens' are zeros there)
+    // steps s0, s0 + 4, .. of the rows (those there are); past a row's end any
+    // of its bytes (the tokens' are zeros there)
     __device__ __forceinline__ void load(const int8_t *const (&w)[G], int K, int s0) {
 #pragma unroll
-        for (int u = 0; u < GEMV_U; ++u)
+        for (int u = 0; u < GEMV_U; ++u) {
+            if ((s0 + 4 * u) * 128 >= K) break;
 #pragma unroll
             for (int g = 0; g < G; ++g)
                 v[u][g] = __builtin_nontemporal_load(reinterpret_cast<const i32x4 *>(
                     w[g] + 16 * int64_t(min((s0 + 4 * u) * 8 + int(threadIdx.x) % 8, K / 16 - 1))));
+        }
     }
 };
 

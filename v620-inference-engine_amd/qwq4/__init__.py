@@ -494,35 +494,35 @@ def moe_combine(yp, route, H, shared=None, out=None, out_bf16=True, out_dtype=No
 
 # ------------------------------------------------------------------- W8A8
 def _here(fn, *ts):
-    """Every tensor on the current GPU: the call goes to its current stream."""
+    """The raw handle of the current GPU's current stream (as _stream gives it); every tensor has to be on that GPU."""
     import torch
-    dev = None
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
+        if t is not None and not t.is_cuda:
             raise RuntimeError(f"{fn}: all tensors must be on the GPU")
-        if dev is None:
-            dev = torch.cuda.current_device()
-        if t.get_device() != dev:
+    dev = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != dev:
             raise RuntimeError(f"{fn}: a tensor is on GPU {t.get_device()}, the current one is {dev}")
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(dev) if raw is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
-def _matrix(fn, name, t, shape, dtype=None):
-    """The row stride of a [rows][cols] tensor whose rows are contiguous (a dimension of None is any size)."""
-    if t.dim() != 2 or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        raise ValueError(f"{fn}: {name} is {tuple(t.shape)}, not {shape}")
+def _matrix(fn, name, t, rows, cols, dtype=None):
+    """The row stride of a [rows][cols] tensor whose rows are contiguous (None: any number)."""
+    shape = t.shape
+    if len(shape) != 2 or (rows is not None and shape[0] != rows) or (cols is not None and shape[1] != cols):
+        raise ValueError(f"{fn}: {name} is {tuple(shape)}, not ({rows}, {cols})")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{fn}: {name} is {t.dtype}, not {dtype}")
-    rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    stride = t.stride()
+    if stride[1] != 1 and shape[1] > 1:
         raise ValueError(f"{fn}: the rows of {name} must be contiguous")
-    return t.stride(0) if rows > 1 else cols
+    return stride[0] if shape[0] > 1 else shape[1]
 
 
 def _whole(fn, name, t, shape, dtype):
     """A contiguous tensor of this shape and type."""
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{fn}: {name} is {tuple(t.shape)}, not {shape}")
     if t.dtype != dtype:
         raise TypeError(f"{fn}: {name} is {t.dtype}, not {dtype}")
@@ -535,17 +535,17 @@ def quant_tokens_i8(x, q=None, scale=None):
     q = rint(x (1 / scale)), scale = max |x| / 127."""
     import torch
     fn = "quant_tokens_i8"
-    ldx = _matrix(fn, "x", x, (None, None))
+    ldx = _matrix(fn, "x", x, None, None)
     T, K = x.shape
     if q is None:
         q = torch.empty((T, K), dtype=torch.int8, device=x.device)
     if scale is None:
         scale = torch.empty(T, dtype=torch.float32, device=x.device)
-    ldq = _matrix(fn, "q", q, (T, K), torch.int8)
+    ldq = _matrix(fn, "q", q, T, K, torch.int8)
     _whole(fn, "scale", scale, (T,), torch.float32)
     code = _tcode(x)
-    _here(fn, x, q, scale)
-    _check(lib().qw_quant_tokens_i8(_ptr(x), code, ldx, T, K, _ptr(q), ldq, _ptr(scale), _stream()),
+    stream = _here(fn, x, q, scale)
+    _check(lib().qw_quant_tokens_i8(_ptr(x), code, ldx, T, K, _ptr(q), ldq, _ptr(scale), stream),
            "qw_quant_tokens_i8")
     return q, scale
 
@@ -557,7 +557,7 @@ def _w8_out(fn, Y, y_dtype, T, N, default, device):
         Y = torch.empty((T, N), dtype=y_dtype if y_dtype is not None else default, device=device)
     elif y_dtype is not None and Y.dtype != y_dtype:
         raise TypeError(f"{fn}: the output is {Y.dtype}, not {y_dtype}")
-    return Y, _matrix(fn, "the output", Y, (T, N)), _tcode(Y)
+    return Y, _matrix(fn, "the output", Y, T, N), _tcode(Y)
 
 
 def gemm_w8a8(W, sw, q, sx, Y=None, y_dtype=None):
@@ -565,13 +565,13 @@ def gemm_w8a8(W, sw, q, sx, Y=None, y_dtype=None):
     checkpoint holds them, (q, sx) from quant_tokens_i8; any T. Y bfloat16, or y_dtype / the dtype of a given Y."""
     import torch
     fn = "gemm_w8a8"
-    ldq, ldw = _matrix(fn, "q", q, (None, None), torch.int8), _matrix(fn, "W", W, (None, q.shape[-1]), torch.int8)
+    ldq, ldw = _matrix(fn, "q", q, None, None, torch.int8), _matrix(fn, "W", W, None, q.shape[-1], torch.int8)
     (T, K), N = q.shape, W.shape[0]
     _whole(fn, "sw", sw, (N,), torch.float32)
     _whole(fn, "sx", sx, (T,), torch.float32)
     Y, ldy, code = _w8_out(fn, Y, y_dtype, T, N, torch.bfloat16, q.device)
-    _here(fn, W, sw, q, sx, Y)
-    _check(lib().qw_w8a8_gemm(_ptr(W), ldw, _ptr(sw), _ptr(q), ldq, _ptr(sx), T, _ptr(Y), ldy, code, N, K, _stream()),
+    stream = _here(fn, W, sw, q, sx, Y)
+    _check(lib().qw_w8a8_gemm(_ptr(W), ldw, _ptr(sw), _ptr(q), ldq, _ptr(sx), T, _ptr(Y), ldy, code, N, K, stream),
            "qw_w8a8_gemm")
     return Y
 
@@ -585,16 +585,16 @@ def linear_w8a8(W, sw, x, Y=None, y_dtype=None, workspace=None):
     x's type, or y_dtype / the dtype of a given Y."""
     import torch
     fn = "linear_w8a8"
-    ldx, ldw = _matrix(fn, "x", x, (None, None)), _matrix(fn, "W", W, (None, x.shape[-1]), torch.int8)
+    ldx, ldw = _matrix(fn, "x", x, None, None), _matrix(fn, "W", W, None, x.shape[-1], torch.int8)
     (T, K), N = x.shape, W.shape[0]
     _whole(fn, "sw", sw, (N,), torch.float32)
     code = _tcode(x)
     Y, ldy, ycode = _w8_out(fn, Y, y_dtype, T, N, x.dtype, x.device)
     if workspace is None:
         workspace = torch.empty(w8a8_workspace_size(T, K), dtype=torch.uint8, device=x.device)
-    _here(fn, W, sw, x, Y, workspace)
+    stream = _here(fn, W, sw, x, Y, workspace)
     _check(lib().qw_w8a8_linear(_ptr(W), ldw, _ptr(sw), _ptr(x), code, ldx, T, _ptr(Y), ldy, ycode, N, K,
-                                _ptr(workspace), workspace.numel() * workspace.element_size(), _stream()),
+                                _ptr(workspace), workspace.numel() * workspace.element_size(), stream),
            "qw_w8a8_linear")
     return Y
 
@@ -635,11 +635,11 @@ def moe_experts_w8a8(gate, up, down, route, x, h=None, yp=None, yp_dtype=None, w
     ycode = _tcode(yp)
     if workspace is None:
         workspace = torch.empty(moe_w8a8_workspace_size(T, topk, H, F), dtype=torch.uint8, device=x.device)
-    _here(fn, x, h, yp, workspace, route.offsets, *gate, *up, *down)
+    stream = _here(fn, x, h, yp, workspace, route.offsets, *gate, *up, *down)
     rc = lib().qw_moe_experts_w8a8(*[_ptr(t) for t in (*gate, *up, *down)], E, H, F, _ptr(route.offsets),
                                    _ptr(route.pair_tok), _ptr(route.tile_e), _ptr(route.tile_m0), _ptr(route.n_tiles),
                                    _ptr(x), code, T, topk, _ptr(h), _ptr(yp), ycode, _ptr(workspace),
-                                   workspace.numel() * workspace.element_size(), _stream())
+                                   workspace.numel() * workspace.element_size(), stream)
     _check(rc, "qw_moe_experts_w8a8")
     return h, yp
 
@@ -671,10 +671,10 @@ def moe_sort(top_e, E, tile_m=0, out=None):
             raise ValueError(f"{fn}: out was made for T, E, k, tile_m = {r.T, r.E, r.topk, r.tile_m}")
         r.top_w = None
     r.top_e = top_e
-    _here(fn, top_e, r.pair_tok)
+    stream = _here(fn, top_e, r.pair_tok)
     rc = lib().qw_moe_sort(_ptr(top_e), T, E, k, tile_m, _ptr(r.counts), _ptr(r.offsets), _ptr(r.tok_slot),
                            _ptr(r.pair_tok), _ptr(r.active), _ptr(r.n_active), _ptr(r.tile_e), _ptr(r.tile_m0),
-                           _ptr(r.n_tiles), _stream())
+                           _ptr(r.n_tiles), stream)
     _check(rc, "qw_moe_sort")
     return r
 
@@ -683,7 +683,7 @@ def _slots(fn, tok_slot):
     import torch
     if tok_slot.dim() != 2:
         raise ValueError(f"{fn}: tok_slot is {tuple(tok_slot.shape)}, not [T][k]")
-    _whole(fn, "tok_slot", tok_slot, tuple(tok_slot.shape), torch.int32)
+    _whole(fn, "tok_slot", tok_slot, tok_slot.shape, torch.int32)
     return tok_slot.shape
 
 
@@ -693,13 +693,13 @@ def moe_permute(x, tok_slot, xs=None):
     import torch
     fn = "moe_permute"
     T, k = _slots(fn, tok_slot)
-    ldx = _matrix(fn, "x", x, (T, None))
+    ldx = _matrix(fn, "x", x, T, None)
     H = x.shape[1]
     if xs is None:
         xs = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
-    ldxs = _matrix(fn, "xs", xs, (T * k, H), x.dtype)
-    _here(fn, x, tok_slot, xs)
-    _check(lib().qw_moe_permute(_ptr(x), ldx, x.element_size(), T, k, H, _ptr(tok_slot), _ptr(xs), ldxs, _stream()),
+    ldxs = _matrix(fn, "xs", xs, T * k, H, x.dtype)
+    stream = _here(fn, x, tok_slot, xs)
+    _check(lib().qw_moe_permute(_ptr(x), ldx, x.element_size(), T, k, H, _ptr(tok_slot), _ptr(xs), ldxs, stream),
            "qw_moe_permute")
     return xs
 
@@ -711,15 +711,15 @@ def moe_unpermute(yp, tok_slot, tok_w=None, out=None, out_dtype=None):
     import torch
     fn = "moe_unpermute"
     T, k = _slots(fn, tok_slot)
-    ldyp = _matrix(fn, "yp", yp, (T * k, None))
+    ldyp = _matrix(fn, "yp", yp, T * k, None)
     H = yp.shape[1]
     if tok_w is not None:
         _whole(fn, "tok_w", tok_w, (T, k), torch.float32)
     code = _tcode(yp)
     out, ldo, ocode = _w8_out(fn, out, out_dtype, T, H, yp.dtype, yp.device)
-    _here(fn, yp, tok_slot, tok_w, out)
+    stream = _here(fn, yp, tok_slot, tok_w, out)
     _check(lib().qw_moe_unpermute(_ptr(yp), code, ldyp, _ptr(tok_slot), _ptr(tok_w), T, k, H, _ptr(out), ocode, ldo,
-                                  _stream()), "qw_moe_unpermute")
+                                  stream), "qw_moe_unpermute")
     return out
 
 
@@ -734,9 +734,9 @@ def moe_unpermute_backward(dout, yp, tok_slot, tok_w=None, dyp=None, dw=None, ne
     import torch
     fn = "moe_unpermute_backward"
     T, k = _slots(fn, tok_slot)
-    ldyp = _matrix(fn, "yp", yp, (T * k, None))
+    ldyp = _matrix(fn, "yp", yp, T * k, None)
     H = yp.shape[1]
-    ldd = _matrix(fn, "dout", dout, (T, H))
+    ldd = _matrix(fn, "dout", dout, T, H)
     dcode, code = _tcode(dout), _tcode(yp)
     if tok_w is not None:
         _whole(fn, "tok_w", tok_w, (T, k), torch.float32)
@@ -748,12 +748,12 @@ def moe_unpermute_backward(dout, yp, tok_slot, tok_w=None, dyp=None, dw=None, ne
         dw = None
     elif dw is None:
         dw = torch.empty((T, k), dtype=torch.float32, device=yp.device)
-    lddyp = _matrix(fn, "dyp", dyp, (T * k, H), yp.dtype) if dyp is not None else H
+    lddyp = _matrix(fn, "dyp", dyp, T * k, H, yp.dtype) if dyp is not None else H
     if dw is not None:
         _whole(fn, "dw", dw, (T, k), torch.float32)
-    _here(fn, dout, yp, tok_slot, tok_w, dyp, dw)
+    stream = _here(fn, dout, yp, tok_slot, tok_w, dyp, dw)
     _check(lib().qw_moe_unpermute_backward(_ptr(dout), dcode, ldd, _ptr(yp), code, ldyp, _ptr(tok_slot), _ptr(tok_w), T,
-                                           k, H, _ptr(dyp), lddyp, _ptr(dw), _stream()), "qw_moe_unpermute_backward")
+                                           k, H, _ptr(dyp), lddyp, _ptr(dw), stream), "qw_moe_unpermute_backward")
     return dyp, dw
 
 
