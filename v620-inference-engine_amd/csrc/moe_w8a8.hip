@@ -8,8 +8,8 @@
 //   yp[p] = W8A8 product of h[p], quantised per slot
 //
 // Work is the routing's tile list (an entry: an expert and 32 to 160 of its
-// slots) times blocks of weight rows. Above 8 tokens a block runs its entry in
-// tiles of 128 or 64 slots on the int8 MFMA (w8a8_core.cuh); up to 8 it streams
+// slots) times blocks of weight rows. Above 16 tokens a block runs its entry in
+// tiles of 128 or 64 slots on the int8 MFMA (w8a8_core.cuh); up to 16 it streams
 // the weights past the slots' rows in LDS (w8a8_gemv.cuh). The sums being
 // whole numbers, both give a slot the same bits.
 #include <algorithm>
@@ -47,7 +47,10 @@ __device__ __forceinline__ int mw8_place(int b, int nt, int &col) {
     return b / 8 / nt * 8 + b % 8;
 }
 
-// The tile heights of a launch, and what its buffers are made for.
+// The tile heights of a launch; the first is what its buffers are made for. An
+// entry of up to 160 slots takes its weights once or twice; heights of 192,
+// 128 and 64 (once, two buffers) took 1521 us where these take 1437 (4096
+// tokens, 256 experts of 1536), tiles of 128 x 128 in two buffers 1477.
 template <bool LARGE>
 struct MW8Tiles {
     using H1 = W8Shape<128, 256, 2, 4, 1, 128, 3>;
@@ -257,9 +260,13 @@ void launch_moe_w8a8(MoeW8A8Args a, const void *x, int x_type, int T, int topk, 
     // entries of the list at most (each has a slot)
     const unsigned tiles = unsigned(std::min(P, P / size_t(-MW8_TILE_M) + size_t(a.E)));
     auto blocks = [](int rows, int per) { return unsigned((rows + per - 1) / per); };
-    const bool stream = T <= 8 && gemv_lds(8, std::max(a.H, a.F)) <= W8_GEMV_LDS;
+    // Streamed or in tiles, 256 experts of 1536, 8 chosen (device us): 1 token
+    // 35.7 and 46.0, 8 tokens 166 and 199, 16 tokens 275 and 305, 32 tokens 455
+    // and 434.
+    const bool stream = T <= 16 && gemv_lds(8, std::max(a.H, a.F)) <= W8_GEMV_LDS;
     if (stream && T <= 2) {
-        // one or two tokens: the blocks quantise the rows they stage
+        // one or two tokens: the blocks quantise the rows they stage (two
+        // launches less: 35.7 us against 39.4 and 59.4 against 63.4)
         const unsigned gu = tiles * blocks(a.F, 8), dn = tiles * blocks(a.H, 16);
         w8_by_rows(x, x_type, a.H, T, [&](auto xt, auto vec) {
             moe_gate_up_gemv_kernel<decltype(xt)::value, decltype(vec)::value>
@@ -275,7 +282,10 @@ void launch_moe_w8a8(MoeW8A8Args a, const void *x, int x_type, int T, int topk, 
         moe_down_gemv_kernel<3, true><<<tiles * blocks(a.H, 16), 256, gemv_lds(8, a.F), s>>>(a);
     } else {
         launch_quant_tokens(x, x_type, a.H, T, a.H, qx, a.H, sx, s);
-        if (P > size_t(32) * size_t(a.E)) launch_moe_tiles<true>(a, tiles, P, qh, sh, s);
+        // tall tiles from 24 slots per expert (512 tokens of 8 choices over 256
+        // experts, 16 each: 912 us tall, 895 low; 1024: 998 and 1075; 2048: 1168
+        // and 1358)
+        if (P > size_t(24) * size_t(a.E)) launch_moe_tiles<true>(a, tiles, P, qh, sh, s);
         else launch_moe_tiles<false>(a, tiles, P, qh, sh, s);
     }
 }

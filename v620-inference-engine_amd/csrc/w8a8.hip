@@ -142,10 +142,17 @@ static void launch_shape(const W8GemmArgs &a, hipStream_t s) {
 }
 
 // ------------------------------------------------------------ few tokens
-// Up to 8 tokens the product is a stream of the weights (w8a8_gemv.cuh), 8 G
-// rows of them per block. For one or two tokens the block quantises their rows
-// itself, which saves the quantiser's launch (one token, 4096 -> 12288 from
-// bf16: 12.6 us against 15.2 in two launches).
+// Up to 4 tokens the product is a stream of the weights (w8a8_gemv.cuh), 8 G
+// rows of them per block, bound by memory (one token, 4096 -> 12288: 9.9 us,
+// 5.1 TB/s; a large copy reaches 5.2). Device times from bf16 rows of 4096:
+//                          1 token   2      4      8
+//   4096 rows, streamed    4.7 us    6.1    8.1    11.1
+//              tiles       10.7      10.6   11.1   11.1
+//   12288 rows, streamed   9.9       11.5   14.5   18.8
+//               tiles      14.3      14.5   14.3   14.8
+// For one or two tokens the block quantises their rows itself, which saves the
+// quantiser's launch (one token: 4.7 against 5.8 us and 9.9 against 11.5; two:
+// 6.1 against 6.6 and 11.5 against 12.2).
 template <int XT, bool VEC, int TM, int G>
 __global__ __launch_bounds__(256) void w8a8_gemv_kernel(W8GemmArgs a, const void *x, int64_t ldx) {
     extern __shared__ __align__(16) unsigned char s_q[];
@@ -168,10 +175,12 @@ __global__ __launch_bounds__(256) void w8a8_gemv_kernel(W8GemmArgs a, const void
     });
 }
 
-static bool gemv_takes(int T, int K) { return T <= 8 && gemv_lds(T, K) <= W8_GEMV_LDS; }
+static bool gemv_takes(int T, int K) { return T <= 4 && gemv_lds(T, K) <= W8_GEMV_LDS; }
 
 template <int XT, bool VEC>
 static void launch_gemv(const W8GemmArgs &a, const void *x, int64_t ldx, hipStream_t s) {
+    // (16 rows a block where that leaves blocks enough: 2 tokens and 12288 rows
+    // take 11.5 us against 13.8 with 8, 4096 rows 6.3 against 6.1)
     auto run = [&](auto tm) {
         constexpr int TM = decltype(tm)::value;
         const size_t lds = gemv_lds(TM, a.K);
@@ -181,14 +190,14 @@ static void launch_gemv(const W8GemmArgs &a, const void *x, int64_t ldx, hipStre
     };
     if (a.T <= 1) run(std::integral_constant<int, 1>{});
     else if (a.T <= 2) run(std::integral_constant<int, 2>{});
-    else if constexpr (XT == 3) {
-        if (a.T <= 4) run(std::integral_constant<int, 4>{});
-        else run(std::integral_constant<int, 8>{});
-    }
+    else if constexpr (XT == 3) run(std::integral_constant<int, 4>{});
 }
 
 // Few tokens stream the weights; else the largest tile that still makes about
-// a block for every CU.
+// a block for every CU. Measured (us; rows x weight rows x K, tiles of 256, 128,
+// 64, 32): 4096 x 12288 x 4096: 237, 270, 406, 685; 1024 x 4096 x 4096: 55, 34, 36,
+// 71; 600 x 4096 x 6144: 75, 46, 38, 61; 256 x 4096 x 4096: 55, 31, 12.9, 21.7;
+// 37 x 12288 x 4096: 52, 33, 14.5, 17.5; 37 x 4096 x 6144: 74, 45, 16.6, 15.2.
 void launch_w8a8_gemm(const W8GemmArgs &a, hipStream_t s) {
     auto tiles = [&](int b) { return int64_t((a.T + b - 1) / b) * ((a.N + b - 1) / b); };
     if (gemv_takes(a.T, a.K)) launch_gemv<3, true>(a, nullptr, 0, s);
