@@ -357,3 +357,71 @@ def test_layer_graph_and_streams(gpu):
         eager = layer(x.clone(), e.clone(), w.clone(), None, None)
         torch.cuda.synchronize()
         assert torch.equal(got, eager)
+
+
+# -------------------------------------------------- edges of the kernels' choice
+@pytest.mark.parametrize("T", [3, 8, 9, 15, 16, 17, 24])
+@pytest.mark.parametrize("E,k", [(3, 2), (40, 5)])
+def test_experts_few_tokens(gpu, T, E, k):
+    """Around the number of tokens up to which the weights are streamed, with few and many slots per expert."""
+    print(f"experts_w8a8 T={T} E={E} k={k}", flush=True)
+    _check_experts(gpu, T, E, k, 208, 336, "f16", "bf16", "spread", seed=71)
+
+
+@pytest.mark.parametrize("xt", ["bf16", "f32"])
+@pytest.mark.parametrize("T", [1, 8, 40])
+def test_experts_buffers_at_any_address(gpu, T, xt):
+    """Rows, h and yp that start at their element's alignment only."""
+    import torch
+    E, k, H, F = 6, 2, 144, 80
+    (g, u, d), _ = _experts(81, E, H, F, gpu)
+    x, _ = _rows(82, T, H, xt, gpu)
+    r = qwq4.moe_sort(to_dev(_choices(83, T, E, k, "spread"), gpu), E, tile_m=qwq4.moe_w8a8_tile_m())
+
+    def odd(shape, dtype):
+        return torch.empty(shape[0] * shape[1] + 1, dtype=dtype, device=gpu)[1:].view(shape)
+    x1 = odd((T, H), x.dtype)
+    x1.copy_(x)
+    h, yp = qwq4.moe_experts_w8a8(g, u, d, r, x, yp_dtype=torch.bfloat16)
+    h1, yp1 = qwq4.moe_experts_w8a8(g, u, d, r, x1, h=odd((T * k, F), torch.float16),
+                                    yp=odd((T * k, H), torch.bfloat16))
+    assert torch.equal(h, h1) and torch.equal(yp, yp1)
+
+
+@pytest.mark.parametrize("T,K", [(1, 65536), (2, 32768), (3, 16384), (4, 16384), (4, 16400), (1, 65552)])
+def test_gemv_longest_rows(gpu, T, K):
+    """The longest rows that are staged whole, and the next longer ones."""
+    Wd, swd, W, sw = _weights(91, 40, K, gpu)
+    x, v = _rows(92, T, K, "bf16", gpu)
+    _same(qwq4.linear_w8a8(Wd, swd, x), ref.bf16(ref.product(*ref.quant(v), W, sw)))
+
+
+@pytest.mark.parametrize("T", [1, 2, 8])
+def test_experts_longest_rows(gpu, T):
+    _check_experts(gpu, T, 2, 1, 8192, 48, "bf16", "f32", "spread", seed=95)
+    _check_experts(gpu, T, 2, 1, 8208, 48, "bf16", "f32", "spread", seed=96)
+    _check_experts(gpu, T, 2, 1, 48, 8192, "bf16", "f32", "spread", seed=97)
+
+
+def test_two_streams_at_once(gpu):
+    """Calls in flight on two streams, each with its own workspace."""
+    import torch
+    T, N, K, E, k, H, F = 300, 700, 1024, 8, 2, 256, 192
+    Wd, swd, _, _ = _weights(101, N, K, gpu)
+    x, _ = _rows(102, T, K, "bf16", gpu)
+    (g, u, d), _ = _experts(103, E, H, F, gpu)
+    xe, _ = _rows(104, T, H, "f16", gpu)
+    r = qwq4.moe_sort(to_dev(_choices(105, T, E, k, "spread"), gpu), E, tile_m=qwq4.moe_w8a8_tile_m())
+    want_y, (_, want_yp) = qwq4.linear_w8a8(Wd, swd, x), qwq4.moe_experts_w8a8(g, u, d, r, xe)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(4):
+        with torch.cuda.stream(a):
+            y = qwq4.linear_w8a8(Wd, swd, x)
+        with torch.cuda.stream(b):
+            yp = qwq4.moe_experts_w8a8(g, u, d, r, xe)[1]
+        got.append((y, yp))
+    torch.cuda.synchronize()
+    for y, yp in got:
+        assert torch.equal(y, want_y) and torch.equal(yp, want_yp)

@@ -154,3 +154,45 @@ def test_binding_refusals():
         qwq4.moe_unpermute_backward(x, torch.zeros(6, 32), slot, dyp=torch.zeros(6, 32).half())
     with pytest.raises(RuntimeError, match="on the GPU"):
         qwq4.moe_unpermute_backward(x, torch.zeros(6, 32), slot)
+
+
+def test_binding_wants_the_current_device(monkeypatch):
+    """A tensor of another GPU than the current one is refused: its call would go to the wrong device's stream."""
+    import types
+
+    import torch
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 70 + d, raising=False)
+    on = lambda d: types.SimpleNamespace(is_cuda=True, get_device=lambda: d)  # noqa: E731
+    assert qwq4._here("f", on(0), None, on(0)) == 70
+    with pytest.raises(RuntimeError, match="f: a tensor is on GPU 1"):
+        qwq4._here("f", on(0), on(1))
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        qwq4._here("f", types.SimpleNamespace(is_cuda=False))
+
+
+def test_experts_binding_refusals():
+    import torch
+    E, F, H, T, k = 4, 32, 48, 3, 2
+    w = lambda *s: torch.zeros(s, dtype=torch.int8)  # noqa: E731
+    gate, down = (w(E, F, H), torch.zeros(E, F)), (w(E, H, F), torch.zeros(E, H))
+    route = qwq4.Route(T, E, k, "cpu", tile_m=qwq4.moe_w8a8_tile_m())
+    x = torch.zeros(T, H)
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        qwq4.moe_experts_w8a8(gate, gate, down, route, x)
+    with pytest.raises(ValueError, match="tile list"):
+        qwq4.moe_experts_w8a8(gate, gate, down, qwq4.Route(T, E, k, "cpu"), x)
+    with pytest.raises(ValueError, match="down is"):
+        qwq4.moe_experts_w8a8(gate, gate, gate, route, x)
+    with pytest.raises(ValueError, match="up scales is"):
+        qwq4.moe_experts_w8a8(gate, (gate[0], torch.zeros(E, H)), down, route, x)
+    with pytest.raises(TypeError, match="gate is"):
+        qwq4.moe_experts_w8a8((gate[0].float(), gate[1]), gate, down, route, x)
+    with pytest.raises(ValueError, match="x is"):
+        qwq4.moe_experts_w8a8(gate, gate, down, route, torch.zeros(T + 1, H))
+    with pytest.raises(TypeError, match="h is"):
+        qwq4.moe_experts_w8a8(gate, gate, down, route, x, h=torch.zeros(T * k, F))
+    with pytest.raises(TypeError, match="yp is"):
+        qwq4.moe_experts_w8a8(gate, gate, down, route, x, yp=torch.zeros(T * k, H), yp_dtype=torch.float16)
+    with pytest.raises(ValueError, match="contiguous"):
+        qwq4.moe_experts_w8a8(gate, gate, down, route, torch.zeros(H, T).t())
