@@ -425,3 +425,12 @@ def test_two_streams_at_once(gpu):
     torch.cuda.synchronize()
     for y, yp in got:
         assert torch.equal(y, want_y) and torch.equal(yp, want_yp)
+
+
+@pytest.mark.parametrize("T", [4, 5, 9, 16, 17])
+@pytest.mark.parametrize("F", [2048, 2032])
+def test_large_experts_few_tokens(gpu, T, F):
+    """Large experts stream their weights for more tokens than small ones; both sides of the edge."""
+    print(f"experts_w8a8 T={T} F={F}", flush=True)
+    _check_experts(gpu, T, 3, 2, 2048, F, "bf16", "f16", "uneven", seed=111)
+    _check_experts(gpu, T, 3, 2, 2048, F, "f16", "f32", "one", seed=115)

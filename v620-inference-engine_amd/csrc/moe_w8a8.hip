@@ -129,11 +129,14 @@ __device__ __forceinline__ void down_tile(const MoeW8A8Args &a, const MW8Entry &
     });
 }
 
-// DOWN: the down projection, else gate/up.
+// DOWN: the down projection, else gate/up. Where experts have few slots their
+// weights are read once and streamed past the caches (250 tokens, 256 experts:
+// 755 -> 697 us, 7.0 TB/s); with several entries an expert the second finds them
+// there (4096 tokens: streamed 1729 us, else 1435).
 template <bool DOWN, bool LARGE>
 __global__ __launch_bounds__(MW8Tiles<LARGE>::H1::THREADS, 2) void moe_w8a8_kernel(MoeW8A8Args a) {
     using T = MW8Tiles<LARGE>;
-    using L = W8Lds<typename T::H1, DOWN ? 2 : 1>;
+    using L = W8Lds<typename T::H1, DOWN ? 2 : 1, !LARGE>;
     constexpr int COLS = DOWN ? T::H1::BN : T::H1::BN / 2;
     int col;
     MW8Entry t;
@@ -260,10 +263,15 @@ void launch_moe_w8a8(MoeW8A8Args a, const void *x, int x_type, int T, int topk, 
     // entries of the list at most (each has a slot)
     const unsigned tiles = unsigned(std::min(P, P / size_t(-MW8_TILE_M) + size_t(a.E)));
     auto blocks = [](int rows, int per) { return unsigned((rows + per - 1) / per); };
-    // Streamed or in tiles, 256 experts of 1536, 8 chosen (device us): 1 token
-    // 35.7 and 46.0, 8 tokens 166 and 199, 16 tokens 275 and 305, 32 tokens 455
-    // and 434.
-    const bool stream = T <= 16 && gemv_lds(8, std::max(a.H, a.F)) <= W8_GEMV_LDS;
+    // Streamed or in tiles (device us, 8 of 256 experts of 4096 x 1536): 1 token
+    // 35.7 and 46.0, 8 tokens 166 and 179, 16 tokens 276 and 277; 8 of 64: 6
+    // tokens 115 and 128, 8 tokens 140 and 150. Small experts leave a block of the
+    // streaming kernels little to read per row staged, and turn sooner: 6 of 64
+    // of 2048 x 1024, 4 tokens 37.6 and 41.5, 6 tokens 45.9 and 43.1, 16 tokens
+    // 80 and 59; 8 of 128 of 2048 x 768, 4 tokens 39.8 and 40.3, 8 tokens 57 and
+    // 50.
+    const bool stream = T <= (size_t(a.H) * size_t(a.F) >= (4u << 20) ? 16 : 4) &&
+                        gemv_lds(8, std::max(a.H, a.F)) <= W8_GEMV_LDS;
     if (stream && T <= 2) {
         // one or two tokens: the blocks quantise the rows they stage (two
         // launches less: 35.7 us against 39.4 and 59.4 against 63.4)
@@ -282,9 +290,9 @@ void launch_moe_w8a8(MoeW8A8Args a, const void *x, int x_type, int T, int topk, 
         moe_down_gemv_kernel<3, true><<<tiles * blocks(a.H, 16), 256, gemv_lds(8, a.F), s>>>(a);
     } else {
         launch_quant_tokens(x, x_type, a.H, T, a.H, qx, a.H, sx, s);
-        // tall tiles from 24 slots per expert (512 tokens of 8 choices over 256
-        // experts, 16 each: 912 us tall, 895 low; 1024: 998 and 1075; 2048: 1168
-        // and 1358)
+        // tall tiles from 24 slots per expert (8 of 256 experts: 512 tokens, 16
+        // each, 912 us tall and 855 low; 768: 1019 and 1014; 896: 945 and 1002;
+        // 1024: 972 and 1059; 1536: 1053 and 1256)
         if (P > size_t(24) * size_t(a.E)) launch_moe_tiles<true>(a, tiles, P, qh, sh, s);
         else launch_moe_tiles<false>(a, tiles, P, qh, sh, s);
     }

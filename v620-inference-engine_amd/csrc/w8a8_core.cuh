@@ -76,9 +76,11 @@ struct W8Shape {
 };
 
 // The stage buffers of shape S; a kernel that runs several shapes takes those
-// of its largest for all of them.
-template <class S, int USE>
+// of its largest for all of them. STREAM: the weights are read by no other
+// block, and go past the caches' replacement (non-temporal loads).
+template <class S, int USE, bool STREAM = false>
 struct W8Lds {
+    static constexpr int W_AUX = STREAM ? 2 : 0;
     template <int I>
     __device__ static __forceinline__ unsigned char *a() {
         __shared__ __align__(16) unsigned char s[I < S::NS ? S::BM * S::KB : 16];
@@ -149,7 +151,7 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
             __builtin_amdgcn_global_load_lds(k < K ? ap[n] + k : zeros, da + (n * S::NW + wave) * 1024, 16, 0, 0);
         else
             __builtin_amdgcn_global_load_lds(bp[n - S::AJ] + min(k, K - 16),
-                                             db + ((n - S::AJ) * S::NW + wave) * 1024, 16, 0, 0);
+                                             db + ((n - S::AJ) * S::NW + wave) * 1024, 16, 0, L::W_AUX);
     };
     auto issue = [&](int ks, unsigned char *da, unsigned char *db) {
 #pragma unroll
