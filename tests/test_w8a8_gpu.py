@@ -434,3 +434,22 @@ def test_large_experts_few_tokens(gpu, T, F):
     print(f"experts_w8a8 T={T} F={F}", flush=True)
     _check_experts(gpu, T, 3, 2, 2048, F, "bf16", "f16", "uneven", seed=111)
     _check_experts(gpu, T, 3, 2, 2048, F, "f16", "f32", "one", seed=115)
+
+
+@pytest.mark.parametrize("K", [16, 64, 128, 144, 256, 272, 384, 400])
+@pytest.mark.parametrize("T,N", [(20, 300), (60, 9000), (100, 20000), (300, 25000)])
+def test_fewer_stages_than_buffers(gpu, T, N, K):
+    """Rows of one to four stages: loads that nobody reads must have landed before their buffers are used again."""
+    print(f"gemm_w8a8 T={T} N={N} K={K}", flush=True)
+    Wd, swd, W, sw = _weights(121, N, K, gpu)
+    r = np.random.default_rng(122)
+    q, sx = r.integers(-127, 128, (T, K), dtype=np.int8), (r.random(T) + 0.5).astype(np.float32)
+    _same(qwq4.gemm_w8a8(Wd, swd, to_dev(q, gpu), to_dev(sx, gpu)), ref.bf16(ref.product(q, sx, W, sw)))
+
+
+@pytest.mark.parametrize("H,F", [(16, 16), (128, 128), (64, 256), (256, 112), (272, 400)])
+@pytest.mark.parametrize("T", [40, 700])
+def test_experts_of_few_stages(gpu, T, H, F):
+    """The same for the experts, whose blocks run several tiles in the same buffers."""
+    print(f"experts_w8a8 T={T} H={H} F={F}", flush=True)
+    _check_experts(gpu, T, 4, 2, H, F, "bf16", "bf16", "one", seed=131)

@@ -267,7 +267,9 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
             multiply(0);
         }
     }
-    __syncthreads();  // the last stage is read
+    // The last stage is read, and no load is in flight any more (a K of one
+    // stage has not waited for those that nobody reads): the buffers are free.
+    w8_stage_barrier<0>();
     const int w = wave % NS;
     spare = (w == 0 ? sb0 : w == 1 ? sb1 : w == 2 ? sb2 : w == 3 ? sb3 : sb4) + wave / NS * S::SPARE;
     if constexpr (S::KW > 1) {
