@@ -320,7 +320,8 @@ int qw_moe_combine(const void *yp, int yp_f16, const int32_t *tok_slot, const fl
 
 /* ---- W8A8: int8 rows with a scale per token times int8 weights with a scale
  * per output row (checkpoints quantised to 8 bits; the engine's own int8 copy
- * of its dense weights keeps 16-bit rows: qw_i8_gemv).
+ * of its dense weights keeps 16-bit rows: qw_i8_gemv). What a call writes must
+ * not overlap what it reads.
  *
  * The rows' quantiser (the recipe of quant_rows_kernel,
  * src/kernels/moe_w4a8.hip:17-36, over whole rows), in fp32:
@@ -377,7 +378,9 @@ int qw_moe_experts_w8a8(const int8_t *gw, const float *gs, const int8_t *uw, con
                         int x_type, int T, int topk, uint16_t *h, void *yp, int yp_type, void *workspace,
                         size_t workspace_bytes, void *stream);
 
-/* ---- Tokens sorted by expert and back, with the gradients.
+/* ---- Tokens sorted by expert and back, with the gradients. What a call writes
+ * must not overlap what it reads; 1 <= H <= 2^28, T <= 2^23.
+ *
  * The slots of given choices top_e [T][k] (another router's, or qw_moe_route's
  * top_e with some of them removed; qw_moe_route gives its own choices' slots):
  * experts ascending, within one the choices in order (t, i). A choice outside
@@ -385,7 +388,9 @@ int qw_moe_experts_w8a8(const int8_t *gw, const float *gs, const int8_t *uw, con
  * the calls below skip it; a token may name an expert twice. Outputs and tile
  * list as qw_moe_route's, with offsets[E] the number of slots; pair_tok of the
  * T*k - offsets[E] places behind them is -1. Limits: 1 <= E <= 1024,
- * 1 <= k <= 64, T * k < 2^30. */
+ * 1 <= k <= 64, T * k < 2^30. For qw_moe_experts_w8a8, qw_moe_combine and the
+ * calls below. (qw_moe_experts_gemv relies on a router's distinct choices: an
+ * expert named twice by a token can have more slots there than it computes.) */
 int qw_moe_sort(const int32_t *top_e, int T, int E, int topk, int tile_m, int32_t *counts, int32_t *offsets,
                 int32_t *tok_slot, int32_t *pair_tok, int32_t *active, int32_t *n_active, int32_t *tile_e,
                 int32_t *tile_m0, int32_t *n_tiles, void *stream);
@@ -394,8 +399,8 @@ int qw_moe_sort(const int32_t *top_e, int T, int E, int topk, int tile_m, int32_
  * choice with a slot (0 <= slot < T*k; others are skipped, and rows no choice
  * has are left as they were). Elements of elem_bytes 1, 2 or 4 are moved as
  * they are (int8 rows, their fp32 scales with H = 1, 16- and 32-bit rows);
- * strides ldx, ldxs >= H in elements, any alignment of the element. xs must
- * not overlap x. T <= 2^23. Its gradient is qw_moe_unpermute without weights. */
+ * strides ldx, ldxs >= H in elements, any alignment of the element. Its
+ * gradient is qw_moe_unpermute without weights. */
 int qw_moe_permute(const void *x, int ldx, int elem_bytes, int T, int topk, int H, const int32_t *tok_slot, void *xs,
                    int ldxs, void *stream);
 

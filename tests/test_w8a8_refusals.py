@@ -196,3 +196,38 @@ def test_experts_binding_refusals():
         qwq4.moe_experts_w8a8(gate, gate, down, route, x, yp=torch.zeros(T * k, H), yp_dtype=torch.float16)
     with pytest.raises(ValueError, match="contiguous"):
         qwq4.moe_experts_w8a8(gate, gate, down, route, torch.zeros(H, T).t())
+
+
+WIDE = {"permute": permute(H=(1 << 28) + 1, ldx=1 << 29, ldxs=1 << 29),
+        "unpermute": unpermute(H=(1 << 28) + 1, ldyp=1 << 29, ldo=1 << 29),
+        "grad": grad(H=(1 << 28) + 1, ldd=1 << 29, ldyp=1 << 29, lddyp=1 << 29)}
+
+
+@pytest.mark.parametrize("name", sorted(WIDE))
+def test_rows_too_wide(lib, name):
+    fn, args = WIDE[name]
+    assert getattr(lib, fn)(*args) == -1
+    assert "2^28" in lib.qw_q4_last_error().decode()
+
+
+def test_binding_refuses_what_passes_32_bits():
+    """Sizes and strides that a 32-bit argument would cut, and workspaces with holes."""
+    import torch
+    big = 2**32 + 32
+    wide = torch.empty_strided((3, 32), (big, 1), dtype=torch.float32, device="meta")
+    slot = torch.zeros(3, 2, dtype=torch.int32)
+    W, sw, x = torch.zeros(8, 32, dtype=torch.int8), torch.zeros(8), torch.zeros(3, 32)
+    for call in (lambda: qwq4.quant_tokens_i8(wide), lambda: qwq4.linear_w8a8(W, sw, wide),
+                 lambda: qwq4.moe_permute(wide, slot), lambda: qwq4.moe_unpermute_backward(wide, x.repeat(2, 1), slot),
+                 lambda: qwq4.quant_tokens_i8(torch.empty((big, 16), device="meta")),
+                 lambda: qwq4.quant_tokens_i8(torch.empty((1, big), device="meta"))):
+        with pytest.raises(ValueError, match="2\\^31"):
+            call()
+    with pytest.raises(ValueError, match="2\\^30"):
+        qwq4.moe_permute(torch.empty((big, 1), device="meta"), torch.empty((big, 1), dtype=torch.int32, device="meta"))
+    for e, E in ((torch.empty((2**30, 1), dtype=torch.int32, device="meta"), 4), (slot, 1025), (slot, 0)):
+        with pytest.raises(ValueError, match="need T \\* k below"):
+            qwq4.moe_sort(e, E)
+    with pytest.raises(ValueError, match="workspace must be contiguous"):
+        qwq4._space("f", torch.zeros(1, dtype=torch.uint8).expand(4096))
+    assert qwq4._space("f", torch.zeros(8, 2)) == 64

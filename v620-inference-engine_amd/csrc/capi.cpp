@@ -497,8 +497,10 @@ int qw_moe_sort(const int32_t *top_e, int T, int E, int topk, int tile_m, int32_
 }
 
 static int check_rows(const char *fn, int T, int topk, int H) {
-    REQUIRE(T >= 1 && T <= kMaxRows && topk >= 1 && topk <= 64 && int64_t(T) * topk < (1 << 30) && H >= 1,
-            "%s: T = %d (1..%d), topk = %d (1..64), H = %d (from 1), T * topk below 2^30", fn, T, kMaxRows, topk, H);
+    // (H: a thread's column, some turns of the block past the row's end, has to stay an int)
+    REQUIRE(T >= 1 && T <= kMaxRows && topk >= 1 && topk <= 64 && int64_t(T) * topk < (1 << 30) && H >= 1 &&
+                H <= (1 << 28),
+            "%s: T = %d (1..%d), topk = %d (1..64), H = %d (1..2^28), T * topk below 2^30", fn, T, kMaxRows, topk, H);
     return 0;
 }
 

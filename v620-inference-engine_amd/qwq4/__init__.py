@@ -507,8 +507,12 @@ def _here(fn, *ts):
     return raw(dev) if raw is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
+_INT_MAX = 2**31 - 1
+
+
 def _matrix(fn, name, t, rows, cols, dtype=None):
-    """The row stride of a [rows][cols] tensor whose rows are contiguous (None: any number)."""
+    """The row stride of a [rows][cols] tensor whose rows are contiguous (None: any number). Sizes and strides are
+    passed on as 32-bit numbers."""
     shape = t.shape
     if len(shape) != 2 or (rows is not None and shape[0] != rows) or (cols is not None and shape[1] != cols):
         raise ValueError(f"{fn}: {name} is {tuple(shape)}, not ({rows}, {cols})")
@@ -517,7 +521,20 @@ def _matrix(fn, name, t, rows, cols, dtype=None):
     stride = t.stride()
     if stride[1] != 1 and shape[1] > 1:
         raise ValueError(f"{fn}: the rows of {name} must be contiguous")
-    return stride[0] if shape[0] > 1 else shape[1]
+    if shape[0] > 1:
+        if shape[0] > _INT_MAX or stride[0] > _INT_MAX:
+            raise ValueError(f"{fn}: {name} has {shape[0]} rows of stride {stride[0]}, more than 2^31 - 1")
+        return stride[0]
+    if shape[1] > _INT_MAX:
+        raise ValueError(f"{fn}: {name} has rows of {shape[1]}, more than 2^31 - 1")
+    return shape[1]
+
+
+def _space(fn, workspace):
+    """The bytes of a workspace."""
+    if not workspace.is_contiguous():
+        raise ValueError(f"{fn}: workspace must be contiguous")
+    return workspace.numel() * workspace.element_size()
 
 
 def _whole(fn, name, t, shape, dtype):
@@ -594,8 +611,7 @@ def linear_w8a8(W, sw, x, Y=None, y_dtype=None, workspace=None):
         workspace = torch.empty(w8a8_workspace_size(T, K), dtype=torch.uint8, device=x.device)
     stream = _here(fn, W, sw, x, Y, workspace)
     _check(lib().qw_w8a8_linear(_ptr(W), ldw, _ptr(sw), _ptr(x), code, ldx, T, _ptr(Y), ldy, ycode, N, K,
-                                _ptr(workspace), workspace.numel() * workspace.element_size(), stream),
-           "qw_w8a8_linear")
+                                _ptr(workspace), _space(fn, workspace), stream), "qw_w8a8_linear")
     return Y
 
 
@@ -639,7 +655,7 @@ def moe_experts_w8a8(gate, up, down, route, x, h=None, yp=None, yp_dtype=None, w
     rc = lib().qw_moe_experts_w8a8(*[_ptr(t) for t in (*gate, *up, *down)], E, H, F, _ptr(route.offsets),
                                    _ptr(route.pair_tok), _ptr(route.tile_e), _ptr(route.tile_m0), _ptr(route.n_tiles),
                                    _ptr(x), code, T, topk, _ptr(h), _ptr(yp), ycode, _ptr(workspace),
-                                   workspace.numel() * workspace.element_size(), stream)
+                                   _space(fn, workspace), stream)
     _check(rc, "qw_moe_experts_w8a8")
     return h, yp
 
@@ -653,6 +669,9 @@ def moe_sort(top_e, E, tile_m=0, out=None):
     if top_e.dim() != 2:
         raise ValueError(f"{fn}: top_e is {tuple(top_e.shape)}, not [T][k]")
     T, k = top_e.shape
+    if T * k >= 1 << 30 or not 1 <= E <= 1024 or abs(tile_m) >= 4096:
+        raise ValueError(f"{fn}: T = {T}, k = {k}, E = {E}, tile_m = {tile_m} (need T * k below 2^30, E 1..1024, "
+                         "|tile_m| below 4096)")
     _whole(fn, "top_e", top_e, (T, k), torch.int32)
     if out is None:
         r = Route.__new__(Route)
@@ -684,6 +703,8 @@ def _slots(fn, tok_slot):
     if tok_slot.dim() != 2:
         raise ValueError(f"{fn}: tok_slot is {tuple(tok_slot.shape)}, not [T][k]")
     _whole(fn, "tok_slot", tok_slot, tok_slot.shape, torch.int32)
+    if tok_slot.numel() >= 1 << 30:
+        raise ValueError(f"{fn}: tok_slot is {tuple(tok_slot.shape)}, need fewer than 2^30 choices")
     return tok_slot.shape
 
 
