@@ -201,10 +201,10 @@ static void launch_gemv(const W8GemmArgs &a, const void *x, int64_t ldx, hipStre
 void launch_w8a8_gemm(const W8GemmArgs &a, hipStream_t s) {
     auto tiles = [&](int b) { return int64_t((a.T + b - 1) / b) * ((a.N + b - 1) / b); };
     if (gemv_takes(a.T, a.K)) launch_gemv<3, true>(a, nullptr, 0, s);
-    else if (a.T > 128 && tiles(256) >= 192) launch_shape<W8Shape<256, 256, 2, 4, 1, 128, 2>>(a, s);
-    else if (a.T > 64 && tiles(128) >= 128) launch_shape<W8Shape<128, 128, 2, 2, 1, 128, 2>>(a, s);
-    else if (a.T > 32 && tiles(64) >= 128) launch_shape<W8Shape<64, 64, 2, 2, 1, 128, 4>>(a, s);
-    else launch_shape<W8Shape<32, 32, 1, 1, 4, 128, 4>>(a, s);
+    else if (a.T > 128 && tiles(256) >= 192) launch_shape<W8A8Shape<256, 256, 2, 4, 1, 2>>(a, s);
+    else if (a.T > 64 && tiles(128) >= 128) launch_shape<W8A8Shape<128, 128, 2, 2, 1, 2>>(a, s);
+    else if (a.T > 32 && tiles(64) >= 128) launch_shape<W8A8Shape<64, 64, 2, 2, 1, 4>>(a, s);
+    else launch_shape<W8A8Shape<32, 32, 1, 1, 4, 4>>(a, s);
 }
 
 static size_t up256(size_t b) { return (b + 255) & ~size_t(255); }

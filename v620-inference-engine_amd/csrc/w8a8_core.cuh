@@ -7,7 +7,7 @@
 // stages and waves, nor the batch changes a result: every shape of this loop
 // gives the same bits, and a variant is chosen by speed alone.
 //
-// Schedule. K runs in stages of KB (64 or 128) bytes through NS buffers of LDS, filled by
+// Schedule. K runs in stages of 128 bytes through NS buffers of LDS, filled by
 // direct global -> LDS loads (a wave instruction moves 8 rows of 128 bytes,
 // whole cache lines, from any row addresses: gathered rows cost the same as
 // neighbours) NS - 1 stages ahead. One barrier per stage: a wave waits for its
@@ -35,18 +35,17 @@ __device__ __forceinline__ i32x16 w8_mfma(const uint4 &a, const uint4 &b, const 
                                                  0);
 }
 
-template <int BM_, int BN_, int WM_, int WN_, int KW_, int KB_, int NS_>
-struct W8Shape {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KW = KW_, KB = KB_, NS = NS_;
+template <int BM_, int BN_, int WM_, int WN_, int KW_, int NS_>
+struct W8A8Shape {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KW = KW_, KB = 128, NS = NS_;
     static constexpr int NW = WM * WN * KW, THREADS = NW * WAVE;
     static constexpr int MT = BM / 32 / WM, NT = BN / 32 / WN;  // 32 x 32 tiles per wave
     static constexpr int CH = KB / 16, RPL = 1024 / KB;         // chunks per row, rows per load instruction
     static constexpr int AJ = BM / RPL / NW, BJ = BN / RPL / NW;  // load instructions per wave and stage
     static constexpr int NQ = KB / 32 / KW;                     // slabs per wave and stage
-    static_assert(KB == 64 || KB == 128, "a stage's row is half a cache line or one");
     static_assert(BM % (RPL * NW) == 0 && BN % (RPL * NW) == 0 && BM % (32 * WM) == 0 && BN % (32 * WN) == 0, "tile");
     static_assert(NQ >= 1 && NQ * 32 * KW == KB, "whole slabs per wave");
-    static_assert(NS >= 2 && NS <= 5 && (KW == 1 || KW <= NS + 1), "one buffer per partial sum");
+    static_assert(NS >= 2 && NS <= 4 && (KW == 1 || KW <= NS + 1), "one buffer per partial sum");
     static_assert(NS * NQ % 2 == 0, "the fragments alternate between two sets of registers");
     static_assert(KW == 1 || WM * WN == 1, "partial sums are exchanged per wave tile");
     static_assert(KW == 1 || BN * 4 <= KB, "a partial sum fits a buffer of rows");
@@ -55,7 +54,7 @@ struct W8Shape {
     // fragment read takes 32 consecutive rows at chunk c (lanes 0-31) and
     // c + 1 (lanes 32-63); under this XOR each 16 lanes of it fall on the 64
     // banks once.
-    __device__ static __forceinline__ int swz_x(int r) { return KB == 128 ? (r & 7) ^ ((r >> 3) & 1) : (r >> 2) & 3; }
+    __device__ static __forceinline__ int swz_x(int r) { return (r & 7) ^ ((r >> 3) & 1); }
     __device__ static __forceinline__ int swz(int r, int c) { return r * KB + ((c ^ swz_x(r)) << 4); }
     // The tile row that part j of this lane's loads belongs to: A rows for
     // j < AJ, weight rows likewise for j < BJ.
@@ -119,24 +118,22 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
     // (distinct arrays picked at compile time: the compiler then sees that the
     // loads in flight into one do not touch the buffer being read)
     unsigned char *const sa0 = L::template a<0>(), *const sa1 = L::template a<1>(), *const sa2 = L::template a<2>(),
-                  *const sa3 = L::template a<3>(), *const sa4 = L::template a<4>();
+                  *const sa3 = L::template a<3>();
     unsigned char *const sb0 = L::template b<0>(), *const sb1 = L::template b<1>(), *const sb2 = L::template b<2>(),
-                  *const sb3 = L::template b<3>(), *const sb4 = L::template b<4>();
+                  *const sb3 = L::template b<3>();
     const int wave = S::wave(), lane = int(threadIdx.x) % WAVE, l32 = lane % 32, lh = lane / 32;
     const int nk = (K + S::KB - 1) / S::KB;
     auto buf_a = [&](auto i) -> unsigned char * {
         if constexpr (decltype(i)::value == 0) return sa0;
         else if constexpr (decltype(i)::value == 1) return sa1;
         else if constexpr (decltype(i)::value == 2) return sa2;
-        else if constexpr (decltype(i)::value == 3) return sa3;
-        else return sa4;
+        else return sa3;
     };
     auto buf_b = [&](auto i) -> unsigned char * {
         if constexpr (decltype(i)::value == 0) return sb0;
         else if constexpr (decltype(i)::value == 1) return sb1;
         else if constexpr (decltype(i)::value == 2) return sb2;
-        else if constexpr (decltype(i)::value == 3) return sb3;
-        else return sb4;
+        else return sb3;
     };
     // Load n of a stage's LPW. Past the end of the rows (the last stage of a K
     // that is no multiple of KB) Q's chunks are zeros and W's any of the row's:
@@ -220,13 +217,11 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
     using I1 = std::integral_constant<int, 1>;
     using I2 = std::integral_constant<int, 2>;
     using I3 = std::integral_constant<int, 3>;
-    using I4 = std::integral_constant<int, 4>;
     // (a K of fewer stages loads its last one again, where nobody reads it)
     issue(0, sa0, sb0);
     issue(min(1, nk - 1), sa1, sb1);
     if constexpr (NS > 2) issue(min(2, nk - 1), sa2, sb2);
     if constexpr (NS > 3) issue(min(3, nk - 1), sa3, sb3);
-    if constexpr (NS > 4) issue(min(4, nk - 1), sa4, sb4);
     w8_stage_barrier<(NS - 1) * LPW>();
     read(0, sa0, sb0, 0);
     inner(0, sa0, sb0);
@@ -236,13 +231,12 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
         step(I1{}, ks + 1);
         if constexpr (NS > 2) step(I2{}, ks + 2);
         if constexpr (NS > 3) step(I3{}, ks + 3);
-        if constexpr (NS > 4) step(I4{}, ks + 4);
     }
     // The last stages (up to 2 NS - 1; ks is at buffer 0 again), in one piece
     // of code for every buffer.
     constexpr int TWO = NQ % 2 ? 2 : 1;  // (with one slab a stage the sets change places every stage)
-    auto pick_a = [&](int i) { return i == 0 ? sa0 : i == 1 ? sa1 : i == 2 ? sa2 : i == 3 ? sa3 : sa4; };
-    auto pick_b = [&](int i) { return i == 0 ? sb0 : i == 1 ? sb1 : i == 2 ? sb2 : i == 3 ? sb3 : sb4; };
+    auto pick_a = [&](int i) { return i == 0 ? sa0 : i == 1 ? sa1 : i == 2 ? sa2 : sa3; };
+    auto pick_b = [&](int i) { return i == 0 ? sb0 : i == 1 ? sb1 : i == 2 ? sb2 : sb3; };
     auto last = [&](int s, int p0) {
         const int cur = s % NS, next = (s + 1) % NS;
         if (s + NS <= nk) w8_stage_barrier<(NS - 2) * LPW>();
@@ -271,7 +265,7 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
     // stage has not waited for those that nobody reads): the buffers are free.
     w8_stage_barrier<0>();
     const int w = wave % NS;
-    spare = (w == 0 ? sb0 : w == 1 ? sb1 : w == 2 ? sb2 : w == 3 ? sb3 : sb4) + wave / NS * S::SPARE;
+    spare = (w == 0 ? sb0 : w == 1 ? sb1 : w == 2 ? sb2 : sb3) + wave / NS * S::SPARE;
     if constexpr (S::KW > 1) {
         auto part = [&](int w) -> int * {
             return reinterpret_cast<int *>(w == 1 ? sa0 : w == 2 ? sa1 : sa2);
