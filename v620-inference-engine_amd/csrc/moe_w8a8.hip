@@ -8,10 +8,10 @@
 //   yp[p] = W8A8 product of h[p], quantised per slot
 //
 // Work is the routing's tile list (an entry: an expert and 32 to 160 of its
-// slots) times blocks of weight rows. Above 16 tokens a block runs its entry in
-// tiles of 128 or 64 slots on the int8 MFMA (w8a8_core.cuh); up to 16 it streams
-// the weights past the slots' rows in LDS (w8a8_gemv.cuh). The sums being
-// whole numbers, both give a slot the same bits.
+// slots) times blocks of weight rows. A block runs its entry in tiles of 128 or
+// 64 slots on the int8 MFMA (w8a8_core.cuh); for few tokens (up to 16, or 4 with
+// small experts) it streams the weights past the slots' rows in LDS
+// (w8a8_gemv.cuh). The sums being whole numbers, both give a slot the same bits.
 #include <algorithm>
 #include <type_traits>
 
