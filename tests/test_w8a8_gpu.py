@@ -453,3 +453,16 @@ def test_experts_of_few_stages(gpu, T, H, F):
     """The same for the experts, whose blocks run several tiles in the same buffers."""
     print(f"experts_w8a8 T={T} H={H} F={F}", flush=True)
     _check_experts(gpu, T, 4, 2, H, F, "bf16", "bf16", "one", seed=131)
+
+
+@pytest.mark.parametrize("K", [496, 512, 528, 1040, 1168, 1552, 2064])
+@pytest.mark.parametrize("T,N", [(3, 8191), (3, 8193), (32, 10001), (33, 4096), (33, 4128), (64, 8192), (64, 8193), (45, 7003)])
+def test_split_tiles(gpu, T, N, K):
+    """Waves that split K, with even and uneven shares, one or two tiles side by side, and the next larger tiles."""
+    print(f"gemm_w8a8 T={T} N={N} K={K}", flush=True)
+    Wd, swd, W, sw = _weights(141, N, K, gpu)
+    r = np.random.default_rng(142)
+    q, sx = r.integers(-128, 128, (T, K), dtype=np.int8), (r.random(T) + 0.5).astype(np.float32)
+    want = ref.product(q, sx, W, sw)
+    for t in ("bf16", "f32"):
+        _same(qwq4.gemm_w8a8(Wd, swd, to_dev(q, gpu), to_dev(sx, gpu), y_dtype=_types()[t]), ref.ROUND[t](want))

@@ -53,12 +53,12 @@ __device__ __forceinline__ int mw8_place(int b, int nt, int &col) {
 // tokens, 256 experts of 1536), tiles of 128 x 128 in two buffers 1477.
 template <bool LARGE>
 struct MW8Tiles {
-    using H1 = W8A8Shape<128, 256, 2, 4, 1, 3>;
-    using H0 = W8A8Shape<64, 256, 2, 4, 1, 3>;
+    using H1 = W8A8Shape<128, 256, 2, 4, 3>;
+    using H0 = W8A8Shape<64, 256, 2, 4, 3>;
 };
 template <>
 struct MW8Tiles<false> {
-    using H1 = W8A8Shape<64, 128, 2, 2, 1, 2>;
+    using H1 = W8A8Shape<64, 128, 2, 2, 2>;
     using H0 = H1;
 };
 

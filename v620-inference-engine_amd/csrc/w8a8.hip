@@ -120,7 +120,7 @@ __global__ __launch_bounds__(S::THREADS) void w8a8_gemm_kernel(W8GemmArgs a) {
     i32x16 acc[S::MT][S::NT];
     w8_clear<S>(acc);
     unsigned char *spare;
-    if (!w8_tile<S, 0>(ap, bp, a.K, acc, spare)) return;
+    w8_tile<S, 0>(ap, bp, a.K, acc, spare);
     const int m_first = m0 + S::m_base(), n_first = n0 + S::n_base(), l32 = int(threadIdx.x) % 32;
     float sx[S::MT], sw[S::NT][16];
 #pragma unroll
@@ -141,16 +141,185 @@ static void launch_shape(const W8GemmArgs &a, hipStream_t s) {
     w8a8_gemm_kernel<S><<<tiles, S::THREADS, 0, s>>>(a);
 }
 
+// ------------------------------------------------------------ tens of tokens
+// Tiles of 32 tokens by 32 NT weight rows whose four waves split K. Such a tile
+// has little to multiply and is bound by the latency of its loads, so each wave
+// runs alone: it loads every fourth 128-byte stage of K into two buffers of its
+// own, waits for its own loads only, and no barrier joins the waves before
+// their sums meet. (With a barrier per stage and four buffers shared by the
+// waves: 37 x 4096 x 6144 15.2 us, here 8.3; 20 x 4096 x 4096 12.0 and 7.0. Three or
+// four buffers or eight waves a block: no better, and fewer blocks on a CU.)
+template <int NT_>
+struct W8Split {
+    static constexpr int NT = NT_, NS = 2, KW = 4, THREADS = KW * WAVE, BN = 32 * NT, LPW = 4 + 4 * NT;
+    // Stage buffer I: [waves][rows][128 bytes].
+    template <int I>
+    __device__ static __forceinline__ unsigned char *a() {
+        __shared__ __align__(16) unsigned char s[KW * 4096];
+        return s;
+    }
+    template <int I>
+    __device__ static __forceinline__ unsigned char *b() {
+        __shared__ __align__(16) unsigned char s[KW * NT * 4096];
+        return s;
+    }
+};
+
+// Until at most N of this wave's loads are in flight, and its LDS reads done.
+template <int N>
+__device__ __forceinline__ void w8_wave_wait() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (0 << 8));
+    asm volatile("" ::: "memory");
+}
+
+template <class S>
+__device__ __forceinline__ void w8_split_tile(const W8GemmArgs &a) {
+    constexpr int NT = S::NT, NS = S::NS, KW = S::KW, LPW = S::LPW;
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE), lane = int(threadIdx.x) % WAVE;
+    const int l32 = lane % 32, lh = lane / 32;
+    int mi, ni;
+    w8_place<8>(int(blockIdx.x), (a.T + 31) / 32, (a.N + S::BN - 1) / S::BN, mi, ni);
+    const int m0 = mi * 32, n0 = ni * S::BN;
+    // (this thread's part of the output: row l32, columns 32 j + col .. + 3)
+    const int col = 8 * wave + 4 * lh;
+    float sw[NT][4];
+    const float sx = a.sx[min(m0 + l32, a.T - 1)];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sw[j][e] = a.sw[min(n0 + 32 * j + col + e, a.N - 1)];
+    const int8_t *ap[4], *bp[4 * NT];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ap[j] = a.q + int64_t(min(m0 + 8 * j + lane / 8, a.T - 1)) * a.ldq;
+#pragma unroll
+    for (int j = 0; j < 4 * NT; ++j) bp[j] = a.W + int64_t(min(n0 + 8 * j + lane / 8, a.N - 1)) * a.ldw;
+    // (16-byte chunk c of row r lies at place c ^ (r & 7) ^ (r >> 3 & 1) of its 128 bytes: without bank conflicts)
+    const int c0 = (lane % 8) ^ (lane / 8), place = (l32 & 7) ^ ((l32 >> 3) & 1);
+    const int nk = (a.K + 127) / 128, n = (nk - wave + KW - 1) / KW;  // stages wave, wave + KW, .. of K
+    const int8_t *zeros = reinterpret_cast<const int8_t *>(&w8_zeros);
+    unsigned char *const sa0 = S::template a<0>() + wave * 4096, *const sa1 = S::template a<1>() + wave * 4096;
+    unsigned char *const sb0 = S::template b<0>() + wave * NT * 4096, *const sb1 = S::template b<1>() + wave * NT * 4096;
+    auto issue = [&](int i, unsigned char *da, unsigned char *db) {
+        const int k0 = min(wave + KW * i, nk - 1) * 128;  // (past the last: again, where nobody reads it)
+#pragma unroll
+        for (int j = 0; j < 4 + 4 * NT; ++j) {
+            const int k = k0 + (c0 ^ (j & 1)) * 16;
+            if (j < 4) __builtin_amdgcn_global_load_lds(k < a.K ? ap[j] + k : zeros, da + j * 1024, 16, 0, 0);
+            else __builtin_amdgcn_global_load_lds(bp[j - 4] + min(k, a.K - 16), db + (j - 4) * 1024, 16, 0, 0);
+        }
+    };
+    i32x16 acc[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j] = i32x16{};
+    // One stage, landed: its fragments are read, and with MORE the loads of
+    // stage `next` go into its buffers, in front of the products.
+    auto stage = [&](unsigned char *sa, unsigned char *sb, auto more, int next) {
+        uint4 af[4], bf[4][NT];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const int at = ((2 * s + lh) ^ place) << 4;
+            af[s] = *reinterpret_cast<const uint4 *>(sa + l32 * 128 + at);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) bf[s][j] = *reinterpret_cast<const uint4 *>(sb + (32 * j + l32) * 128 + at);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (decltype(more)::value) {
+            w8_wave_wait<63>();
+            issue(next, sa, sb);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) acc[j] = w8_mfma(bf[s][j], af[s], acc[j]);
+    };
+    issue(0, sa0, sb0);
+    issue(1, sa1, sb1);
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    int i = 0;
+    auto turn = [&](unsigned char *sa, unsigned char *sb, int at) {
+        w8_wave_wait<(NS - 1) * LPW>();
+        stage(sa, sb, yes, at + NS);
+    };
+    for (; i + NS < n; i += NS) {
+        turn(sa0, sb0, i);
+        turn(sa1, sb1, i + 1);
+    }
+    // the last one or two (of a K of few stages: none), both on their way
+    auto last = [&](unsigned char *sa, unsigned char *sb) { stage(sa, sb, no, 0); };
+    if (i < n) {
+        w8_wave_wait<(NS - 1) * LPW>();
+        last(sa0, sb0);
+    }
+    if (i + 1 < n) {
+        w8_wave_wait<0>();
+        last(sa1, sb1);
+    }
+    // the waves' sums through their buffers; each wave then has a quarter of the columns
+    w8_wave_wait<0>();
+    int *part = reinterpret_cast<int *>(sb0);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) part[(j * 16 + r) * WAVE + lane] = acc[j][r];
+    __syncthreads();
+    const int *parts = reinterpret_cast<const int *>(S::template b<0>());
+    const int m = m0 + l32;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            int sum = 0;
+#pragma unroll
+            for (int w = 0; w < KW; ++w) sum += parts[(w * NT * 16 + j * 16 + 4 * wave + e) * WAVE + lane];
+            v[e] = w8_value(sum, sw[j][e], sx);
+        }
+        const int at = n0 + 32 * j + col;
+        if (m >= a.T) continue;
+        const int64_t y = int64_t(m) * a.ldy + at;
+        if (a.y_type == 0) {
+            float *p = static_cast<float *>(a.Y) + y;
+            if (at + 4 <= a.N && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+                *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+                continue;
+            }
+        } else {
+            uint16_t *p = static_cast<uint16_t *>(a.Y) + y;
+            if (at + 4 <= a.N && reinterpret_cast<uintptr_t>(p) % 8 == 0) {
+                *reinterpret_cast<uint2 *>(p) =
+                    make_uint2(w8_bits16(a.y_type, v[0]) | uint32_t(w8_bits16(a.y_type, v[1])) << 16,
+                               w8_bits16(a.y_type, v[2]) | uint32_t(w8_bits16(a.y_type, v[3])) << 16);
+                continue;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (at + e < a.N) w8_store(a.Y, a.y_type, y + e, v[e]);
+    }
+}
+
+template <class S>
+__global__ __launch_bounds__(S::THREADS) void w8a8_split_kernel(W8GemmArgs a) {
+    w8_split_tile<S>(a);
+}
+
+template <int NT>
+static void launch_split(const W8GemmArgs &a, hipStream_t s) {
+    using S = W8Split<NT>;
+    const unsigned tiles = unsigned((a.T + 31) / 32) * unsigned((a.N + S::BN - 1) / S::BN);
+    w8a8_split_kernel<S><<<tiles, S::THREADS, 0, s>>>(a);
+}
+
 // ------------------------------------------------------------ few tokens
-// Up to 4 tokens the product is a stream of the weights (w8a8_gemv.cuh), 8 G
+// Up to 2 tokens the product is a stream of the weights (w8a8_gemv.cuh), 8 G
 // rows of them per block, bound by memory (one token, 4096 -> 12288: 9.9 us,
-// 5.1 TB/s; a large copy reaches 5.2). Device times from bf16 rows of 4096:
-//                          1 token   2      4      8
-//   4096 rows, streamed    4.7 us    6.1    8.1    11.1
-//              tiles       10.7      10.6   11.1   11.1
-//   12288 rows, streamed   9.9       11.5   14.5   18.8
-//               tiles      14.3      14.5   14.3   14.8
-// For one or two tokens the block quantises their rows itself, which saves the
+// 5.1 TB/s; a large copy reaches 5.2). Streamed and in tiles of 32, K 4096: 2
+// rows to 4096 5.4 and 6.4 us, to 12288 12.3 and 12.3; 4 rows 6.9 and 6.4, 14.5
+// and 12.3.
+// From 16- or 32-bit rows the block quantises them itself, which saves the
 // quantiser's launch (one token: 4.7 against 5.8 us and 9.9 against 11.5; two:
 // 6.1 against 6.6 and 11.5 against 12.2).
 template <int XT, bool VEC, int TM, int G>
@@ -175,7 +344,7 @@ __global__ __launch_bounds__(256) void w8a8_gemv_kernel(W8GemmArgs a, const void
     });
 }
 
-static bool gemv_takes(int T, int K) { return T <= 4 && gemv_lds(T, K) <= W8_GEMV_LDS; }
+static bool gemv_takes(int T, int K) { return T <= 2 && gemv_lds(T, K) <= W8_GEMV_LDS; }
 
 template <int XT, bool VEC>
 static void launch_gemv(const W8GemmArgs &a, const void *x, int64_t ldx, hipStream_t s) {
@@ -189,22 +358,26 @@ static void launch_gemv(const W8GemmArgs &a, const void *x, int64_t ldx, hipStre
         else w8a8_gemv_kernel<XT, VEC, TM, 1><<<unsigned((a.N + 7) / 8), 256, lds, s>>>(a, x, ldx);
     };
     if (a.T <= 1) run(std::integral_constant<int, 1>{});
-    else if (a.T <= 2) run(std::integral_constant<int, 2>{});
-    else if constexpr (XT == 3) run(std::integral_constant<int, 4>{});
+    else run(std::integral_constant<int, 2>{});
 }
 
-// Few tokens stream the weights; else the largest tile that still makes about
-// a block for every CU. Measured (us; rows x weight rows x K, tiles of 256, 128,
-// 64, 32): 4096 x 12288 x 4096: 237, 270, 406, 685; 1024 x 4096 x 4096: 55, 34, 36,
-// 71; 600 x 4096 x 6144: 75, 46, 38, 61; 256 x 4096 x 4096: 55, 31, 12.9, 21.7;
-// 37 x 12288 x 4096: 52, 33, 14.5, 17.5; 37 x 4096 x 6144: 74, 45, 16.6, 15.2.
+// One or two tokens stream the weights. Else the largest tile that makes about
+// a block for every CU (us; rows x weight rows x K, tiles of 256, 128, 64: 4096 x
+// 12288 x 4096: 237, 270, 406; 1024 x 4096 x 4096: 55, 34, 36; 256 x 4096 x 4096: 55,
+// 31, 12.9). Where those of 32 are no more than two rounds of the CUs, or there
+// are no more than 32 rows, those, two side by side between one round and two
+// (tiles of 64, of 32, of 32 x 64: 64 x 4096 x 4096, 256 of 32: 14.0, 7.4, 9.8; 32 x
+// 9216 x 4096, 288: 14.3, 12.9, 11.0; 128 x 4096 x 4096, 512: 13.9, 10.8, 9.7; 96 x
+// 6144 x 4096, 576: 13.1, 15.0, 17.6; 150 x 4096 x 4096, 640: 12.8, 13.6, 16.2; 16 x
+// 20480 x 4096, 640: 23.9, 19.1, 23.8; 8 x 100000 x 4096: 85, 72, 91).
 void launch_w8a8_gemm(const W8GemmArgs &a, hipStream_t s) {
     auto tiles = [&](int b) { return int64_t((a.T + b - 1) / b) * ((a.N + b - 1) / b); };
     if (gemv_takes(a.T, a.K)) launch_gemv<3, true>(a, nullptr, 0, s);
-    else if (a.T > 128 && tiles(256) >= 192) launch_shape<W8A8Shape<256, 256, 2, 4, 1, 2>>(a, s);
-    else if (a.T > 64 && tiles(128) >= 128) launch_shape<W8A8Shape<128, 128, 2, 2, 1, 2>>(a, s);
-    else if (a.T > 32 && tiles(64) >= 128) launch_shape<W8A8Shape<64, 64, 2, 2, 1, 4>>(a, s);
-    else launch_shape<W8A8Shape<32, 32, 1, 1, 4, 4>>(a, s);
+    else if (a.T > 128 && tiles(256) >= 192) launch_shape<W8A8Shape<256, 256, 2, 4, 2>>(a, s);
+    else if (a.T > 64 && tiles(128) >= 128) launch_shape<W8A8Shape<128, 128, 2, 2, 2>>(a, s);
+    else if (a.T > 32 && tiles(32) > 512) launch_shape<W8A8Shape<64, 64, 2, 2, 4>>(a, s);
+    else if (tiles(32) > 256 && tiles(32) <= 512) launch_split<2>(a, s);
+    else launch_split<1>(a, s);
 }
 
 static size_t up256(size_t b) { return (b + 255) & ~size_t(255); }

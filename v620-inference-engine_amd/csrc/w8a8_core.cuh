@@ -3,9 +3,8 @@
 // checkpoint holds them: row-major), summed exactly in int32 on
 // v_mfma_i32_32x32x32_i8.
 //
-// The sums are whole numbers, so neither the tile, nor how K is split over
-// stages and waves, nor the batch changes a result: every shape of this loop
-// gives the same bits, and a variant is chosen by speed alone.
+// The sums are whole numbers, so neither the tile, nor the order of K, nor the
+// batch changes a result: every shape of this loop gives the same bits, and a variant is chosen by speed alone.
 //
 // Schedule. K runs in stages of 128 bytes through NS buffers of LDS, filled by
 // direct global -> LDS loads (a wave instruction moves 8 rows of 128 bytes,
@@ -13,8 +12,7 @@
 // neighbours) NS - 1 stages ahead. One barrier per stage: a wave waits for its
 // own loads of the stage, and the barrier then makes everyone's visible and
 // tells that the buffer of the stage before is free for the next loads.
-// The waves are WM x WN over the tile and KW over the 32-wide slabs of a
-// stage; the KW partial sums meet in LDS at the end.
+// The waves are WM x WN over the tile.
 #pragma once
 
 #include <type_traits>
@@ -35,20 +33,16 @@ __device__ __forceinline__ i32x16 w8_mfma(const uint4 &a, const uint4 &b, const 
                                                  0);
 }
 
-template <int BM_, int BN_, int WM_, int WN_, int KW_, int NS_>
+template <int BM_, int BN_, int WM_, int WN_, int NS_>
 struct W8A8Shape {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KW = KW_, KB = 128, NS = NS_;
-    static constexpr int NW = WM * WN * KW, THREADS = NW * WAVE;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = 128, NS = NS_;
+    static constexpr int NW = WM * WN, THREADS = NW * WAVE;
     static constexpr int MT = BM / 32 / WM, NT = BN / 32 / WN;  // 32 x 32 tiles per wave
     static constexpr int CH = KB / 16, RPL = 1024 / KB;         // chunks per row, rows per load instruction
     static constexpr int AJ = BM / RPL / NW, BJ = BN / RPL / NW;  // load instructions per wave and stage
-    static constexpr int NQ = KB / 32 / KW;                     // slabs per wave and stage
+    static constexpr int NQ = KB / 32;                          // slabs per stage
     static_assert(BM % (RPL * NW) == 0 && BN % (RPL * NW) == 0 && BM % (32 * WM) == 0 && BN % (32 * WN) == 0, "tile");
-    static_assert(NQ >= 1 && NQ * 32 * KW == KB, "whole slabs per wave");
-    static_assert(NS >= 2 && NS <= 4 && (KW == 1 || KW <= NS + 1), "one buffer per partial sum");
-    static_assert(NS * NQ % 2 == 0, "the fragments alternate between two sets of registers");
-    static_assert(KW == 1 || WM * WN == 1, "partial sums are exchanged per wave tile");
-    static_assert(KW == 1 || BN * 4 <= KB, "a partial sum fits a buffer of rows");
+    static_assert(NS >= 2 && NS <= 4 && NQ % 2 == 0, "the fragments alternate between two sets of registers");
 
     // Byte offset of 16-byte chunk c of row r in a [rows][KB] buffer. A
     // fragment read takes 32 consecutive rows at chunk c (lanes 0-31) and
@@ -67,8 +61,8 @@ struct W8A8Shape {
     // of accumulator (i, j) is row m_base() + 32 i + lane % 32 of Q and row
     // n_base() + 32 j + n_of(r) of W.
     __device__ static __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE); }
-    __device__ static __forceinline__ int m_base() { return wave() / KW / WN * MT * 32; }
-    __device__ static __forceinline__ int n_base() { return wave() / KW % WN * NT * 32; }
+    __device__ static __forceinline__ int m_base() { return wave() / WN * MT * 32; }
+    __device__ static __forceinline__ int n_base() { return wave() % WN * NT * 32; }
     __device__ static __forceinline__ int n_of(int r) { return 8 * (r / 4) + 4 * (int(threadIdx.x) % WAVE / 32) + r % 4; }
     // LDS that a wave has to itself after the sums
     static constexpr int SPARE = BN * KB / ((NW + NS - 1) / NS);  // (of the weights' buffers)
@@ -105,14 +99,13 @@ __device__ __forceinline__ void w8_stage_barrier() {
 
 // acc += the tile's sums over K (a multiple of 16, >= 16). ap[j] / bp[j]: the
 // start of the int8 row load_row(j) of Q / W (any valid row where the tile
-// passes the matrix). With KW > 1 the sums end in the waves with wave % KW
-// == 0 (acc of the others is void); returns whether this wave holds sums.
+// passes the matrix).
 // spare: S::SPARE bytes of LDS for this wave until the block's next barrier,
 // which has to come before another tile. (USE tags the caller: each call site
 // instantiates its own specialization; the host compilation pass rejects a
 // second call site of a shared one.)
 template <class S, int USE, class L = W8Lds<S, USE>>
-__device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t *(&bp)[S::BJ], int K,
+__device__ __forceinline__ void w8_tile(const int8_t *(&ap)[S::AJ], const int8_t *(&bp)[S::BJ], int K,
                                         i32x16 (&acc)[S::MT][S::NT], unsigned char *&spare) {
     constexpr int NS = S::NS, LPW = S::AJ + S::BJ;
     // (distinct arrays picked at compile time: the compiler then sees that the
@@ -154,15 +147,15 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
 #pragma unroll
         for (int n = 0; n < LPW; ++n) issue_one(ks, n, da, db);
     };
-    const int wm = wave / S::KW / S::WN, wn = wave / S::KW % S::WN, kw = wave % S::KW;
-    // Fragments of slab n of a stage (of this wave's NQ), read while the slab
+    const int wm = wave / S::WN, wn = wave % S::WN;
+    // Fragments of slab n of a stage, read while the slab
     // before is multiplied. (The scheduling barrier keeps the reads in front:
     // left to itself the compiler moves them behind the products, and every
     // slab then waits for its own.)
     constexpr int NQ = S::NQ;
     uint4 af[2][S::MT], bf[2][S::NT];
     auto read = [&](int p, const unsigned char *a, const unsigned char *b, int n) {
-        const int c = 2 * (n * S::KW + kw) + lh;
+        const int c = 2 * n + lh;
 #pragma unroll
         for (int i = 0; i < S::MT; ++i)
             af[p][i] = *reinterpret_cast<const uint4 *>(a + S::swz((wm * S::MT + i) * 32 + l32, c));
@@ -190,13 +183,13 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // A stage up to its last slab, whose fragments are then held; the first
-    // slab's are in set p0.
-    auto inner = [&](int p0, const unsigned char *a, const unsigned char *b) {
+    // A stage up to its last slab, whose fragments are then held in set 1; the
+    // first slab's are in set 0.
+    auto inner = [&](const unsigned char *a, const unsigned char *b) {
 #pragma unroll
         for (int n = 0; n + 1 < NQ; ++n) {
-            read((p0 + n + 1) % 2, a, b, n + 1);
-            multiply((p0 + n) % 2);
+            read((n + 1) % 2, a, b, n + 1);
+            multiply(n % 2);
         }
     };
     // From stage ks in buffer I to the next. Before the last slab of ks is
@@ -209,9 +202,9 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
         constexpr int I = decltype(i)::value;
         constexpr std::integral_constant<int, (I + 1) % NS> next{};
         w8_stage_barrier<(NS - 2) * LPW>();
-        read((I * NQ + NQ) % 2, buf_a(next), buf_b(next), 0);
-        multiply_and_issue((I * NQ + NQ - 1) % 2, ks + NS, buf_a(i), buf_b(i));
-        inner((I * NQ + NQ) % 2, buf_a(next), buf_b(next));
+        read(0, buf_a(next), buf_b(next), 0);
+        multiply_and_issue(1, ks + NS, buf_a(i), buf_b(i));
+        inner(buf_a(next), buf_b(next));
     };
     using I0 = std::integral_constant<int, 0>;
     using I1 = std::integral_constant<int, 1>;
@@ -224,7 +217,7 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
     if constexpr (NS > 3) issue(min(3, nk - 1), sa3, sb3);
     w8_stage_barrier<(NS - 1) * LPW>();
     read(0, sa0, sb0, 0);
-    inner(0, sa0, sb0);
+    inner(sa0, sb0);
     int ks = 0;
     for (; ks + 2 * NS - 1 < nk; ks += NS) {
         step(I0{}, ks);
@@ -234,65 +227,24 @@ __device__ __forceinline__ bool w8_tile(const int8_t *(&ap)[S::AJ], const int8_t
     }
     // The last stages (up to 2 NS - 1; ks is at buffer 0 again), in one piece
     // of code for every buffer.
-    constexpr int TWO = NQ % 2 ? 2 : 1;  // (with one slab a stage the sets change places every stage)
     auto pick_a = [&](int i) { return i == 0 ? sa0 : i == 1 ? sa1 : i == 2 ? sa2 : sa3; };
     auto pick_b = [&](int i) { return i == 0 ? sb0 : i == 1 ? sb1 : i == 2 ? sb2 : sb3; };
-    auto last = [&](int s, int p0) {
+    auto last = [&](int s) {
         const int cur = s % NS, next = (s + 1) % NS;
         if (s + NS <= nk) w8_stage_barrier<(NS - 2) * LPW>();
         else w8_stage_barrier<0>();
-        read(p0, pick_a(next), pick_b(next), 0);
+        read(0, pick_a(next), pick_b(next), 0);
         if (s + NS < nk) issue(s + NS, pick_a(cur), pick_b(cur));
-        multiply(1 - p0);
-        inner(p0, pick_a(next), pick_b(next));
-    };
-    if constexpr (TWO == 1) {
-        for (; ks < nk - 1; ++ks) last(ks, 0);
         multiply(1);
-    } else {
-        for (; ks < nk - 2; ks += 2) {
-            last(ks, 1);
-            last(ks + 1, 0);
-        }
-        if (ks < nk - 1) {
-            last(ks, 1);
-            multiply(1);
-        } else {
-            multiply(0);
-        }
-    }
+        inner(pick_a(next), pick_b(next));
+    };
+    for (; ks < nk - 1; ++ks) last(ks);
+    multiply(1);
     // The last stage is read, and no load is in flight any more (a K of one
     // stage has not waited for those that nobody reads): the buffers are free.
     w8_stage_barrier<0>();
     const int w = wave % NS;
     spare = (w == 0 ? sb0 : w == 1 ? sb1 : w == 2 ? sb2 : sb3) + wave / NS * S::SPARE;
-    if constexpr (S::KW > 1) {
-        auto part = [&](int w) -> int * {
-            return reinterpret_cast<int *>(w == 1 ? sa0 : w == 2 ? sa1 : sa2);
-        };
-        if (kw > 0) {
-            int *p = part(kw);
-#pragma unroll
-            for (int i = 0; i < S::MT; ++i)
-#pragma unroll
-                for (int j = 0; j < S::NT; ++j)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) p[((i * S::NT + j) * 16 + r) * WAVE + lane] = acc[i][j][r];
-        }
-        __syncthreads();
-        if (kw > 0) return false;
-#pragma unroll
-        for (int w = 1; w < S::KW; ++w) {
-            const int *p = part(w);
-#pragma unroll
-            for (int i = 0; i < S::MT; ++i)
-#pragma unroll
-                for (int j = 0; j < S::NT; ++j)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[i][j][r] += p[((i * S::NT + j) * 16 + r) * WAVE + lane];
-        }
-    }
-    return true;
 }
 
 template <class S>
@@ -377,22 +329,10 @@ __device__ __forceinline__ void w8_store_rows(unsigned char *spare, void *Y, int
         }
 }
 
-// w8_store_rows for either width of the output's type; the tiles whose waves
-// split K have little to store and do it as they hold it.
+// w8_store_rows for either width of the output's type.
 template <class S, int NC, class ValueF, class RowF>
 __device__ __forceinline__ void w8_output(unsigned char *spare, void *Y, int type, int cols, ValueF value, RowF row) {
-    if constexpr (S::KW > 1) {
-#pragma unroll
-        for (int i = 0; i < S::MT; ++i) {
-            const int64_t at = row(32 * i + int(threadIdx.x) % 32);
-            if (at < 0) continue;
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (32 * c + S::n_of(r) < cols) w8_store(Y, type, at + 32 * c + S::n_of(r), value(i, c, r));
-        }
-    } else if (type == 0) {
+    if (type == 0) {
         w8_store_rows<S, NC, 4>(spare, Y, type, cols, value, row);
     } else {
         w8_store_rows<S, NC, 2>(spare, Y, type, cols, value, row);
