@@ -350,7 +350,8 @@ int qw_w8a8_gemm(const int8_t *W, int ldw, const float *sw, const int8_t *q, int
 /* qw_quant_tokens_i8 followed by qw_w8a8_gemm, bit for bit, from rows x of
  * x_type. workspace: qw_w8a8_workspace_size(T, K) bytes, 256-byte aligned,
  * scratch (it holds nothing between calls; calls that share it must not
- * overlap). */
+ * overlap); 0, and NULL then, for the one or two rows that the product itself
+ * quantises. */
 size_t qw_w8a8_workspace_size(int T, int K);
 int qw_w8a8_linear(const int8_t *W, int ldw, const float *sw, const void *x, int x_type, int ldx, int T, void *Y,
                    int ldy, int y_type, int N, int K, void *workspace, size_t workspace_bytes, void *stream);

@@ -466,3 +466,13 @@ def test_split_tiles(gpu, T, N, K):
     want = ref.product(q, sx, W, sw)
     for t in ("bf16", "f32"):
         _same(qwq4.gemm_w8a8(Wd, swd, to_dev(q, gpu), to_dev(sx, gpu), y_dtype=_types()[t]), ref.ROUND[t](want))
+
+
+@pytest.mark.parametrize("T", [1, 2])
+def test_few_rows_without_workspace(gpu, T):
+    import torch
+    Wd, swd, W, sw = _weights(151, 70, 528, gpu)
+    x, v = _rows(152, T, 528, "bf16", gpu)
+    want = ref.bf16(ref.product(*ref.quant(v), W, sw))
+    for ws in (None, torch.empty(0, dtype=torch.uint8, device=gpu), torch.empty(4096, dtype=torch.uint8, device=gpu)):
+        _same(qwq4.linear_w8a8(Wd, swd, x, workspace=ws), want)

@@ -231,3 +231,12 @@ def test_binding_refuses_what_passes_32_bits():
     with pytest.raises(ValueError, match="workspace must be contiguous"):
         qwq4._space("f", torch.zeros(1, dtype=torch.uint8).expand(4096))
     assert qwq4._space("f", torch.zeros(8, 2)) == 64
+
+
+def test_workspace_of_few_rows(lib):
+    """One and two rows need no workspace as long as they fit a block; longer ones and more rows do."""
+    assert lib.qw_w8a8_workspace_size(1, 4096) == 0 and lib.qw_w8a8_workspace_size(2, 32768) == 0
+    assert lib.qw_w8a8_workspace_size(2, 32784) >= 2 * 32784 + 8 and lib.qw_w8a8_workspace_size(3, 64) >= 3 * 64 + 12
+    for T, K in ((3, 64), (2, 32784)):
+        fn, args = linear(T=T, K=K, ldw=K, ldx=K, ws=None, wb=0)
+        assert getattr(lib, fn)(*args) == -1 and "workspace needs" in lib.qw_q4_last_error().decode()

@@ -437,7 +437,7 @@ int qw_w8a8_linear(const int8_t *W, int ldw, const float *sw, const void *x, int
     if (int r = check_w8_product(fn, W, ldw, sw, T, Y, ldy, y_type, N, K)) return r;
     if (int r = check_w8_rows(fn, x, x_type, ldx, T, K)) return r;
     const size_t need = qwq4::w8a8_workspace_bytes(T, K);
-    REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 256),
+    REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 256)),
             "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", fn, need, workspace_bytes);
     qwq4::launch_w8a8_linear(qwq4::W8GemmArgs{W, ldw, sw, nullptr, 0, nullptr, T, Y, ldy, y_type, N, K}, x, x_type, ldx,
                              workspace, st(stream));

@@ -382,10 +382,13 @@ void launch_w8a8_gemm(const W8GemmArgs &a, hipStream_t s) {
 
 static size_t up256(size_t b) { return (b + 255) & ~size_t(255); }
 
-size_t w8a8_workspace_bytes(int T, int K) { return up256(size_t(T) * size_t(K)) + up256(size_t(T) * 4); }
+// (none where the product's blocks quantise the rows)
+size_t w8a8_workspace_bytes(int T, int K) {
+    return gemv_takes(T, K) ? 0 : up256(size_t(T) * size_t(K)) + up256(size_t(T) * 4);
+}
 
 void launch_w8a8_linear(W8GemmArgs a, const void *x, int x_type, int64_t ldx, void *ws, hipStream_t s) {
-    if (a.T <= 2 && gemv_takes(a.T, a.K)) {
+    if (gemv_takes(a.T, a.K)) {
         w8_by_rows(x, x_type, ldx, a.T, [&](auto xt, auto vec) {
             launch_gemv<decltype(xt)::value, decltype(vec)::value>(a, x, ldx, s);
         });

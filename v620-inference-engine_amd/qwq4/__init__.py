@@ -496,12 +496,15 @@ def moe_combine(yp, route, H, shared=None, out=None, out_bf16=True, out_dtype=No
 def _here(fn, *ts):
     """The raw handle of the current GPU's current stream (as _stream gives it); every tensor has to be on that GPU."""
     import torch
+    dev = None
     for t in ts:
-        if t is not None and not t.is_cuda:
+        if t is None:
+            continue
+        if not t.is_cuda:
             raise RuntimeError(f"{fn}: all tensors must be on the GPU")
-    dev = torch.cuda.current_device()
-    for t in ts:
-        if t is not None and t.get_device() != dev:
+        if dev is None:
+            dev = torch.cuda.current_device()
+        if t.get_device() != dev:
             raise RuntimeError(f"{fn}: a tensor is on GPU {t.get_device()}, the current one is {dev}")
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     return raw(dev) if raw is not None else torch.cuda.current_stream(dev).cuda_stream
@@ -531,7 +534,9 @@ def _matrix(fn, name, t, rows, cols, dtype=None):
 
 
 def _space(fn, workspace):
-    """The bytes of a workspace."""
+    """The bytes of a workspace (None: none)."""
+    if workspace is None:
+        return 0
     if not workspace.is_contiguous():
         raise ValueError(f"{fn}: workspace must be contiguous")
     return workspace.numel() * workspace.element_size()
@@ -608,7 +613,9 @@ def linear_w8a8(W, sw, x, Y=None, y_dtype=None, workspace=None):
     code = _tcode(x)
     Y, ldy, ycode = _w8_out(fn, Y, y_dtype, T, N, x.dtype, x.device)
     if workspace is None:
-        workspace = torch.empty(w8a8_workspace_size(T, K), dtype=torch.uint8, device=x.device)
+        need = w8a8_workspace_size(T, K)
+        if need:  # (one or two rows need none)
+            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
     stream = _here(fn, W, sw, x, Y, workspace)
     _check(lib().qw_w8a8_linear(_ptr(W), ldw, _ptr(sw), _ptr(x), code, ldx, T, _ptr(Y), ldy, ycode, N, K,
                                 _ptr(workspace), _space(fn, workspace), stream), "qw_w8a8_linear")
