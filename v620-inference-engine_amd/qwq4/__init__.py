@@ -687,7 +687,7 @@ def moe_sort(top_e, E, tile_m=0, out=None):
         nt = P // abs(tile_m) + E if tile_m else 0
         # (one buffer for all of the lists: an allocation each would cost more than the sort)
         own = torch.empty(2 * P + 3 * E + 3 + 2 * nt, dtype=torch.int32, device=top_e.device)
-        slot, r.pair_tok, r.counts, r.offsets, r.active, r.n_active, tile_e, tile_m0, n_tiles = own.split(
+        slot, r.pair_tok, r.counts, r.offsets, r.active, r.n_active, tile_e, tile_m0, n_tiles = own.split_with_sizes(
             (P, P, E, E + 1, E, 1, nt, nt, 1))
         r.tok_slot = slot.view(T, k)
         r.tile_e, r.tile_m0, r.n_tiles = (tile_e, tile_m0, n_tiles) if tile_m else (None, None, None)
