@@ -400,8 +400,9 @@ int qw_moe_sort(const int32_t *top_e, int T, int E, int topk, int tile_m, int32_
  * choice with a slot (0 <= slot < T*k; others are skipped, and rows no choice
  * has are left as they were). Elements of elem_bytes 1, 2 or 4 are moved as
  * they are (int8 rows, their fp32 scales with H = 1, 16- and 32-bit rows);
- * strides ldx, ldxs >= H in elements, any alignment of the element. Its
- * gradient is qw_moe_unpermute without weights. */
+ * strides ldx, ldxs >= H in elements, any alignment of the element. Where a
+ * slot is named twice, by a tok_slot that qw_moe_sort did not write, its row
+ * holds elements of either. Its gradient is qw_moe_unpermute without weights. */
 int qw_moe_permute(const void *x, int ldx, int elem_bytes, int T, int topk, int H, const int32_t *tok_slot, void *xs,
                    int ldxs, void *stream);
 
