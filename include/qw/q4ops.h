@@ -412,7 +412,8 @@ int qw_moe_permute(const void *x, int ldx, int elem_bytes, int T, int topk, int 
  * (fp16: finite values beyond +-65504 saturate). tok_w fp32 [T][k], or NULL:
  * all 1 (the gradient of qw_moe_permute). A token without slots gets zeros.
  * yp_type and out_type QW_T_F32, QW_T_BF16 or QW_T_F16; strides ldyp, ldo >= H
- * in elements. qw_moe_combine is the form with a shared expert's rows. */
+ * in elements. qw_moe_combine is the form with a shared expert's rows; it takes
+ * fp32 and fp16 yp, not bf16. */
 int qw_moe_unpermute(const void *yp, int yp_type, int ldyp, const int32_t *tok_slot, const float *tok_w, int T,
                      int topk, int H, void *out, int out_type, int ldo, void *stream);
 

@@ -240,3 +240,26 @@ def test_workspace_of_few_rows(lib):
     for T, K in ((3, 64), (2, 32784)):
         fn, args = linear(T=T, K=K, ldw=K, ldx=K, ws=None, wb=0)
         assert getattr(lib, fn)(*args) == -1 and "workspace needs" in lib.qw_q4_last_error().decode()
+
+
+def _combine_route(T=3, E=4, k=2):
+    import torch
+    r = qwq4.Route(T, E, k, "cpu")
+    r.tok_slot.copy_(torch.arange(T * k, dtype=torch.int32).view(T, k))
+    r.top_w.fill_(0.5)
+    return r
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float64", "int16", "int8"])
+def test_combine_refuses_rows_it_would_misread(dtype):
+    """moe_combine knows fp32 and fp16 rows: others (the bf16 yp that moe_experts_w8a8 can write) are refused, as the
+    expert rows and as the shared ones, before anything is launched."""
+    import torch
+    r, bad, good = _combine_route(), torch.zeros(6, 8, dtype=getattr(torch, dtype)), torch.zeros(6, 8)
+    with pytest.raises(TypeError, match="moe_combine: yp is torch." + dtype):
+        qwq4.moe_combine(bad, r, 8)
+    with pytest.raises(TypeError, match="moe_combine: shared is torch." + dtype):
+        qwq4.moe_combine(good, r, 8, shared=bad[:3])
+    for t in (torch.float32, torch.float16):  # (these go on to the check of the device)
+        with pytest.raises(RuntimeError, match="on the GPU"):
+            qwq4.moe_combine(good.to(t), r, 8, shared=good[:3].to(t))

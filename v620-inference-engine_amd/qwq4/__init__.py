@@ -478,9 +478,14 @@ def moe_experts_w4a8(gate, up, down, route, x, E, F, h=None, yp=None, workspace=
 
 def moe_combine(yp, route, H, shared=None, out=None, out_bf16=True, out_dtype=None):
     """out = shared + sum_i w_i yp[slot_i]; yp and shared fp32 or float16 (by dtype), out bf16
-    (out_bf16), fp32, or the dtype given (out_dtype, or that of a given out)."""
+    (out_bf16), fp32, or the dtype given (out_dtype, or that of a given out). Other rows (the bfloat16 yp of
+    moe_experts_w8a8) are refused: moe_unpermute takes those."""
     import torch
     T, topk = route.T, route.topk
+    for name, t in (("yp", yp), ("shared", shared)):
+        if t is not None and t.dtype != torch.float32 and t.dtype != torch.float16:
+            raise TypeError(f"moe_combine: {name} is {t.dtype}, not torch.float32 or torch.float16 (moe_unpermute "
+                            "takes bfloat16 rows)")
     if out is None:
         dt = out_dtype if out_dtype is not None else torch.bfloat16 if out_bf16 else torch.float32
         out = torch.empty((T, H), dtype=dt, device=yp.device)
