@@ -64,8 +64,11 @@ struct W8A8Shape {
     __device__ static __forceinline__ int m_base() { return wave() / WN * MT * 32; }
     __device__ static __forceinline__ int n_base() { return wave() % WN * NT * 32; }
     __device__ static __forceinline__ int n_of(int r) { return 8 * (r / 4) + 4 * (int(threadIdx.x) % WAVE / 32) + r % 4; }
-    // LDS that a wave has to itself after the sums
-    static constexpr int SPARE = BN * KB / ((NW + NS - 1) / NS);  // (of the weights' buffers)
+    // LDS that a wave has to itself after the sums, of the weights' buffers
+    // (whole banks' turns: several waves share a buffer, three of 10922 bytes in
+    // the tall expert tiles, and each of them starts aligned)
+    static constexpr int SPARE = BN * KB / ((NW + NS - 1) / NS) / 128 * 128;
+    static_assert(SPARE % 16 == 0, "16-byte pieces go through it");
 };
 
 // The stage buffers of shape S; a kernel that runs several shapes takes those
