@@ -13,7 +13,7 @@
  *   qw_quant_rows_i8      quant_rows_kernel         src/kernels/moe_w4a8.hip:17-36
  *   qw_moe_combine        gpu::moe_combine_B/T      src/kernels/moe.hpp:42-46
  *   qw_w8a8_gemm, qw_w8a8_linear, qw_moe_experts_w8a8, qw_moe_sort, qw_moe_permute,
- *   qw_moe_unpermute and its gradient have no counterpart there: products of
+ *   qw_moe_unpermute and their gradients have no counterpart there: products of
  *   checkpoints quantised to 8 bits, and expert rows held in memory.
  *   qw_w16_gemv           gpu::gemv_rows (fp16 W)   src/kernels/gemv.hpp:13-14
  *   qw_w16_gemv_tiled     gpu::gemv_rows (fp16 W)   src/kernels/gemv.hpp:13-14 (weights tiled at load)
@@ -402,15 +402,21 @@ int qw_moe_sort(const int32_t *top_e, int T, int E, int topk, int tile_m, int32_
  * they are (int8 rows, their fp32 scales with H = 1, 16- and 32-bit rows);
  * strides ldx, ldxs >= H in elements, any alignment of the element. Where a
  * slot is named twice, by a tok_slot that qw_moe_sort did not write, its row
- * holds elements of either. Its gradient is qw_moe_unpermute without weights. */
+ * holds elements of either. */
 int qw_moe_permute(const void *x, int ldx, int elem_bytes, int T, int topk, int H, const int32_t *tok_slot, void *xs,
                    int ldxs, void *stream);
+
+/* Its gradient: dx[t][j] = sum_i dxs[tok_slot[t][i]][j], as qw_moe_unpermute
+ * without weights, but fp16 dx beyond +-65504 rounds to infinities (a loss
+ * scaler has to see an overflow). */
+int qw_moe_permute_backward(const void *dxs, int dxs_type, int lddxs, const int32_t *tok_slot, int T, int topk, int H,
+                            void *dx, int dx_type, int lddx, void *stream);
 
 /* The rows back at their tokens:
  *   out[t][j] = sum_i tok_w[t][i] * yp[tok_slot[t][i]][j]
  * over the choices with a slot, in order, in fp32, rounded once to out_type
  * (fp16: finite values beyond +-65504 saturate). tok_w fp32 [T][k], or NULL:
- * all 1 (the gradient of qw_moe_permute). A token without slots gets zeros.
+ * all 1. A token without slots gets zeros.
  * yp_type and out_type QW_T_F32, QW_T_BF16 or QW_T_F16; strides ldyp, ldo >= H
  * in elements. qw_moe_combine is the form with a shared expert's rows; it takes
  * fp32 and fp16 yp, not bf16. */
@@ -418,8 +424,9 @@ int qw_moe_unpermute(const void *yp, int yp_type, int ldyp, const int32_t *tok_s
                      int topk, int H, void *out, int out_type, int ldo, void *stream);
 
 /* The gradients of qw_moe_unpermute, from dout [T][H] of dout_type:
- *   dyp[tok_slot[t][i]][j] = tok_w[t][i] * dout[t][j]   (of yp_type, one rounding;
- *                            rows no choice has are left as they were)
+ *   dyp[tok_slot[t][i]][j] = tok_w[t][i] * dout[t][j]   (of yp_type, one rounding,
+ *                            fp16 beyond +-65504 to infinities; rows no choice
+ *                            has are left as they were)
  *   dw[t][i] = sum_j yp[tok_slot[t][i]][j] * dout[t][j] (fp32; 0 without a slot)
  * Either of dyp and dw may be NULL (not wanted); yp is read for dw only. tok_w
  * NULL: all 1. Every sum has a fixed order. Where a slot is named twice, by a

@@ -318,3 +318,34 @@ def test_offsets_past_32_bits(gpu):
     dyp, dw = qwq4.moe_unpermute_backward(x, xs, r.tok_slot)
     assert torch.equal(dyp[at], xs[at])
     assert torch.equal(dw[-3:], (x[-3:].float() ** 2).sum(1)[:, None].expand(3, k))
+
+
+# fp16 beside and beyond its largest value 65504: 65519.996 rounds down to it, 65520 is the tie that rounds to infinity
+EDGE = [65504.0, 65519.996, 65520.0, -65520.0, 70000.0, -1e6, 3.0, float("inf")]
+
+
+@pytest.mark.parametrize("pad", [0, 1])
+def test_fp16_gradients_overflow(gpu, pad):
+    """Gradients that fp16 cannot hold are infinite, as a plain rounding makes them (a loss scaler looks for those);
+    the forward saturates. Whole 16-byte pieces, and one element at a time."""
+    import torch
+    H = len(EDGE)
+    d = torch.zeros(2, H + pad, device=gpu)[:, :H]
+    d[0], d[1] = torch.tensor(EDGE, device=gpu), 30000.0
+    slot = torch.tensor([[0, 2], [1, 3]], dtype=torch.int32, device=gpu)
+    w = torch.tensor([[1.0, 2.0], [2.0, 3.0]], device=gpu)
+    yp = torch.ones(4, H + pad, dtype=torch.float16, device=gpu)[:, :H]
+    dyp, _ = qwq4.moe_unpermute_backward(d, yp, slot, w)
+    with np.errstate(over="ignore"):
+        want = np.stack([host(d[0]), 2 * host(d[1]), 2 * host(d[0]), 3 * host(d[1])]).astype(np.float16)
+        want_dx = np.stack([host(d[0]), 2 * host(d[1])]).astype(np.float16)
+    assert np.array_equal(host(dyp), want)
+    assert np.isinf(want).any() and (want[3] == np.inf).all()
+    # its other choice's row is of zeros: the sum is the edge itself
+    dxs = torch.zeros(4, H + pad, device=gpu)[:, :H]
+    dxs[0], dxs[1], dxs[3] = d[0], d[1], d[1]
+    dx = torch.full((2, H + pad), GUARD, dtype=torch.float16, device=gpu)[:, :H]
+    assert np.array_equal(host(qwq4.moe_permute_backward(dxs, slot, dx=dx)), want_dx)
+    half = torch.full((4, H), 40000.0, dtype=torch.float16, device=gpu)  # (a sum of two: 80000)
+    assert (host(qwq4.moe_permute_backward(half, slot)) == np.inf).all()
+    assert (host(qwq4.moe_unpermute(half, slot)) == 65504).all()

@@ -263,3 +263,35 @@ def test_combine_refuses_rows_it_would_misread(dtype):
     for t in (torch.float32, torch.float16):  # (these go on to the check of the device)
         with pytest.raises(RuntimeError, match="on the GPU"):
             qwq4.moe_combine(good.to(t), r, 8, shared=good[:3].to(t))
+
+
+def permute_grad(dxs=P, dt=1, lddxs=64, slot=P, T=4, k=2, H=64, dx=P, xt=1, lddx=64):
+    return "qw_moe_permute_backward", (dxs, dt, lddxs, slot, T, k, H, dx, xt, lddx, None)
+
+
+PERMUTE_GRAD = {
+    "null dxs": permute_grad(dxs=None), "null dx": permute_grad(dx=None), "null slot": permute_grad(slot=None),
+    "dxs type": permute_grad(dt=3), "dx type": permute_grad(xt=-1), "lddxs": permute_grad(lddxs=63),
+    "lddx": permute_grad(lddx=63), "T": permute_grad(T=0), "topk": permute_grad(k=65), "H": permute_grad(H=0),
+    "too wide": permute_grad(H=(1 << 28) + 1, lddxs=1 << 29, lddx=1 << 29), "dx odd": permute_grad(dx=ODD),
+}
+
+
+@pytest.mark.parametrize("name", sorted(PERMUTE_GRAD))
+def test_permute_gradient_refused(lib, name):
+    fn, args = PERMUTE_GRAD[name]
+    assert getattr(lib, fn)(*args) == -1
+    assert lib.qw_q4_last_error().decode().startswith("qw_moe_permute_backward:")
+
+
+def test_permute_gradient_binding_refusals():
+    import torch
+    slot = torch.zeros(3, 2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="moe_permute_backward: dxs is"):
+        qwq4.moe_permute_backward(torch.zeros(5, 32), slot)
+    with pytest.raises(TypeError, match="element type"):
+        qwq4.moe_permute_backward(torch.zeros(6, 32, dtype=torch.int8), slot)
+    with pytest.raises(TypeError, match="moe_permute_backward: the output is"):
+        qwq4.moe_permute_backward(torch.zeros(6, 32), slot, dx=torch.zeros(3, 32), dx_dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="moe_permute_backward: all tensors must be on the GPU"):
+        qwq4.moe_permute_backward(torch.zeros(6, 32), slot)

@@ -517,20 +517,32 @@ int qw_moe_permute(const void *x, int ldx, int elem_bytes, int T, int topk, int 
     return launched(fn);
 }
 
-int qw_moe_unpermute(const void *yp, int yp_type, int ldyp, const int32_t *tok_slot, const float *tok_w, int T,
-                     int topk, int H, void *out, int out_type, int ldo, void *stream) {
-    const char *fn = "qw_moe_unpermute";
+static int unpermute(const char *fn, const void *yp, int yp_type, int ldyp, const int32_t *tok_slot,
+                     const float *tok_w, int T, int topk, int H, void *out, int out_type, int ldo, bool saturate,
+                     void *stream) {
     REQUIRE(yp && tok_slot && out, "%s: null pointer", fn);
     if (int r = check_rows(fn, T, topk, H)) return r;
-    REQUIRE(is_type(yp_type) && is_type(out_type), "%s: yp_type = %d, out_type = %d (0 fp32, 1 bf16, 2 fp16)", fn,
+    REQUIRE(is_type(yp_type) && is_type(out_type), "%s: types of the rows = %d, %d (0 fp32, 1 bf16, 2 fp16)", fn,
             yp_type, out_type);
     REQUIRE((int64_t(T) * topk == 1 || ldyp >= H) && (T == 1 || ldo >= H), "%s: stride %d or %d < H = %d", fn, ldyp, ldo,
             H);
     REQUIRE(aligned(yp, type_bytes(yp_type)) && aligned(out, type_bytes(out_type)) && aligned(tok_slot, 4) &&
                 aligned(tok_w, 4),
             "%s: misaligned buffer", fn);
-    qwq4::launch_unpermute(yp, yp_type, ldyp, tok_slot, tok_w, T, topk, H, out, out_type, ldo, st(stream));
+    qwq4::launch_unpermute(yp, yp_type, ldyp, tok_slot, tok_w, T, topk, H, out, out_type, ldo, saturate, st(stream));
     return launched(fn);
+}
+
+int qw_moe_unpermute(const void *yp, int yp_type, int ldyp, const int32_t *tok_slot, const float *tok_w, int T,
+                     int topk, int H, void *out, int out_type, int ldo, void *stream) {
+    return unpermute("qw_moe_unpermute", yp, yp_type, ldyp, tok_slot, tok_w, T, topk, H, out, out_type, ldo, true,
+                     stream);
+}
+
+int qw_moe_permute_backward(const void *dxs, int dxs_type, int lddxs, const int32_t *tok_slot, int T, int topk, int H,
+                            void *dx, int dx_type, int lddx, void *stream) {
+    return unpermute("qw_moe_permute_backward", dxs, dxs_type, lddxs, tok_slot, nullptr, T, topk, H, dx, dx_type, lddx,
+                     false, stream);
 }
 
 int qw_moe_unpermute_backward(const void *dout, int dout_type, int ldd, const void *yp, int yp_type, int ldyp,

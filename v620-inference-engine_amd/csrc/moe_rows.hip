@@ -7,7 +7,8 @@
 //   out[t] = sum_i w[t][i] yp[slot(t, i)]                    unpermute
 //   dyp[slot(t, i)] = w[t][i] dout[t]                        its gradients
 //   dw[t][i] = <yp[slot(t, i)], dout[t]>
-// The gradient of permute is unpermute with all weights 1. Choices outside
+// The gradient of permute is unpermute with all weights 1 (and fp16 that
+// overflows instead of saturating). Choices outside
 // 0 .. E - 1 (an expert that another rank holds, in the engine's
 // expert-parallel layout, src/core/shard.hpp:34) have no slot (-1) and add
 // nothing. No atomics on values: every sum has a fixed order.
@@ -184,8 +185,19 @@ __device__ __forceinline__ void row_load(const void *x, int64_t i, float (&v)[V]
         for (int j = 0; j < V; ++j) v[j] = TY == 1 ? bf16_bits_to_f32(b[j]) : f16_bits_to_f32(b[j]);
     }
 }
+// fp32 -> the nearest fp16, infinite beyond its range. (The value is taken as it
+// is: the compiler would otherwise join the conversion with the multiplication
+// before it, which then rounds once, and differently in 16-byte pieces and single
+// elements.)
+__device__ __forceinline__ _Float16 f32_to_f16_rne(float v) {
+    asm volatile("" : "+v"(v));
+    return _Float16(v);
+}
+
+// saturate: finite values beyond fp16's +-65504 become those (activations);
+// else they round to infinities (gradients: a loss scaler has to see them).
 template <int TY, int V>
-__device__ __forceinline__ void row_store(void *y, int64_t i, const float (&v)[V]) {
+__device__ __forceinline__ void row_store(void *y, int64_t i, const float (&v)[V], bool saturate) {
     if constexpr (TY == 0 && V == 1) {
         static_cast<float *>(y)[i] = v[0];
     } else if constexpr (TY == 0) {
@@ -198,7 +210,8 @@ __device__ __forceinline__ void row_store(void *y, int64_t i, const float (&v)[V
         uint16_t b[V];
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            b[j] = TY == 1 ? f32_to_bf16_rne(v[j]) : __builtin_bit_cast(uint16_t, f32_to_f16_satfinite(v[j]));
+            b[j] = TY == 1 ? f32_to_bf16_rne(v[j])
+                           : __builtin_bit_cast(uint16_t, saturate ? f32_to_f16_satfinite(v[j]) : f32_to_f16_rne(v[j]));
         if constexpr (V == 8) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(b);
         else if constexpr (V == 4) *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(b);
         else p[0] = b[0];
@@ -220,7 +233,8 @@ template <int YT, int OT, int V>
 __global__ __launch_bounds__(256) void unpermute_kernel(const void *__restrict__ yp, int64_t ldy,
                                                         const int32_t *__restrict__ tok_slot,
                                                         const float *__restrict__ tok_w, int T, int topk, int H,
-                                                        void *__restrict__ out, int64_t ldo, int cols) {
+                                                        void *__restrict__ out, int64_t ldo, int cols,
+                                                        bool saturate) {
     const int t = int(blockIdx.x) / cols, P = T * topk;
     const int32_t *slots = tok_slot + int64_t(t) * topk;
     const float *weights = tok_w ? tok_w + int64_t(t) * topk : nullptr;
@@ -247,7 +261,7 @@ __global__ __launch_bounds__(256) void unpermute_kernel(const void *__restrict__
                 }
             }
         }
-        row_store<OT, V>(out, t * ldo + j, sum);
+        row_store<OT, V>(out, t * ldo + j, sum, saturate);
     }
 }
 
@@ -263,14 +277,14 @@ static void by_type(int type, F f) {
 }
 
 void launch_unpermute(const void *yp, int yp_type, int64_t ldy, const int32_t *tok_slot, const float *tok_w, int T,
-                      int topk, int H, void *out, int out_type, int64_t ldo, hipStream_t s) {
+                      int topk, int H, void *out, int out_type, int64_t ldo, bool saturate, hipStream_t s) {
     auto run = [&](auto yt, auto ot, auto v) {
         constexpr int V = decltype(v)::value;
         const int items = (H + V - 1) / V, threads = items > 128 ? 256 : items > 64 ? 128 : 64;
         // (a grid holds less than 2^32 threads: with very many tokens a block takes more of a row)
         const int cols = std::max(1, std::min((items + threads - 1) / threads, (1 << 23) / T));
         unpermute_kernel<decltype(yt)::value, decltype(ot)::value, V><<<unsigned(T) * unsigned(cols), threads, 0, s>>>(
-            yp, ldy, tok_slot, tok_w, T, topk, H, out, ldo, cols);
+            yp, ldy, tok_slot, tok_w, T, topk, H, out, ldo, cols, saturate);
     };
     by_type(yp_type, [&](auto yt) {
         by_type(out_type, [&](auto ot) {
@@ -315,7 +329,7 @@ __device__ __forceinline__ void choice_backward(const UnpermuteGradArgs &a, int 
                     float g[V];
 #pragma unroll
                     for (int c = 0; c < V; ++c) g[c] = w * d[u][c];
-                    row_store<YT, V>(a.dyp, g0 + j, g);
+                    row_store<YT, V>(a.dyp, g0 + j, g, false);
                 }
             }
         }

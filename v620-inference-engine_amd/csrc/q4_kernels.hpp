@@ -312,7 +312,7 @@ void launch_sort(const SortArgs &a, hipStream_t s);
 void launch_permute(const void *x, int64_t ldx, int elem_bytes, int T, int topk, int H, const int32_t *tok_slot,
                     void *xs, int64_t ldxs, hipStream_t s);
 void launch_unpermute(const void *yp, int yp_type, int64_t ldy, const int32_t *tok_slot, const float *tok_w, int T,
-                      int topk, int H, void *out, int out_type, int64_t ldo, hipStream_t s);
+                      int topk, int H, void *out, int out_type, int64_t ldo, bool saturate, hipStream_t s);
 struct UnpermuteGradArgs {
     const void *dout;
     int dout_type;

@@ -24,8 +24,8 @@ SYMBOLS = (
     "qw_w16_gemv", "qw_w16_tiled_size", "qw_w16_tile", "qw_w16_gemv_tiled", "qw_w16_swiglu_gemv_tiled", "qw_i8_gemv", "qw_i8_tiled_size", "qw_i8_tile",
     "qw_moe_w4a8_tile_m", "qw_moe_w4a8_workspace_size", "qw_moe_experts_w4a8", "qw_quant_rows_i8", "qw_swiglu_gate",
     "qw_quant_tokens_i8", "qw_w8a8_gemm", "qw_w8a8_workspace_size", "qw_w8a8_linear", "qw_moe_w8a8_tile_m",
-    "qw_moe_w8a8_workspace_size", "qw_moe_experts_w8a8", "qw_moe_sort", "qw_moe_permute", "qw_moe_unpermute",
-    "qw_moe_unpermute_backward",
+    "qw_moe_w8a8_workspace_size", "qw_moe_experts_w8a8", "qw_moe_sort", "qw_moe_permute",
+    "qw_moe_permute_backward", "qw_moe_unpermute", "qw_moe_unpermute_backward",
     "qw_wcache_open", "qw_wcache_put", "qw_wcache_get", "qw_wcache_finish", "qw_wcache_close",
 )
 
@@ -79,6 +79,7 @@ _SIGS = {
     "qw_moe_experts_w8a8": ([_P] * 6 + [_I, _I, _I] + [_P] * 6 + [_I, _I, _I, _P, _P, _I, _P, _SZ, _P], _I),
     "qw_moe_sort": ([_P, _I, _I, _I, _I] + [_P] * 10, _I),
     "qw_moe_permute": ([_P, _I, _I, _I, _I, _I, _P, _P, _I, _P], _I),
+    "qw_moe_permute_backward": ([_P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _P], _I),
     "qw_moe_unpermute": ([_P, _I, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P], _I),
     "qw_moe_unpermute_backward": ([_P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _P, _I, _P, _P], _I),
     "qw_moe_decode_static": ([_P, _I, _P, _I, _I, _I, _I] + [_P] * 9 + [_I, _I, _P, _P, _I] + [_P] * 6 + [_I, _P], _I),
@@ -757,13 +758,24 @@ def moe_unpermute(yp, tok_slot, tok_w=None, out=None, out_dtype=None):
 
 
 def moe_permute_backward(dxs, tok_slot, dx=None, dx_dtype=None):
-    """The gradient of moe_permute: dx[t] = sum_i dxs[tok_slot[t][i]]."""
-    return moe_unpermute(dxs, tok_slot, None, dx, dx_dtype)
+    """The gradient of moe_permute: dx[t] = sum_i dxs[tok_slot[t][i]], summed and typed as moe_unpermute does, but
+    float16 dx beyond +-65504 becomes infinite."""
+    fn = "moe_permute_backward"
+    T, k = _slots(fn, tok_slot)
+    lddxs = _matrix(fn, "dxs", dxs, T * k, None)
+    H = dxs.shape[1]
+    code = _tcode(dxs)
+    dx, lddx, xcode = _w8_out(fn, dx, dx_dtype, T, H, dxs.dtype, dxs.device)
+    stream = _here(fn, dxs, tok_slot, dx)
+    _check(lib().qw_moe_permute_backward(_ptr(dxs), code, lddxs, _ptr(tok_slot), T, k, H, _ptr(dx), xcode, lddx,
+                                         stream), "qw_moe_permute_backward")
+    return dx
 
 
 def moe_unpermute_backward(dout, yp, tok_slot, tok_w=None, dyp=None, dw=None, need_dyp=True, need_dw=True):
     """The gradients of moe_unpermute from dout [T][H]: (dyp [T*k][H] of yp's type, dw fp32 [T][k]), either None
-    where it is not needed. Rows of dyp that no choice has are left as they were (a new dyp: not set)."""
+    where it is not needed. float16 dyp beyond +-65504 becomes infinite. Rows of dyp that no choice has are left as
+    they were (a new dyp: not set)."""
     import torch
     fn = "moe_unpermute_backward"
     T, k = _slots(fn, tok_slot)
