@@ -295,3 +295,35 @@ def test_permute_gradient_binding_refusals():
         qwq4.moe_permute_backward(torch.zeros(6, 32), slot, dx=torch.zeros(3, 32), dx_dtype=torch.float16)
     with pytest.raises(RuntimeError, match="moe_permute_backward: all tensors must be on the GPU"):
         qwq4.moe_permute_backward(torch.zeros(6, 32), slot)
+
+
+def test_sort_into_a_route_keeps_the_routers_buffers(monkeypatch):
+    """moe_sort(out=route) shows the given choices as route.top_e; the next moe_route into it writes the route's own
+    buffers again, not the caller's choices, and a Route that moe_sort made has none to write."""
+    import types
+
+    import torch
+    calls = []
+    stub = types.SimpleNamespace(qw_moe_sort=lambda *a: calls.append(("sort", a)) or 0,
+                                 qw_moe_route=lambda *a: calls.append(("route", a)) or 0)
+    monkeypatch.setattr(qwq4, "lib", lambda: stub)
+    monkeypatch.setattr(qwq4, "_here", lambda *a: None)
+    monkeypatch.setattr(qwq4, "_dev", lambda *a: None)
+    monkeypatch.setattr(qwq4, "_stream", lambda: None)
+    T, E, k = 5, 4, 2
+    r = qwq4.Route(T, E, k, "cpu")
+    own_e, own_w, logits = r.top_e, r.top_w, torch.zeros(T, E)
+    for _ in range(2):
+        for e in (torch.zeros(T, k, dtype=torch.int32), torch.ones(T, k, dtype=torch.int32)):
+            assert qwq4.moe_sort(e, E, out=r) is r and r.top_e is e and r.top_w is None
+        r.top_w = torch.ones(T, k)  # (the caller's weights of these choices)
+        assert qwq4.moe_route(logits, k, out=r) is r and r.top_e is own_e and r.top_w is own_w
+        assert calls[-1][0] == "route" and calls[-1][1][5:7] == (own_e.data_ptr(), own_w.data_ptr())
+    w = torch.ones(T, k)
+    r.top_w = w  # (buffers that a caller put there stay: no sort came between)
+    assert qwq4.moe_route(logits, k, out=r).top_w is w
+    n, made = len(calls) + 1, qwq4.moe_sort(own_e, E)
+    made.top_w = torch.ones(T, k)
+    with pytest.raises(ValueError, match="moe_route: out was made by moe_sort"):
+        qwq4.moe_route(logits, k, out=made)
+    assert len(calls) == n and made.top_e is own_e

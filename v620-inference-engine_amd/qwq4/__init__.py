@@ -361,6 +361,8 @@ def gemm(W, S, Z, X, N, K, Y=None, y_bf16=False, workspace=None, x_f16=None, y_d
 class Route:
     """Device outputs of qw_moe_route."""
 
+    _router = None  # (the router's top_e and top_w, while the lists are those of moe_sort's choices)
+
     def __init__(self, T, E, topk, device, tile_m=0):
         import torch
         i32 = dict(dtype=torch.int32, device=device)
@@ -382,6 +384,10 @@ class Route:
 def moe_route(logits, topk, tile_m=0, out=None):
     T, E = logits.shape
     r = out if out is not None else Route(T, E, topk, logits.device, tile_m)
+    if r._router is not None:
+        if r._router[1] is None:
+            raise ValueError("moe_route: out was made by moe_sort and has no buffers for choices and weights")
+        (r.top_e, r.top_w), r._router = r._router, None
     _dev(logits)
     rc = lib().qw_moe_route(_ptr(logits), T, E, topk, tile_m, _ptr(r.top_e), _ptr(r.top_w), _ptr(r.counts),
                             _ptr(r.offsets), _ptr(r.tok_slot), _ptr(r.pair_tok), _ptr(r.active), _ptr(r.n_active),
@@ -675,8 +681,9 @@ def moe_experts_w8a8(gate, up, down, route, x, h=None, yp=None, yp_dtype=None, w
 
 # ----------------------------------------- tokens sorted by expert and back
 def moe_sort(top_e, E, tile_m=0, out=None):
-    """The slots of given choices top_e int32 [T][k], as a Route (top_w is not set): experts ascending, within one
-    the choices in order; a choice outside 0 .. E - 1 has slot -1, a place behind the last slot token -1."""
+    """The slots of given choices top_e int32 [T][k], as a Route (its top_e is the tensor given, top_w is None):
+    experts ascending, within one the choices in order; a choice outside 0 .. E - 1 has slot -1, a place behind the
+    last slot token -1. A Route given as out has its own top_e and top_w back with the next moe_route into it."""
     import torch
     fn = "moe_sort"
     if top_e.dim() != 2:
@@ -688,7 +695,7 @@ def moe_sort(top_e, E, tile_m=0, out=None):
     _whole(fn, "top_e", top_e, (T, k), torch.int32)
     if out is None:
         r = Route.__new__(Route)
-        r.T, r.E, r.topk, r.tile_m, r.top_w = T, E, k, tile_m, None
+        r.T, r.E, r.topk, r.tile_m, r.top_w, r._router = T, E, k, tile_m, None, (None, None)
         P = T * k
         nt = P // abs(tile_m) + E if tile_m else 0
         # (one buffer for all of the lists: an allocation each would cost more than the sort)
@@ -701,9 +708,10 @@ def moe_sort(top_e, E, tile_m=0, out=None):
         r = out
         if (r.T, r.E, r.topk, r.tile_m) != (T, E, k, tile_m):
             raise ValueError(f"{fn}: out was made for T, E, k, tile_m = {r.T, r.E, r.topk, r.tile_m}")
-        r.top_w = None
-    r.top_e = top_e
     stream = _here(fn, top_e, r.pair_tok)
+    if r._router is None:
+        r._router = r.top_e, r.top_w
+    r.top_e, r.top_w = top_e, None
     rc = lib().qw_moe_sort(_ptr(top_e), T, E, k, tile_m, _ptr(r.counts), _ptr(r.offsets), _ptr(r.tok_slot),
                            _ptr(r.pair_tok), _ptr(r.active), _ptr(r.n_active), _ptr(r.tile_e), _ptr(r.tile_m0),
                            _ptr(r.n_tiles), stream)
