@@ -327,3 +327,32 @@ def test_sort_into_a_route_keeps_the_routers_buffers(monkeypatch):
     with pytest.raises(ValueError, match="moe_route: out was made by moe_sort"):
         qwq4.moe_route(logits, k, out=made)
     assert len(calls) == n and made.top_e is own_e
+
+
+def test_combine_of_a_sorted_route_wants_weights(monkeypatch):
+    """A route of given choices has no router's weights: moe_combine takes them as tok_w (fp32 [T][k]), and without
+    any says what is missing."""
+    import types
+
+    import torch
+    r, yp, w = _combine_route(), torch.zeros(6, 8), torch.ones(3, 2)
+    r.top_w = None
+    with pytest.raises(ValueError, match="moe_combine: the route has no weights"):
+        qwq4.moe_combine(yp, r, 8)
+    with pytest.raises(ValueError, match="tok_w is"):
+        qwq4.moe_combine(yp, r, 8, tok_w=torch.ones(3, 3))
+    with pytest.raises(TypeError, match="tok_w is"):
+        qwq4.moe_combine(yp, r, 8, tok_w=w.half())
+    with pytest.raises(ValueError, match="tok_w must be contiguous"):
+        qwq4.moe_combine(yp, r, 8, tok_w=torch.ones(2, 3).t())
+    with pytest.raises(RuntimeError, match="on the GPU"):
+        qwq4.moe_combine(yp, r, 8, tok_w=w)
+    seen = []
+    monkeypatch.setattr(qwq4, "lib", lambda: types.SimpleNamespace(qw_moe_combine=lambda *a: seen.append(a[3]) or 0))
+    monkeypatch.setattr(qwq4, "_dev", lambda *a: None)
+    monkeypatch.setattr(qwq4, "_stream", lambda: None)
+    qwq4.moe_combine(yp, r, 8, tok_w=w)
+    r.top_w = torch.ones(3, 2)  # (a router's, or set by the caller; tok_w goes before it)
+    qwq4.moe_combine(yp, r, 8)
+    qwq4.moe_combine(yp, r, 8, tok_w=w)
+    assert seen == [w.data_ptr(), r.top_w.data_ptr(), w.data_ptr()]

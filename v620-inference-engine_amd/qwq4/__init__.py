@@ -483,8 +483,9 @@ def moe_experts_w4a8(gate, up, down, route, x, E, F, h=None, yp=None, workspace=
     return h, yp
 
 
-def moe_combine(yp, route, H, shared=None, out=None, out_bf16=True, out_dtype=None):
-    """out = shared + sum_i w_i yp[slot_i]; yp and shared fp32 or float16 (by dtype), out bf16
+def moe_combine(yp, route, H, shared=None, out=None, out_bf16=True, out_dtype=None, tok_w=None):
+    """out = shared + sum_i w_i yp[slot_i], w the route's top_w or tok_w (float32 [T][k]; a route of moe_sort has no
+    weights of its own, and choices without a slot add nothing); yp and shared fp32 or float16 (by dtype), out bf16
     (out_bf16), fp32, or the dtype given (out_dtype, or that of a given out). Other rows (the bfloat16 yp of
     moe_experts_w8a8) are refused: moe_unpermute takes those."""
     import torch
@@ -493,11 +494,17 @@ def moe_combine(yp, route, H, shared=None, out=None, out_bf16=True, out_dtype=No
         if t is not None and t.dtype != torch.float32 and t.dtype != torch.float16:
             raise TypeError(f"moe_combine: {name} is {t.dtype}, not torch.float32 or torch.float16 (moe_unpermute "
                             "takes bfloat16 rows)")
+    if tok_w is not None:
+        _whole("moe_combine", "tok_w", tok_w, (T, topk), torch.float32)
+    elif route.top_w is None:
+        raise ValueError("moe_combine: the route has no weights (moe_sort made it): give tok_w")
+    else:
+        tok_w = route.top_w
     if out is None:
         dt = out_dtype if out_dtype is not None else torch.bfloat16 if out_bf16 else torch.float32
         out = torch.empty((T, H), dtype=dt, device=yp.device)
-    _dev(yp, shared, out)
-    rc = lib().qw_moe_combine(_ptr(yp), int(yp.dtype == torch.float16), _ptr(route.tok_slot), _ptr(route.top_w),
+    _dev(yp, shared, out, tok_w)
+    rc = lib().qw_moe_combine(_ptr(yp), int(yp.dtype == torch.float16), _ptr(route.tok_slot), _ptr(tok_w),
                               _ptr(shared), int(shared is not None and shared.dtype == torch.float16), T, topk, H,
                               _ptr(out), _tcode(out), _stream())
     _check(rc, "qw_moe_combine")
@@ -683,7 +690,7 @@ def moe_experts_w8a8(gate, up, down, route, x, h=None, yp=None, yp_dtype=None, w
 def moe_sort(top_e, E, tile_m=0, out=None):
     """The slots of given choices top_e int32 [T][k], as a Route (its top_e is the tensor given, top_w is None):
     experts ascending, within one the choices in order; a choice outside 0 .. E - 1 has slot -1, a place behind the
-    last slot token -1. A Route given as out has its own top_e and top_w back with the next moe_route into it."""
+    last slot token -1. moe_combine and moe_unpermute take the choices' weights. A Route given as out has its own top_e and top_w back with the next moe_route into it."""
     import torch
     fn = "moe_sort"
     if top_e.dim() != 2:
