@@ -349,3 +349,37 @@ def test_fp16_gradients_overflow(gpu, pad):
     half = torch.full((4, H), 40000.0, dtype=torch.float16, device=gpu)  # (a sum of two: 80000)
     assert (host(qwq4.moe_permute_backward(half, slot)) == np.inf).all()
     assert (host(qwq4.moe_unpermute(half, slot)) == 65504).all()
+
+
+@pytest.mark.parametrize("t", ["i8", "u16", "e4m3", "bf16", "f32"])
+def test_new_rows_are_defined(gpu, t):
+    """Sorted rows and dyp that a call allocates are zero where no choice has a slot (a product over all of them, such as
+    an expert's weight gradient, must not meet what the memory held before)."""
+    import torch
+    T, k, H = 96, 4, 512
+    dtype = {"i8": torch.int8, "u16": torch.uint16, "e4m3": torch.float8_e4m3fn, "bf16": torch.bfloat16,
+             "f32": torch.float32}[t]
+    e = _choices(17, T, 9, k, "dropped")
+    _, offsets, slot, tok = ref.sort(e, 9)
+    n, slots = int(offsets[-1]), to_dev(slot.astype(np.int32), gpu)
+    assert 0 < n < T * k
+    x = torch.from_numpy(np.random.default_rng(18).integers(1, 99, (T, H)).astype(np.int8)).to(gpu)
+    x = x.repeat(1, dtype.itemsize).view(dtype)
+
+    def used():  # the allocator's block that the call below takes, full of ones (a NaN in any float type)
+        block = torch.full((T * k, H * dtype.itemsize), 255, dtype=torch.uint8, device=gpu)
+        torch.cuda.synchronize()
+        return block.data_ptr()
+    torch.cuda.empty_cache()
+    at = used()
+    xs = qwq4.moe_permute(x, slots)
+    print(f"moe_permute {t}: block taken again: {at == xs.data_ptr()}", flush=True)
+    bits = host(xs.view(torch.uint8))
+    assert np.array_equal(bits[:n], host(x.view(torch.uint8))[tok[:n]]) and (bits[n:] == 0).all()
+    if t not in ("bf16", "f32"):
+        return
+    yp, dout = torch.ones(T * k, H, dtype=dtype, device=gpu), torch.ones(T, H, device=gpu)
+    del xs
+    used()
+    dyp, _ = qwq4.moe_unpermute_backward(dout, yp, slots)
+    assert (host(dyp)[:n] == 1).all() and (host(dyp)[n:] == 0).all()

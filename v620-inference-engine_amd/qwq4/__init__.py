@@ -652,7 +652,8 @@ def moe_w8a8_workspace_size(T, topk, H, F):
 def moe_experts_w8a8(gate, up, down, route, x, h=None, yp=None, yp_dtype=None, workspace=None):
     """The routed experts in W8A8 (route from moe_route or moe_sort with tile_m = moe_w8a8_tile_m()): gate and up
     (int8 [E][F][H], fp32 [E][F]), down (int8 [E][H][F], fp32 [E][H]), x [T][H] float32, bfloat16 or float16. Returns
-    (h fp16 [T*k][F], yp [T*k][H]); yp float16, or yp_dtype / the dtype of a given yp."""
+    (h fp16 [T*k][F], yp [T*k][H]); yp float16, or yp_dtype / the dtype of a given yp. Rows that no choice has (behind
+    route.offsets[E]) are left as they were, in a new h and yp not set: read yp through route.tok_slot."""
     import torch
     fn = "moe_experts_w8a8"
     T, topk, E = route.T, route.topk, route.E
@@ -738,14 +739,15 @@ def _slots(fn, tok_slot):
 
 def moe_permute(x, tok_slot, xs=None):
     """The rows in slot order: xs[tok_slot[t][i]] = x[t] (x [T][H] of 1, 2 or 4 bytes an element). Rows of xs
-    [T*k][H] that no choice has are left as they were (a new xs: not set). Its gradient is moe_permute_backward."""
+    [T*k][H] that no choice has are left as they were; a new xs has zeros there, which a caller who does not need
+    them saves by giving one. Its gradient is moe_permute_backward."""
     import torch
     fn = "moe_permute"
     T, k = _slots(fn, tok_slot)
     ldx = _matrix(fn, "x", x, T, None)
     H = x.shape[1]
     if xs is None:
-        xs = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
+        xs = torch.zeros((T * k, H), dtype=x.dtype, device=x.device)
     ldxs = _matrix(fn, "xs", xs, T * k, H, x.dtype)
     stream = _here(fn, x, tok_slot, xs)
     _check(lib().qw_moe_permute(_ptr(x), ldx, x.element_size(), T, k, H, _ptr(tok_slot), _ptr(xs), ldxs, stream),
@@ -790,7 +792,7 @@ def moe_permute_backward(dxs, tok_slot, dx=None, dx_dtype=None):
 def moe_unpermute_backward(dout, yp, tok_slot, tok_w=None, dyp=None, dw=None, need_dyp=True, need_dw=True):
     """The gradients of moe_unpermute from dout [T][H]: (dyp [T*k][H] of yp's type, dw fp32 [T][k]), either None
     where it is not needed. float16 dyp beyond +-65504 becomes infinite. Rows of dyp that no choice has are left as
-    they were (a new dyp: not set)."""
+    they were; a new dyp has zeros there."""
     import torch
     fn = "moe_unpermute_backward"
     T, k = _slots(fn, tok_slot)
@@ -803,7 +805,7 @@ def moe_unpermute_backward(dout, yp, tok_slot, tok_w=None, dyp=None, dw=None, ne
     if not need_dyp:
         dyp = None
     elif dyp is None:
-        dyp = torch.empty((T * k, H), dtype=yp.dtype, device=yp.device)
+        dyp = torch.zeros((T * k, H), dtype=yp.dtype, device=yp.device)
     if not need_dw:
         dw = None
     elif dw is None:
