@@ -383,3 +383,34 @@ def test_new_rows_are_defined(gpu, t):
     used()
     dyp, _ = qwq4.moe_unpermute_backward(dout, yp, slots)
     assert (host(dyp)[:n] == 1).all() and (host(dyp)[n:] == 0).all()
+
+
+@pytest.mark.parametrize("T,k,H", [(1, 1, 8), (37, 4, 96), (130, 8, 257)])
+def test_functions_of_the_guide(gpu, T, k, H):
+    """The integration guide's autograd Functions around a user's own expert (a product per column): they run, and
+    their gradients are the formula's."""
+    import os
+    import re
+
+    import torch
+    guide = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")).read()
+    code, = (b for b in re.findall(r"```python\n(.*?)```", guide, flags=re.S) if "class Unpermute" in b)
+    names = {"torch": torch, "qwq4": qwq4}
+    exec(code, names)
+    r = np.random.default_rng(T)
+    slot = ref.sort(_choices(T + k, T, 7, k, "dropped" if T > 1 else "spread"), 7)[2]
+    x, w, a, m = (r.standard_normal(s).astype(np.float32) for s in ((T, H), (T, k), (H,), (T, H)))
+    leaf = [torch.from_numpy(v).to(gpu).requires_grad_() for v in (x, w)]
+    s = to_dev(slot.astype(np.int32), gpu)
+    out = names["Unpermute"].apply(names["Permute"].apply(leaf[0], s) * to_dev(a, gpu), s, leaf[1])
+    (out * to_dev(m, gpu)).sum().backward()
+    x, w, a, m = (v.astype(np.float64) for v in (x, w, a, m))
+    kept = slot >= 0
+    each = np.where(kept[..., None], (w[..., None] * m[:, None]) * a, 0.0)
+    # w m, its product with a, and k sums: k + 2 roundings of 2^-24 of the sum of magnitudes
+    assert np.all(np.abs(host(leaf[0].grad) - each.sum(1)) <= (k + 2) * 2.0**-24 * np.abs(each).sum(1))
+    # x a, H products and H sums
+    part = np.where(kept[..., None], ((x * a) * m)[:, None], 0.0)
+    assert np.all(np.abs(host(leaf[1].grad) - part.sum(-1)) <= (2 * H + 1) * 2.0**-24 * np.abs(part).sum(-1))
+    only, = torch.autograd.grad(names["Unpermute"].apply(torch.ones(T * k, H, device=gpu), s, leaf[1]).sum(), leaf[1])
+    assert np.array_equal(host(only), np.where(kept, H, 0).astype(np.float32))

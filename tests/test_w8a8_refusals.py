@@ -356,3 +356,17 @@ def test_combine_of_a_sorted_route_wants_weights(monkeypatch):
     qwq4.moe_combine(yp, r, 8)
     qwq4.moe_combine(yp, r, 8, tok_w=w)
     assert seen == [w.data_ptr(), r.top_w.data_ptr(), w.data_ptr()]
+
+
+def test_expert_rows_refuse_what_autograd_follows():
+    """A result that is cut off from its inputs would train nothing and say nothing."""
+    import torch
+    x, yp, w = (torch.zeros(*s, requires_grad=True) for s in ((3, 32), (6, 32), (3, 2)))
+    slot = torch.zeros(3, 2, dtype=torch.int32)
+    calls = (("moe_permute", lambda: qwq4.moe_permute(x, slot)), ("moe_unpermute", lambda: qwq4.moe_unpermute(yp, slot)),
+             ("moe_unpermute", lambda: qwq4.moe_unpermute(yp.detach(), slot, w)))
+    for fn, call in calls:
+        with pytest.raises(RuntimeError, match=fn + ": an input requires grad.*" + fn + "_backward"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="on the GPU"):  # (goes on to the check of the device)
+            call()

@@ -737,12 +737,23 @@ def _slots(fn, tok_slot):
     return tok_slot.shape
 
 
+def _no_autograd(fn, *ts):
+    """Nothing here is recorded for autograd: an input whose gradient torch follows is refused, not cut off silently."""
+    import torch
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{fn}: an input requires grad, which this call does not record (use torch.no_grad(), "
+                                   f"or a torch.autograd.Function with {fn}_backward)")
+
+
 def moe_permute(x, tok_slot, xs=None):
     """The rows in slot order: xs[tok_slot[t][i]] = x[t] (x [T][H] of 1, 2 or 4 bytes an element). Rows of xs
     [T*k][H] that no choice has are left as they were; a new xs has zeros there, which a caller who does not need
-    them saves by giving one. Its gradient is moe_permute_backward."""
+    them saves by giving one. Its gradient is moe_permute_backward; autograd does not record the call."""
     import torch
     fn = "moe_permute"
+    _no_autograd(fn, x)
     T, k = _slots(fn, tok_slot)
     ldx = _matrix(fn, "x", x, T, None)
     H = x.shape[1]
@@ -758,9 +769,10 @@ def moe_permute(x, tok_slot, xs=None):
 def moe_unpermute(yp, tok_slot, tok_w=None, out=None, out_dtype=None):
     """out[t] = sum_i tok_w[t][i] yp[tok_slot[t][i]] over the choices with a slot, in order, in fp32 (tok_w None: all
     1); yp [T*k][H]. out of yp's type, or out_dtype / the dtype of a given out. moe_combine is the form with a shared
-    expert's rows."""
+    expert's rows. Its gradients are moe_unpermute_backward; autograd does not record the call."""
     import torch
     fn = "moe_unpermute"
+    _no_autograd(fn, yp, tok_w)
     T, k = _slots(fn, tok_slot)
     ldyp = _matrix(fn, "yp", yp, T * k, None)
     H = yp.shape[1]
