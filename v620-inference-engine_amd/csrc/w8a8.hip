@@ -147,8 +147,9 @@ static void launch_shape(const W8GemmArgs &a, hipStream_t s) {
 // runs alone: it loads every fourth 128-byte stage of K into two buffers of its
 // own, waits for its own loads only, and no barrier joins the waves before
 // their sums meet. (With a barrier per stage and four buffers shared by the
-// waves: 37 x 4096 x 6144 15.2 us, here 8.3; 20 x 4096 x 4096 12.0 and 7.0. Three or
-// four buffers or eight waves a block: no better, and fewer blocks on a CU.)
+// waves: 37 x 4096 x 6144 15.2 us, here 8.3; 20 x 4096 x 4096 12.0 and 7.0, weights
+// in the last-level cache; from memory 10.2 and 8.1 here. Three or four buffers
+// or eight waves a block: no better, and fewer blocks on a CU.)
 template <int NT_>
 struct W8Split {
     static constexpr int NT = NT_, NS = 2, KW = 4, THREADS = KW * WAVE, BN = 32 * NT, LPW = 4 + 4 * NT;
@@ -315,13 +316,15 @@ static void launch_split(const W8GemmArgs &a, hipStream_t s) {
 
 // ------------------------------------------------------------ few tokens
 // Up to 2 tokens the product is a stream of the weights (w8a8_gemv.cuh), 8 G
-// rows of them per block, bound by memory (one token, 4096 -> 12288: 9.9 us,
-// 5.1 TB/s; a large copy reaches 5.2). Streamed and in tiles of 32, K 4096: 2
-// rows to 4096 5.4 and 6.4 us, to 12288 12.3 and 12.3; 4 rows 6.9 and 6.4, 14.5
-// and 12.3.
+// rows of them per block, bound by memory and by the launch's ramp (one token,
+// 4096 -> 12288, rows quantised on the way: 12.1 us, 4.2 TB/s; a large copy
+// reaches 5.2). Times here and at launch_w8a8_gemm: calls in a graph over 0.8 GB
+// of weights in turn, which no cache holds. Streamed and in tiles of 32, K 4096:
+// 1 row to 4096 5.2 and 6.6 us, to 12288 11.7 and 13.5; 2 rows 5.9 and 6.6, 12.5
+// and 13.6. (4 rows, weights in the last-level cache: 6.9 and 6.4, 14.5 and 12.3.)
 // From 16- or 32-bit rows the block quantises them itself, which saves the
-// quantiser's launch (one token: 4.7 against 5.8 us and 9.9 against 11.5; two:
-// 6.1 against 6.6 and 11.5 against 12.2).
+// quantiser's launch (one token: 6.0 against 7.3 us and 12.1 against 13.7; two:
+// 7.4 against 7.9 and 14.2 against 14.6).
 template <int XT, bool VEC, int TM, int G>
 __global__ __launch_bounds__(256) void w8a8_gemv_kernel(W8GemmArgs a, const void *x, int64_t ldx) {
     extern __shared__ __align__(16) unsigned char s_q[];
@@ -349,7 +352,8 @@ static bool gemv_takes(int T, int K) { return T <= 2 && gemv_lds(T, K) <= W8_GEM
 template <int XT, bool VEC>
 static void launch_gemv(const W8GemmArgs &a, const void *x, int64_t ldx, hipStream_t s) {
     // (16 rows a block where that leaves blocks enough: 2 tokens and 12288 rows
-    // take 11.5 us against 13.8 with 8, 4096 rows 6.3 against 6.1)
+    // take 14.2 us against 15.3 with 8, 8192 rows 11.1 and 11.0, 4096 rows 8.0
+    // and 7.7. One token has less to gain from it: 12288 rows 12.4 and 11.5.)
     auto run = [&](auto tm) {
         constexpr int TM = decltype(tm)::value;
         const size_t lds = gemv_lds(TM, a.K);
@@ -362,14 +366,15 @@ static void launch_gemv(const W8GemmArgs &a, const void *x, int64_t ldx, hipStre
 }
 
 // One or two tokens stream the weights. Else the largest tile that makes about
-// a block for every CU (us; rows x weight rows x K, tiles of 256, 128, 64: 4096 x
-// 12288 x 4096: 237, 270, 406; 1024 x 4096 x 4096: 55, 34, 36; 256 x 4096 x 4096: 55,
-// 31, 12.9). Where those of 32 are no more than two rounds of the CUs, or there
-// are no more than 32 rows, those, two side by side between one round and two
-// (tiles of 64, of 32, of 32 x 64: 64 x 4096 x 4096, 256 of 32: 14.0, 7.4, 9.8; 32 x
-// 9216 x 4096, 288: 14.3, 12.9, 11.0; 128 x 4096 x 4096, 512: 13.9, 10.8, 9.7; 96 x
-// 6144 x 4096, 576: 13.1, 15.0, 17.6; 150 x 4096 x 4096, 640: 12.8, 13.6, 16.2; 16 x
-// 20480 x 4096, 640: 23.9, 19.1, 23.8; 8 x 100000 x 4096: 85, 72, 91).
+// a block for every CU (us, weights from memory; rows x weight rows x K, tiles of
+// 256 and 128: 4096 x 12288 x 4096: 190, 235; 1024 x 12288 x 4096: 60, 78; 1024 x
+// 4096 x 4096: 54, 34; of 256, 128, 64: 256 x 12288 x 4096: 58, 35, 34; 256 x 4096 x
+// 4096: 56, 32, 13.9). Where those of 32 are no more than two rounds of the CUs,
+// or there are no more than 32 rows, those, two side by side between one round
+// and two (tiles of 64, of 32, of 32 x 64: 64 x 4096 x 4096, 256 of 32: 13.4, 8.3,
+// 10.3; 32 x 9216 x 4096, 288: 15.6, 14.4, 13.3; 128 x 4096 x 4096, 512: 13.3, 11.3,
+// 10.5; 96 x 6144 x 4096, 576: 13.3, 15.6, 18.2; 150 x 4096 x 4096, 640: 12.4, 14.0,
+// 16.9; 16 x 20480 x 4096, 640: 25.2, 20.4, 25.0; 8 x 100000 x 4096: 87, 75, 92).
 void launch_w8a8_gemm(const W8GemmArgs &a, hipStream_t s) {
     auto tiles = [&](int b) { return int64_t((a.T + b - 1) / b) * ((a.N + b - 1) / b); };
     if (gemv_takes(a.T, a.K)) launch_gemv<3, true>(a, nullptr, 0, s);
