@@ -370,3 +370,21 @@ def test_expert_rows_refuse_what_autograd_follows():
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="on the GPU"):  # (goes on to the check of the device)
             call()
+
+
+def test_lists_of_any_object(monkeypatch):
+    """moe_route and moe_sort write into any object that has a Route's lists."""
+    import types
+
+    import torch
+    calls = []
+    stub = types.SimpleNamespace(qw_moe_sort=lambda *a: calls.append(a) or 0, qw_moe_route=lambda *a: calls.append(a) or 0)
+    monkeypatch.setattr(qwq4, "lib", lambda: stub)
+    monkeypatch.setattr(qwq4, "_here", lambda *a: None)
+    monkeypatch.setattr(qwq4, "_dev", lambda *a: None)
+    monkeypatch.setattr(qwq4, "_stream", lambda: None)
+    like = types.SimpleNamespace(**vars(qwq4.Route(3, 4, 2, "cpu")))
+    own_e, own_w, e = like.top_e, like.top_w, torch.zeros(3, 2, dtype=torch.int32)
+    assert qwq4.moe_route(torch.zeros(3, 4), 2, out=like) is like
+    assert qwq4.moe_sort(e, 4, out=like) is like and like.top_e is e
+    assert qwq4.moe_route(torch.zeros(3, 4), 2, out=like).top_e is own_e and like.top_w is own_w and len(calls) == 3

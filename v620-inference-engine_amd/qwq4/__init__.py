@@ -361,8 +361,6 @@ def gemm(W, S, Z, X, N, K, Y=None, y_bf16=False, workspace=None, x_f16=None, y_d
 class Route:
     """Device outputs of qw_moe_route."""
 
-    _router = None  # (the router's top_e and top_w, while the lists are those of moe_sort's choices)
-
     def __init__(self, T, E, topk, device, tile_m=0):
         import torch
         i32 = dict(dtype=torch.int32, device=device)
@@ -384,10 +382,12 @@ class Route:
 def moe_route(logits, topk, tile_m=0, out=None):
     T, E = logits.shape
     r = out if out is not None else Route(T, E, topk, logits.device, tile_m)
-    if r._router is not None:
-        if r._router[1] is None:
+    kept = getattr(r, "_router", None)
+    if kept is not None:  # (moe_sort's choices are shown in their place)
+        if kept[1] is None:
             raise ValueError("moe_route: out was made by moe_sort and has no buffers for choices and weights")
-        (r.top_e, r.top_w), r._router = r._router, None
+        r.top_e, r.top_w = kept
+        r._router = None
     _dev(logits)
     rc = lib().qw_moe_route(_ptr(logits), T, E, topk, tile_m, _ptr(r.top_e), _ptr(r.top_w), _ptr(r.counts),
                             _ptr(r.offsets), _ptr(r.tok_slot), _ptr(r.pair_tok), _ptr(r.active), _ptr(r.n_active),
@@ -691,7 +691,8 @@ def moe_experts_w8a8(gate, up, down, route, x, h=None, yp=None, yp_dtype=None, w
 def moe_sort(top_e, E, tile_m=0, out=None):
     """The slots of given choices top_e int32 [T][k], as a Route (its top_e is the tensor given, top_w is None):
     experts ascending, within one the choices in order; a choice outside 0 .. E - 1 has slot -1, a place behind the
-    last slot token -1. moe_combine and moe_unpermute take the choices' weights. A Route given as out has its own top_e and top_w back with the next moe_route into it."""
+    last slot token -1. moe_combine and moe_unpermute take the choices' weights. A Route given as out has its own
+    top_e and top_w back with the next moe_route into it."""
     import torch
     fn = "moe_sort"
     if top_e.dim() != 2:
@@ -717,8 +718,8 @@ def moe_sort(top_e, E, tile_m=0, out=None):
         if (r.T, r.E, r.topk, r.tile_m) != (T, E, k, tile_m):
             raise ValueError(f"{fn}: out was made for T, E, k, tile_m = {r.T, r.E, r.topk, r.tile_m}")
     stream = _here(fn, top_e, r.pair_tok)
-    if r._router is None:
-        r._router = r.top_e, r.top_w
+    if getattr(r, "_router", None) is None:
+        r._router = r.top_e, r.top_w  # (the router's own buffers, for the next moe_route)
     r.top_e, r.top_w = top_e, None
     rc = lib().qw_moe_sort(_ptr(top_e), T, E, k, tile_m, _ptr(r.counts), _ptr(r.offsets), _ptr(r.tok_slot),
                            _ptr(r.pair_tok), _ptr(r.active), _ptr(r.n_active), _ptr(r.tile_e), _ptr(r.tile_m0),
