@@ -15,6 +15,9 @@
  *   qw_w8a8_gemm, qw_w8a8_linear, qw_moe_experts_w8a8, qw_moe_sort, qw_moe_permute,
  *   qw_moe_unpermute and their gradients have no counterpart there: products of
  *   checkpoints quantised to 8 bits, and expert rows held in memory.
+ *   qw_rms_norm, qw_rms_norm_i8, qw_lora, qw_logprobs and their gradients: the
+ *   rows in front of a projection, low-rank adapters beside one, and what the
+ *   LM head's logits say of a token.
  *   qw_w16_gemv           gpu::gemv_rows (fp16 W)   src/kernels/gemv.hpp:13-14
  *   qw_w16_gemv_tiled     gpu::gemv_rows (fp16 W)   src/kernels/gemv.hpp:13-14 (weights tiled at load)
  *   qw_w16_swiglu_gemv_tiled  gpu::swiglu_T + gemv_rows  src/kernels/moe_route.hip:187-197, gemv.hpp:13-14
@@ -434,6 +437,105 @@ int qw_moe_unpermute(const void *yp, int yp_type, int ldyp, const int32_t *tok_s
 int qw_moe_unpermute_backward(const void *dout, int dout_type, int ldd, const void *yp, int yp_type, int ldyp,
                               const int32_t *tok_slot, const float *tok_w, int T, int topk, int H, void *dyp,
                               int lddyp, float *dw, void *stream);
+
+/* ---- Around a projection: the norm in front of it, adapters beside it, and
+ * log probabilities behind the last one.
+ *
+ * Root-mean-square norm of rows x [T][H], with the residual's addition:
+ *   h = x + residual (fp32),  y = h w / sqrt(mean(h^2) + eps)
+ * residual [T][H] of x's type or fp32, or NULL (h = x); res_out [T][H] of its
+ * type gets h, rounded (with a residual only; it may be the residual itself, at
+ * the same stride). y is normalised from h as added, before that rounding.
+ * x and y of any QW_T_* type, w [H] of x's type or fp32; y may be x where type and
+ * stride are the same. fp16 outputs saturate at +-65504. Sums in fp32: rows with values
+ * past 1e19 overflow them and give zeros. Any H from 1 to 2^28, any stride >= H and
+ * alignment of the elements; rows of a multiple of 8 on 16 bytes are fastest. */
+int qw_rms_norm(const void *x, int x_type, int ldx, const void *residual, int res_type, int ldr, void *res_out,
+                int ldro, const void *w, int w_type, float eps, int T, int H, void *y, int y_type, int ldy,
+                void *stream);
+
+/* The same with y in 8 bits and a scale per row, as qw_w8a8_gemm takes them:
+ *   u = h w,  c = max_j |u_j| / 127,  q = rint(u (1 / c)),  scale = c / sqrt(mean(h^2) + eps)
+ * (q is what qw_quant_tokens_i8 gives for the rows u in fp32: c is 1 for a row of
+ * zeros and at least 2^-126; an infinity or a NaN in u gives a NaN scale and q of
+ * zeros). q [T][H] of stride ldq >= H, scale fp32 [T]. */
+int qw_rms_norm_i8(const void *x, int x_type, int ldx, const void *residual, int res_type, int ldr, void *res_out,
+                   int ldro, const void *w, int w_type, float eps, int T, int H, int8_t *q, int ldq, float *scale,
+                   void *stream);
+
+/* The gradients of y = h w r, r = 1 / sqrt(mean(h^2) + eps), from dy [T][H]:
+ *   dx_t = r (g - h r^2 mean(g h)) + dres_t,  g = dy_t w     (of h's type)
+ *   dw = sum_t dy_t h_t r_t                                  (fp32 [H])
+ * h [T][H] is the row that was normalised (res_out where there was a residual),
+ * of dy's type or fp32; dres [T][H] of h's type (the gradient of res_out; the sum
+ * is the gradient of x and of the residual alike) or NULL; w of dy's type or fp32. dw may be NULL; its sum
+ * over tokens has a fixed order that depends on T. fp16 dx beyond +-65504 becomes
+ * infinite. dx may be dy, h or dres of the same type and stride. H up to 16384.
+ * workspace (with dw): qw_rms_norm_backward_workspace_size bytes, 256-byte
+ * aligned. */
+size_t qw_rms_norm_backward_workspace_size(int T, int H);
+int qw_rms_norm_backward(const void *dy, int dy_type, int lddy, const void *h, int h_type, int ldh, const void *w,
+                         int w_type, float eps, const void *dres, int lddr, int T, int H, void *dx, int lddx, float *dw,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
+/* Low-rank adapters beside a projection, a token's own each:
+ *   v_t = A[ids_t] x_t,   out_t = y_t + scaling[ids_t] B[ids_t] v_t
+ * x [T][K], A [L][R][K] and B [L][N][R] all bf16 (f16 = 0) or all fp16 (f16 = 1);
+ * ids int32 [T], a token with an id outside 0 .. L - 1 has no adapter (out_t = y_t);
+ * scaling fp32 [L] or NULL (all 1). y and out [T][N] of y_type; out may be y (the
+ * same stride). fp16 outputs saturate. v fp32 [T][R] is the call's workspace and
+ * what qw_lora_backward needs again; rows without an adapter are left as they
+ * were. Tokens need no order (those of a request stand together as a rule, which
+ * is fastest); adapters of smaller rank are padded with zeros to R. Sums in fp32,
+ * a row's bits depend on neither the batch nor its place in it; an infinity or a
+ * NaN in a token's row or its adapter does not reach other tokens (in its own the
+ * result may be NaN where the sum is infinite).
+ * K, N, R multiples of 8, R at most 128, K and N at most 2^20, L at most 4096; strides ldx, ldy,
+ * ldo multiples of 8 elements (4 in fp32); x, A, B, v, y and out 16-byte aligned. */
+int qw_lora(const void *x, int ldx, int f16, const void *A, const void *B, const int32_t *ids, const float *scaling,
+            int T, int K, int N, int R, int L, float *v, const void *y, int ldy, void *out, int ldo, int y_type,
+            void *stream);
+
+/* The gradients of qw_lora from dy [T][N] of x's type, with v as qw_lora left it:
+ *   dv_t = B[ids_t]^T dy_t (fp32),  dx_out_t = dx_t + scaling A[ids_t]^T dv_t
+ *   dA[l] = scaling[l] sum_t dv_t x_t^T,  dB[l] = scaling[l] sum_t dy_t v_t^T   over the tokens of adapter l
+ * dx [T][K] of x's type is the gradient through the shared projection; dx_out may
+ * be dx (the same stride); both NULL: not wanted. dA fp32 [L][R][K] and dB fp32
+ * [L][N][R] are written whole (zeros for an adapter without tokens) and may be
+ * NULL each, x is read for dA only and v for dB only. fp16 dx_out beyond +-65504
+ * becomes infinite. Sums over tokens have a fixed order. Limits as qw_lora's.
+ * workspace: qw_lora_backward_workspace_size bytes, 256-byte aligned. */
+size_t qw_lora_backward_workspace_size(int T, int K, int N, int R, int L);
+int qw_lora_backward(const void *dy, int lddy, const void *x, int ldx, int f16, const void *A, const void *B,
+                     const int32_t *ids, const float *v, const float *scaling, int T, int K, int N, int R, int L,
+                     const void *dx, int lddx, void *dx_out, int lddxo, float *dA, float *dB, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* What rows of logits [T][V] (of type, stride ld >= V, any alignment of the
+ * element) say of tokens int32 [T], all fp32 [T]:
+ *   lse = log sum_j exp(l_j),  logp = l[token] - lse (0 for a token outside 0 .. V - 1),
+ *   entropy = -sum_j p_j log p_j
+ * and, with top > 0, the top (at most 64 and V) largest logits' indices
+ * top_ids int32 [T][top] and log probabilities top_logp fp32 [T][top], largest
+ * first, ties by the lowest index. A logit of -infinity is masked: it has p = 0
+ * and adds nothing. A row of only such has lse, logp and top_logp of -infinity and
+ * entropy 0. A row with a NaN or +infinity gives NaN, and top_ids of -1.
+ * workspace: qw_logprobs_workspace_size bytes (0 from 2048 rows on), 256-byte
+ * aligned. */
+size_t qw_logprobs_workspace_size(int T, int V, int top);
+int qw_logprobs(const void *logits, int type, int ld, const int32_t *tokens, int T, int V, int top, float *logp,
+                float *entropy, float *lse, int32_t *top_ids, float *top_logp, void *workspace, size_t workspace_bytes,
+                void *stream);
+
+/* The gradient of logp and entropy, from lse and entropy as qw_logprobs gave them:
+ *   dl_j = dlogp ([j = token] - p_j) - dentropy p_j (log p_j + entropy)
+ * of the logits' type, in dlogits [T][V] of stride ldd (it may be the logits, at
+ * the same stride). dlogp, dentropy fp32 [T], either may be NULL (none; entropy is
+ * read with dentropy only); a token outside 0 .. V - 1 has no dlogp. Masked logits and rows of
+ * only such get 0; fp16 beyond +-65504 becomes infinite. */
+int qw_logprobs_backward(const void *logits, int type, int ld, const int32_t *tokens, const float *lse,
+                         const float *entropy, const float *dlogp, const float *dentropy, int T, int V, void *dlogits,
+                         int ldd, void *stream);
 
 /* Format surface (bit-exact): nibbles as bytes [N][K]; dequantised fp32
  * weights [N][K]; reference-engine word order -> checkpoint word order. */

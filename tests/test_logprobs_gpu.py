@@ -1,0 +1,185 @@
+"""qw_logprobs and qw_logprobs_backward against 64 bits."""
+import pytest
+import torch
+
+import qwq4
+import _projection_ref as ref
+from _projection_ref import TYPES, assert_close, f64
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+def make(seed, T, V, t, gpu, pad=0, off=0, kind="peaks"):
+    g = torch.Generator().manual_seed(seed)
+    l = torch.randn(T, V + pad, generator=g) * 2 - 3
+    if kind == "peaks":
+        l[torch.arange(T), torch.randint(0, V, (T,), generator=g)] += 14
+    elif kind == "masked":
+        l[torch.rand(T, V + pad, generator=g) < 0.9] = -INF
+        l[::3, V // 2:] = -INF
+    elif kind == "ties":
+        l = torch.randint(-2, 3, (T, V + pad), generator=g).float()
+        l[l == 0] = -0.0
+        l[:, ::5] += 0.0
+    elif kind == "same":
+        l[:] = 0.25
+    elif kind == "lowest":
+        l[:] = torch.finfo(TYPES[t]).min
+        l[1::2, V // 3] = 1.0
+    elif kind == "rising":
+        l = torch.arange(T * (V + pad)).view(T, V + pad).float() / (T * V) * 20
+    elif kind == "wide":
+        l *= 30
+    tokens = torch.randint(0, V, (T,), generator=g).to(torch.int32)
+    tokens[3::7] = -1
+    tokens[5::7] = V
+    flat = torch.empty(T * (V + pad) + off, dtype=TYPES[t], device=gpu)
+    flat[off:] = l.to(TYPES[t]).flatten().to(gpu)
+    return flat[off:].view(T, V + pad)[:, :V], tokens.to(gpu), g
+
+
+def check(logits, tokens, top, got):
+    (logp, ent, lse, ids, tops), (blp, bent, blse) = ref.logprobs(logits, tokens, top)
+    assert_close(got[0], logp, blp, "logp")
+    assert_close(got[1], ent, bent, "entropy")
+    assert_close(got[2], lse, blse, "lse")
+    if top:
+        assert torch.equal(got[3].cpu(), ids)
+        assert_close(got[4], tops, (blse[:, None] + 2 * ref.U * torch.where(torch.isfinite(tops), tops, 0.0).abs()), "top")
+    else:
+        assert got[3] is None and got[4] is None
+
+
+CASES = [(1, 1, 1), (1, 2, 2), (3, 7, 5), (2, 64, 64), (5, 513, 0), (1, 151936, 20), (1, 151669, 5), (4, 50257, 64),
+         (33, 32000, 8), (64, 4099, 1), (65, 8192, 3), (300, 2051, 20), (2100, 777, 4), (700, 9001, 0)]
+
+
+@pytest.mark.parametrize("T,V,top", CASES)
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_logprobs(gpu, T, V, top, t):
+    print(f"logprobs T={T} V={V} top={top} {t}", flush=True)
+    logits, tokens, _ = make(T + V, T, V, t, gpu)
+    check(logits, tokens, top, qwq4.logprobs(logits, tokens, top=top))
+
+
+@pytest.mark.parametrize("kind", ["masked", "ties", "same", "lowest", "rising", "wide"])
+@pytest.mark.parametrize("T,V", [(1, 40000), (2, 12), (70, 5000), (2100, 300)])
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_kinds_of_rows(gpu, kind, T, V, t):
+    """Masked vocabularies, ties (also of both zeros), constant rows, the type's lowest value, every value the best so
+    far: alternatives in order with ties by the lowest index."""
+    print(f"logprobs {kind} T={T} V={V} {t}", flush=True)
+    logits, tokens, _ = make(V, T, V, t, gpu, kind=kind)
+    for top in (1, 7, min(64, V)):
+        check(logits, tokens, min(top, V), qwq4.logprobs(logits, tokens, top=min(top, V)))
+
+
+@pytest.mark.parametrize("pad,off", [(0, 1), (1, 0), (3, 5), (8, 0), (8, 3)])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_strides_and_alignment(gpu, pad, off, t):
+    for T, V in ((3, 9001), (70, 1030), (2050, 77)):
+        logits, tokens, g = make(off, T, V, t, gpu, pad, off)
+        got = qwq4.logprobs(logits, tokens, top=6)
+        check(logits, tokens, 6, got)
+        dlogp, dent = torch.randn(T, generator=g).to(gpu), torch.randn(T, generator=g).to(gpu)
+        want, bound = ref.logprobs_grad(logits, tokens, got[2], got[1], dlogp, dent)
+        for other in (0, 2):  # (the gradient's rows aligned as the logits', and otherwise)
+            buf = torch.full((T, V + pad + other), 7.0, dtype=logits.dtype, device=gpu)
+            d = qwq4.logprobs_backward(logits, tokens, got[2], got[1], dlogp, dent, dlogits=buf[:, :V])
+            assert_close(d, want, bound, f"pad {pad + other}")
+            assert (buf[:, V:] == 7).all()
+
+
+@pytest.mark.parametrize("T,V", [(6, 30000), (2100, 200)])
+def test_rows_without_an_answer(gpu, T, V):
+    """Everything masked; a NaN; an infinity: each in its own row."""
+    logits, tokens, g = make(1, T, V, "f32", gpu)
+    logits, tokens = logits.contiguous(), tokens.clamp(0, V - 1)
+    logits[1] = -INF
+    logits[2, V - 1] = float("nan")
+    logits[3, 0] = INF
+    logits[4] = float("nan")
+    logits[5, 1:] = -INF
+    got = qwq4.logprobs(logits, tokens, top=5)
+    check(logits, tokens, 5, got)
+    assert got[1][1] == 0 and got[0][1] == -INF and (got[4][1] == -INF).all() and got[3][1].tolist() == [0, 1, 2, 3, 4]
+    assert got[1][5] == 0 and got[3][5].tolist() == [0, 1, 2, 3, 4] and (got[4][5, 1:] == -INF).all()
+    dlogp = torch.ones(T, device=gpu)
+    d = qwq4.logprobs_backward(logits, tokens, got[2], got[1], dlogp, dlogp)
+    assert (d[1] == 0).all() and torch.isnan(d[2]).all() and torch.isnan(d[3]).all() and torch.isfinite(d[5]).all()
+    assert torch.isfinite(d[0]).all()
+
+
+def test_bad_tokens_of_bad_rows(gpu):
+    """A token outside the vocabulary has logp 0 in any row."""
+    logits = torch.full((3, 100), -INF, device=gpu)
+    logits[1] = 1.0
+    tokens = torch.tensor([-5, 100, 2**31 - 1], dtype=torch.int32, device=gpu)
+    assert (qwq4.logprobs(logits, tokens)[0] == 0).all()
+
+
+@pytest.mark.parametrize("T,V", [(1, 1), (1, 151936), (7, 30), (33, 5001), (601, 2048), (2, 70001)])
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind", ["peaks", "masked"])
+def test_backward(gpu, T, V, t, kind):
+    print(f"logprobs_backward T={T} V={V} {t} {kind}", flush=True)
+    logits, tokens, g = make(T + V, T, V, t, gpu, kind=kind)
+    _, ent, lse, _, _ = qwq4.logprobs(logits, tokens)
+    dlogp, dent = torch.randn(T, generator=g).to(gpu), torch.randn(T, generator=g).to(gpu)
+    for a, b in ((dlogp, dent), (dlogp, None), (None, dent)):
+        d = qwq4.logprobs_backward(logits, tokens, lse, ent if b is not None else None, a, b)
+        want, bound = ref.logprobs_grad(logits, tokens, lse, ent, a, b)
+        assert_close(d, want, bound, f"{a is not None} {b is not None}")
+    same = logits.clone()
+    assert qwq4.logprobs_backward(same, tokens, lse, ent, dlogp, dent, dlogits=same) is same
+    assert torch.equal(same, qwq4.logprobs_backward(logits, tokens, lse, ent, dlogp, dent))
+
+
+def test_backward_is_the_derivative(gpu):
+    """Along random directions, against central differences in 64 bits."""
+    T, V, step = 5, 300, 1e-5
+    logits, tokens, g = make(3, T, V, "f32", gpu)
+    _, ent, lse, _, _ = qwq4.logprobs(logits, tokens)
+    dlogp, dent = torch.randn(T, generator=g).to(gpu), torch.randn(T, generator=g).to(gpu)
+    d = qwq4.logprobs_backward(logits, tokens, lse, ent, dlogp, dent)
+    (_, _, _, _, _), (_, bent, blse) = ref.logprobs(logits, tokens)
+    _, bound = ref.logprobs_grad(logits, tokens, lse, ent, dlogp, dent)
+    p = torch.exp(f64(logits) - f64(lse)[:, None])
+    size = f64(dlogp).abs()[:, None] + f64(dent).abs()[:, None] * (2 + (f64(logits) - f64(lse)[:, None]).abs() + f64(ent)[:, None])
+    # (lse and entropy are rounded: p moves by lse's error, the entropy's part by its own)
+    bound = bound + p * (size * (blse + 2.0**-20)[:, None] + f64(dent).abs()[:, None] * (bent + 2.0**-20)[:, None])
+    for seed in range(5):
+        e = torch.randn(T, V, generator=g).double()
+
+        def f(s):
+            (logp, h, *_), _ = ref.logprobs(f64(logits) + s * e, tokens)
+            return float((logp * f64(dlogp)).sum() + (h * f64(dent)).sum())
+
+        slope = (f(step) - f(-step)) / (2 * step)
+        got = float((f64(d) * e).sum())
+        limit = float(((bound + ref.U * f64(d).abs()) * e.abs()).sum()) + 1e-7 * float(size.sum())
+        assert abs(got - slope) <= limit, (got, slope, limit)
+
+
+def test_fp16_gradient_overflows(gpu):
+    logits, tokens = torch.zeros(2, 64, dtype=torch.float16, device=gpu), torch.zeros(2, dtype=torch.int32, device=gpu)
+    _, ent, lse, _, _ = qwq4.logprobs(logits, tokens)
+    d = qwq4.logprobs_backward(logits, tokens, lse, ent, torch.tensor([1e6, 1.0], device=gpu))
+    assert torch.isposinf(d[0, 0]) and torch.isfinite(d[1]).all()
+
+
+def test_offsets_past_32_bits(gpu):
+    """The last rows of more than 2^32 bytes."""
+    T, V = 20000, 60007
+    logits = torch.zeros(T, V, device=gpu)
+    few, tokens, g = make(5, 3, V, "f32", gpu)
+    logits[-3:] = few
+    tok = torch.zeros(T, dtype=torch.int32, device=gpu)
+    tok[-3:] = torch.tensor([5, V - 1, -1], dtype=torch.int32)
+    got = qwq4.logprobs(logits, tok, top=3)
+    check(logits[-3:], tok[-3:], 3, tuple(x[-3:] for x in got))
+    dlogp = torch.ones(T, device=gpu)
+    d = qwq4.logprobs_backward(logits, tok, got[2], got[1], dlogp, dlogp, dlogits=logits.clone())
+    want, bound = ref.logprobs_grad(logits[-3:], tok[-3:], got[2][-3:], got[1][-3:], dlogp[-3:], dlogp[-3:])
+    assert_close(d[-3:], want, bound)

@@ -1,0 +1,204 @@
+"""qw_lora and qw_lora_backward against 64 bits."""
+import pytest
+import torch
+
+import qwq4
+import _projection_ref as ref
+from _projection_ref import TYPES, assert_close, f64
+
+pytestmark = pytest.mark.gpu
+GUARD = 77.0
+
+
+def make(seed, T, K, N, R, L, t, gpu, kind="mixed"):
+    g = torch.Generator().manual_seed(seed)
+    dt = TYPES[t]
+    rnd = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    x, A, B = rnd(T, K), rnd(L, R, K) * K**-0.5, rnd(L, N, R) * R**-0.5
+    if kind == "runs":  # requests one after another
+        ids = torch.sort(torch.randint(-1, L, (T,), generator=g)).values
+    elif kind == "none":
+        ids = torch.full((T,), -1)
+    elif kind == "one":
+        ids = torch.full((T,), L - 1)
+    else:
+        ids = torch.randint(-1, L + 1, (T,), generator=g)
+        ids[::11] = -(2**31)
+        ids[5::13] = 2**31 - 1
+    scaling = 0.5 + torch.rand(L, generator=g)
+    to = lambda v, d=dt: v.to(d).to(gpu)  # noqa: E731
+    return to(x), to(A), to(B), ids.to(torch.int32).to(gpu), scaling.to(gpu), g
+
+
+CASES = [(1, 64, 64, 16, 1, "one"), (1, 4096, 256, 16, 8, "one"), (2, 8, 8, 8, 2, "mixed"), (15, 136, 72, 24, 3, "mixed"),
+         (16, 64, 1032, 32, 4, "runs"), (17, 520, 264, 40, 2, "mixed"), (37, 1536, 640, 16, 32, "mixed"),
+         (63, 640, 328, 64, 5, "mixed"), (64, 72, 64, 128, 3, "runs"), (65, 2560, 320, 120, 2, "mixed"),
+         (130, 256, 200, 16, 64, "mixed"), (601, 264, 520, 16, 4, "runs"), (1030, 128, 136, 8, 3, "runs"),
+         (40, 64, 64, 16, 3, "none"), (300, 4096, 64, 56, 1, "one")]
+
+
+@pytest.mark.parametrize("T,K,N,R,L,kind", CASES)
+@pytest.mark.parametrize("t,y", [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32"), ("f16", "bf16")])
+def test_lora(gpu, T, K, N, R, L, kind, t, y):
+    print(f"lora T={T} K={K} N={N} R={R} L={L} {kind} {t} {y}", flush=True)
+    x, A, B, ids, scaling, g = make(T + K + R, T, K, N, R, L, t, gpu, kind)
+    ys = torch.randn(T, N, generator=g).to(TYPES[y]).to(gpu)
+    v = torch.full((T, R), GUARD, device=gpu)
+    out = torch.full((T, N + 8), GUARD, dtype=ys.dtype, device=gpu)
+    got = qwq4.lora(x, A, B, ids, ys, scaling=scaling, out=out[:, :N], v=v)
+    wv, bv, want, bound = ref.lora(x, A, B, ids, ys, scaling)
+    has = ((ids >= 0) & (ids < L)).cpu()
+    assert_close(v[has.to(gpu)], wv[has], bv[has], "v")
+    assert (v[~has.to(gpu)] == GUARD).all()
+    assert_close(got, want, bound, "out")
+    assert torch.equal(got[~has.to(gpu)], ys[~has.to(gpu)]) and (out[:, N:] == GUARD).all()
+    same = ys.clone()
+    assert qwq4.lora(x, A, B, ids, same, scaling=scaling) is same and torch.equal(same, got)
+    ones = qwq4.lora(x, A, B, ids, ys.clone())
+    assert torch.equal(ones, qwq4.lora(x, A, B, ids, ys.clone(), scaling=torch.ones_like(scaling)))
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_rows_do_not_depend_on_the_batch(gpu, t):
+    T, K, N, R, L = 300, 1544, 392, 32, 6
+    x, A, B, ids, scaling, g = make(1, T, K, N, R, L, t, gpu)
+    for y in ("f32", t):
+        ys = torch.randn(T, N, generator=g).to(TYPES[y]).to(gpu)
+        whole = qwq4.lora(x, A, B, ids, ys, scaling=scaling, out=torch.empty_like(ys))
+        for at in ([0], [7, 8], list(range(100, 137)), list(range(299, -1, -1))):
+            i = torch.tensor(at, device=gpu)
+            part = qwq4.lora(x[i], A, B, ids[i], ys[i], scaling=scaling)
+            assert torch.equal(part, whole[i])
+
+
+def test_strided_rows(gpu):
+    T, K, N, R, L = 50, 128, 96, 16, 3
+    x, A, B, ids, scaling, g = make(2, T, K, N, R, L, "bf16", gpu)
+    wide_x, wide_y = torch.zeros(T, K + 24, dtype=x.dtype, device=gpu), torch.zeros(T, 3 * N, device=gpu)
+    wide_x[:, 8:8 + K] = x
+    wide_y[:] = torch.randn(T, 3 * N, generator=g).to(gpu)
+    before = wide_y.clone()
+    qwq4.lora(wide_x[:, 8:8 + K], A, B, ids, wide_y[:, N:2 * N], scaling=scaling)  # one slice of a fused projection
+    assert torch.equal(wide_y[:, N:2 * N], qwq4.lora(x, A, B, ids, before[:, N:2 * N].contiguous(), scaling=scaling))
+    assert torch.equal(wide_y[:, :N], before[:, :N]) and torch.equal(wide_y[:, 2 * N:], before[:, 2 * N:])
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_bad_values_stay_with_their_token(gpu, t):
+    """A NaN or an infinity in one token's row, or in the weights of its adapter, reaches no other token."""
+    T, K, N, R, L = 40, 128, 128, 16, 4
+    x, A, B, ids, scaling, g = make(3, T, K, N, R, L, t, gpu)
+    ids[:] = torch.arange(T) % 3  # (tokens of three adapters in every tile, none of the fourth)
+    for y in (t, "f32"):
+        ys = torch.randn(T, N, generator=g).to(TYPES[y]).to(gpu)
+        clean = qwq4.lora(x, A, B, ids, ys, scaling=scaling, out=torch.empty_like(ys))
+        x2, A2, B2 = x.clone(), A.clone(), B.clone()
+        x2[4, 5], x2[7, 0] = float("nan"), float("inf")
+        A2[2, 3, 9], B2[2, 11, 2], B2[3] = float("nan"), float("inf"), float("nan")
+        got = qwq4.lora(x2, A2, B2, ids, ys, scaling=scaling, out=torch.empty_like(ys))
+        good = (ids != 2) & (torch.arange(T, device=gpu) != 4) & (torch.arange(T, device=gpu) != 7)
+        assert torch.equal(got[good], clean[good]) and torch.isnan(got[4]).all()
+        dy, dx = torch.randn(T, N, generator=g).to(x.dtype).to(gpu), torch.randn(T, K, generator=g).to(x.dtype).to(gpu)
+        v = torch.zeros(T, R, device=gpu)
+        qwq4.lora(x, A, B, ids, ys.clone(), v=v)
+        want = qwq4.lora_backward(dy, x, A, B, ids, v, dx=dx, dx_out=torch.empty_like(dx))
+        back = qwq4.lora_backward(dy, x2, A2, B2, ids, v, dx=dx, dx_out=torch.empty_like(dx))
+        clean_t = ids != 2
+        assert torch.equal(back[0][clean_t], want[0][clean_t])
+        assert torch.equal(back[1][0], want[1][0]) and torch.equal(back[2][:2], want[2][:2]) and (back[1][3] == 0).all()
+
+
+def test_fp16_over_its_range(gpu):
+    """v beyond fp16's range and far below its smallest step: the product still is the sum of 64 bits."""
+    T, K, N, R, L = 33, 256, 64, 16, 2
+    x, A, B, ids, scaling, g = make(4, T, K, N, R, L, "f16", gpu, "one")
+    for by in (3000.0, 2.0**-14):
+        xs = (x.float() * by).half()
+        ys = torch.zeros(T, N, device=gpu)
+        v = torch.empty(T, R, device=gpu)
+        out = qwq4.lora(xs, A * 8 if by > 1 else A, B, ids, ys, out=torch.empty_like(ys), v=v)
+        assert by < 1 or float(v.abs().max()) > 65504
+        _, _, want, bound = ref.lora(xs, A * 8 if by > 1 else A, B, ids, ys)
+        assert_close(out, want, bound)
+    big = qwq4.lora((x.float() * 3000).half(), A * 8, B, ids, torch.zeros(T, N, dtype=torch.float16, device=gpu))
+    assert torch.isfinite(big).all() and float(big.abs().max()) == 65504
+
+
+GRAD_CASES = [(1, 64, 64, 16, 1, "one"), (2, 8, 8, 8, 2, "mixed"), (17, 520, 264, 40, 2, "mixed"),
+              (37, 640, 1032, 16, 32, "mixed"), (64, 72, 64, 128, 3, "runs"), (130, 256, 200, 24, 3, "mixed"),
+              (601, 264, 520, 64, 2, "runs"), (2500, 128, 136, 16, 3, "runs"), (40, 64, 64, 16, 3, "none"),
+              (4100, 64, 72, 8, 1, "one"), (300, 1536, 640, 16, 4, "runs")]
+
+
+@pytest.mark.parametrize("T,K,N,R,L,kind", GRAD_CASES)
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_lora_backward(gpu, T, K, N, R, L, kind, t):
+    print(f"lora_backward T={T} K={K} N={N} R={R} L={L} {kind} {t}", flush=True)
+    x, A, B, ids, scaling, g = make(T + N + R, T, K, N, R, L, t, gpu, kind)
+    dy, dx = (torch.randn(T, n, generator=g).to(x.dtype).to(gpu) for n in (N, K))
+    v = torch.full((T, R), float("nan"), device=gpu)  # (rows without an adapter are not read)
+    qwq4.lora(x, A, B, ids, torch.zeros(T, N, device=gpu), v=v)
+    out, dA, dB = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling, dx=dx, dx_out=torch.empty_like(dx))
+    (wx, bx), wA, bA, wB, bB = ref.lora_grad(dy, x, A, B, ids, torch.nan_to_num(v), scaling, dx)
+    assert_close(out, wx, bx, "dx")
+    assert_close(dA, wA, bA, "dA")
+    assert_close(dB, wB, bB, "dB")
+    same = dx.clone()
+    a, b, c = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling, dx=same, need_weights=False)
+    assert a is same and torch.equal(a, out) and b is None and c is None
+    a, b, c = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling)
+    assert a is None and torch.equal(b, dA) and torch.equal(c, dB)
+
+
+def test_one_gradient_alone(gpu):
+    """dA or dB alone through the C call, the other side's inputs not given."""
+    T, K, N, R, L = 70, 128, 648, 16, 2
+    x, A, B, ids, scaling, g = make(9, T, K, N, R, L, "bf16", gpu)
+    dy = torch.randn(T, N, generator=g).to(x.dtype).to(gpu)
+    v = torch.zeros(T, R, device=gpu)
+    qwq4.lora(x, A, B, ids, torch.zeros(T, N, device=gpu), v=v)
+    _, dA, dB = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling)
+    lib, s = qwq4.lib(), torch.cuda.current_stream().cuda_stream
+    n = qwq4.lora_backward_workspace_size(T, K, N, R, L)
+    ws, a, b = torch.empty(n, dtype=torch.uint8, device=gpu), torch.empty_like(dA), torch.empty_like(dB)
+    p = lambda t: t.data_ptr()  # noqa: E731
+    for want_a in (True, False):
+        rc = lib.qw_lora_backward(p(dy), N, p(x) if want_a else None, K, 0, p(A), p(B), p(ids), None if want_a else p(v),
+                                  p(scaling), T, K, N, R, L, None, 0, None, 0, p(a) if want_a else None,
+                                  None if want_a else p(b), p(ws), n, s)
+        assert rc == 0, lib.qw_q4_last_error()
+    assert torch.equal(a, dA) and torch.equal(b, dB)
+
+
+def test_backward_is_the_derivative(gpu):
+    """Along random directions, against central differences of the adapters in 64 bits."""
+    T, K, N, R, L, step = 21, 64, 72, 8, 2, 1e-4
+    x, A, B, ids, scaling, g = make(10, T, K, N, R, L, "bf16", gpu)
+    dy = torch.randn(T, N, generator=g).to(x.dtype).to(gpu)
+    v = torch.zeros(T, R, device=gpu)
+    y0 = torch.zeros(T, N, device=gpu)
+    qwq4.lora(x, A, B, ids, y0.clone(), v=v)
+    dx0 = torch.zeros(T, K, dtype=x.dtype, device=gpu)
+    dx, dA, dB = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling, dx=dx0)
+    (_, bx), _, bA, _, bB = ref.lora_grad(dy, x, A, B, ids, v, scaling, torch.zeros_like(dx0))
+    for seed in range(4):
+        d = [torch.randn(t.shape, generator=g).double() for t in (x, A, B)]
+        f = lambda s: float((ref.lora(*(f64(t) + s * e for t, e in zip((x, A, B), d)), ids, y0, scaling)[2] * f64(dy)).sum())  # noqa: E731
+        # (the function is a cubic along a line: the difference's error is its third coefficient times step^2)
+        slope = (f(step) - f(-step)) / (2 * step)
+        third = abs((f(1.0) - f(-1.0)) / 2 - slope)
+        got = sum(float((f64(t) * e).sum()) for t, e in zip((dx, dA, dB), d))
+        # (dx is rounded to 16 bits, the other two to fp32)
+        limit = sum(float(((b + h * f64(t).abs()) * e.abs()).sum()) for t, e, b, h in zip(
+            (dx, dA, dB), d, (bx, bA, bB), (2.0**-8, ref.U, ref.U))) + third * step**2 * 2 + 1e-8 * abs(slope)
+        assert abs(got - slope) <= limit, (got, slope, limit)
+
+
+def test_fp16_gradient_overflows(gpu):
+    T, K, N, R, L = 3, 64, 64, 16, 1
+    x, A, B, ids, scaling, g = make(11, T, K, N, R, L, "f16", gpu, "one")
+    dy = torch.zeros(T, N, dtype=torch.float16, device=gpu)
+    dy[1] = 60000
+    v = torch.zeros(T, R, device=gpu)
+    dx, dA, _ = qwq4.lora_backward(dy, x, A * 100, B * 100, ids, v, dx=torch.zeros_like(x))
+    assert torch.isinf(dx[1]).any() and (dx[0] == 0).all() and torch.isfinite(dA).all()

@@ -566,6 +566,222 @@ int qw_moe_unpermute_backward(const void *dout, int dout_type, int ldd, const vo
     return launched(fn);
 }
 
+// ---- around a projection
+// Rows of a type: a stride >= n (one row: any), elements aligned.
+static int check_plain_rows(const char *fn, const char *name, const void *p, int type, int ld, int T, int n) {
+    REQUIRE(p, "%s: null %s", fn, name);
+    REQUIRE(is_type(type), "%s: type of %s = %d (0 fp32, 1 bf16, 2 fp16)", fn, name, type);
+    REQUIRE((T == 1 || ld >= n) && aligned(p, type_bytes(type)), "%s: stride %d of %s < %d, or misaligned", fn, ld, name,
+            n);
+    return 0;
+}
+
+// An output that may be an input has that input's rows, or none of them.
+static int check_in_place(const char *fn, const char *name, const void *out, int ldo, const void *in, int ldi, int T) {
+    REQUIRE(out != in || T == 1 || ldo == ldi, "%s: %s lies on its input with another stride (%d, %d)", fn, name, ldo,
+            ldi);
+    return 0;
+}
+
+static int check_norm(const char *fn, const qwq4::NormArgs &a) {
+    REQUIRE(a.T >= 1 && a.T <= kMaxRows && a.H >= 1 && a.H <= (1 << 28), "%s: T = %d (1..%d), H = %d (1..2^28)", fn, a.T,
+            kMaxRows, a.H);
+    if (int r = check_plain_rows(fn, "x", a.x, a.x_type, int(a.ldx), a.T, a.H)) return r;
+    if (int r = check_plain_rows(fn, "w", a.w, a.w_type, a.H, 1, a.H)) return r;
+    REQUIRE(a.w_type == QW_T_F32 || a.w_type == a.x_type, "%s: w_type = %d (fp32 or x's type)", fn, a.w_type);
+    REQUIRE(a.eps >= 0.f && a.eps < 1e30f, "%s: eps = %g", fn, double(a.eps));
+    REQUIRE(!a.res == !a.res_out, "%s: residual and res_out are given together or not at all", fn);
+    if (!a.res) return 0;
+    REQUIRE(a.res_type == QW_T_F32 || a.res_type == a.x_type, "%s: res_type = %d (fp32 or x's type)", fn, a.res_type);
+    if (int r = check_plain_rows(fn, "residual", a.res, a.res_type, int(a.ldr), a.T, a.H)) return r;
+    if (int r = check_plain_rows(fn, "res_out", a.res_out, a.res_type, int(a.ldro), a.T, a.H)) return r;
+    return check_in_place(fn, "res_out", a.res_out, int(a.ldro), a.res, int(a.ldr), a.T);
+}
+
+int qw_rms_norm(const void *x, int x_type, int ldx, const void *residual, int res_type, int ldr, void *res_out,
+                int ldro, const void *w, int w_type, float eps, int T, int H, void *y, int y_type, int ldy,
+                void *stream) {
+    const char *fn = "qw_rms_norm";
+    const qwq4::NormArgs a{x,      x_type, ldx,    residual, res_type, ldr, res_out, ldro, w,
+                           w_type, y,      y_type, ldy,      nullptr,  T,   H,       eps};
+    if (int r = check_norm(fn, a)) return r;
+    if (int r = check_plain_rows(fn, "y", y, y_type, ldy, T, H)) return r;
+    REQUIRE(y != x || (y_type == x_type && (T == 1 || ldy == ldx)), "%s: y lies on x with another type or stride", fn);
+    REQUIRE(y != residual && y != res_out, "%s: y lies on the residual", fn);
+    qwq4::launch_rms_norm(a, st(stream));
+    return launched(fn);
+}
+
+int qw_rms_norm_i8(const void *x, int x_type, int ldx, const void *residual, int res_type, int ldr, void *res_out,
+                   int ldro, const void *w, int w_type, float eps, int T, int H, int8_t *q, int ldq, float *scale,
+                   void *stream) {
+    const char *fn = "qw_rms_norm_i8";
+    REQUIRE(q && scale, "%s: null q or scale", fn);
+    const qwq4::NormArgs a{x,      x_type, ldx, residual, res_type, ldr, res_out, ldro, w,
+                           w_type, q,      0,   ldq,      scale,    T,   H,       eps};
+    if (int r = check_norm(fn, a)) return r;
+    REQUIRE((T == 1 || ldq >= H) && aligned(scale, 4), "%s: ldq %d < H = %d, or scale misaligned", fn, ldq, H);
+    qwq4::launch_rms_norm(a, st(stream));
+    return launched(fn);
+}
+
+size_t qw_rms_norm_backward_workspace_size(int T, int H) {
+    return T < 1 || H < 1 ? 0 : qwq4::rms_norm_backward_workspace_bytes(T, H);
+}
+
+int qw_rms_norm_backward(const void *dy, int dy_type, int lddy, const void *h, int h_type, int ldh, const void *w,
+                         int w_type, float eps, const void *dres, int lddr, int T, int H, void *dx, int lddx, float *dw,
+                         void *workspace, size_t workspace_bytes, void *stream) {
+    const char *fn = "qw_rms_norm_backward";
+    REQUIRE(T >= 1 && T <= kMaxRows && H >= 1 && H <= 16384, "%s: T = %d (1..%d), H = %d (1..16384)", fn, T, kMaxRows, H);
+    if (int r = check_plain_rows(fn, "dy", dy, dy_type, lddy, T, H)) return r;
+    if (int r = check_plain_rows(fn, "h", h, h_type, ldh, T, H)) return r;
+    REQUIRE(h_type == QW_T_F32 || h_type == dy_type, "%s: h_type = %d (fp32 or dy's type)", fn, h_type);
+    if (int r = check_plain_rows(fn, "w", w, w_type, H, 1, H)) return r;
+    REQUIRE(w_type == QW_T_F32 || w_type == dy_type, "%s: w_type = %d (fp32 or dy's type)", fn, w_type);
+    if (dres)
+        if (int r = check_plain_rows(fn, "dres", dres, h_type, lddr, T, H)) return r;
+    if (int r = check_plain_rows(fn, "dx", dx, h_type, lddx, T, H)) return r;
+    REQUIRE(dx != dy || h_type == dy_type, "%s: dx lies on dy with another type", fn);
+    if (int r = check_in_place(fn, "dx", dx, lddx, dy, lddy, T)) return r;
+    if (int r = check_in_place(fn, "dx", dx, lddx, h, ldh, T)) return r;
+    if (int r = check_in_place(fn, "dx", dx, lddx, dres, lddr, T)) return r;
+    REQUIRE(eps >= 0.f && eps < 1e30f, "%s: eps = %g", fn, double(eps));
+    REQUIRE(aligned(dw, 4), "%s: dw misaligned", fn);
+    const size_t need = dw ? qwq4::rms_norm_backward_workspace_bytes(T, H) : 0;
+    REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 256)),
+            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", fn, need, workspace_bytes);
+    qwq4::launch_rms_norm_backward(
+        qwq4::NormGradArgs{dy, dy_type, lddy, h, h_type, ldh, w, w_type, dres, lddr, dx, lddx, dw,
+                           static_cast<float *>(workspace), T, H, eps},
+        st(stream));
+    return launched(fn);
+}
+
+// Sizes of an adapter call: the grids' bounds, and 16-byte pieces of 16-bit elements.
+static int check_lora(const char *fn, const void *A, const void *B, const int32_t *ids, const float *scaling, int T,
+                      int K, int N, int R, int L) {
+    REQUIRE(A && B && ids, "%s: null A, B or ids", fn);
+    REQUIRE(T >= 1 && T <= (1 << 20) && L >= 1 && L <= 4096, "%s: T = %d (1..2^20), L = %d (1..4096)", fn, T, L);
+    REQUIRE(K >= 8 && K % 8 == 0 && K <= (1 << 20) && N >= 8 && N % 8 == 0 && N <= (1 << 20),
+            "%s: K = %d, N = %d must be multiples of 8 up to 2^20", fn, K, N);
+    REQUIRE(R >= 8 && R % 8 == 0 && R <= 128, "%s: R = %d must be a multiple of 8 from 8 to 128", fn, R);
+    REQUIRE(int64_t(T) * (K > N ? K : N) <= (int64_t(1) << 36), "%s: T = %d rows of %d are too many for one call", fn, T,
+            K > N ? K : N);
+    REQUIRE(aligned(A, 16) && aligned(B, 16) && aligned(ids, 4) && aligned(scaling, 4),
+            "%s: A and B must be 16-byte aligned, ids and scaling 4-byte", fn);
+    return 0;
+}
+
+// Rows that are moved in 16-byte pieces.
+static int check_wide_rows(const char *fn, const char *name, const void *p, int type, int ld, int T, int n) {
+    REQUIRE(p, "%s: null %s", fn, name);
+    const int e = 16 / int(type_bytes(type));
+    REQUIRE(aligned(p, 16) && (T == 1 || (ld >= n && ld % e == 0)),
+            "%s: stride %d of %s must be >= %d and a multiple of %d, the rows 16-byte aligned", fn, ld, name, n, e);
+    return 0;
+}
+
+int qw_lora(const void *x, int ldx, int f16, const void *A, const void *B, const int32_t *ids, const float *scaling,
+            int T, int K, int N, int R, int L, float *v, const void *y, int ldy, void *out, int ldo, int y_type,
+            void *stream) {
+    const char *fn = "qw_lora";
+    if (int r = check_lora(fn, A, B, ids, scaling, T, K, N, R, L)) return r;
+    REQUIRE(is_type(y_type), "%s: y_type = %d (0 fp32, 1 bf16, 2 fp16)", fn, y_type);
+    if (int r = check_wide_rows(fn, "x", x, QW_T_BF16, ldx, T, K)) return r;
+    if (int r = check_wide_rows(fn, "v", v, QW_T_F32, R, T, R)) return r;
+    if (int r = check_wide_rows(fn, "y", y, y_type, ldy, T, N)) return r;
+    if (int r = check_wide_rows(fn, "out", out, y_type, ldo, T, N)) return r;
+    if (int r = check_in_place(fn, "out", out, ldo, y, ldy, T)) return r;
+    qwq4::launch_lora_shrink(qwq4::LoraShrinkArgs{static_cast<const uint16_t *>(x), ldx,
+                                                  static_cast<const uint16_t *>(A), ids, T, K, R, L, v, f16 != 0},
+                             st(stream));
+    qwq4::launch_lora_expand(qwq4::LoraExpandArgs{v, static_cast<const uint16_t *>(B), ids, scaling, T, N, R, L,
+                                                  f16 != 0, y, ldy, out, ldo, y_type, false},
+                             st(stream));
+    return launched(fn);
+}
+
+size_t qw_lora_backward_workspace_size(int T, int K, int N, int R, int L) {
+    return T < 1 || K < 8 || N < 8 || R < 8 || L < 1 ? 0 : qwq4::lora_backward_workspace_bytes(T, K, N, R, L);
+}
+
+int qw_lora_backward(const void *dy, int lddy, const void *x, int ldx, int f16, const void *A, const void *B,
+                     const int32_t *ids, const float *v, const float *scaling, int T, int K, int N, int R, int L,
+                     const void *dx, int lddx, void *dx_out, int lddxo, float *dA, float *dB, void *workspace,
+                     size_t workspace_bytes, void *stream) {
+    const char *fn = "qw_lora_backward";
+    if (int r = check_lora(fn, A, B, ids, scaling, T, K, N, R, L)) return r;
+    REQUIRE(!dx == !dx_out && (dx || dA || dB), "%s: dx and dx_out are given together; dx, dA or dB has to be asked for",
+            fn);
+    if (int r = check_wide_rows(fn, "dy", dy, QW_T_BF16, lddy, T, N)) return r;
+    if (dA)
+        if (int r = check_wide_rows(fn, "x", x, QW_T_BF16, ldx, T, K)) return r;
+    if (dB)
+        if (int r = check_wide_rows(fn, "v", v, QW_T_F32, R, T, R)) return r;
+    if (dx) {
+        if (int r = check_wide_rows(fn, "dx", dx, QW_T_BF16, lddx, T, K)) return r;
+        if (int r = check_wide_rows(fn, "dx_out", dx_out, QW_T_BF16, lddxo, T, K)) return r;
+        if (int r = check_in_place(fn, "dx_out", dx_out, lddxo, dx, lddx, T)) return r;
+    }
+    REQUIRE(aligned(dA, 16) && aligned(dB, 16), "%s: dA and dB must be 16-byte aligned", fn);
+    const size_t need = qwq4::lora_backward_workspace_bytes(T, K, N, R, L);
+    REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 256),
+            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", fn, need, workspace_bytes);
+    qwq4::launch_lora_backward(
+        qwq4::LoraGradArgs{static_cast<const uint16_t *>(dy), lddy, static_cast<const uint16_t *>(x), ldx,
+                           static_cast<const uint16_t *>(A), static_cast<const uint16_t *>(B), ids, v, scaling, T, K, N,
+                           R, L, f16 != 0, dx, lddx, dx_out, lddxo, dA, dB},
+        workspace, st(stream));
+    return launched(fn);
+}
+
+size_t qw_logprobs_workspace_size(int T, int V, int top) {
+    return T < 1 || V < 1 || top < 0 ? 0 : qwq4::logprobs_workspace_bytes(T, V, top);
+}
+
+static int check_logits(const char *fn, const void *logits, int type, int ld, const int32_t *tokens, int T, int V) {
+    REQUIRE(T >= 1 && T <= kMaxRows && V >= 1 && V <= (1 << 28), "%s: T = %d (1..%d), V = %d (1..2^28)", fn, T, kMaxRows,
+            V);
+    REQUIRE(tokens && aligned(tokens, 4), "%s: tokens null or misaligned", fn);
+    return check_plain_rows(fn, "logits", logits, type, ld, T, V);
+}
+
+int qw_logprobs(const void *logits, int type, int ld, const int32_t *tokens, int T, int V, int top, float *logp,
+                float *entropy, float *lse, int32_t *top_ids, float *top_logp, void *workspace, size_t workspace_bytes,
+                void *stream) {
+    const char *fn = "qw_logprobs";
+    if (int r = check_logits(fn, logits, type, ld, tokens, T, V)) return r;
+    REQUIRE(top >= 0 && top <= 64 && top <= V, "%s: top = %d (0..64, at most V = %d)", fn, top, V);
+    REQUIRE(logp && entropy && lse && (!top || (top_ids && top_logp)), "%s: null output", fn);
+    REQUIRE(aligned(logp, 4) && aligned(entropy, 4) && aligned(lse, 4) && aligned(top_ids, 4) && aligned(top_logp, 4),
+            "%s: misaligned output", fn);
+    const size_t need = qwq4::logprobs_workspace_bytes(T, V, top);
+    REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 256)),
+            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", fn, need, workspace_bytes);
+    qwq4::LogprobArgs a{};
+    a.logits = logits, a.type = type, a.ld = ld, a.tokens = tokens, a.T = T, a.V = V, a.top = top;
+    a.logp = logp, a.entropy = entropy, a.lse = lse, a.top_i = top_ids, a.top_v = top_logp;
+    qwq4::launch_logprobs(a, workspace, st(stream));
+    return launched(fn);
+}
+
+int qw_logprobs_backward(const void *logits, int type, int ld, const int32_t *tokens, const float *lse,
+                         const float *entropy, const float *dlogp, const float *dentropy, int T, int V, void *dlogits,
+                         int ldd, void *stream) {
+    const char *fn = "qw_logprobs_backward";
+    if (int r = check_logits(fn, logits, type, ld, tokens, T, V)) return r;
+    if (int r = check_plain_rows(fn, "dlogits", dlogits, type, ldd, T, V)) return r;
+    if (int r = check_in_place(fn, "dlogits", dlogits, ldd, logits, ld, T)) return r;
+    REQUIRE(lse && (dlogp || dentropy) && (entropy || !dentropy),
+            "%s: null pointer (lse; dlogp or dentropy; entropy with dentropy)", fn);
+    REQUIRE(aligned(lse, 4) && aligned(entropy, 4) && aligned(dlogp, 4) && aligned(dentropy, 4), "%s: misaligned input",
+            fn);
+    qwq4::launch_logprobs_backward(
+        qwq4::LogprobGradArgs{logits, type, ld, tokens, lse, entropy, dlogp, dentropy, T, V, dlogits, ldd}, st(stream));
+    return launched(fn);
+}
+
 void qw_q4_tiled_size(int64_t N, int64_t K, size_t *wt_bytes, size_t *st_bytes, size_t *zt_bytes) {
     const int64_t G = K / 128, GC = (G + 3) / 4;
     if (wt_bytes) *wt_bytes = size_t(N) * size_t(K) / 2;

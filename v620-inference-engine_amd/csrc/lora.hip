@@ -1,0 +1,560 @@
+// Low-rank adapters of many requests beside a projection that all share, and
+// their gradients.
+//
+//   v_t = A[id_t] x_t                              shrink: [R][K] x [K]
+//   y_t += scaling[id_t] B[id_t] v_t               expand: [N][R] x [R]
+//   dv_t = B[id_t]^T dy_t                          shrink, with B transposed
+//   dx_t += scaling[id_t] A[id_t]^T dv_t           expand, with A transposed
+//   dA[l] = scaling[l] sum_t dv_t x_t^T,  dB[l] = scaling[l] sum_t dy_t v_t^T     over the tokens of adapter l
+//
+// A token with an id outside 0 .. L - 1 has no adapter. Tokens need no order:
+// a tile of tokens is taken once for each adapter in it, with the others'
+// results dropped, so a batch of long requests pays one product per tile and
+// a batch of single tokens reads each adapter's weights where it has to
+// anyway. All products run on the 16-bit MFMA with sums in fp32. v is kept in
+// fp32; where it meets 16-bit weights again it goes in as two (16-bit outputs)
+// or three (fp32 outputs) 16-bit parts whose sum it is, to 2^-17 or exactly:
+// with ranks of tens the added products cost less than the rows' traffic.
+#include <algorithm>
+
+#include "q4_kernels.hpp"
+#include "row_io.cuh"
+
+namespace qwq4 {
+
+// fp32 pairs -> 16-bit pairs (nearest even) and back
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const f32x2 f = {a, b};
+    if constexpr (__is_same(T, BF16)) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, f16x2));
+}
+template <class T>
+__device__ __forceinline__ void unpack2(uint32_t w, float &a, float &b) {
+    if constexpr (__is_same(T, BF16)) {
+        a = __builtin_bit_cast(float, w << 16);
+        b = __builtin_bit_cast(float, w & 0xffff0000u);
+    } else {
+        a = f16_bits_to_f32(uint16_t(w));
+        b = f16_bits_to_f32(uint16_t(w >> 16));
+    }
+}
+
+// 8 fp32 values as PARTS operands of 8 16-bit values that add up to them.
+template <class T, int PARTS>
+__device__ __forceinline__ void split8(const float (&f)[8], uint4 (&part)[PARTS]) {
+    float r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = f[j];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            w[j] = pack2<T>(r[2 * j], r[2 * j + 1]);
+            if (p + 1 < PARTS) {
+                float a, b;
+                unpack2<T>(w[j], a, b);
+                r[2 * j] -= a;
+                r[2 * j + 1] -= b;
+            }
+        }
+        part[p] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+__device__ __forceinline__ void load8(const float *p, float (&f)[8]) {
+    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
+    f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+}
+
+// The adapters among a wave's tokens (lane i: token i's, or -1), every `of`-th
+// from `from` on: f(adapter, mask of its tokens). The same in every wave that
+// asks for the same tokens.
+template <class F>
+__device__ __forceinline__ void each_adapter(int id, int from, int of, F f) {
+    unsigned long long left = __ballot(id >= 0);
+    for (int j = 0; left; ++j) {
+        const int a = __builtin_amdgcn_readlane(id, __builtin_ctzll(left));
+        const unsigned long long mine = __ballot(id == a);
+        left &= ~mine;
+        if (j % of == from) f(a, mine);
+    }
+}
+
+__device__ __forceinline__ int adapter_of(const int32_t *ids, int t, int T, int L) {
+    if (t >= T) return -1;
+    const int id = ids[t];
+    return id >= 0 && id < L ? id : -1;
+}
+
+// ------------------------------------------------------------ shrink
+// v[t][r] = sum_k A[id_t][r][k] x[t][k] for 16 tokens by a block whose 8 waves
+// split K in 64-wide steps and join their sums in LDS, in order: a row's bits
+// depend on neither the batch nor its place in it. RF: 16-row pieces of A.
+template <class T16, int RF>
+__global__ __launch_bounds__(512) void lora_shrink_kernel(LoraShrinkArgs a) {
+    constexpr int NW = 8, U = RF == 1 ? 4 : RF == 2 ? 2 : 1;
+    __shared__ f32x4 s_part[NW][RF][WAVE];
+    const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
+    const int c = lane % 16, g = lane / 16, t0 = int(blockIdx.x) * 16, t = min(t0 + c, a.T - 1);
+    const int id = lane < 16 ? adapter_of(a.ids, t0 + lane, a.T, a.L) : -1;
+    const int steps = (a.K + 63) / 64;
+    const uint16_t *x = a.x + int64_t(t) * a.ldx + 16 * g;
+    each_adapter(id, int(blockIdx.y), int(gridDim.y), [&](int l, unsigned long long mine) {
+        const uint16_t *w[RF];
+#pragma unroll
+        for (int f = 0; f < RF; ++f)
+            w[f] = a.A + (int64_t(l) * a.R + min(16 * f + c, a.R - 1)) * a.K + 16 * g;
+        f32x4 acc[RF];
+#pragma unroll
+        for (int f = 0; f < RF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int s0 = wave; s0 < steps; s0 += NW * U) {
+            uint4 xf[U][2], wf[U][RF][2];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int k = (s0 + NW * u) * 64 + 8 * h;
+                    const bool in = k + 16 * g < a.K;  // (K is a multiple of 8)
+                    xf[u][h] = in ? *reinterpret_cast<const uint4 *>(x + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int f = 0; f < RF; ++f)
+                        wf[u][f][h] = in ? *reinterpret_cast<const uint4 *>(w[f] + k) : make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int f = 0; f < RF; ++f) acc[f] = mfma16<T16>(wf[u][f][h], xf[u][h], acc[f]);
+        }
+#pragma unroll
+        for (int f = 0; f < RF; ++f) s_part[wave][f][lane] = acc[f];
+        __syncthreads();
+        const int f = wave, r = 16 * f + 4 * g;  // (a wave adds a piece: RF <= 8)
+        if (f < RF && r < a.R && ((mine >> c) & 1)) {
+            f32x4 sum = s_part[0][f][lane];
+#pragma unroll
+            for (int i = 1; i < NW; ++i) sum += s_part[i][f][lane];
+            *reinterpret_cast<f32x4 *>(a.v + int64_t(t) * a.R + r) = sum;
+        }
+        __syncthreads();
+    });
+}
+
+void launch_lora_shrink(const LoraShrinkArgs &a, hipStream_t s) {
+    const int tiles = (a.T + 15) / 16;
+    // Adapters of a tile in parallel while there are few tiles (37 requests with an adapter each: every block takes
+    // one), all of a tile's by one block where the tiles fill the chip.
+    const int side = std::max(1, std::min({512 / tiles, 16, a.L, a.T}));
+    auto run = [&](auto t16, auto rf) {
+        lora_shrink_kernel<decltype(t16), decltype(rf)::value>
+            <<<dim3(unsigned(tiles), unsigned(side)), 512, 0, s>>>(a);
+    };
+    auto by_rank = [&](auto t16) {
+        if (a.R <= 16) run(t16, Int<1>{});
+        else if (a.R <= 32) run(t16, Int<2>{});
+        else if (a.R <= 64) run(t16, Int<4>{});
+        else run(t16, Int<8>{});
+    };
+    if (a.f16) by_rank(F16{});
+    else by_rank(BF16{});
+}
+
+// ------------------------------------------------------------ expand
+// out[t][n] = y[t][n] + scaling[id_t] sum_r B[id_t][n][r] v[t][r]: 16 NT tokens by
+// 64 columns a wave. The MFMA's rows are columns of y, dealt so that a lane
+// holds 16 neighbouring ones of a token (16-byte loads and stores; a row's 64
+// are written whole by its four lanes). K of the MFMA runs over the R values
+// of each of v's parts in turn. fp16 parts are of v times a power of two per
+// token, so that none of them overflows or loses bits to the range.
+template <class T16, int YT>
+__global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
+    constexpr bool HALF = __is_same(T16, F16);
+    constexpr int PARTS = YT == 0 ? 3 : 2, NT = YT == 0 ? 2 : 4;
+    const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
+    const int c = lane % 16, g = lane / 16;
+    const int t0 = int(blockIdx.y) * (16 * NT), n0 = (int(blockIdx.x) * 4 + wave) * 64;
+    if (n0 >= a.N) return;  // (no barrier below)
+    const int id = lane < 16 * NT ? adapter_of(a.ids, t0 + lane, a.T, a.L) : -1;
+    const int octets = a.R / 8, steps = (PARTS * octets + 3) / 4;
+    const int at = n0 + 16 * g;  // the lane's columns of y
+    if (a.out != a.y && blockIdx.z == 0) {  // (rows without an adapter)
+        const unsigned long long none = ~__ballot(id >= 0);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int t = t0 + 16 * i + c;
+            if (t >= a.T || !((none >> (16 * i + c)) & 1)) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (at + 8 * h < a.N) {
+                    float f[8];
+                    row_load<YT == GRAD_F16 ? 2 : YT, 8>(a.y, t * a.ldy + at + 8 * h, f);
+                    row_store<YT, 8>(a.out, t * a.ldo + at + 8 * h, f);
+                }
+        }
+    }
+    each_adapter(id, int(blockIdx.z), int(gridDim.z), [&](int l, unsigned long long mine) {
+        const float scale = a.scaling ? a.scaling[l] : 1.f;
+        float y[NT][2][8];
+        f32x4 acc[NT][4];
+        int shift[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            const int t = t0 + 16 * i + c;
+            const bool own = (mine >> (16 * i + c)) & 1;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (own && at + 8 * h < a.N) row_load<YT == GRAD_F16 ? 2 : YT, 8>(a.y, t * a.ldy + at + 8 * h, y[i][h]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (HALF) {
+                float top = 0.f;
+                for (int o = g; own && o < octets; o += 4) {
+                    float f[8];
+                    load8(a.v + int64_t(t) * a.R + 8 * o, f);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j] * scale));
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                // (2^shift top below 2^15)
+                shift[i] = 141 - int((__builtin_bit_cast(uint32_t, top) >> 23) & 255u);
+            }
+        }
+        const uint16_t *w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int n = min(n0 + 16 * (c / 4) + 4 * j + c % 4, a.N - 1);
+            w[j] = a.B + (int64_t(l) * a.N + n) * a.R;
+        }
+        for (int q = 0; q < steps; ++q) {
+            const int o = 4 * q + g, p = o / octets, ro = p < PARTS ? o - p * octets : 0;
+            uint4 wf[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wf[j] = *reinterpret_cast<const uint4 *>(w[j] + 8 * ro);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                if (!((mine >> (16 * i)) & 0xffffu)) continue;
+                const int t = t0 + 16 * i + c;
+                float f[8] = {};
+                if (((mine >> (16 * i + c)) & 1) && p < PARTS) {
+                    load8(a.v + int64_t(t) * a.R + 8 * ro, f);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        f[j] *= scale;
+                        if constexpr (HALF) f[j] = __builtin_ldexpf(f[j], shift[i]);
+                    }
+                }
+                uint4 part[PARTS];
+                split8<T16, PARTS>(f, part);
+                uint4 vf = part[0];
+                if (p == 1) vf = part[1];
+                if constexpr (PARTS == 3) {
+                    if (p == 2) vf = part[2];
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = mfma16<T16>(wf[j], vf, acc[i][j]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            if (!((mine >> (16 * i + c)) & 1)) continue;
+            const int64_t row = int64_t(t0 + 16 * i + c) * a.ldo;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (at + 8 * h >= a.N) continue;
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float d = acc[i][2 * h + j / 4][j % 4];
+                    if constexpr (HALF) d = __builtin_ldexpf(d, -shift[i]);
+                    f[j] = y[i][h][j] + d;
+                }
+                row_store<YT, 8>(a.out, row + at + 8 * h, f);
+            }
+        }
+    });
+}
+
+void launch_lora_expand(const LoraExpandArgs &a, hipStream_t s) {
+    auto run = [&](auto t16, auto yt) {
+        constexpr int YT = decltype(yt)::value, GROUP = YT == 0 ? 32 : 64;
+        const int groups = (a.T + GROUP - 1) / GROUP, cols = (a.N + 255) / 256;
+        const int side = std::max(1, std::min({1024 / (groups * cols), GROUP, a.L, a.T}));
+        lora_expand_kernel<decltype(t16), YT>
+            <<<dim3(unsigned(cols), unsigned(groups), unsigned(side)), 256, 0, s>>>(a);
+    };
+    auto by_16 = [&](auto yt) {
+        if (a.f16) run(F16{}, yt);
+        else run(BF16{}, yt);
+    };
+    if (a.y_type == 2 && a.grad) by_16(Int<GRAD_F16>{});
+    else by_type(a.y_type, by_16);
+}
+
+// ------------------------------------------------------------ gradients
+// out[l][c][r] = in[l][r][c] of 16-bit elements, 64 x 64 a block; two such
+// problems in one launch. Rows and columns are multiples of 8.
+__global__ __launch_bounds__(256) void lora_transpose_kernel(LoraTransposeArgs a0, LoraTransposeArgs a1) {
+    __shared__ __align__(16) uint16_t s[64][72];
+    int b = int(blockIdx.x);
+    const int n0 = a0.blocks();
+    const LoraTransposeArgs a = b < n0 ? a0 : a1;
+    if (b >= n0) b -= n0;
+    const int rt = (a.rows + 63) / 64, ct = (a.cols + 63) / 64;
+    const int64_t l = b / (rt * ct), base = l * a.rows * a.cols;
+    const int r0 = b % (rt * ct) / ct * 64, c0 = b % ct * 64;
+    const int q = int(threadIdx.x) % 8 * 8, p = int(threadIdx.x) / 8;  // 8 elements of row p (+ 32)
+#pragma unroll
+    for (int i = 0; i < 64; i += 32) {
+        if (r0 + p + i < a.rows && c0 + q < a.cols) {
+            const Halves<8> e = __builtin_bit_cast(
+                Halves<8>, *reinterpret_cast<const uint4 *>(a.in + base + int64_t(r0 + p + i) * a.cols + c0 + q));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s[p + i][q + j] = e.h[j];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 64; i += 32) {
+        if (c0 + p + i < a.cols && r0 + q < a.rows) {
+            Halves<8> e;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e.h[j] = s[q + j][p + i];
+            *reinterpret_cast<uint4 *>(a.out + base + int64_t(c0 + p + i) * a.rows + r0 + q) =
+                __builtin_bit_cast(uint4, e);
+        }
+    }
+}
+
+constexpr int OUTER_COLS = 512, OUTER_TOKENS = 2048;  // of a block: columns, tokens whose ids it looks at
+
+// G[r][c] = scaling sum_t u[t][r] m[t][c] over the tokens of one adapter in one
+// part of the batch: 128 columns a wave, 16 RF ranks. The tokens are listed in
+// LDS in order. The sum runs over tokens, whose values lie a row apart: a lane
+// loads 8 columns of 8 tokens and turns them in registers (v_perm) into 8
+// operands of one column each, so the wide rows come in 16-byte loads and
+// never pass through LDS. u goes in as three bf16 parts (exact), fp16 rows as
+// two (exact; fp16 products of unscaled sums would overflow).
+template <class T16, int RF>
+__global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
+    constexpr bool HALF = __is_same(T16, F16);
+    __shared__ int s_tok[OUTER_TOKENS];
+    __shared__ int s_count[4];
+    const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
+    const int c = lane % 16, g = lane / 16;
+    const int part = int(blockIdx.z), l = int(blockIdx.y) % a.L, r0 = int(blockIdx.y) / a.L * (16 * RF);
+    const bool second = int(blockIdx.x) >= a.m[0].blocks();
+    const LoraOuterSide &m = a.m[second];
+    const int c0 = (int(blockIdx.x) - (second ? a.m[0].blocks() : 0)) * OUTER_COLS + wave * 128;
+
+    int n = 0;
+    const int from = part * a.per, to = min(a.T, from + a.per);
+    for (int b = from; b < to; b += 256) {
+        const int t = b + int(threadIdx.x);
+        const bool mine = t < to && a.ids[t] == l;
+        const unsigned long long which = __ballot(mine);
+        if (lane == 0) s_count[wave] = __popcll(which);
+        __syncthreads();
+        int before = n;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            before += w < wave ? s_count[w] : 0;
+            n += s_count[w];
+        }
+        if (mine) s_tok[before + __popcll(which & ((1ull << lane) - 1ull))] = t;
+        __syncthreads();
+    }
+    if (a.parts > 1 && blockIdx.x == 0 && r0 == 0 && threadIdx.x == 0) a.count[part * a.L + l] = n;
+    if (n == 0 && a.parts > 1) return;  // (the joining launch goes by the count)
+    if (c0 >= m.C) return;              // (no barrier below)
+
+    const uint16_t *col = m.m + min(c0 + 8 * c, m.C - 8);
+    const int steps = (n + 31) / 32;
+    f32x4 acc[RF][8];
+#pragma unroll
+    for (int f = 0; f < RF; ++f)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    uint4 next[8];
+    float nu[RF][8];
+    auto load = [&](int s) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int p = 32 * s + 8 * g + e;
+            const int64_t t = s_tok[min(p, n - 1)];
+            const bool in = p < n;
+            next[e] = in ? *reinterpret_cast<const uint4 *>(col + t * m.ldm) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int f = 0; f < RF; ++f) nu[f][e] = in ? m.u[t * a.R + min(r0 + 16 * f + c, a.R - 1)] : 0.f;
+        }
+    };
+    if (steps > 0) load(0);
+    for (int s = 0; s < steps; ++s) {
+        uint32_t d[8][4];
+        uint4 part[RF][3];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e][0] = next[e].x, d[e][1] = next[e].y, d[e][2] = next[e].z, d[e][3] = next[e].w;
+#pragma unroll
+        for (int f = 0; f < RF; ++f) split8<BF16, 3>(nu[f], part[f]);
+        if (s + 1 < steps) load(s + 1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t w[4];  // column j of the 8 tokens
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                w[e] = __builtin_amdgcn_perm(d[2 * e + 1][j / 2], d[2 * e][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+            if constexpr (HALF) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) unpack2<F16>(w[e], v[2 * e], v[2 * e + 1]);
+                uint4 h[2];
+                split8<BF16, 2>(v, h);
+#pragma unroll
+                for (int f = 0; f < RF; ++f) {
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) acc[f][j] = mfma16<BF16>(part[f][p], h[0], acc[f][j]);
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) acc[f][j] = mfma16<BF16>(part[f][p], h[1], acc[f][j]);
+                }
+            } else {
+                const uint4 h = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                for (int f = 0; f < RF; ++f)
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) acc[f][j] = mfma16<BF16>(part[f][p], h, acc[f][j]);
+            }
+        }
+    }
+
+    if (c0 + 8 * c >= m.C) return;
+    const float scale = a.scaling ? a.scaling[l] : 1.f;
+    float *out = m.out + (int64_t(part) * a.L + l) * a.R * m.C;
+#pragma unroll
+    for (int f = 0; f < RF; ++f) {
+        const int r = r0 + 16 * f + 4 * g;
+        if (r >= a.R) continue;
+        if (m.by_column) {  // [C][R]
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                *reinterpret_cast<f32x4 *>(out + int64_t(c0 + 8 * c + j) * a.R + r) = acc[f][j] * scale;
+        } else {  // [R][C]
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float *p = out + int64_t(r + i) * m.C + c0 + 8 * c;
+#pragma unroll
+                for (int j = 0; j < 8; j += 4)
+                    *reinterpret_cast<f32x4 *>(p + j) = f32x4{acc[f][j][i], acc[f][j + 1][i], acc[f][j + 2][i], acc[f][j + 3][i]} * scale;
+            }
+        }
+    }
+}
+
+// out[l] = the parts of adapter l that have tokens, in order (none: zeros).
+__global__ __launch_bounds__(256) void lora_outer_join_kernel(LoraOuterArgs a, float *dA, float *dB) {
+    const int l = int(blockIdx.y);
+    const int64_t i = (int64_t(blockIdx.x) * 256 + int(threadIdx.x)) * 4;
+    const int64_t n0 = dA ? int64_t(a.R) * a.m[0].C : 0;
+    const bool second = i >= n0;
+    float *out = second ? dB : dA;
+    const LoraOuterSide &m = a.m[second];
+    const int64_t at = second ? i - n0 : i, each = int64_t(a.R) * m.C;
+    if (!out || at >= each) return;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < a.parts; ++p)
+        if (a.count[p * a.L + l])
+            sum += *reinterpret_cast<const f32x4 *>(m.out + (int64_t(p) * a.L + l) * each + at);
+    *reinterpret_cast<f32x4 *>(out + l * each + at) = sum;
+}
+
+// Parts of the batch whose sums over tokens run side by side: until about 2048
+// blocks are there (a block whose adapter has no token in its part ends at
+// once), of at most OUTER_TOKENS tokens each.
+static int outer_ranks(int R) { return R <= 16 ? 16 : 32; }
+static int outer_parts(int T, int K, int N, int R, int L) {
+    const int ranks = outer_ranks(R);
+    const int64_t blocks = int64_t((K + OUTER_COLS - 1) / OUTER_COLS + (N + OUTER_COLS - 1) / OUTER_COLS) *
+                           ((R + ranks - 1) / ranks) * L;
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((2048 + blocks - 1) / blocks, (T + 127) / 128));
+    return int(std::max<int64_t>(want, (T + OUTER_TOKENS - 1) / OUTER_TOKENS));
+}
+
+// Workspace of the gradients: B and A transposed, dv, and the parts of dA and
+// dB with their counts, each at a multiple of 256 bytes.
+struct LoraSpace {
+    size_t bt, at, dv, pa, pb, count, bytes;
+    LoraSpace(int T, int K, int N, int R, int L, int parts) {
+        size_t end = 0;
+        auto take = [&](size_t n) {
+            const size_t at0 = end;
+            end = (end + n + 255) / 256 * 256;
+            return at0;
+        };
+        const size_t rk = size_t(L) * R * K, rn = size_t(L) * R * N;
+        bt = take(rn * 2);
+        at = take(rk * 2);
+        dv = take(size_t(T) * R * 4);
+        pa = take(parts > 1 ? rk * 4 * parts : 0);
+        pb = take(parts > 1 ? rn * 4 * parts : 0);
+        count = take(parts > 1 ? size_t(L) * parts * 4 : 0);
+        bytes = end;
+    }
+};
+
+size_t lora_backward_workspace_bytes(int T, int K, int N, int R, int L) {
+    return LoraSpace(T, K, N, R, L, outer_parts(T, K, N, R, L)).bytes;
+}
+
+void launch_lora_backward(const LoraGradArgs &a, void *ws, hipStream_t s) {
+    const int parts = outer_parts(a.T, a.K, a.N, a.R, a.L);
+    const LoraSpace at(a.T, a.K, a.N, a.R, a.L, parts);
+    char *base = static_cast<char *>(ws);
+    uint16_t *bt = reinterpret_cast<uint16_t *>(base + at.bt), *att = reinterpret_cast<uint16_t *>(base + at.at);
+    float *dv = reinterpret_cast<float *>(base + at.dv);
+    const bool need_dv = a.dx || a.dA;
+    if (need_dv) {
+        const LoraTransposeArgs tb{a.B, bt, a.L, a.N, a.R}, ta{a.A, att, a.dx ? a.L : 0, a.R, a.K};
+        lora_transpose_kernel<<<unsigned(tb.blocks() + ta.blocks()), 256, 0, s>>>(tb, ta);
+        launch_lora_shrink(LoraShrinkArgs{a.dy, a.lddy, bt, a.ids, a.T, a.N, a.R, a.L, dv, a.f16}, s);
+    }
+    if (a.dx)
+        launch_lora_expand(LoraExpandArgs{dv, att, a.ids, a.scaling, a.T, a.K, a.R, a.L, a.f16, a.dx, a.lddx, a.dx_out,
+                                          a.lddxo, a.f16 ? 2 : 1, true},
+                           s);
+    if (!a.dA && !a.dB) return;
+    float *pa = parts > 1 ? reinterpret_cast<float *>(base + at.pa) : a.dA;
+    float *pb = parts > 1 ? reinterpret_cast<float *>(base + at.pb) : a.dB;
+    LoraOuterArgs o{};
+    // (a side that is not wanted has no columns)
+    o.m[0] = LoraOuterSide{a.x, a.ldx, dv, a.dA ? a.K : 0, pa, false};
+    o.m[1] = LoraOuterSide{a.dy, a.lddy, a.v, a.dB ? a.N : 0, pb, true};
+    o.ids = a.ids;
+    o.scaling = a.scaling;
+    o.T = a.T;
+    o.R = a.R;
+    o.L = a.L;
+    o.parts = parts;
+    o.per = (a.T + parts - 1) / parts;
+    o.count = reinterpret_cast<int *>(base + at.count);
+    const int ranks = outer_ranks(a.R);
+    const dim3 grid(unsigned(o.m[0].blocks() + o.m[1].blocks()), unsigned((a.R + ranks - 1) / ranks * a.L),
+                    unsigned(parts));
+    auto run = [&](auto t16) {
+        if (ranks == 16) lora_outer_kernel<decltype(t16), 1><<<grid, 256, 0, s>>>(o);
+        else lora_outer_kernel<decltype(t16), 2><<<grid, 256, 0, s>>>(o);
+    };
+    if (a.f16) run(F16{});
+    else run(BF16{});
+    if (parts > 1) {
+        const int64_t n = int64_t(a.R) * ((a.dA ? a.K : 0) + int64_t(a.dB ? a.N : 0)) / 4;
+        lora_outer_join_kernel<<<dim3(unsigned((n + 255) / 256), unsigned(a.L)), 256, 0, s>>>(o, a.dA, a.dB);
+    }
+}
+
+}  // namespace qwq4

@@ -15,8 +15,8 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "q4_common.cuh"
 #include "q4_kernels.hpp"
+#include "row_io.cuh"
 
 namespace qwq4 {
 
@@ -160,76 +160,6 @@ void launch_permute(const void *x, int64_t ldx, int elem_bytes, int T, int topk,
     else run(uint8_t{});
 }
 
-// V consecutive elements of type TY (QW_T_*), V a vector load's worth (16
-// bytes: 4 or 8) or 1.
-template <int TY, int V>
-__device__ __forceinline__ void row_load(const void *x, int64_t i, float (&v)[V]) {
-    if constexpr (TY == 0 && V == 1) {
-        v[0] = static_cast<const float *>(x)[i];
-    } else if constexpr (TY == 0) {
-#pragma unroll
-        for (int j = 0; j < V; j += 4) {
-            const float4 f = *reinterpret_cast<const float4 *>(static_cast<const float *>(x) + i + j);
-            v[j] = f.x;
-            v[j + 1] = f.y;
-            v[j + 2] = f.z;
-            v[j + 3] = f.w;
-        }
-    } else {
-        const uint16_t *p = static_cast<const uint16_t *>(x) + i;
-        uint16_t b[V];
-        if constexpr (V == 8) *reinterpret_cast<uint4 *>(b) = *reinterpret_cast<const uint4 *>(p);
-        else if constexpr (V == 4) *reinterpret_cast<uint2 *>(b) = *reinterpret_cast<const uint2 *>(p);
-        else b[0] = p[0];
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = TY == 1 ? bf16_bits_to_f32(b[j]) : f16_bits_to_f32(b[j]);
-    }
-}
-// fp32 -> the nearest fp16, infinite beyond its range. (The value is taken as it
-// is: the compiler would otherwise join the conversion with the multiplication
-// before it, which then rounds once, and differently in 16-byte pieces and single
-// elements.)
-__device__ __forceinline__ _Float16 f32_to_f16_rne(float v) {
-    asm volatile("" : "+v"(v));
-    return _Float16(v);
-}
-
-// Finite values beyond fp16's +-65504 become those (activations), or, as type
-// GRAD_F16, infinities (gradients: a loss scaler has to see them). A flag at run
-// time would cost the forward 3% (4096 tokens of 8 choices, 4096 wide: 59.3 us
-// against 57.7).
-constexpr int GRAD_F16 = 3;
-template <int TY, int V>
-__device__ __forceinline__ void row_store(void *y, int64_t i, const float (&v)[V]) {
-    if constexpr (TY == 0 && V == 1) {
-        static_cast<float *>(y)[i] = v[0];
-    } else if constexpr (TY == 0) {
-#pragma unroll
-        for (int j = 0; j < V; j += 4)
-            *reinterpret_cast<float4 *>(static_cast<float *>(y) + i + j) =
-                make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-    } else {
-        uint16_t *p = static_cast<uint16_t *>(y) + i;
-        uint16_t b[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            b[j] = TY == 1   ? f32_to_bf16_rne(v[j])
-                   : TY == 2 ? __builtin_bit_cast(uint16_t, f32_to_f16_satfinite(v[j]))
-                             : __builtin_bit_cast(uint16_t, f32_to_f16_rne(v[j]));
-        if constexpr (V == 8) *reinterpret_cast<uint4 *>(p) = *reinterpret_cast<const uint4 *>(b);
-        else if constexpr (V == 4) *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(b);
-        else p[0] = b[0];
-    }
-}
-
-// Elements per thread: 8 of 16-bit rows or 4 of fp32 rows (16-byte loads of
-// the rows that are read k times), where every row starts on what the widest
-// of them needs, else 1.
-static bool rows_aligned(const void *p, int type, int64_t ld, int V) {
-    const int64_t z = type == 0 ? 4 : 2, a = V * z < 16 ? V * z : 16;
-    return !p || (reinterpret_cast<uintptr_t>(p) % size_t(a) == 0 && ld * z % a == 0);
-}
-
 // A thread's V columns of one token: up to 8 selections' rows requested
 // together, then added in selection order. Bound by memory: 4096 tokens of 8
 // choices, 4096 bf16 wide, take 63 us (4.8 TB/s; a large copy reaches 5.2).
@@ -266,17 +196,6 @@ __global__ __launch_bounds__(256) void unpermute_kernel(const void *__restrict__
         }
         row_store<OT, V>(out, t * ldo + j, sum);
     }
-}
-
-template <int N>
-using Int = std::integral_constant<int, N>;
-
-// f with a type code as a constant
-template <class F>
-static void by_type(int type, F f) {
-    if (type == 0) f(Int<0>{});
-    else if (type == 1) f(Int<1>{});
-    else f(Int<2>{});
 }
 
 void launch_unpermute(const void *yp, int yp_type, int64_t ldy, const int32_t *tok_slot, const float *tok_w, int T,

@@ -329,6 +329,144 @@ struct UnpermuteGradArgs {
 };
 void launch_unpermute_backward(const UnpermuteGradArgs &a, hipStream_t s);
 
+// Norm of rows, types QW_T_*; the residual's strides and type also for its sum.
+struct NormArgs {
+    const void *x;
+    int x_type;
+    int64_t ldx;
+    const void *res;  // or null
+    int res_type;     // fp32 or x's
+    int64_t ldr;
+    void *res_out;
+    int64_t ldro;
+    const void *w;
+    int w_type;  // fp32 or x's
+    void *y;     // rows of y_type, or int8 (scale not null)
+    int y_type;
+    int64_t ldy;
+    float *scale;
+    int T, H;
+    float eps;
+};
+void launch_rms_norm(const NormArgs &a, hipStream_t s);
+struct NormGradArgs {
+    const void *dy;
+    int dy_type;
+    int64_t lddy;
+    const void *h;
+    int h_type;  // of dres and dx too: fp32 or dy's
+    int64_t ldh;
+    const void *w;
+    int w_type;  // fp32 or dy's
+    const void *dres;  // or null
+    int64_t lddr;
+    void *dx;
+    int64_t lddx;
+    float *dw;    // or null
+    float *part;  // rms_norm_backward_workspace_bytes (with dw)
+    int T, H;
+    float eps;
+};
+size_t rms_norm_backward_workspace_bytes(int T, int H);
+void launch_rms_norm_backward(const NormGradArgs &a, hipStream_t s);
+
+// Low-rank adapters: 16-bit rows and weights of one type (fp16 with f16, else
+// bf16), v fp32 [T][R].
+struct LoraShrinkArgs {
+    const uint16_t *x;
+    int64_t ldx;
+    const uint16_t *A;  // [L][R][K]
+    const int32_t *ids;
+    int T, K, R, L;
+    float *v;
+    bool f16;
+};
+void launch_lora_shrink(const LoraShrinkArgs &a, hipStream_t s);
+struct LoraExpandArgs {
+    const float *v;
+    const uint16_t *B;  // [L][N][R]
+    const int32_t *ids;
+    const float *scaling;  // or null: all 1
+    int T, N, R, L;
+    bool f16;
+    const void *y;  // y and out of y_type
+    int64_t ldy;
+    void *out;
+    int64_t ldo;
+    int y_type;
+    bool grad;  // fp16 overflows to infinities (else saturates)
+};
+void launch_lora_expand(const LoraExpandArgs &a, hipStream_t s);
+struct LoraTransposeArgs {
+    const uint16_t *in;  // [L][rows][cols]
+    uint16_t *out;
+    int L, rows, cols;
+    __host__ __device__ int blocks() const { return L * ((rows + 63) / 64) * ((cols + 63) / 64); }
+};
+// One of the two products over tokens: rows m [T][C], factors u [T][R].
+struct LoraOuterSide {
+    const uint16_t *m;
+    int64_t ldm;
+    const float *u;
+    int C;
+    float *out;      // [parts][L][R][C], or [parts][L][C][R]
+    bool by_column;  // the latter
+    __host__ __device__ int blocks() const { return (C + 511) / 512; }
+};
+struct LoraOuterArgs {
+    LoraOuterSide m[2];
+    const int32_t *ids;
+    const float *scaling;
+    int T, R, L, parts, per;  // per: tokens of a part
+    int *count;               // [parts][L] tokens
+};
+struct LoraGradArgs {
+    const uint16_t *dy;
+    int64_t lddy;
+    const uint16_t *x;
+    int64_t ldx;
+    const uint16_t *A, *B;
+    const int32_t *ids;
+    const float *v, *scaling;
+    int T, K, N, R, L;
+    bool f16;
+    const void *dx;  // or null; dx_out = dx + the adapters' part
+    int64_t lddx;
+    void *dx_out;
+    int64_t lddxo;
+    float *dA, *dB;  // or null
+};
+size_t lora_backward_workspace_bytes(int T, int K, int N, int R, int L);
+void launch_lora_backward(const LoraGradArgs &a, void *ws, hipStream_t s);
+
+struct LogprobArgs {
+    const void *logits;
+    int type;
+    int64_t ld;
+    const int32_t *tokens;
+    int T, V, top;
+    float *logp, *entropy, *lse;
+    int32_t *top_i;
+    float *top_v;
+    // set by the launch:
+    int splits;
+    float *part_st, *part_v;  // [T][splits][3], [T][splits][top]
+    int *part_i;
+};
+size_t logprobs_workspace_bytes(int T, int V, int top);
+void launch_logprobs(LogprobArgs a, void *ws, hipStream_t s);
+struct LogprobGradArgs {
+    const void *logits;
+    int type;  // of dlogits too
+    int64_t ld;
+    const int32_t *tokens;
+    const float *lse, *entropy, *dlogp, *dentropy;  // either gradient may be null
+    int T, V;
+    void *dlogits;
+    int64_t ldd;
+};
+void launch_logprobs_backward(const LogprobGradArgs &a, hipStream_t s);
+
 struct GemmArgs {
     const uint32_t *W;
     const uint16_t *S;

@@ -1,0 +1,391 @@
+// Root-mean-square norm of rows, with the residual's addition in front and an
+// output in 16 bits, fp32 or int8 with a scale per row, and its gradients.
+//
+//   h = x + residual,  r = 1 / sqrt(mean(h^2) + eps),  y = h r w
+//   int8: u = h w,  c = max |u| / 127,  q = rint(u (1 / c)),  scale = r c
+//   g = dy w,  dh = r (g - h r^2 mean(g h)) + dres,  dw = sum_t dy h r
+//
+// The 8-bit values do not depend on r (it cancels in u / max |u|), so the
+// row's sum of squares and its largest |u| come out of the same pass, and q
+// does not change with the order of the sum. Sums are in fp32; h is
+// normalised as added, the residual is rounded to its own type beside it.
+#include <algorithm>
+
+#include "q4_kernels.hpp"
+#include "row_io.cuh"
+
+namespace qwq4 {
+
+// 8 elements from index j on of a row of n (VEC: n is a multiple of 8 and the
+// row starts on 16 bytes), those behind the row's end as zeros. Single elements
+// go to the same threads as vectors do: a row's bits do not depend on how it
+// lies.
+template <int TY, bool VEC>
+__device__ __forceinline__ void part_load(const void *x, int64_t row, int j, int n, float (&v)[8]) {
+    if constexpr (VEC) {
+        row_load<TY, 8>(x, row + j, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float one[1];
+            row_load<TY, 1>(x, row + min(j + e, n - 1), one);
+            v[e] = j + e < n ? one[0] : 0.f;
+        }
+    }
+}
+template <int TY, bool VEC>
+__device__ __forceinline__ void part_store(void *y, int64_t row, int j, int n, const float (&v)[8]) {
+    if constexpr (VEC) {
+        row_store<TY, 8>(y, row + j, v);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float one[1] = {v[e]};
+            if (j + e < n) row_store<TY, 1>(y, row + j + e, one);
+        }
+    }
+}
+
+// The same with a type known at run time (one for the whole launch). Stores
+// only: with three loads to choose from at run time the compiler has left
+// values undefined that the third passes by.
+template <bool VEC>
+__device__ __forceinline__ void any_store(void *y, int type, int64_t row, int j, int n, const float (&v)[8]) {
+    if (type == 0) part_store<0, VEC>(y, row, j, n, v);
+    else if (type == 1) part_store<1, VEC>(y, row, j, n, v);
+    else part_store<2, VEC>(y, row, j, n, v);
+}
+
+__device__ __forceinline__ float wave_add(float v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// 8 elements of h = x + residual (RT < 0: no residual).
+template <int XT, int RT, bool VEC>
+__device__ __forceinline__ void load_h(const NormArgs &a, int64_t x0, int64_t r0, int j, float (&h)[8]) {
+    part_load<XT, VEC>(a.x, x0, j, a.H, h);
+    if constexpr (RT >= 0) {
+        float r[8];
+        part_load<RT, VEC>(a.res, r0, j, a.H, r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] += r[e];
+    }
+}
+
+// A row by G threads (64: a wave, four rows a block; 256: the block), 8
+// elements per thread and turn. C > 0: the row is held in C turns' registers
+// and read once; C = 0: any length, read twice (the second time from the
+// caches; the residual is written then, since it may lie on its input).
+// Bound by memory.
+template <int XT, int RT, int WT, bool I8, bool VEC, int G, int C>
+__global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
+    const int li = int(threadIdx.x) % G, H = a.H;
+    const int64_t t = int64_t(blockIdx.x) * (256 / G) + int(threadIdx.x) / G;
+    if (t >= a.T) return;  // (whole waves, where G = 64: they meet no barrier)
+    const int64_t x0 = t * a.ldx, r0 = t * a.ldr, o0 = t * a.ldro, y0 = t * a.ldy;
+    float h[C > 0 ? C : 1][8], w[C > 0 ? C : 1][8];
+    float sum = 0.f;
+    uint32_t top = 0u;
+    auto count = [&](const float (&v)[8], const float (&wv)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sum = __builtin_fmaf(v[e], v[e], sum);
+            if constexpr (I8) top = max(top, __builtin_bit_cast(uint32_t, v[e] * wv[e]) & 0x7fffffffu);
+        }
+    };
+    if constexpr (C > 0) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int j = (li + c * G) * 8;
+            if (j < H) {
+                load_h<XT, RT, VEC>(a, x0, r0, j, h[c]);
+                part_load<WT, VEC>(a.w, 0, j, H, w[c]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[c][e] = w[c][e] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int j = (li + c * G) * 8;
+            if constexpr (RT >= 0) {
+                if (j < H) part_store<RT, VEC>(a.res_out, o0, j, H, h[c]);
+            }
+            count(h[c], w[c]);
+        }
+    } else {
+        for (int j = li * 8; j < H; j += G * 8) {
+            load_h<XT, RT, VEC>(a, x0, r0, j, h[0]);
+            if constexpr (I8) part_load<WT, VEC>(a.w, 0, j, H, w[0]);
+            count(h[0], w[0]);
+        }
+    }
+    sum = wave_add(sum);
+    if constexpr (I8) {
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) top = max(top, uint32_t(__shfl_xor(int(top), o)));
+    }
+    if constexpr (G == 256) {
+        __shared__ float s_sum[4];
+        __shared__ uint32_t s_top[4];
+        if (li % WAVE == 0) {
+            s_sum[li / WAVE] = sum;
+            if constexpr (I8) s_top[li / WAVE] = top;
+        }
+        __syncthreads();
+        sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+        if constexpr (I8) top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+    }
+    const float r = 1.f / sqrtf(sum / float(H) + a.eps);
+    // (as the quantiser of rows: a row of zeros has step 1, an infinity or a NaN gives a NaN scale)
+    const bool finite = top < 0x7f800000u;
+    float step = 1.f, inv = 1.f;
+    if constexpr (I8) {
+        step = !finite ? __builtin_nanf("") : top ? fmaxf(__builtin_bit_cast(float, top) / 127.f, 1.17549435e-38f) : 1.f;
+        inv = 1.f / step;
+    }
+    auto put = [&](int j, const float (&v)[8], const float (&wv)[8]) {
+        if constexpr (I8) {
+            uint32_t q[2] = {0u, 0u};
+            if (finite) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    q[e / 4] |= uint32_t(int(__builtin_rintf(v[e] * wv[e] * inv)) & 0xff) << (8 * (e % 4));
+            }
+            int8_t *p = static_cast<int8_t *>(a.y) + y0 + j;
+            if constexpr (VEC) {
+                *reinterpret_cast<uint2 *>(p) = make_uint2(q[0], q[1]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (j + e < H) p[e] = int8_t(q[e / 4] >> (8 * (e % 4)));
+            }
+        } else {
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = v[e] * r * wv[e];
+            any_store<VEC>(a.y, a.y_type, y0, j, H, o);
+        }
+    };
+    if constexpr (C > 0) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int j = (li + c * G) * 8;
+            if (j < H) put(j, h[c], w[c]);
+        }
+    } else {
+        for (int j = li * 8; j < H; j += G * 8) {
+            load_h<XT, RT, VEC>(a, x0, r0, j, h[0]);
+            part_load<WT, VEC>(a.w, 0, j, H, w[0]);
+            if constexpr (RT >= 0) part_store<RT, VEC>(a.res_out, o0, j, H, h[0]);
+            put(j, h[0], w[0]);
+        }
+    }
+    if constexpr (I8) {
+        if (li == 0) a.scale[t] = step * r;
+    }
+}
+
+template <int XT, int RT, int WT, bool I8>
+static void launch_norm(const NormArgs &a, hipStream_t s) {
+    auto run = [&](auto vec, auto g, auto c) {
+        constexpr int G = decltype(g)::value, ROWS = 256 / G;
+        rms_norm_kernel<XT, RT, WT, I8, decltype(vec)::value, G, decltype(c)::value>
+            <<<unsigned((a.T + ROWS - 1) / ROWS), 256, 0, s>>>(a);
+    };
+    auto by_length = [&](auto vec) {
+        if (a.H <= 512) run(vec, Int<64>{}, Int<1>{});
+        else if (a.H <= 2048) run(vec, Int<256>{}, Int<1>{});
+        else if (a.H <= 4096) run(vec, Int<256>{}, Int<2>{});
+        else if (a.H <= 8192) run(vec, Int<256>{}, Int<4>{});
+        else run(vec, Int<256>{}, Int<0>{});
+    };
+    const int64_t one = a.T == 1 ? 0 : 1;  // (a single row's stride does not matter)
+    const bool out = I8 ? reinterpret_cast<uintptr_t>(a.y) % 8 == 0 && one * a.ldy % 8 == 0
+                        : rows_aligned(a.y, a.y_type, one * a.ldy, 8);
+    if (a.H % 8 == 0 && out && rows_aligned(a.x, XT, one * a.ldx, 8) && rows_aligned(a.w, WT, 0, 8) &&
+        (RT < 0 || (rows_aligned(a.res, RT, one * a.ldr, 8) && rows_aligned(a.res_out, RT, one * a.ldro, 8))))
+        by_length(std::true_type{});
+    else
+        by_length(std::false_type{});
+}
+
+void launch_rms_norm(const NormArgs &a, hipStream_t s) {
+    by_type(a.x_type, [&](auto xt) {
+        constexpr int XT = decltype(xt)::value;
+        auto run = [&](auto rt, auto wt) {
+            constexpr int RT = decltype(rt)::value, WT = decltype(wt)::value;
+            if (a.scale) launch_norm<XT, RT, WT, true>(a, s);
+            else launch_norm<XT, RT, WT, false>(a, s);
+        };
+        auto by_residual = [&](auto wt) {
+            if (!a.res) run(Int<-1>{}, wt);
+            else if (a.res_type == 0) run(Int<0>{}, wt);
+            else run(xt, wt);
+        };
+        if (a.w_type == 0) by_residual(Int<0>{});
+        else by_residual(xt);
+    });
+}
+
+// ------------------------------------------------------------ gradients
+// A block of TH threads takes rows blockIdx.x, blockIdx.x + gridDim.x, .., 8
+// elements per thread and C turns each, with the next row's h and dy requested
+// before the current one's sums, and keeps its columns' part of dw in
+// registers; the blocks' parts are added in order by a second launch.
+template <int DT, int HT, int WT, bool VEC, int TH, int C>
+__global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
+    constexpr int NW = TH / WAVE;
+    __shared__ float s_sum[2][2][NW];
+    const int tid = int(threadIdx.x), H = a.H;
+    float w[C][8], dw[C][8], h[2][C][8], d[2][C][8];
+    auto load = [&](int64_t t, float (&hv)[C][8], float (&dv)[C][8]) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int j = (tid + c * TH) * 8;
+            if (j < H) {
+                part_load<HT, VEC>(a.h, t * a.ldh, j, H, hv[c]);
+                part_load<DT, VEC>(a.dy, t * a.lddy, j, H, dv[c]);
+            }
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int j = (tid + c * TH) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[c][e] = dw[c][e] = h[0][c][e] = d[0][c][e] = h[1][c][e] = d[1][c][e] = 0.f;
+        if (j < H) part_load<WT, VEC>(a.w, 0, j, H, w[c]);
+    }
+    auto row = [&](int64_t t, int p, const float (&hv)[C][8], const float (&dv)[C][8]) {
+        float res[C][8];
+        float sum = 0.f, dot = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int j = (tid + c * TH) * 8;
+            if (a.dres && j < H) part_load<HT, VEC>(a.dres, t * a.lddr, j, H, res[c]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                sum = __builtin_fmaf(hv[c][e], hv[c][e], sum);
+                dot = __builtin_fmaf(dv[c][e] * w[c][e], hv[c][e], dot);
+            }
+        }
+        sum = wave_add(sum);
+        dot = wave_add(dot);
+        if (tid % WAVE == 0) {
+            s_sum[p][0][tid / WAVE] = sum;
+            s_sum[p][1][tid / WAVE] = dot;
+        }
+        __syncthreads();  // (one per row: the next row's sums go to the other pair of lists)
+        sum = dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            sum += s_sum[p][0][i];
+            dot += s_sum[p][1][i];
+        }
+        const float r = 1.f / sqrtf(sum / float(H) + a.eps), k = r * r * (dot / float(H));
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int j = (tid + c * TH) * 8;
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                o[e] = r * (dv[c][e] * w[c][e] - hv[c][e] * k);
+                dw[c][e] = __builtin_fmaf(dv[c][e], hv[c][e] * r, dw[c][e]);
+            }
+            if (j >= H) continue;
+            if (a.dres) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] += res[c][e];
+            }
+            part_store<HT == 2 ? GRAD_F16 : HT, VEC>(a.dx, t * a.lddx, j, H, o);
+        }
+    };
+    int64_t t = blockIdx.x;
+    const int64_t step = gridDim.x;
+    if (t < a.T) load(t, h[0], d[0]);
+    for (; t < a.T; t += 2 * step) {
+        if (t + step < a.T) load(t + step, h[1], d[1]);
+        row(t, 0, h[0], d[0]);
+        if (t + step >= a.T) break;
+        if (t + 2 * step < a.T) load(t + 2 * step, h[0], d[0]);
+        row(t + step, 1, h[1], d[1]);
+    }
+    if (!a.dw) return;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int j = (tid + c * TH) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (j + e < H) a.part[int64_t(blockIdx.x) * H + j + e] = dw[c][e];
+    }
+}
+
+// dw[j] = the blocks' parts in order: 64 columns a block, each of 16 waves
+// adding a run of the parts.
+__global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float *__restrict__ part, int parts, int H,
+                                                           float *__restrict__ dw) {
+    __shared__ float s[16][WAVE];
+    const int lane = int(threadIdx.x) % WAVE, wave = int(threadIdx.x) / WAVE;
+    const int64_t j = int64_t(blockIdx.x) * WAVE + lane;
+    const int per = (parts + 15) / 16, b0 = wave * per, b1 = min(parts, b0 + per);
+    float sum = 0.f;
+    if (j < H) {
+#pragma unroll 8
+        for (int b = b0; b < b1; ++b) sum += part[int64_t(b) * H + j];
+    }
+    s[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && j < H) {
+#pragma unroll
+        for (int i = 1; i < 16; ++i) sum += s[i][lane];
+        dw[j] = sum;
+    }
+}
+
+// Blocks of the gradients' launch: as many parts of dw are written and read.
+static int norm_grad_blocks(int T) { return std::min(T, 512); }
+
+size_t rms_norm_backward_workspace_bytes(int T, int H) { return size_t(norm_grad_blocks(T)) * size_t(H) * 4; }
+
+template <int DT, int HT, int WT>
+static void launch_norm_grad(const NormGradArgs &a, hipStream_t s) {
+    const int blocks = norm_grad_blocks(a.T);
+    auto run = [&](auto vec, auto th, auto c) {
+        constexpr int TH = decltype(th)::value;
+        rms_norm_backward_kernel<DT, HT, WT, decltype(vec)::value, TH, decltype(c)::value>
+            <<<unsigned(blocks), TH, 0, s>>>(a);
+    };
+    auto by_length = [&](auto vec) {
+        if (a.H <= 512) run(vec, Int<64>{}, Int<1>{});
+        else if (a.H <= 2048) run(vec, Int<256>{}, Int<1>{});
+        else if (a.H <= 4096) run(vec, Int<256>{}, Int<2>{});
+        else if (a.H <= 8192) run(vec, Int<1024>{}, Int<1>{});
+        else run(vec, Int<1024>{}, Int<2>{});
+    };
+    const int64_t one = a.T == 1 ? 0 : 1;  // (a single row's stride does not matter)
+    if (a.H % 8 == 0 && rows_aligned(a.dy, DT, one * a.lddy, 8) && rows_aligned(a.h, HT, one * a.ldh, 8) &&
+        rows_aligned(a.w, WT, 0, 8) && rows_aligned(a.dres, HT, one * a.lddr, 8) &&
+        rows_aligned(a.dx, HT, one * a.lddx, 8))
+        by_length(std::true_type{});
+    else
+        by_length(std::false_type{});
+    if (a.dw) rms_norm_dw_kernel<<<unsigned((a.H + WAVE - 1) / WAVE), 1024, 0, s>>>(a.part, blocks, a.H, a.dw);
+}
+
+void launch_rms_norm_backward(const NormGradArgs &a, hipStream_t s) {
+    by_type(a.dy_type, [&](auto dt) {
+        auto run = [&](auto ht, auto wt) {
+            launch_norm_grad<decltype(dt)::value, decltype(ht)::value, decltype(wt)::value>(a, s);
+        };
+        auto by_row = [&](auto wt) {
+            if (a.h_type == 0) run(Int<0>{}, wt);
+            else run(dt, wt);
+        };
+        if (a.w_type == 0) by_row(Int<0>{});
+        else by_row(dt);
+    });
+}
+
+}  // namespace qwq4

@@ -26,6 +26,9 @@ SYMBOLS = (
     "qw_quant_tokens_i8", "qw_w8a8_gemm", "qw_w8a8_workspace_size", "qw_w8a8_linear", "qw_moe_w8a8_tile_m",
     "qw_moe_w8a8_workspace_size", "qw_moe_experts_w8a8", "qw_moe_sort", "qw_moe_permute",
     "qw_moe_permute_backward", "qw_moe_unpermute", "qw_moe_unpermute_backward",
+    "qw_rms_norm", "qw_rms_norm_i8", "qw_rms_norm_backward_workspace_size", "qw_rms_norm_backward", "qw_lora",
+    "qw_lora_backward_workspace_size", "qw_lora_backward", "qw_logprobs_workspace_size", "qw_logprobs",
+    "qw_logprobs_backward",
     "qw_wcache_open", "qw_wcache_put", "qw_wcache_get", "qw_wcache_finish", "qw_wcache_close",
 )
 
@@ -33,6 +36,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
+_F = ctypes.c_float
 
 _SIGS = {
     "qw_q4_abi_version": ([], _I),
@@ -82,6 +86,16 @@ _SIGS = {
     "qw_moe_permute_backward": ([_P, _I, _I, _P, _I, _I, _I, _P, _I, _I, _P], _I),
     "qw_moe_unpermute": ([_P, _I, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P], _I),
     "qw_moe_unpermute_backward": ([_P, _I, _I, _P, _I, _I, _P, _P, _I, _I, _I, _P, _I, _P, _P], _I),
+    "qw_rms_norm": ([_P, _I, _I, _P, _I, _I, _P, _I, _P, _I, _F, _I, _I, _P, _I, _I, _P], _I),
+    "qw_rms_norm_i8": ([_P, _I, _I, _P, _I, _I, _P, _I, _P, _I, _F, _I, _I, _P, _I, _P, _P], _I),
+    "qw_rms_norm_backward_workspace_size": ([_I, _I], _SZ),
+    "qw_rms_norm_backward": ([_P, _I, _I, _P, _I, _I, _P, _I, _F, _P, _I, _I, _I, _P, _I, _P, _P, _SZ, _P], _I),
+    "qw_lora": ([_P, _I, _I, _P, _P, _P, _P] + [_I] * 5 + [_P, _P, _I, _P, _I, _I, _P], _I),
+    "qw_lora_backward_workspace_size": ([_I] * 5, _SZ),
+    "qw_lora_backward": ([_P, _I, _P, _I, _I] + [_P] * 5 + [_I] * 5 + [_P, _I, _P, _I, _P, _P, _P, _SZ, _P], _I),
+    "qw_logprobs_workspace_size": ([_I, _I, _I], _SZ),
+    "qw_logprobs": ([_P, _I, _I, _P, _I, _I, _I] + [_P] * 6 + [_SZ, _P], _I),
+    "qw_logprobs_backward": ([_P, _I, _I] + [_P] * 5 + [_I, _I, _P, _I, _P], _I),
     "qw_moe_decode_static": ([_P, _I, _P, _I, _I, _I, _I] + [_P] * 9 + [_I, _I, _P, _P, _I] + [_P] * 6 + [_I, _P], _I),
     "qw_moe_decode_with_shared_workspace_size": ([_I, _I, _I, _I, _I, _I], _SZ),
     "qw_moe_decode_with_shared": ([_P, _I, _P, _I, _I, _I, _I] + [_P] * 9 + [_I, _I, _P, _P, _I, _P, _P, _P, _I]
@@ -830,6 +844,233 @@ def moe_unpermute_backward(dout, yp, tok_slot, tok_w=None, dyp=None, dw=None, ne
     _check(lib().qw_moe_unpermute_backward(_ptr(dout), dcode, ldd, _ptr(yp), code, ldyp, _ptr(tok_slot), _ptr(tok_w), T,
                                            k, H, _ptr(dyp), lddyp, _ptr(dw), stream), "qw_moe_unpermute_backward")
     return dyp, dw
+
+
+# ------------------------------------------------------ around a projection
+def _norm_rows(fn, x, w, residual, residual_out):
+    """(T, H, arguments of the C call up to eps, residual_out)"""
+    import torch
+    _no_autograd(fn, x, w, residual)
+    ldx = _matrix(fn, "x", x, None, None)
+    T, H = x.shape
+    if w.shape != (H,) or not w.is_contiguous():
+        raise ValueError(f"{fn}: w is {tuple(w.shape)}, not ({H},), or not contiguous")
+    if residual is None:
+        if residual_out is not None:
+            raise ValueError(f"{fn}: residual_out without a residual")
+        return T, H, (_ptr(x), _tcode(x), ldx, None, 0, 0, None, 0, _ptr(w), _tcode(w)), None
+    ldr = _matrix(fn, "residual", residual, T, H)
+    if residual_out is None:
+        residual_out = torch.empty((T, H), dtype=residual.dtype, device=x.device)
+    ldro = _matrix(fn, "residual_out", residual_out, T, H, residual.dtype)
+    return T, H, (_ptr(x), _tcode(x), ldx, _ptr(residual), _tcode(residual), ldr, _ptr(residual_out), ldro, _ptr(w),
+                  _tcode(w)), residual_out
+
+
+def rms_norm(x, w, eps=1e-6, residual=None, y=None, y_dtype=None, residual_out=None):
+    """y = h w / sqrt(mean(h^2) + eps) of rows x [T][H], w [H] (of x's type or float32), in fp32; y of x's type, or y_dtype / the dtype of a
+    given y. With a residual (of x's type or float32) h = x + residual, and the result is (y, residual_out): h
+    rounded to the residual's type, in a new tensor or the one given, which may be the residual. Its gradients are
+    rms_norm_backward; autograd does not record the call."""
+    fn = "rms_norm"
+    T, H, args, residual_out = _norm_rows(fn, x, w, residual, residual_out)
+    y, ldy, ycode = _w8_out(fn, y, y_dtype, T, H, x.dtype, x.device)
+    stream = _here(fn, x, w, residual, residual_out, y)
+    _check(lib().qw_rms_norm(*args, eps, T, H, _ptr(y), ycode, ldy, stream), "qw_rms_norm")
+    return y if residual is None else (y, residual_out)
+
+
+def rms_norm_i8(x, w, eps=1e-6, residual=None, q=None, scale=None, residual_out=None):
+    """rms_norm with its rows in 8 bits, as gemm_w8a8 takes them: (q int8 [T][H], scale fp32 [T]), and residual_out
+    behind them where there is a residual. The values of q are quant_tokens_i8's of the rows h w in fp32."""
+    import torch
+    fn = "rms_norm_i8"
+    T, H, args, residual_out = _norm_rows(fn, x, w, residual, residual_out)
+    if q is None:
+        q = torch.empty((T, H), dtype=torch.int8, device=x.device)
+    if scale is None:
+        scale = torch.empty(T, dtype=torch.float32, device=x.device)
+    ldq = _matrix(fn, "q", q, T, H, torch.int8)
+    _whole(fn, "scale", scale, (T,), torch.float32)
+    stream = _here(fn, x, w, residual, residual_out, q, scale)
+    _check(lib().qw_rms_norm_i8(*args, eps, T, H, _ptr(q), ldq, _ptr(scale), stream), "qw_rms_norm_i8")
+    return (q, scale) if residual is None else (q, scale, residual_out)
+
+
+def rms_norm_backward_workspace_size(T, H):
+    return lib().qw_rms_norm_backward_workspace_size(T, H)
+
+
+def rms_norm_backward(dy, h, w, eps=1e-6, dres=None, dx=None, dw=None, need_dw=True, workspace=None):
+    """The gradients of rms_norm from dy [T][H]: (dx of h's type, dw fp32 [H] or None where it is not needed). h
+    [T][H], of dy's type or float32 as w is, is what was normalised (residual_out where there was a residual); dres, of h's
+    type, is the gradient of residual_out and is added to dx, which is then that of x and of the residual alike.
+    dx may be dy, h or dres. float16 dx beyond +-65504 becomes infinite."""
+    import torch
+    fn = "rms_norm_backward"
+    lddy = _matrix(fn, "dy", dy, None, None)
+    T, H = dy.shape
+    ldh = _matrix(fn, "h", h, T, H)
+    if w.shape != (H,) or not w.is_contiguous():
+        raise ValueError(f"{fn}: w is {tuple(w.shape)}, not ({H},), or not contiguous")
+    lddr = _matrix(fn, "dres", dres, T, H, h.dtype) if dres is not None else 0
+    if dx is None:
+        dx = torch.empty((T, H), dtype=h.dtype, device=h.device)
+    lddx = _matrix(fn, "dx", dx, T, H, h.dtype)
+    if not need_dw:
+        dw = None
+    else:
+        if dw is None:
+            dw = torch.empty(H, dtype=torch.float32, device=h.device)
+        _whole(fn, "dw", dw, (H,), torch.float32)
+        if workspace is None:
+            workspace = torch.empty(rms_norm_backward_workspace_size(T, H), dtype=torch.uint8, device=h.device)
+    stream = _here(fn, dy, h, w, dres, dx, dw, workspace)
+    _check(lib().qw_rms_norm_backward(_ptr(dy), _tcode(dy), lddy, _ptr(h), _tcode(h), ldh, _ptr(w), _tcode(w), eps,
+                                      _ptr(dres), lddr, T, H, _ptr(dx), lddx, _ptr(dw), _ptr(workspace),
+                                      _space(fn, workspace), stream), "qw_rms_norm_backward")
+    return dx, dw
+
+
+def _adapters(fn, x, A, B, ids, scaling):
+    """(T, K, N, R, L, whether fp16) of an adapter call"""
+    import torch
+    if A.dim() != 3 or B.dim() != 3:
+        raise ValueError(f"{fn}: A is {tuple(A.shape)}, B {tuple(B.shape)}, not [L][R][K] and [L][N][R]")
+    (L, R, K), N, T = A.shape, B.shape[1], x.shape[0]
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{fn}: rows are {x.dtype}, not bfloat16 or float16")
+    _whole(fn, "A", A, (L, R, K), x.dtype)
+    _whole(fn, "B", B, (L, N, R), x.dtype)
+    _whole(fn, "ids", ids, (T,), torch.int32)
+    if scaling is not None:
+        _whole(fn, "scaling", scaling, (L,), torch.float32)
+    if max(T, L, R, K, N) > _INT_MAX:
+        raise ValueError(f"{fn}: T, K, N, R, L = {T, K, N, R, L}, more than 2^31 - 1")
+    return T, K, N, R, L, int(x.dtype == torch.float16)
+
+
+def lora(x, A, B, ids, y, scaling=None, out=None, v=None):
+    """Low-rank adapters beside a projection whose rows y [T][N] are given: out_t = y_t + scaling[i] B[i] (A[i] x_t),
+    i = ids[t] (int32 [T]; outside 0 .. L - 1: no adapter, out_t = y_t). x [T][K], A [L][R][K], B [L][N][R] all
+    bfloat16 or all float16; y of any type; scaling fp32 [L] (None: all 1). out is y unless another is given. v fp32
+    [T][R] takes A[i] x_t, which lora_backward needs; rows without an adapter are left as they were. Its gradients are
+    lora_backward; autograd does not record the call."""
+    import torch
+    fn = "lora"
+    _no_autograd(fn, x, A, B, y, scaling)
+    ldx = _matrix(fn, "x", x, None, None)
+    T, K, N, R, L, f16 = _adapters(fn, x, A, B, ids, scaling)
+    if x.shape[1] != K:
+        raise ValueError(f"{fn}: x is {tuple(x.shape)}, not ({T}, {K})")
+    ldy = _matrix(fn, "y", y, T, N)
+    code = _tcode(y)
+    if out is None:
+        out = y
+    ldo = _matrix(fn, "out", out, T, N, y.dtype)
+    if v is None:
+        v = torch.empty((T, R), dtype=torch.float32, device=x.device)
+    else:
+        _whole(fn, "v", v, (T, R), torch.float32)
+    stream = _here(fn, x, A, B, ids, y, scaling, out, v)
+    _check(lib().qw_lora(_ptr(x), ldx, f16, _ptr(A), _ptr(B), _ptr(ids), _ptr(scaling), T, K, N, R, L, _ptr(v), _ptr(y),
+                         ldy, _ptr(out), ldo, code, stream), "qw_lora")
+    return out
+
+
+def lora_backward_workspace_size(T, K, N, R, L):
+    return lib().qw_lora_backward_workspace_size(T, K, N, R, L)
+
+
+def lora_backward(dy, x, A, B, ids, v, scaling=None, dx=None, dx_out=None, dA=None, dB=None, need_weights=True,
+                  workspace=None):
+    """The gradients of lora from dy [T][N] (of x's type) and v as lora left it: (dx_out, dA fp32 [L][R][K], dB fp32
+    [L][N][R]). dx [T][K], of x's type, is the gradient through the shared projection; the adapters' is added to it, in
+    place unless another dx_out is given; None: not wanted. dA and dB are written whole, zeros for an adapter without
+    tokens, and None with need_weights = False. float16 dx_out beyond +-65504 becomes infinite."""
+    import torch
+    fn = "lora_backward"
+    lddy, ldx = _matrix(fn, "dy", dy, None, None, x.dtype), _matrix(fn, "x", x, None, None)
+    T, K, N, R, L, f16 = _adapters(fn, x, A, B, ids, scaling)
+    if x.shape[1] != K or dy.shape != (T, N):
+        raise ValueError(f"{fn}: x is {tuple(x.shape)}, dy {tuple(dy.shape)}, not ({T}, {K}) and ({T}, {N})")
+    _whole(fn, "v", v, (T, R), torch.float32)
+    lddx = lddxo = 0
+    if dx is not None:
+        dx_out = dx if dx_out is None else dx_out
+        lddx, lddxo = _matrix(fn, "dx", dx, T, K, x.dtype), _matrix(fn, "dx_out", dx_out, T, K, x.dtype)
+    elif dx_out is not None:
+        raise ValueError(f"{fn}: dx_out without dx")
+    if need_weights:
+        dA = torch.empty((L, R, K), dtype=torch.float32, device=x.device) if dA is None else dA
+        dB = torch.empty((L, N, R), dtype=torch.float32, device=x.device) if dB is None else dB
+        _whole(fn, "dA", dA, (L, R, K), torch.float32)
+        _whole(fn, "dB", dB, (L, N, R), torch.float32)
+    else:
+        dA = dB = None
+    if workspace is None:
+        workspace = torch.empty(lora_backward_workspace_size(T, K, N, R, L), dtype=torch.uint8, device=x.device)
+    stream = _here(fn, dy, x, A, B, ids, v, scaling, dx, dx_out, dA, dB, workspace)
+    _check(lib().qw_lora_backward(_ptr(dy), lddy, _ptr(x), ldx, f16, _ptr(A), _ptr(B), _ptr(ids), _ptr(v), _ptr(scaling),
+                                  T, K, N, R, L, _ptr(dx), lddx, _ptr(dx_out), lddxo, _ptr(dA), _ptr(dB),
+                                  _ptr(workspace), _space(fn, workspace), stream), "qw_lora_backward")
+    return dx_out, dA, dB
+
+
+def logprobs_workspace_size(T, V, top):
+    return lib().qw_logprobs_workspace_size(T, V, top)
+
+
+def logprobs(logits, tokens, top=0, workspace=None):
+    """Of logits [T][V] and tokens int32 [T]: (logp, entropy, lse, top_ids, top_logp). logp = logits[t][tokens[t]] -
+    lse (0 for a token outside 0 .. V - 1), entropy and lse fp32 [T]; top_ids int32 and top_logp fp32 [T][top]: the
+    most likely tokens, largest first, ties by the lowest index (None with top = 0). Logits of -inf are masked; a row
+    of only such has lse, logp and top_logp of -inf and entropy 0. Its gradient is logprobs_backward; autograd does
+    not record the call."""
+    import torch
+    fn = "logprobs"
+    _no_autograd(fn, logits)
+    ld = _matrix(fn, "logits", logits, None, None)
+    T, V = logits.shape
+    _whole(fn, "tokens", tokens, (T,), torch.int32)
+    if not 0 <= top <= min(64, V):
+        raise ValueError(f"{fn}: top = {top} (0..64, at most V = {V})")
+    code = _tcode(logits)
+    # (one buffer for the fp32 outputs: an allocation each would cost more than the call)
+    own = torch.empty(T * (3 + top), dtype=torch.float32, device=logits.device)
+    logp, entropy, lse, top_logp = own.split_with_sizes((T, T, T, T * top))
+    top_ids = torch.empty((T, top), dtype=torch.int32, device=logits.device) if top else None
+    top_logp = top_logp.view(T, top) if top else None
+    if workspace is None:
+        need = logprobs_workspace_size(T, V, top)
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+    stream = _here(fn, logits, tokens, own, workspace)
+    _check(lib().qw_logprobs(_ptr(logits), code, ld, _ptr(tokens), T, V, top, _ptr(logp), _ptr(entropy), _ptr(lse),
+                             _ptr(top_ids), _ptr(top_logp), _ptr(workspace), _space(fn, workspace), stream),
+           "qw_logprobs")
+    return logp, entropy, lse, top_ids, top_logp
+
+
+def logprobs_backward(logits, tokens, lse, entropy, dlogp=None, dentropy=None, dlogits=None):
+    """The gradient of logprobs' logp and entropy (dlogp, dentropy fp32 [T], either None: none) in the logits' type,
+    from lse and entropy as logprobs gave them. dlogits may be the logits. float16 beyond +-65504 becomes infinite."""
+    import torch
+    fn = "logprobs_backward"
+    ld = _matrix(fn, "logits", logits, None, None)
+    T, V = logits.shape
+    _whole(fn, "tokens", tokens, (T,), torch.int32)
+    for name, t in (("lse", lse), ("entropy", entropy), ("dlogp", dlogp), ("dentropy", dentropy)):
+        if t is not None:
+            _whole(fn, name, t, (T,), torch.float32)
+    if dlogits is None:
+        dlogits = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
+    ldd = _matrix(fn, "dlogits", dlogits, T, V, logits.dtype)
+    stream = _here(fn, logits, tokens, lse, entropy, dlogp, dentropy, dlogits)
+    _check(lib().qw_logprobs_backward(_ptr(logits), _tcode(logits), ld, _ptr(tokens), _ptr(lse), _ptr(entropy),
+                                      _ptr(dlogp), _ptr(dentropy), T, V, _ptr(dlogits), ldd, stream),
+           "qw_logprobs_backward")
+    return dlogits
 
 
 def unpack(W, N, K):
