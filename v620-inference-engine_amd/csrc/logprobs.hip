@@ -40,7 +40,24 @@ struct SoftStats {
         m = to;
         return ref;
     }
-    // (the difference is bounded where it is a factor: 0 times a masked value's would be a NaN)
+    // The values of one step, summed among themselves first: next to a likely
+    // token each of the others alone is too small to change the sum so far, all
+    // of them are not. (The difference is bounded where it is a factor: 0 times
+    // a masked value's would be a NaN.)
+    template <int N>
+    __device__ __forceinline__ void add(const float (&v)[N][8], float ref) {
+        float ps[4] = {}, pu[4] = {};
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float d = v[n][j] - ref, e = exp_fast(d);
+                ps[j % 4] += e;
+                pu[j % 4] = __builtin_fmaf(e, fmaxf(d, NEARLY_NONE), pu[j % 4]);
+            }
+        s += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        u += (pu[0] + pu[1]) + (pu[2] + pu[3]);
+    }
     __device__ __forceinline__ void add(float v, float ref) {
         const float d = v - ref, e = exp_fast(d);
         s += e;
@@ -70,7 +87,8 @@ __device__ __forceinline__ SoftStats wave_join(SoftStats a) {
 
 // Order of alternatives: by value, ties by the lowest index (unused places of
 // a list hold -infinity and INT_MAX: last).
-__device__ __forceinline__ bool ahead(float v, int i, float w, int j) { return v > w || (v == w && i < j); }
+// (Without branches: they would make every comparison wait for the one before.)
+__device__ __forceinline__ bool ahead(float v, int i, float w, int j) { return (v > w) | ((v == w) & (i < j)); }
 
 // whole numbers in the order of the values
 __device__ __forceinline__ int ordered(float v) {
@@ -78,6 +96,16 @@ __device__ __forceinline__ int ordered(float v) {
     return b >= 0 ? b : b ^ 0x7fffffff;
 }
 __device__ __forceinline__ float unordered(int b) { return __builtin_bit_cast(float, b >= 0 ? b : b ^ 0x7fffffff); }
+
+// The same order in one number (both zeros are one value): 0 is an unused
+// place, behind every value; a NaN has none.
+typedef unsigned long long TopKey;
+__device__ __forceinline__ TopKey top_key(float v, int i) {
+    const TopKey high = uint32_t(ordered(v + 0.f)) ^ 0x80000000u;
+    return i == INT_MAX || v != v ? 0 : high << 32 | uint32_t(~i);
+}
+__device__ __forceinline__ float key_value(TopKey k) { return unordered(int(uint32_t(k >> 32) ^ 0x80000000u)); }
+__device__ __forceinline__ int key_index(TopKey k) { return int(~uint32_t(k)); }
 
 __device__ __forceinline__ float lane_value(float v, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
@@ -107,25 +135,6 @@ struct TopList {
         const int pv = lane_before(__builtin_bit_cast(int, v)), pi = lane_before(i);
         v = lane == at ? w : lane > at ? __builtin_bit_cast(float, pv) : v;
         i = lane == at ? j : lane > at ? pi : i;
-        set_last();
-    }
-    // The list of the 64 lanes' own (w, j), sorted (a bitonic network).
-    __device__ __forceinline__ void seed(float w, int j) {
-        const int lane = int(threadIdx.x) % WAVE;
-        v = w;
-        i = j;
-#pragma unroll
-        for (int n = 2; n <= WAVE; n *= 2)
-#pragma unroll
-            for (int o = n / 2; o >= 1; o /= 2) {
-                const float ov = __shfl_xor(v, o);
-                const int oi = __shfl_xor(i, o);
-                const bool down = (lane & n) == 0, low = (lane & o) == 0;
-                if (ahead(ov, oi, v, i) == (down == low)) {  // (equal pairs are both unused: swapped or not is alike)
-                    v = ov;
-                    i = oi;
-                }
-            }
         set_last();
     }
 };
@@ -184,50 +193,178 @@ __device__ __forceinline__ float finish_row(const LogprobArgs &a, int64_t t, con
     return lse;
 }
 
-__device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t t, int rank, float v, int i, float lse) {
+__device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t t, int rank, TopKey key, float lse) {
     const bool bad = lse != lse;
-    a.top_i[t * a.top + rank] = bad ? -1 : i;
-    a.top_v[t * a.top + rank] = bad ? lse : lse == neg_inf() ? lse : v - lse;
+    a.top_i[t * a.top + rank] = bad ? -1 : key_index(key);
+    a.top_v[t * a.top + rank] = bad ? lse : lse == neg_inf() ? lse : key_value(key) - lse;
 }
 
-// Places of n lists (sorted, k entries each, in LDS) in the order of all:
-// put(rank, v, i) for the first k. An entry's rank is its own place and, for
-// every other list, how many of that are ahead of it.
+// put(rank, key) for the first k of n keys in LDS, none alike (0 for the places
+// behind the n-th): a key's rank is how many are ahead of it. Every comparison
+// is independent of the others, where a search or a sorted list would wait.
 template <class Put>
-__device__ __forceinline__ void merge_lists(const float *lv, const int *li, int n, int k, Put put) {
-    for (int e = int(threadIdx.x); e < n * k; e += int(blockDim.x)) {
-        const int own = e / k;
-        const float v = lv[e];
-        const int i = li[e];
-        int rank = e % k;
-        for (int q = 0; q < n && rank < k; ++q) {
-            if (q == own) continue;
-            int lo = 0, hi = k;  // (how many of list q are ahead; unused places go by their list's number)
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                const float w = lv[q * k + mid];
-                const int j = li[q * k + mid];
-                if (ahead(w, j, v, i) || (w == v && j == i && q < own)) lo = mid + 1;
-                else hi = mid;
-            }
-            rank += lo;
+__device__ __forceinline__ void rank_keys(const TopKey *keys, int n, int k, Put put) {
+    for (int e = int(threadIdx.x); e < n; e += int(blockDim.x)) {
+        const TopKey own = keys[e];
+        int rank = 0;
+#pragma unroll 16
+        for (int c = 0; c < n; ++c) rank += int(keys[c] > own);
+        if (rank < k) put(rank, own);
+    }
+    for (int e = n + int(threadIdx.x); e < k; e += int(blockDim.x)) put(e, TopKey(0));
+}
+
+// A part of a row by four waves with 2 pieces a lane: all of it in registers.
+// The k-th of a wave's lanes' largest has k values at or ahead of it, and so
+// has the farthest of the four waves': only values not behind that can be
+// among the part's first k. They go to a list in LDS (k and a few, and never
+// more than the part has) and are ranked.
+constexpr int MAX_SPLITS = 64;  // parts of a row at most
+constexpr int FEW_PIECES = 4 * WAVE * 2;
+template <int TY, bool TOP>
+__global__ __launch_bounds__(256) void logprobs_few_kernel(LogprobArgs a) {
+    constexpr int Z = TY == 0 ? 4 : 2;
+    __shared__ float s_st[4][3];
+    __shared__ TopKey s_last;
+    __shared__ int s_n;
+    __shared__ TopKey s_best[TOP ? 4 : 1][WAVE];
+    __shared__ TopKey s_keys[TOP ? 8 * FEW_PIECES + WAVE : 1];  // (and the row's head and tail)
+    const int tid = int(threadIdx.x), lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+    const int64_t t = int64_t(blockIdx.x) / a.splits;
+    const int split = int(blockIdx.x) % a.splits;
+    const char *row = static_cast<const char *>(a.logits) + t * a.ld * Z;
+    const RowCut cut(row, Z, a.V);
+    const char *body = row + int64_t(cut.head) * Z;
+    if (tid == 0) {
+        s_last = 0;
+        s_n = 0;
+    }
+    const int p0 = split * FEW_PIECES + tid;
+    Raw8<TY> raw[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+        if (p0 + 256 * u < cut.pieces) raw[u].load(body + int64_t(p0 + 256 * u) * (8 * Z));
+    // (single elements before and behind the pieces: one each by the first lanes)
+    const int alone = tid < cut.head ? tid : 8 * cut.pieces + tid;
+    const bool has_alone = split == 0 && tid < cut.head + cut.tail;
+    const float extra = has_alone ? logit_at<TY>(row, alone) : neg_inf();
+    float v[2][8], largest = extra;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const bool in = p0 + 256 * u < cut.pieces;
+        raw[u].values(v[u]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[u][j] = in ? v[u][j] : neg_inf();
+            largest = fmaxf(largest, v[u][j]);
         }
-        if (rank < k) put(rank, v, i);
+    }
+    SoftStats st;
+    st.clear();
+    const float ref = st.raise(largest);
+    st.add(v, ref);
+    st.add(extra, ref);
+    st = wave_join(st);
+    if (lane == 0) {
+        s_st[wave][0] = st.m;
+        s_st[wave][1] = st.s;
+        s_st[wave][2] = st.u;
+    }
+    // f(value, index) for all that the lane holds, single elements behind the row's before it
+    auto each = [&](auto f) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int p = p0 + 256 * u;
+            if (p < cut.pieces) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f(v[u][j], cut.head + 8 * p + j);
+            }
+        }
+        if (has_alone) f(extra, alone);
+    };
+    TopKey best = 0;
+    if constexpr (TOP) {
+        float w = neg_inf();
+        int i = INT_MAX;
+        each([&](float x, int at) {
+            const bool first = ahead(x, at, w, i);
+            w = first ? x : w;
+            i = first ? at : i;
+        });
+        best = top_key(w, i);
+        s_best[wave][lane] = best;
+    }
+    __syncthreads();
+    st = SoftStats{s_st[0][0], s_st[0][1], s_st[0][2]};
+#pragma unroll
+    for (int w = 1; w < 4; ++w) st.join(SoftStats{s_st[w][0], s_st[w][1], s_st[w][2]});
+    const int64_t part = t * a.splits + split;
+    if constexpr (TOP) {
+        int rank = 0;
+#pragma unroll 16
+        for (int l = 0; l < WAVE; ++l) rank += int(s_best[wave][l] > best);
+        if (rank == a.top - 1) atomicMax(&s_last, best);
+        __syncthreads();
+        const TopKey last = max(s_last, TopKey(1));
+        const float last_v = key_value(last);
+        const int last_i = key_index(last);
+        const bool any = last == 1;  // (the part has fewer than k values: all of them)
+        auto kept = [&](float x, int at) { return (x > last_v) | ((x == last_v) & (at <= last_i)) | (any & (x == x)); };
+        int mine = 0;
+        if (best >= last) each([&](float x, int at) { mine += int(kept(x, at)); });
+        int before = mine;
+#pragma unroll
+        for (int o = 1; o < WAVE; o <<= 1) {
+            const int u = __shfl_up(before, o);
+            if (lane >= o) before += u;
+        }
+        int base = 0;
+        if (lane == WAVE - 1) base = atomicAdd(&s_n, before);
+        before += __builtin_amdgcn_readlane(base, WAVE - 1) - mine;
+        if (mine > 0) each([&](float x, int at) {
+            if (kept(x, at)) s_keys[before++] = top_key(x, at);
+        });
+        __syncthreads();
+        float lse = 0.f;
+        __shared__ float s_lse;
+        if (a.splits == 1) {
+            if (tid == 0) s_lse = finish_row<TY>(a, t, row, st);
+            __syncthreads();
+            lse = s_lse;
+        }
+        rank_keys(s_keys, s_n, a.top, [&](int r, TopKey k) {
+            if (a.splits == 1) put_top(a, t, r, k, lse);
+            else a.part_key[part * a.top + r] = k;
+        });
+    } else if (a.splits == 1 && tid == 0) {
+        finish_row<TY>(a, t, row, st);
+    }
+    if (a.splits > 1 && tid == 0) {
+        a.part_st[3 * part] = st.m;
+        a.part_st[3 * part + 1] = st.s;
+        a.part_st[3 * part + 2] = st.u;
     }
 }
 
 // Part `split` of row t by a block of four waves, each taking every fourth
-// step of 64 U pieces. TOP: a wave keeps a list of the most likely values; a
-// piece is looked at value by value only where its largest would come into the
-// list and is not below the last of another wave's.
+// step of 64 U pieces. TOP: the largest value of each lane's step is left in LDS
+// on the way. The lanes make 64 groups (a lane of each wave); the k-th of the
+// groups' largest has k values at or above it, and only steps whose largest is
+// not below it are read a second time: of a row of 151936 and k = 5, some 6 of
+// 4736, from which some 5 values go to the list that is ranked. (A sorted list per
+// wave kept up to date on the way: 5 alternatives 45 us more in 4096 rows, 20
+// alternatives 130.) Where more than the list takes are left (rows with thousands of
+// equal values, fewer than k unmasked ones), the part is read again into sorted lists.
+constexpr int TOP_SLOTS = 32, TOP_LIST = 512;
 template <int TY, bool TOP, int U>
 __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     constexpr int Z = TY == 0 ? 4 : 2;
-    __shared__ int s_last;
-    __shared__ float s_st[4][3];
-    __shared__ float s_lv[TOP ? 4 * WAVE : 1];
-    __shared__ int s_li[TOP ? 4 * WAVE : 1];
-    const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
+    extern __shared__ float s_max[];  // TOP: [slots][256]
+    __shared__ int s_n;
+    __shared__ float s_st[4][3], s_bound, s_lse;
+    __shared__ float s_lane[TOP ? 256 : 1];
+    __shared__ TopKey s_keys[TOP ? TOP_LIST : 1];
+    const int tid = int(threadIdx.x), lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int64_t t = int64_t(blockIdx.x) / a.splits;
     const int split = int(blockIdx.x) % a.splits;
     const char *row = static_cast<const char *>(a.logits) + t * a.ld * Z;
@@ -235,63 +372,15 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     const char *body = row + int64_t(cut.head) * Z;
     const int steps = (cut.pieces + WAVE * U - 1) / (WAVE * U);
     const int per = (steps + a.splits - 1) / a.splits, first = split * per, end = min(steps, first + per);
-    if constexpr (TOP) {
-        if (threadIdx.x == 0) s_last = INT_MIN;
-        __syncthreads();
-    }
+    if (TOP && tid == 0) s_n = 0;
+    // (single elements before and behind the pieces: one each by the first lanes)
+    const int alone = tid < cut.head ? tid : 8 * cut.pieces + tid;
+    const bool has_alone = split == 0 && tid < cut.head + cut.tail;
+    const float extra = has_alone ? logit_at<TY>(row, alone) : neg_inf();
     SoftStats st;
     st.clear();
-    TopList list;
-    list.clear(a.top);
-    bool empty = true;
+    st.add(extra, st.raise(extra));
 
-    // the values of one step, `mine` of them in order from index at: into the sums and the list
-    auto take = [&](const float (&v)[8], float largest, int at, bool have, int seeded) {
-        if constexpr (TOP) {
-            const float other = unordered(__hip_atomic_load(&s_last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
-            auto wanted = [&] { return __ballot(have && list.wants(largest, at) && !(largest < other)); };
-            unsigned long long lanes = wanted();
-            if (!lanes) return;
-            while (lanes) {
-                const int l = __builtin_ctzll(lanes);
-                float w = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) w = lane == j ? lane_value(v[j], l) : w;
-                const int i0 = __builtin_amdgcn_readlane(at, l), skip = __builtin_amdgcn_readlane(seeded, l);
-                const int i = i0 + lane;
-                unsigned long long which = __ballot(lane < 8 && i != skip && list.wants(w, i));
-                while (which) {
-                    const int j = __builtin_ctzll(which);
-                    which &= which - 1;
-                    const float x = lane_value(w, j);
-                    if (list.wants(x, i0 + j)) list.insert(x, i0 + j);
-                }
-                lanes = l == WAVE - 1 ? 0 : wanted() & (~0ull << (l + 1));
-            }
-            if (lane == 0 && list.last_i != INT_MAX)
-                __hip_atomic_fetch_max(&s_last, ordered(list.last_v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        }
-    };
-
-    // (single elements before and behind the pieces: by the first wave)
-    if (split == 0 && wave == 0 && cut.head + cut.tail > 0) {
-        const int at = lane < cut.head ? lane : cut.head + 8 * cut.pieces + lane - cut.head;
-        const bool have = lane < cut.head + cut.tail;
-        const float v = have ? logit_at<TY>(row, at) : neg_inf();
-        st.add(v, st.raise(v));
-        if constexpr (TOP) {
-            unsigned long long lanes = __ballot(have);
-            while (lanes) {
-                const int l = __builtin_ctzll(lanes);
-                lanes &= lanes - 1;
-                const float x = lane_value(v, l);
-                const int i = __builtin_amdgcn_readlane(at, l);
-                if (list.wants(x, i)) list.insert(x, i);
-            }
-        }
-    }
-
-    Raw8<TY> raw[U], next[U];
     auto load = [&](int step, Raw8<TY> (&r)[U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -299,145 +388,222 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
             r[u].load(body + int64_t(p) * (8 * Z));
         }
     };
+    // a step's values, -infinity behind the last piece (only in a row's last step)
+    auto values = [&](int step, const Raw8<TY> (&r)[U], float (&v)[U][8]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            r[u].values(v[u]);
+            if ((step * U + u) * WAVE + lane >= cut.pieces) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[u][j] = neg_inf();
+            }
+        }
+    };
+    Raw8<TY> raw[U], next[U];
+    float slot_max = neg_inf();
+    int slot = 0, in_slot = 0;
     int step = first + wave;
     if (step < end) load(step, next);
     for (; step < end; step += 4) {
 #pragma unroll
         for (int u = 0; u < U; ++u) raw[u] = next[u];
         if (step + 4 < end) load(step + 4, next);
-        float v[U][8], largest[U], all = neg_inf();
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            raw[u].values(v[u]);
-            if ((step * U + u) * WAVE + lane >= cut.pieces) {  // (only in a row's last step)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[u][j] = neg_inf();
-            }
-            largest[u] = v[u][0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) largest[u] = fmaxf(largest[u], v[u][j]);
-            all = fmaxf(all, largest[u]);
-        }
-        const float ref = st.raise(all);
+        float v[U][8], largest = neg_inf();
+        values(step, raw, v);
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) st.add(v[u][j], ref);
+            for (int j = 0; j < 8; ++j) largest = fmaxf(largest, v[u][j]);
+        const float ref = st.raise(largest);
+        st.add(v, ref);
         if constexpr (TOP) {
-            int seeded = -1;
-            if (empty && list.last_i == INT_MAX && a.top > 1) {
-                // the lanes' largest are the list to begin with: few other values of the step come before its k-th
-                float w = neg_inf();
-                int i = INT_MAX;
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int p = (step * U + u) * WAVE + lane, at = cut.head + 8 * p;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (p < cut.pieces && ahead(v[u][j], at + j, w, i)) {
-                            w = v[u][j];
-                            i = at + j;
-                        }
-                }
-                // (what the row's head and tail put into the list goes in again behind)
-                TopList before = list;
-                list.seed(w, i);
-                seeded = i;
-                unsigned long long lanes = __ballot(before.i != INT_MAX);
-                while (lanes) {
-                    const int l = __builtin_ctzll(lanes);
-                    lanes &= lanes - 1;
-                    const float x = lane_value(before.v, l);
-                    const int j = __builtin_amdgcn_readlane(before.i, l);
-                    if (list.wants(x, j)) list.insert(x, j);
-                }
-            }
-            empty = false;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int p = (step * U + u) * WAVE + lane;
-                take(v[u], largest[u], cut.head + 8 * p, p < cut.pieces, seeded);
+            slot_max = fmaxf(slot_max, largest);
+            if (++in_slot == a.slot_steps) {
+                s_max[slot * 256 + tid] = slot_max;
+                ++slot;
+                in_slot = 0;
+                slot_max = neg_inf();
             }
         }
     }
-
+    if constexpr (TOP) {
+        if (in_slot) s_max[slot++ * 256 + tid] = slot_max;
+        s_lane[tid] = st.m;
+    }
     st = wave_join(st);
     if (lane == 0) {
         s_st[wave][0] = st.m;
         s_st[wave][1] = st.s;
         s_st[wave][2] = st.u;
     }
-    if constexpr (TOP) {
-        if (lane < a.top) {
-            s_lv[wave * a.top + lane] = list.v;
-            s_li[wave * a.top + lane] = list.i;
+    __syncthreads();
+    if (!TOP || wave == 3) {
+        st = SoftStats{s_st[0][0], s_st[0][1], s_st[0][2]};
+#pragma unroll
+        for (int w = 1; w < 4; ++w) st.join(SoftStats{s_st[w][0], s_st[w][1], s_st[w][2]});
+        if (tid == (TOP ? 3 * WAVE : 0)) {
+            if (a.splits == 1) {
+                s_lse = finish_row<TY>(a, t, row, st);
+            } else {
+                float *p = a.part_st + 3 * (t * a.splits + split);
+                p[0] = st.m;
+                p[1] = st.s;
+                p[2] = st.u;
+            }
+        }
+    }
+    if constexpr (!TOP) return;
+
+    if (wave == 0) {
+        const float own = fmaxf(fmaxf(s_lane[lane], s_lane[lane + 64]), fmaxf(s_lane[lane + 128], s_lane[lane + 192]));
+        int rank = 0;
+#pragma unroll 16
+        for (int l = 0; l < WAVE; ++l) {
+            const float other = lane_value(own, l);
+            rank += int((other > own) | ((other == own) & (l < lane)));
+        }
+        if (rank == a.top - 1) s_bound = own;
+    }
+    __syncthreads();
+    const float bound = s_bound;
+    auto keep = [&](float x, int at) {
+        if (!(x >= bound)) return;
+        const int n = atomicAdd(&s_n, 1);
+        if (n < TOP_LIST) s_keys[n] = top_key(x, at);
+    };
+    if (has_alone) keep(extra, alone);
+    for (int k = 0; k < slot; ++k) {
+        if (!(s_max[k * 256 + tid] >= bound)) continue;
+        for (int c = 0; c < a.slot_steps; ++c) {
+            const int again = first + wave + 4 * (k * a.slot_steps + c);
+            if (again >= end) break;
+            load(again, raw);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int p = (again * U + u) * WAVE + lane;
+                float v[8];
+                raw[u].values(v);
+                if (p < cut.pieces) {
+#pragma unroll 1
+                    for (int j = 0; j < 8; ++j) {
+                        float x = v[0];
+#pragma unroll
+                        for (int i = 1; i < 8; ++i) x = j == i ? v[i] : x;
+                        keep(x, cut.head + 8 * p + j);
+                    }
+                }
+            }
         }
     }
     __syncthreads();
-    st = SoftStats{s_st[0][0], s_st[0][1], s_st[0][2]};
+    int n = s_n;
+    if (n > TOP_LIST) {
+        TopList list;
+        list.clear(a.top);
+        auto take = [&](float w, int i, bool have) {
+            unsigned long long which = __ballot(have && list.wants(w, i));
+            while (which) {
+                const int l = __builtin_ctzll(which);
+                which &= which - 1;
+                const float x = lane_value(w, l);
+                const int j = __builtin_amdgcn_readlane(i, l);
+                if (list.wants(x, j)) list.insert(x, j);
+            }
+        };
+        take(extra, alone, has_alone);
+        for (int again = first + wave; again < end; again += 4) {
+            load(again, raw);
+            float v[U][8];
+            values(again, raw, v);
 #pragma unroll
-    for (int w = 1; w < 4; ++w) st.join(SoftStats{s_st[w][0], s_st[w][1], s_st[w][2]});
-    if (a.splits == 1) {
-        __shared__ float s_lse;
-        if (threadIdx.x == 0) s_lse = finish_row<TY>(a, t, row, st);
-        if constexpr (TOP) {
-            __syncthreads();
-            const float lse = s_lse;
-            merge_lists(s_lv, s_li, 4, a.top, [&](int rank, float v, int i) { put_top(a, t, rank, v, i, lse); });
+            for (int u = 0; u < U; ++u) {
+                const int p = (again * U + u) * WAVE + lane;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) take(v[u][j], cut.head + 8 * p + j, p < cut.pieces);
+            }
         }
-        return;
+        __syncthreads();
+        if (tid == 0) s_n = 0;
+        __syncthreads();
+        const bool used = lane < a.top && list.i != INT_MAX;  // (the first so many places)
+        const int places = __popcll(__ballot(used));
+        int base = 0;
+        if (lane == 0) base = atomicAdd(&s_n, places);
+        base = __builtin_amdgcn_readlane(base, 0);
+        if (used) s_keys[base + lane] = top_key(list.v, list.i);
+        __syncthreads();
+        n = s_n;
     }
+    const float lse = a.splits == 1 ? s_lse : 0.f;
     const int64_t part = t * a.splits + split;
-    if (threadIdx.x == 0) {
-        a.part_st[3 * part] = st.m;
-        a.part_st[3 * part + 1] = st.s;
-        a.part_st[3 * part + 2] = st.u;
-    }
-    if constexpr (TOP) {
-        merge_lists(s_lv, s_li, 4, a.top, [&](int rank, float v, int i) {
-            a.part_v[part * a.top + rank] = v;
-            a.part_i[part * a.top + rank] = i;
-        });
-    }
+    rank_keys(s_keys, n, a.top, [&](int rank, TopKey key) {
+        if (a.splits == 1) put_top(a, t, rank, key, lse);
+        else a.part_key[part * a.top + rank] = key;
+    });
 }
 
-constexpr int MAX_SPLITS = 64;
-
-// The parts of a row joined, in order, by a block.
+// The parts of a row joined, in order, by a block. With j the least such that
+// the parts' first j keys are k or more, the ceil(k / j)-th of the parts' j-th
+// keys has k keys at or ahead of it: what is behind it is left out, and the rest
+// ranked. (Of 38 parts of 20 keys each some 40 are left, and 450 if only the
+// parts' last keys are gone by.)
 template <int TY>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
-    extern __shared__ float s_lists[];
+    __shared__ TopKey s_last, s_keys[MAX_SPLITS * WAVE];
+    __shared__ int s_n;
     __shared__ float s_lse;
+    const int tid = int(threadIdx.x), n = a.splits * a.top;
     const int64_t t = blockIdx.x;
-    const int n = a.splits * a.top;
-    float *lv = s_lists;
-    int *li = reinterpret_cast<int *>(s_lists + n);
-    for (int e = int(threadIdx.x); e < n; e += 256) {
-        lv[e] = a.part_v[t * n + e];
-        li[e] = a.part_i[t * n + e];
+    const TopKey *parts = a.part_key + t * n;
+    const int j = (a.top + a.splits - 1) / a.splits, m = j ? (a.top + j - 1) / j : 0;
+    if (tid == 0) {
+        s_last = 1;
+        s_n = 0;
     }
-    if (threadIdx.x < WAVE) {
+    if (a.top && tid < WAVE) s_keys[tid] = tid < a.splits ? parts[tid * a.top + j - 1] : 0;
+    __syncthreads();
+    if (a.top && tid < WAVE) {
+        const TopKey own = s_keys[tid];
+        int rank = 0;
+#pragma unroll 16
+        for (int l = 0; l < WAVE; ++l) rank += int(s_keys[l] > own);
+        if (rank == m - 1 && own) s_last = own;  // (keys differ: one lane)
+    }
+    if (tid >= 192) {
+        const int lane = tid - 192;
         SoftStats st;
         st.clear();
-        if (int(threadIdx.x) < a.splits) {
-            const float *p = a.part_st + 3 * (t * a.splits + int(threadIdx.x));
+        if (lane < a.splits) {
+            const float *p = a.part_st + 3 * (t * a.splits + lane);
             st = SoftStats{p[0], p[1], p[2]};
         }
         st = wave_join(st);
         constexpr int Z = TY == 0 ? 4 : 2;
-        if (threadIdx.x == 0)
-            s_lse = finish_row<TY>(a, t, static_cast<const char *>(a.logits) + t * a.ld * Z, st);
+        if (lane == 0) s_lse = finish_row<TY>(a, t, static_cast<const char *>(a.logits) + t * a.ld * Z, st);
+    }
+    if (!a.top) return;
+    __syncthreads();
+    const TopKey last = s_last;
+    for (int e = tid; e < n; e += 256) {
+        const TopKey key = parts[e];
+        if (key >= last) s_keys[atomicAdd(&s_n, 1)] = key;
     }
     __syncthreads();
     const float lse = s_lse;
-    merge_lists(lv, li, a.splits, a.top, [&](int rank, float v, int i) { put_top(a, t, rank, v, i, lse); });
+    rank_keys(s_keys, s_n, a.top, [&](int rank, TopKey key) { put_top(a, t, rank, key, lse); });
 }
 
-// Pieces of a step by the row count, and parts of a row: enough blocks for the
-// chip, at least one step for each wave.
-static int logprob_unroll(int T) { return T >= 64 ? 4 : 2; }
-int logprob_splits(int T, int V) {
-    const int wave = 8 * WAVE * logprob_unroll(T), steps = std::max(1, V / wave);
+// Few rows: a part of a row is what four waves hold at once (a row of 151936
+// in 38 parts). Else a block takes a row, or a part of it while there are too few
+// blocks for the chip, with at least a step for each wave.
+static int logprob_few_parts(int T, int V) {
+    const int parts = std::max(1, (V / 8 + FEW_PIECES - 1) / FEW_PIECES);
+    return T < 64 && parts <= MAX_SPLITS ? parts : 0;
+}
+constexpr int LOGPROB_U = 4;
+static int logprob_splits(int T, int V) {
+    if (const int few = logprob_few_parts(T, V)) return few;
+    const int steps = std::max(1, V / (8 * WAVE * LOGPROB_U));
     return std::max(1, std::min({(2048 + T - 1) / T, (steps + 3) / 4, MAX_SPLITS}));
 }
 
@@ -449,20 +615,23 @@ size_t logprobs_workspace_bytes(int T, int V, int top) {
 void launch_logprobs(LogprobArgs a, void *ws, hipStream_t s) {
     a.splits = logprob_splits(a.T, a.V);
     const size_t parts = size_t(a.T) * size_t(a.splits);
-    a.part_st = static_cast<float *>(ws);
-    a.part_v = a.part_st + 3 * parts;
-    a.part_i = reinterpret_cast<int *>(a.part_v + parts * size_t(a.top));
+    a.part_key = static_cast<unsigned long long *>(ws);
+    a.part_st = reinterpret_cast<float *>(a.part_key + parts * size_t(a.top));
     by_type(a.type, [&](auto ty) {
         constexpr int TY = decltype(ty)::value;
-        auto run = [&](auto u) {
-            constexpr int U = decltype(u)::value;
-            if (a.top) logprobs_kernel<TY, true, U><<<unsigned(parts), 256, 0, s>>>(a);
-            else logprobs_kernel<TY, false, U><<<unsigned(parts), 256, 0, s>>>(a);
-        };
-        if (logprob_unroll(a.T) == 4) run(Int<4>{});
-        else run(Int<2>{});
-        if (a.splits > 1)
-            logprobs_join_kernel<TY><<<unsigned(a.T), 256, size_t(a.splits) * size_t(a.top) * 8, s>>>(a);
+        if (logprob_few_parts(a.T, a.V)) {
+            if (a.top) logprobs_few_kernel<TY, true><<<unsigned(parts), 256, 0, s>>>(a);
+            else logprobs_few_kernel<TY, false><<<unsigned(parts), 256, 0, s>>>(a);
+        } else {
+            // (a wave's steps at most; a row's cut can only make them fewer)
+            const int steps = (a.V / 8 + WAVE * LOGPROB_U - 1) / (WAVE * LOGPROB_U);
+            const int wave = ((steps + a.splits - 1) / a.splits + 3) / 4;
+            a.slot_steps = std::max(1, (wave + TOP_SLOTS - 1) / TOP_SLOTS);
+            const size_t lds = size_t((wave + a.slot_steps - 1) / a.slot_steps) * 1024;
+            if (a.top) logprobs_kernel<TY, true, LOGPROB_U><<<unsigned(parts), 256, lds, s>>>(a);
+            else logprobs_kernel<TY, false, LOGPROB_U><<<unsigned(parts), 256, 0, s>>>(a);
+        }
+        if (a.splits > 1) logprobs_join_kernel<TY><<<unsigned(a.T), 256, 0, s>>>(a);
     });
 }
 

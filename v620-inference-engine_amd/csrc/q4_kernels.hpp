@@ -449,9 +449,9 @@ struct LogprobArgs {
     int32_t *top_i;
     float *top_v;
     // set by the launch:
-    int splits;
-    float *part_st, *part_v;  // [T][splits][3], [T][splits][top]
-    int *part_i;
+    int splits, slot_steps;
+    unsigned long long *part_key;  // [T][splits][top], value and index in one number
+    float *part_st;                // [T][splits][3]
 };
 size_t logprobs_workspace_bytes(int T, int V, int top);
 void launch_logprobs(LogprobArgs a, void *ws, hipStream_t s);
