@@ -22,27 +22,6 @@
 
 namespace qwq4 {
 
-// fp32 pairs -> 16-bit pairs (nearest even) and back
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-template <class T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    const f32x2 f = {a, b};
-    if constexpr (__is_same(T, BF16)) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
-    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, f16x2));
-}
-template <class T>
-__device__ __forceinline__ void unpack2(uint32_t w, float &a, float &b) {
-    if constexpr (__is_same(T, BF16)) {
-        a = __builtin_bit_cast(float, w << 16);
-        b = __builtin_bit_cast(float, w & 0xffff0000u);
-    } else {
-        a = f16_bits_to_f32(uint16_t(w));
-        b = f16_bits_to_f32(uint16_t(w >> 16));
-    }
-}
-
 // 8 fp32 values as PARTS operands of 8 16-bit values that add up to them.
 template <class T, int PARTS>
 __device__ __forceinline__ void split8(const float (&f)[8], uint4 (&part)[PARTS]) {
@@ -93,50 +72,90 @@ __device__ __forceinline__ int adapter_of(const int32_t *ids, int t, int T, int 
 }
 
 // ------------------------------------------------------------ shrink
-// v[t][r] = sum_k A[id_t][r][k] x[t][k] for 16 tokens by a block whose 8 waves
-// split K in 64-wide steps and join their sums in LDS, in order: a row's bits
-// depend on neither the batch nor its place in it. RF: 16-row pieces of A.
+// A wave's 16 rows of 64 16-bit elements on their way from memory to MFMA
+// operands: read with eight lanes to a row (a 128-byte line each, where the
+// operand's lane order would touch 16 lines with every 16 lanes and move 7
+// bytes a cycle), turned in LDS. The 16-byte piece p of row r lies at place p ^ (r &
+// 7) of its row: without bank conflicts both ways.
+struct Turned {
+    uint4 w[2];
+    // row(r): the row's pointer; the first n of the 64 elements exist
+    template <class Row>
+    __device__ __forceinline__ void load(Row row, int n) {
+        const int lane = int(threadIdx.x) % WAVE, k = lane % 8 * 8;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            w[i] = k < n ? *reinterpret_cast<const uint4 *>(row(i) + k) : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void turn(uint4 *lds) {
+        const int lane = int(threadIdx.x) % WAVE, r = lane / 8, c = lane % 16, g = lane / 16;
+        wave_lds_order();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) lds[(8 * i + r) * 8 + (lane % 8 ^ r)] = w[i];
+        wave_lds_order();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[h] = lds[c * 8 + ((4 * h + g) ^ (c & 7))];
+    }
+    // (a wave's LDS accesses complete in order; the compiler must keep them so)
+    __device__ static __forceinline__ void wave_lds_order() {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+        __builtin_amdgcn_wave_barrier();
+    }
+};
+
+// v[t][r] = sum_k A[id_t][r][k] x[t][k] for 16 tokens and 16 RF ranks by a block
+// whose 16 waves take a run of 64-wide steps of K each and join their sums in
+// LDS, in order: a row's bits depend on neither the batch nor its place in it.
+// Every wave has U steps of rows and weights on their way.
 template <class T16, int RF>
-__global__ __launch_bounds__(512) void lora_shrink_kernel(LoraShrinkArgs a) {
-    constexpr int NW = 8, U = RF == 1 ? 4 : RF == 2 ? 2 : 1;
-    __shared__ f32x4 s_part[NW][RF][WAVE];
+__global__ __launch_bounds__(1024) void lora_shrink_kernel(LoraShrinkArgs a) {
+    constexpr int NW = 16, U = RF == 1 ? 4 : RF == 2 ? 3 : 2;
+    __shared__ uint4 s_turn[NW][2][128];  // (4 KB a wave, and then the waves' sums)
+    f32x4(*s_part)[RF][WAVE] = reinterpret_cast<f32x4(*)[RF][WAVE]>(s_turn);
+    static_assert(sizeof(f32x4) * NW * RF * WAVE <= sizeof(s_turn), "the sums fit");
     const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
-    const int c = lane % 16, g = lane / 16, t0 = int(blockIdx.x) * 16, t = min(t0 + c, a.T - 1);
+    const int c = lane % 16, g = lane / 16, t0 = int(blockIdx.x) * 16, t = t0 + c;
+    const int r0 = int(blockIdx.z) * (16 * RF);
     const int id = lane < 16 ? adapter_of(a.ids, t0 + lane, a.T, a.L) : -1;
-    const int steps = (a.K + 63) / 64;
-    const uint16_t *x = a.x + int64_t(t) * a.ldx + 16 * g;
+    const int steps = (a.K + 63) / 64, per = (steps + NW - 1) / NW, end = min(steps, (wave + 1) * per);
+    const uint16_t *x[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) x[i] = a.x + int64_t(min(t0 + 8 * i + lane / 8, a.T - 1)) * a.ldx;
     each_adapter(id, int(blockIdx.y), int(gridDim.y), [&](int l, unsigned long long mine) {
-        const uint16_t *w[RF];
+        const uint16_t *w[RF][2];
 #pragma unroll
         for (int f = 0; f < RF; ++f)
-            w[f] = a.A + (int64_t(l) * a.R + min(16 * f + c, a.R - 1)) * a.K + 16 * g;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                w[f][i] = a.A + (int64_t(l) * a.R + min(r0 + 16 * f + 8 * i + lane / 8, a.R - 1)) * a.K;
         f32x4 acc[RF];
 #pragma unroll
         for (int f = 0; f < RF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int s0 = wave; s0 < steps; s0 += NW * U) {
-            uint4 xf[U][2], wf[U][RF][2];
+        for (int s0 = wave * per; s0 < end; s0 += U) {
+            Turned xf[U], wf[U][RF];
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+                const int k = (s0 + u) * 64, n = s0 + u < end ? a.K - k : 0;
+                xf[u].load([&](int i) { return x[i] + k; }, n);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int k = (s0 + NW * u) * 64 + 8 * h;
-                    const bool in = k + 16 * g < a.K;  // (K is a multiple of 8)
-                    xf[u][h] = in ? *reinterpret_cast<const uint4 *>(x + k) : make_uint4(0, 0, 0, 0);
+                for (int f = 0; f < RF; ++f) wf[u][f].load([&](int i) { return w[f][i] + k; }, n);
+            }
 #pragma unroll
-                    for (int f = 0; f < RF; ++f)
-                        wf[u][f][h] = in ? *reinterpret_cast<const uint4 *>(w[f] + k) : make_uint4(0, 0, 0, 0);
+            for (int u = 0; u < U; ++u) {
+                xf[u].turn(s_turn[wave][0]);
+#pragma unroll
+                for (int f = 0; f < RF; ++f) {
+                    wf[u][f].turn(s_turn[wave][1]);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) acc[f] = mfma16<T16>(wf[u][f].w[h], xf[u].w[h], acc[f]);
                 }
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int f = 0; f < RF; ++f) acc[f] = mfma16<T16>(wf[u][f][h], xf[u][h], acc[f]);
+            }
         }
+        __syncthreads();
 #pragma unroll
         for (int f = 0; f < RF; ++f) s_part[wave][f][lane] = acc[f];
         __syncthreads();
-        const int f = wave, r = 16 * f + 4 * g;  // (a wave adds a piece: RF <= 8)
+        const int f = wave, r = r0 + 16 * f + 4 * g;  // (a wave adds a piece: RF <= 16)
         if (f < RF && r < a.R && ((mine >> c) & 1)) {
             f32x4 sum = s_part[0][f][lane];
 #pragma unroll
@@ -150,17 +169,17 @@ __global__ __launch_bounds__(512) void lora_shrink_kernel(LoraShrinkArgs a) {
 void launch_lora_shrink(const LoraShrinkArgs &a, hipStream_t s) {
     const int tiles = (a.T + 15) / 16;
     // Adapters of a tile in parallel while there are few tiles (37 requests with an adapter each: every block takes
-    // one), all of a tile's by one block where the tiles fill the chip.
-    const int side = std::max(1, std::min({512 / tiles, 16, a.L, a.T}));
+    // one), all of a tile's by one block where the tiles fill the chip; ranks likewise, 16 or up to 64 a block.
+    const int side = std::max(1, std::min({256 / tiles, 16, a.L, a.T}));
     auto run = [&](auto t16, auto rf) {
-        lora_shrink_kernel<decltype(t16), decltype(rf)::value>
-            <<<dim3(unsigned(tiles), unsigned(side)), 512, 0, s>>>(a);
+        constexpr int RF = decltype(rf)::value;
+        lora_shrink_kernel<decltype(t16), RF>
+            <<<dim3(unsigned(tiles), unsigned(side), unsigned((a.R + 16 * RF - 1) / (16 * RF))), 1024, 0, s>>>(a);
     };
     auto by_rank = [&](auto t16) {
-        if (a.R <= 16) run(t16, Int<1>{});
+        if (a.R <= 16 || tiles * side < 128) run(t16, Int<1>{});
         else if (a.R <= 32) run(t16, Int<2>{});
-        else if (a.R <= 64) run(t16, Int<4>{});
-        else run(t16, Int<8>{});
+        else run(t16, Int<4>{});
     };
     if (a.f16) by_rank(F16{});
     else by_rank(BF16{});
@@ -168,87 +187,93 @@ void launch_lora_shrink(const LoraShrinkArgs &a, hipStream_t s) {
 
 // ------------------------------------------------------------ expand
 // out[t][n] = y[t][n] + scaling[id_t] sum_r B[id_t][n][r] v[t][r]: 16 NT tokens by
-// 64 columns a wave. The MFMA's rows are columns of y, dealt so that a lane
-// holds 16 neighbouring ones of a token (16-byte loads and stores; a row's 64
-// are written whole by its four lanes). K of the MFMA runs over the R values
-// of each of v's parts in turn. fp16 parts are of v times a power of two per
-// token, so that none of them overflows or loses bits to the range.
-template <class T16, int YT>
+// 128 columns a wave, 16 tokens at a time (NT = a.tiles, at most 4). The columns are dealt to 8 MFMAs so
+// that a lane holds 8 neighbouring ones of four tokens and 16 lanes a row's 128:
+// rows are read and written in 256-byte runs (four lanes to a token's 64 columns:
+// 47 us where this takes %s, 4096 x 12288 in bf16). K of the MFMA runs over the R values of
+// each of v's parts in turn. fp16 parts are of v times a power of two per token,
+// so that none of them overflows or loses bits to the range. Bound by memory.
+template <class T16, int YT, bool ONE>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
     constexpr bool HALF = __is_same(T16, F16);
-    constexpr int PARTS = YT == 0 ? 3 : 2, NT = YT == 0 ? 2 : 4;
+    constexpr int PARTS = YT == 0 ? 3 : 2;
     const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
     const int c = lane % 16, g = lane / 16;
-    const int t0 = int(blockIdx.y) * (16 * NT), n0 = (int(blockIdx.x) * 4 + wave) * 64;
-    if (n0 >= a.N) return;  // (no barrier below)
+    const int NT = a.tiles, t0 = int(blockIdx.y) * (16 * NT);
+    const int at = (int(blockIdx.x) * 4 + wave) * 128 + 8 * c;  // the lane's columns
+    const bool in = at < a.N;                                   // (N is a multiple of 8)
     const int id = lane < 16 * NT ? adapter_of(a.ids, t0 + lane, a.T, a.L) : -1;
-    const int octets = a.R / 8, steps = (PARTS * octets + 3) / 4;
-    const int at = n0 + 16 * g;  // the lane's columns of y
+    const int octets = a.R / 8, steps = ONE ? 1 : (PARTS * octets + 3) / 4;
     if (a.out != a.y && blockIdx.z == 0) {  // (rows without an adapter)
         const unsigned long long none = ~__ballot(id >= 0);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int t = t0 + 16 * i + c;
-            if (t >= a.T || !((none >> (16 * i + c)) & 1)) continue;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (at + 8 * h < a.N) {
-                    float f[8];
-                    row_load<YT == GRAD_F16 ? 2 : YT, 8>(a.y, t * a.ldy + at + 8 * h, f);
-                    row_store<YT, 8>(a.out, t * a.ldo + at + 8 * h, f);
-                }
+        for (int i = 0; i < 16 * NT; i += 4) {
+            const int t = t0 + i + g;
+            if (t < a.T && in && ((none >> (i + g)) & 1)) {
+                RowPiece<YT> y;
+                y.load(a.y, t * a.ldy + at);
+                y.store(a.out, t * a.ldo + at);
+            }
         }
     }
     each_adapter(id, int(blockIdx.z), int(gridDim.z), [&](int l, unsigned long long mine) {
         const float scale = a.scaling ? a.scaling[l] : 1.f;
-        float y[NT][2][8];
-        f32x4 acc[NT][4];
-        int shift[NT];
+        const uint16_t *w = a.B + (int64_t(l) * a.N + min(at, a.N - 8)) * a.R;
+        uint4 wf[8];
+        auto weights = [&](int q, uint4 (&to)[8]) {
+            const int o = 4 * q + g, p = o / octets, ro = p < PARTS ? o - p * octets : 0;
 #pragma unroll
+            for (int j = 0; j < 8; ++j) to[j] = *reinterpret_cast<const uint4 *>(w + j * a.R + 8 * ro);
+        };
+        // the tokens of tile i that are this adapter's, and their rows
+        auto tokens = [&](int i) { return i < NT ? uint32_t(mine >> (16 * i)) & 0xffffu : 0u; };
+        auto rows = [&](int i, RowPiece<YT> (&y)[4]) {
+            const uint32_t here = tokens(i) >> (4 * g);
+            const int64_t row = int64_t(t0 + 16 * i + 4 * g) * a.ldy + at;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (in && ((here >> e) & 1)) y[e].load(a.y, row + e * a.ldy);
+        };
+        RowPiece<YT> next[4];
+        rows(0, next);
+        weights(0, wf);
+#pragma unroll 1
         for (int i = 0; i < NT; ++i) {
-            const int t = t0 + 16 * i + c;
-            const bool own = (mine >> (16 * i + c)) & 1;
+            RowPiece<YT> y[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (own && at + 8 * h < a.N) row_load<YT == GRAD_F16 ? 2 : YT, 8>(a.y, t * a.ldy + at + 8 * h, y[i][h]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < 4; ++e) y[e] = next[e];
+            rows(i + 1, next);
+            const uint32_t here = tokens(i);
+            if (!here) continue;
+            const bool own = (here >> c) & 1;  // (token c's values of v are this lane's operand)
+            const float *v = a.v + int64_t(t0 + 16 * i + c) * a.R;
+            int shift = 0;
             if constexpr (HALF) {
                 float top = 0.f;
                 for (int o = g; own && o < octets; o += 4) {
                     float f[8];
-                    load8(a.v + int64_t(t) * a.R + 8 * o, f);
+                    load8(v + 8 * o, f);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j] * scale));
                 }
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
                 // (2^shift top below 2^15)
-                shift[i] = 141 - int((__builtin_bit_cast(uint32_t, top) >> 23) & 255u);
+                shift = 141 - int((__builtin_bit_cast(uint32_t, top) >> 23) & 255u);
             }
-        }
-        const uint16_t *w[4];
+            f32x4 acc[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int n = min(n0 + 16 * (c / 4) + 4 * j + c % 4, a.N - 1);
-            w[j] = a.B + (int64_t(l) * a.N + n) * a.R;
-        }
-        for (int q = 0; q < steps; ++q) {
-            const int o = 4 * q + g, p = o / octets, ro = p < PARTS ? o - p * octets : 0;
-            uint4 wf[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) wf[j] = *reinterpret_cast<const uint4 *>(w[j] + 8 * ro);
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                if (!((mine >> (16 * i)) & 0xffffu)) continue;
-                const int t = t0 + 16 * i + c;
+            for (int j = 0; j < 8; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int q = 0; q < steps; ++q) {
+                const int o = 4 * q + g, p = o / octets;
+                uint4 after[8];
+                if constexpr (!ONE) weights(q + 1 < steps ? q + 1 : 0, after);  // (the next tile begins anew)
                 float f[8] = {};
-                if (((mine >> (16 * i + c)) & 1) && p < PARTS) {
-                    load8(a.v + int64_t(t) * a.R + 8 * ro, f);
+                if (own && p < PARTS) {
+                    load8(v + 8 * (o - p * octets), f);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         f[j] *= scale;
-                        if constexpr (HALF) f[j] = __builtin_ldexpf(f[j], shift[i]);
+                        if constexpr (HALF) f[j] = __builtin_ldexpf(f[j], shift);
                     }
                 }
                 uint4 part[PARTS];
@@ -259,36 +284,44 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
                     if (p == 2) vf = part[2];
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = mfma16<T16>(wf[j], vf, acc[i][j]);
+                for (int j = 0; j < 8; ++j) {
+                    acc[j] = mfma16<T16>(vf, wf[j], acc[j]);
+                    if constexpr (!ONE) wf[j] = after[j];
+                }
             }
-        }
+            const int64_t row = int64_t(t0 + 16 * i + 4 * g) * a.ldo + at;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            if (!((mine >> (16 * i + c)) & 1)) continue;
-            const int64_t row = int64_t(t0 + 16 * i + c) * a.ldo;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (at + 8 * h >= a.N) continue;
+            for (int e = 0; e < 4; ++e) {
+                int back = 0;
+                if constexpr (HALF) back = -__shfl(shift, 4 * g + e);  // (token 4 g + e's, from the lane that scaled it)
+                if (!in || !((here >> (4 * g + e)) & 1)) continue;
                 float f[8];
+                y[e].values(f);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    float d = acc[i][2 * h + j / 4][j % 4];
-                    if constexpr (HALF) d = __builtin_ldexpf(d, -shift[i]);
-                    f[j] = y[i][h][j] + d;
+                    float d = acc[j][e];
+                    if constexpr (HALF) d = __builtin_ldexpf(d, back);
+                    f[j] += d;
                 }
-                row_store<YT, 8>(a.out, row + at + 8 * h, f);
+                y[e].template set<YT == GRAD_F16>(f);
+                y[e].store(a.out, row + e * a.ldo);
             }
         }
     });
 }
 
-void launch_lora_expand(const LoraExpandArgs &a, hipStream_t s) {
+void launch_lora_expand(LoraExpandArgs a, hipStream_t s) {
     auto run = [&](auto t16, auto yt) {
-        constexpr int YT = decltype(yt)::value, GROUP = YT == 0 ? 32 : 64;
-        const int groups = (a.T + GROUP - 1) / GROUP, cols = (a.N + 255) / 256;
-        const int side = std::max(1, std::min({1024 / (groups * cols), GROUP, a.L, a.T}));
-        lora_expand_kernel<decltype(t16), YT>
-            <<<dim3(unsigned(cols), unsigned(groups), unsigned(side)), 256, 0, s>>>(a);
+        constexpr int YT = decltype(yt)::value;
+        // Tiles of a block: the weights are read once for all of them, but first of all the chip is to be filled; then
+        // the adapters of a block's tokens side by side.
+        const int tiles = (a.T + 15) / 16, cols = (a.N + 511) / 512;
+        a.tiles = tiles * cols >= 2048 ? 4 : tiles * cols >= 1024 ? 2 : 1;
+        const int groups = (tiles + a.tiles - 1) / a.tiles;
+        const int side = std::max(1, std::min({1024 / (groups * cols), 16 * a.tiles, a.L, a.T}));
+        const dim3 grid{unsigned(cols), unsigned(groups), unsigned(side)};
+        if ((YT == 0 ? 3 : 2) * a.R <= 32) lora_expand_kernel<decltype(t16), YT, true><<<grid, 256, 0, s>>>(a);
+        else lora_expand_kernel<decltype(t16), YT, false><<<grid, 256, 0, s>>>(a);
     };
     auto by_16 = [&](auto yt) {
         if (a.f16) run(F16{}, yt);

@@ -394,9 +394,10 @@ struct LoraExpandArgs {
     void *out;
     int64_t ldo;
     int y_type;
-    bool grad;  // fp16 overflows to infinities (else saturates)
+    bool grad;      // fp16 overflows to infinities (else saturates)
+    int tiles = 1;  // of 16 tokens, of a block: set by the launch
 };
-void launch_lora_expand(const LoraExpandArgs &a, hipStream_t s);
+void launch_lora_expand(LoraExpandArgs a, hipStream_t s);
 struct LoraTransposeArgs {
     const uint16_t *in;  // [L][rows][cols]
     uint16_t *out;

@@ -231,48 +231,79 @@ void launch_rms_norm(const NormArgs &a, hipStream_t s) {
 }
 
 // ------------------------------------------------------------ gradients
+// 8 elements of a row on their way: as they lie, or (single elements) values.
+template <int TY, bool VEC>
+struct Part {
+    RowPiece<TY> w;
+    __device__ __forceinline__ void load(const void *x, int64_t row, int j, int) { w.load(x, row + j); }
+    __device__ __forceinline__ void values(float (&v)[8]) const { w.values(v); }
+};
+template <int TY>
+struct Part<TY, false> {
+    float f[8];
+    __device__ __forceinline__ void load(const void *x, int64_t row, int j, int n) { part_load<TY, false>(x, row, j, n, f); }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = f[e];
+    }
+};
+
 // A block of TH threads takes rows blockIdx.x, blockIdx.x + gridDim.x, .., 8
-// elements per thread and C turns each, with the next row's h and dy requested
-// before the current one's sums, and keeps its columns' part of dw in
-// registers; the blocks' parts are added in order by a second launch.
+// elements per thread and C turns each, with the next row on its way while the
+// current one's sums are made, and keeps its columns' part of dw in registers;
+// the blocks' parts are added in order by a second launch. Bound by memory.
 template <int DT, int HT, int WT, bool VEC, int TH, int C>
 __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
     constexpr int NW = TH / WAVE;
     __shared__ float s_sum[2][2][NW];
     const int tid = int(threadIdx.x), H = a.H;
-    float w[C][8], dw[C][8], h[2][C][8], d[2][C][8];
-    auto load = [&](int64_t t, float (&hv)[C][8], float (&dv)[C][8]) {
+    struct Row {
+        Part<HT, VEC> h[C], res[C];
+        Part<DT, VEC> d[C];
+    } next;
+    Part<WT, VEC> wp[C];
+    float dw[C][8];
+    auto load = [&](int64_t t) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int j = (tid + c * TH) * 8;
-            if (j < H) {
-                part_load<HT, VEC>(a.h, t * a.ldh, j, H, hv[c]);
-                part_load<DT, VEC>(a.dy, t * a.lddy, j, H, dv[c]);
-            }
+            if (j >= H) continue;
+            next.h[c].load(a.h, t * a.ldh, j, H);
+            next.d[c].load(a.dy, t * a.lddy, j, H);
+            if (a.dres) next.res[c].load(a.dres, t * a.lddr, j, H);
         }
     };
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int j = (tid + c * TH) * 8;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[c][e] = dw[c][e] = h[0][c][e] = d[0][c][e] = h[1][c][e] = d[1][c][e] = 0.f;
-        if (j < H) part_load<WT, VEC>(a.w, 0, j, H, w[c]);
+        for (int e = 0; e < 8; ++e) dw[c][e] = 0.f;
+        if (j < H) wp[c].load(a.w, 0, j, H);
     }
-    auto row = [&](int64_t t, int p, const float (&hv)[C][8], const float (&dv)[C][8]) {
-        float res[C][8];
-        float sum = 0.f, dot = 0.f;
+    if (int64_t(blockIdx.x) < a.T) load(blockIdx.x);
+    int p = 0;
+    for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x, p ^= 1) {
+        const Row row = next;
+        if (t + gridDim.x < a.T) load(t + gridDim.x);
+        float h[C][8], g[C][8], sum = 0.f, dot = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int j = (tid + c * TH) * 8;
-            if (a.dres && j < H) part_load<HT, VEC>(a.dres, t * a.lddr, j, H, res[c]);
+            if ((tid + c * TH) * 8 >= H) continue;
+            float w[8];
+            row.h[c].values(h[c]);
+            row.d[c].values(g[c]);
+            wp[c].values(w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                sum = __builtin_fmaf(hv[c][e], hv[c][e], sum);
-                dot = __builtin_fmaf(dv[c][e] * w[c][e], hv[c][e], dot);
+                sum = __builtin_fmaf(h[c][e], h[c][e], sum);
+                dot = __builtin_fmaf(g[c][e] * w[e], h[c][e], dot);
             }
         }
-        sum = wave_add(sum);
-        dot = wave_add(dot);
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) {
+            sum += __shfl_xor(sum, o);
+            dot += __shfl_xor(dot, o);
+        }
         if (tid % WAVE == 0) {
             s_sum[p][0][tid / WAVE] = sum;
             s_sum[p][1][tid / WAVE] = dot;
@@ -288,29 +319,22 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int j = (tid + c * TH) * 8;
-            float o[8];
+            if (j >= H) continue;
+            float o[8], w[8];
+            wp[c].values(w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                o[e] = r * (dv[c][e] * w[c][e] - hv[c][e] * k);
-                dw[c][e] = __builtin_fmaf(dv[c][e], hv[c][e] * r, dw[c][e]);
+                o[e] = r * (g[c][e] * w[e] - h[c][e] * k);
+                dw[c][e] = __builtin_fmaf(g[c][e], h[c][e] * r, dw[c][e]);
             }
-            if (j >= H) continue;
             if (a.dres) {
+                float res[8];
+                row.res[c].values(res);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] += res[c][e];
+                for (int e = 0; e < 8; ++e) o[e] += res[e];
             }
             part_store<HT == 2 ? GRAD_F16 : HT, VEC>(a.dx, t * a.lddx, j, H, o);
         }
-    };
-    int64_t t = blockIdx.x;
-    const int64_t step = gridDim.x;
-    if (t < a.T) load(t, h[0], d[0]);
-    for (; t < a.T; t += 2 * step) {
-        if (t + step < a.T) load(t + step, h[1], d[1]);
-        row(t, 0, h[0], d[0]);
-        if (t + step >= a.T) break;
-        if (t + 2 * step < a.T) load(t + 2 * step, h[0], d[0]);
-        row(t + step, 1, h[1], d[1]);
     }
     if (!a.dw) return;
 #pragma unroll

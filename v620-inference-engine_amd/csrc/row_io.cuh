@@ -86,6 +86,71 @@ inline bool rows_aligned(const void *p, int type, int64_t ld, int V) {
     return !p || (reinterpret_cast<uintptr_t>(p) % size_t(a) == 0 && ld * z % a == 0);
 }
 
+// fp32 pairs -> 16-bit pairs (nearest even) and back
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const f32x2 f = {a, b};
+    if constexpr (__is_same(T, BF16)) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, f16x2));
+}
+template <class T>
+__device__ __forceinline__ void unpack2(uint32_t w, float &a, float &b) {
+    if constexpr (__is_same(T, BF16)) {
+        a = __builtin_bit_cast(float, w << 16);
+        b = __builtin_bit_cast(float, w & 0xffff0000u);
+    } else {
+        a = f16_bits_to_f32(uint16_t(w));
+        b = f16_bits_to_f32(uint16_t(w >> 16));
+    }
+}
+
+// 8 elements of a row as they lie (16-byte aligned), and their values.
+template <int YT>
+struct RowPiece {
+    uint4 w[YT == 0 ? 2 : 1];
+    __device__ __forceinline__ void load(const void *p, int64_t i) {
+        const char *at = static_cast<const char *>(p) + i * (YT == 0 ? 4 : 2);
+        w[0] = reinterpret_cast<const uint4 *>(at)[0];
+        if constexpr (YT == 0) w[1] = reinterpret_cast<const uint4 *>(at)[1];
+    }
+    // (fp16: finite values beyond its range saturate, or, as a gradient, become infinite)
+    template <bool GRAD>
+    __device__ __forceinline__ void set(float (&v)[8]) {
+        if constexpr (YT == 0) {
+            w[0] = __builtin_bit_cast(uint4, f32x4{v[0], v[1], v[2], v[3]});
+            w[1] = __builtin_bit_cast(uint4, f32x4{v[4], v[5], v[6], v[7]});
+        } else {
+            using T = std::conditional_t<YT == 1, BF16, F16>;
+            if constexpr (YT != 1 && !GRAD) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = __builtin_isfinite(v[j]) ? fminf(fmaxf(v[j], -65504.f), 65504.f) : v[j];
+            }
+            w[0] = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+        }
+    }
+    __device__ __forceinline__ void store(void *p, int64_t i) const {
+        char *at = static_cast<char *>(p) + i * (YT == 0 ? 4 : 2);
+        reinterpret_cast<uint4 *>(at)[0] = w[0];
+        if constexpr (YT == 0) reinterpret_cast<uint4 *>(at)[1] = w[1];
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        if constexpr (YT == 0) {
+            const f32x4 a = __builtin_bit_cast(f32x4, w[0]), b = __builtin_bit_cast(f32x4, w[1]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = a[j], v[j + 4] = b[j];
+        } else {
+            using T = std::conditional_t<YT == 1, BF16, F16>;
+            unpack2<T>(w[0].x, v[0], v[1]);
+            unpack2<T>(w[0].y, v[2], v[3]);
+            unpack2<T>(w[0].z, v[4], v[5]);
+            unpack2<T>(w[0].w, v[6], v[7]);
+        }
+    }
+};
+
 template <int N>
 using Int = std::integral_constant<int, N>;
 
