@@ -106,10 +106,10 @@ struct Turned {
 // v[t][r] = sum_k A[id_t][r][k] x[t][k] for 16 tokens and 16 RF ranks by a block
 // whose 16 waves take a run of 64-wide steps of K each and join their sums in
 // LDS, in order: a row's bits depend on neither the batch nor its place in it.
-// Every wave has U steps of rows and weights on their way.
+// Every wave has the next U steps of rows and weights on their way.
 template <class T16, int RF>
 __global__ __launch_bounds__(1024) void lora_shrink_kernel(LoraShrinkArgs a) {
-    constexpr int NW = 16, U = RF == 1 ? 4 : RF == 2 ? 3 : 2;
+    constexpr int NW = 16, U = RF == 1 ? 2 : 1;
     __shared__ uint4 s_turn[NW][2][128];  // (4 KB a wave, and then the waves' sums)
     f32x4(*s_part)[RF][WAVE] = reinterpret_cast<f32x4(*)[RF][WAVE]>(s_turn);
     static_assert(sizeof(f32x4) * NW * RF * WAVE <= sizeof(s_turn), "the sums fit");
@@ -122,32 +122,39 @@ __global__ __launch_bounds__(1024) void lora_shrink_kernel(LoraShrinkArgs a) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) x[i] = a.x + int64_t(min(t0 + 8 * i + lane / 8, a.T - 1)) * a.ldx;
     each_adapter(id, int(blockIdx.y), int(gridDim.y), [&](int l, unsigned long long mine) {
-        const uint16_t *w[RF][2];
+        const uint16_t *A = a.A + int64_t(l) * a.R * a.K;
+        uint32_t w[RF][2];  // (R K is below 2^28)
 #pragma unroll
         for (int f = 0; f < RF; ++f)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                w[f][i] = a.A + (int64_t(l) * a.R + min(r0 + 16 * f + 8 * i + lane / 8, a.R - 1)) * a.K;
+            for (int i = 0; i < 2; ++i) w[f][i] = uint32_t(min(r0 + 16 * f + 8 * i + lane / 8, a.R - 1)) * uint32_t(a.K);
         f32x4 acc[RF];
 #pragma unroll
         for (int f = 0; f < RF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int s0 = wave * per; s0 < end; s0 += U) {
-            Turned xf[U], wf[U][RF];
+        struct Steps {
+            Turned x[U], w[U][RF];
+        } next;
+        auto load = [&](int s0) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int k = (s0 + u) * 64, n = s0 + u < end ? a.K - k : 0;
-                xf[u].load([&](int i) { return x[i] + k; }, n);
+                next.x[u].load([&](int i) { return x[i] + k; }, n);
 #pragma unroll
-                for (int f = 0; f < RF; ++f) wf[u][f].load([&](int i) { return w[f][i] + k; }, n);
+                for (int f = 0; f < RF; ++f) next.w[u][f].load([&](int i) { return A + (w[f][i] + uint32_t(k)); }, n);
             }
+        };
+        load(wave * per);
+        for (int s0 = wave * per; s0 < end; s0 += U) {
+            Steps now = next;
+            if (s0 + U < end) load(s0 + U);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                xf[u].turn(s_turn[wave][0]);
+                now.x[u].turn(s_turn[wave][0]);
 #pragma unroll
                 for (int f = 0; f < RF; ++f) {
-                    wf[u][f].turn(s_turn[wave][1]);
+                    now.w[u][f].turn(s_turn[wave][1]);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) acc[f] = mfma16<T16>(wf[u][f].w[h], xf[u].w[h], acc[f]);
+                    for (int h = 0; h < 2; ++h) acc[f] = mfma16<T16>(now.w[u][f].w[h], now.x[u].w[h], acc[f]);
                 }
             }
         }
@@ -187,21 +194,30 @@ void launch_lora_shrink(const LoraShrinkArgs &a, hipStream_t s) {
 
 // ------------------------------------------------------------ expand
 // out[t][n] = y[t][n] + scaling[id_t] sum_r B[id_t][n][r] v[t][r]: 16 NT tokens by
-// 128 columns a wave, 16 tokens at a time (NT = a.tiles, at most 4). The columns are dealt to 8 MFMAs so
-// that a lane holds 8 neighbouring ones of four tokens and 16 lanes a row's 128:
-// rows are read and written in 256-byte runs (four lanes to a token's 64 columns:
-// 47 us where this takes %s, 4096 x 12288 in bf16). K of the MFMA runs over the R values of
+// 128 columns a wave, 16 tokens at a time (NT = a.tiles, at most 4). The columns
+// are dealt to 8 MFMAs so that a lane holds 8 neighbouring ones of four tokens
+// and 16 lanes a row's 128: rows are read and written in 256-byte runs (four lanes
+// to a token's 64 columns: 47 us where this takes @@, 4096 x 12288 in bf16), past
+// the caches (kept in them: 5 us more). K of the MFMA runs over the R values of
 // each of v's parts in turn. fp16 parts are of v times a power of two per token,
 // so that none of them overflows or loses bits to the range. Bound by memory.
+// ONE: one step of the MFMA covers all parts, and its weights stay in registers.
+// Else they lie in LDS, a wave's 128 rows of B as one run of memory (read for
+// every tile in the MFMA's order, they touch a line per lane: 4096 x 12288 of rank 64
+// 172 us where this takes @@); 16-byte piece p of them at place p ^ (row / 8 & 7):
+// without bank conflicts.
 template <class T16, int YT, bool ONE>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
     constexpr bool HALF = __is_same(T16, F16);
     constexpr int PARTS = YT == 0 ? 3 : 2;
+    extern __shared__ uint4 s_weights[];  // ONE: none; [waves][128 R / 8]
     const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
     const int c = lane % 16, g = lane / 16;
     const int NT = a.tiles, t0 = int(blockIdx.y) * (16 * NT);
-    const int at = (int(blockIdx.x) * 4 + wave) * 128 + 8 * c;  // the lane's columns
-    const bool in = at < a.N;                                   // (N is a multiple of 8)
+    const int n0 = (int(blockIdx.x) * (int(blockDim.x) / WAVE) + wave) * 128;
+    if (n0 >= a.N) return;  // (no barrier below)
+    const int at = n0 + 8 * c;    // the lane's columns
+    const bool in = at < a.N;     // (N is a multiple of 8)
     const int id = lane < 16 * NT ? adapter_of(a.ids, t0 + lane, a.T, a.L) : -1;
     const int octets = a.R / 8, steps = ONE ? 1 : (PARTS * octets + 3) / 4;
     if (a.out != a.y && blockIdx.z == 0) {  // (rows without an adapter)
@@ -210,20 +226,15 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
             const int t = t0 + i + g;
             if (t < a.T && in && ((none >> (i + g)) & 1)) {
                 RowPiece<YT> y;
-                y.load(a.y, t * a.ldy + at);
-                y.store(a.out, t * a.ldo + at);
+                y.load_stream(a.y, t * a.ldy + at);
+                y.store_stream(a.out, t * a.ldo + at);
             }
         }
     }
+    uint4 *lds = s_weights + wave * 128 * octets;
     each_adapter(id, int(blockIdx.z), int(gridDim.z), [&](int l, unsigned long long mine) {
         const float scale = a.scaling ? a.scaling[l] : 1.f;
-        const uint16_t *w = a.B + (int64_t(l) * a.N + min(at, a.N - 8)) * a.R;
-        uint4 wf[8];
-        auto weights = [&](int q, uint4 (&to)[8]) {
-            const int o = 4 * q + g, p = o / octets, ro = p < PARTS ? o - p * octets : 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) to[j] = *reinterpret_cast<const uint4 *>(w + j * a.R + 8 * ro);
-        };
+        const uint16_t *B = a.B + (int64_t(l) * a.N + n0) * a.R;  // the wave's rows, min(128, N - n0) of them
         // the tokens of tile i that are this adapter's, and their rows
         auto tokens = [&](int i) { return i < NT ? uint32_t(mine >> (16 * i)) & 0xffffu : 0u; };
         auto rows = [&](int i, RowPiece<YT> (&y)[4]) {
@@ -231,11 +242,31 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
             const int64_t row = int64_t(t0 + 16 * i + 4 * g) * a.ldy + at;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (in && ((here >> e) & 1)) y[e].load(a.y, row + e * a.ldy);
+                if (in && ((here >> e) & 1)) y[e].load_stream(a.y, row + e * a.ldy);
         };
         RowPiece<YT> next[4];
         rows(0, next);
-        weights(0, wf);
+        // place o of v's parts and what it is: octet ro of part p (none from PARTS on)
+        auto place = [&](int q, int &p) {
+            const int o = 4 * q + g;
+            p = ONE ? (o >= octets) + (o >= 2 * octets) + (PARTS == 3 && o >= 3 * octets) : o / octets;
+            return p < PARTS ? o - p * octets : 0;
+        };
+        uint4 wf[8];
+        if constexpr (ONE) {
+            int p;
+            const uint16_t *w = B + min(8 * c, a.N - 8 - n0) * a.R + 8 * place(0, p);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) wf[j] = *reinterpret_cast<const uint4 *>(w + j * a.R);
+        } else {
+            const int n = min(128, a.N - n0) * octets;
+            const uint32_t inverse = (65536u + uint32_t(octets) - 1) / uint32_t(octets);  // (exact below 4096)
+            Turned::wave_lds_order();
+#pragma unroll 4
+            for (int i = lane; i < n; i += WAVE)
+                lds[i ^ int(((uint32_t(i) * inverse >> 16) >> 3) & 7)] = reinterpret_cast<const uint4 *>(B)[i];
+            Turned::wave_lds_order();
+        }
 #pragma unroll 1
         for (int i = 0; i < NT; ++i) {
             RowPiece<YT> y[4];
@@ -264,12 +295,15 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
             for (int q = 0; q < steps; ++q) {
-                const int o = 4 * q + g, p = o / octets;
-                uint4 after[8];
-                if constexpr (!ONE) weights(q + 1 < steps ? q + 1 : 0, after);  // (the next tile begins anew)
+                int p;
+                const int ro = place(q, p);
+                if constexpr (!ONE) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) wf[j] = lds[((8 * c + j) * octets + ro) ^ (c & 7)];
+                }
                 float f[8] = {};
                 if (own && p < PARTS) {
-                    load8(v + 8 * (o - p * octets), f);
+                    load8(v + 8 * ro, f);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         f[j] *= scale;
@@ -284,10 +318,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
                     if (p == 2) vf = part[2];
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    acc[j] = mfma16<T16>(vf, wf[j], acc[j]);
-                    if constexpr (!ONE) wf[j] = after[j];
-                }
+                for (int j = 0; j < 8; ++j) acc[j] = mfma16<T16>(vf, wf[j], acc[j]);
             }
             const int64_t row = int64_t(t0 + 16 * i + 4 * g) * a.ldo + at;
 #pragma unroll
@@ -304,7 +335,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
                     f[j] += d;
                 }
                 y[e].template set<YT == GRAD_F16>(f);
-                y[e].store(a.out, row + e * a.ldo);
+                y[e].store_stream(a.out, row + e * a.ldo);
             }
         }
     });
@@ -313,15 +344,19 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
 void launch_lora_expand(LoraExpandArgs a, hipStream_t s) {
     auto run = [&](auto t16, auto yt) {
         constexpr int YT = decltype(yt)::value;
+        const bool one = (YT == 0 ? 3 : 2) * a.R <= 32;
+        const int waves = !one && a.R > 64 ? 2 : 4;  // (at most 64 KB of weights a block)
         // Tiles of a block: the weights are read once for all of them, but first of all the chip is to be filled; then
         // the adapters of a block's tokens side by side.
-        const int tiles = (a.T + 15) / 16, cols = (a.N + 511) / 512;
+        const int tiles = (a.T + 15) / 16, cols = (a.N + 128 * waves - 1) / (128 * waves);
         a.tiles = tiles * cols >= 2048 ? 4 : tiles * cols >= 1024 ? 2 : 1;
         const int groups = (tiles + a.tiles - 1) / a.tiles;
         const int side = std::max(1, std::min({1024 / (groups * cols), 16 * a.tiles, a.L, a.T}));
         const dim3 grid{unsigned(cols), unsigned(groups), unsigned(side)};
-        if ((YT == 0 ? 3 : 2) * a.R <= 32) lora_expand_kernel<decltype(t16), YT, true><<<grid, 256, 0, s>>>(a);
-        else lora_expand_kernel<decltype(t16), YT, false><<<grid, 256, 0, s>>>(a);
+        const unsigned threads = unsigned(waves * WAVE);
+        if (one) lora_expand_kernel<decltype(t16), YT, true><<<grid, threads, 0, s>>>(a);
+        else
+            lora_expand_kernel<decltype(t16), YT, false><<<grid, threads, size_t(waves) * 256 * size_t(a.R), s>>>(a);
     };
     auto by_16 = [&](auto yt) {
         if (a.f16) run(F16{}, yt);
@@ -544,23 +579,8 @@ size_t lora_backward_workspace_bytes(int T, int K, int N, int R, int L) {
     return LoraSpace(T, K, N, R, L, outer_parts(T, K, N, R, L)).bytes;
 }
 
-void launch_lora_backward(const LoraGradArgs &a, void *ws, hipStream_t s) {
-    const int parts = outer_parts(a.T, a.K, a.N, a.R, a.L);
-    const LoraSpace at(a.T, a.K, a.N, a.R, a.L, parts);
-    char *base = static_cast<char *>(ws);
-    uint16_t *bt = reinterpret_cast<uint16_t *>(base + at.bt), *att = reinterpret_cast<uint16_t *>(base + at.at);
-    float *dv = reinterpret_cast<float *>(base + at.dv);
-    const bool need_dv = a.dx || a.dA;
-    if (need_dv) {
-        const LoraTransposeArgs tb{a.B, bt, a.L, a.N, a.R}, ta{a.A, att, a.dx ? a.L : 0, a.R, a.K};
-        lora_transpose_kernel<<<unsigned(tb.blocks() + ta.blocks()), 256, 0, s>>>(tb, ta);
-        launch_lora_shrink(LoraShrinkArgs{a.dy, a.lddy, bt, a.ids, a.T, a.N, a.R, a.L, dv, a.f16}, s);
-    }
-    if (a.dx)
-        launch_lora_expand(LoraExpandArgs{dv, att, a.ids, a.scaling, a.T, a.K, a.R, a.L, a.f16, a.dx, a.lddx, a.dx_out,
-                                          a.lddxo, a.f16 ? 2 : 1, true},
-                           s);
-    if (!a.dA && !a.dB) return;
+static void launch_lora_outer(const LoraGradArgs &a, char *base, const LoraSpace &at, int parts, const float *dv,
+                              hipStream_t s) {
     float *pa = parts > 1 ? reinterpret_cast<float *>(base + at.pa) : a.dA;
     float *pb = parts > 1 ? reinterpret_cast<float *>(base + at.pb) : a.dB;
     LoraOuterArgs o{};
@@ -588,6 +608,25 @@ void launch_lora_backward(const LoraGradArgs &a, void *ws, hipStream_t s) {
         const int64_t n = int64_t(a.R) * ((a.dA ? a.K : 0) + int64_t(a.dB ? a.N : 0)) / 4;
         lora_outer_join_kernel<<<dim3(unsigned((n + 255) / 256), unsigned(a.L)), 256, 0, s>>>(o, a.dA, a.dB);
     }
+}
+
+void launch_lora_backward(const LoraGradArgs &a, void *ws, hipStream_t s) {
+    const int parts = outer_parts(a.T, a.K, a.N, a.R, a.L);
+    const LoraSpace at(a.T, a.K, a.N, a.R, a.L, parts);
+    char *base = static_cast<char *>(ws);
+    uint16_t *bt = reinterpret_cast<uint16_t *>(base + at.bt), *att = reinterpret_cast<uint16_t *>(base + at.at);
+    float *dv = reinterpret_cast<float *>(base + at.dv);
+    const bool need_dv = a.dx || a.dA;
+    if (need_dv) {
+        const LoraTransposeArgs tb{a.B, bt, a.L, a.N, a.R}, ta{a.A, att, a.dx ? a.L : 0, a.R, a.K};
+        lora_transpose_kernel<<<unsigned(tb.blocks() + ta.blocks()), 256, 0, s>>>(tb, ta);
+        launch_lora_shrink(LoraShrinkArgs{a.dy, a.lddy, bt, a.ids, a.T, a.N, a.R, a.L, dv, a.f16}, s);
+    }
+    if (a.dA || a.dB) launch_lora_outer(a, base, at, parts, dv, s);
+    if (a.dx)
+        launch_lora_expand(LoraExpandArgs{dv, att, a.ids, a.scaling, a.T, a.K, a.R, a.L, a.f16, a.dx, a.lddx, a.dx_out,
+                                          a.lddxo, a.f16 ? 2 : 1, true},
+                           s);
 }
 
 }  // namespace qwq4

@@ -107,6 +107,8 @@ __device__ __forceinline__ void unpack2(uint32_t w, float &a, float &b) {
     }
 }
 
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
 // 8 elements of a row as they lie (16-byte aligned), and their values.
 template <int YT>
 struct RowPiece {
@@ -115,6 +117,17 @@ struct RowPiece {
         const char *at = static_cast<const char *>(p) + i * (YT == 0 ? 4 : 2);
         w[0] = reinterpret_cast<const uint4 *>(at)[0];
         if constexpr (YT == 0) w[1] = reinterpret_cast<const uint4 *>(at)[1];
+    }
+    // the same past the caches, for rows that nobody reads or writes again soon
+    __device__ __forceinline__ void load_stream(const void *p, int64_t i) {
+        const u32x4 *at = reinterpret_cast<const u32x4 *>(static_cast<const char *>(p) + i * (YT == 0 ? 4 : 2));
+#pragma unroll
+        for (int n = 0; n < (YT == 0 ? 2 : 1); ++n) w[n] = __builtin_bit_cast(uint4, __builtin_nontemporal_load(at + n));
+    }
+    __device__ __forceinline__ void store_stream(void *p, int64_t i) const {
+        u32x4 *at = reinterpret_cast<u32x4 *>(static_cast<char *>(p) + i * (YT == 0 ? 4 : 2));
+#pragma unroll
+        for (int n = 0; n < (YT == 0 ? 2 : 1); ++n) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, w[n]), at + n);
     }
     // (fp16: finite values beyond its range saturate, or, as a gradient, become infinite)
     template <bool GRAD>
