@@ -491,7 +491,7 @@ int qw_rms_norm_backward(const void *dy, int dy_type, int lddy, const void *h, i
  * NaN in a token's row or its adapter does not reach other tokens (in its own the
  * result may be NaN where the sum is infinite).
  * K, N, R multiples of 8, R at most 128, K and N at most 2^20, L at most 4096; strides ldx, ldy,
- * ldo multiples of 8 elements (4 in fp32); x, A, B, v, y and out 16-byte aligned. */
+ * ldo multiples of 8 elements (4 in fp32) up to 2^23; x, A, B, v, y and out 16-byte aligned. */
 int qw_lora(const void *x, int ldx, int f16, const void *A, const void *B, const int32_t *ids, const float *scaling,
             int T, int K, int N, int R, int L, float *v, const void *y, int ldy, void *out, int ldo, int y_type,
             void *stream);

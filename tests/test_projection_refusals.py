@@ -68,7 +68,7 @@ CALLS = {
     "lora null v": lora(v=None), "lora null y": lora(y=None), "lora null out": lora(out=None), "lora no rows": lora(T=0),
     "lora too many rows": lora(T=(1 << 20) + 1), "lora K 60": lora(K=60), "lora N 30": lora(N=30), "lora K 0": lora(K=0),
     "lora N 0": lora(N=0), "lora R 0": lora(R=0), "lora R 12": lora(R=12), "lora R 136": lora(R=136), "lora L 0": lora(L=0),
-    "lora L 4097": lora(L=4097), "lora ldx": lora(ldx=60), "lora ldx 68": lora(ldx=68), "lora ldy": lora(ldy=24),
+    "lora L 4097": lora(L=4097), "lora ldx": lora(ldx=60), "lora ldx 68": lora(ldx=68), "lora ldx too wide": lora(ldx=(1 << 23) + 8), "lora ldy": lora(ldy=24),
     "lora ldy 36": lora(ldy=36, ldo=36), "lora fp32 ldy 34": lora(yt=0, ldy=34, ldo=34), "lora ldo 36": lora(out=Q, ldo=36),
     "lora in place, other stride": lora(ldo=40), "lora y type": lora(yt=3), "lora x at 8": lora(x=EIGHT),
     "lora A at 8": lora(A=EIGHT), "lora B at 8": lora(B=EIGHT), "lora v at 8": lora(v=EIGHT), "lora y at 8": lora(y=EIGHT),

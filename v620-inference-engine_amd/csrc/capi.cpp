@@ -677,8 +677,9 @@ static int check_lora(const char *fn, const void *A, const void *B, const int32_
 static int check_wide_rows(const char *fn, const char *name, const void *p, int type, int ld, int T, int n) {
     REQUIRE(p, "%s: null %s", fn, name);
     const int e = 16 / int(type_bytes(type));
-    REQUIRE(aligned(p, 16) && (T == 1 || (ld >= n && ld % e == 0)),
-            "%s: stride %d of %s must be >= %d and a multiple of %d, the rows 16-byte aligned", fn, ld, name, n, e);
+    REQUIRE(aligned(p, 16) && (T == 1 || (ld >= n && ld % e == 0 && ld <= (1 << 23))),
+            "%s: stride %d of %s must be >= %d, at most 2^23 and a multiple of %d, the rows 16-byte aligned", fn, ld, name,
+            n, e);
     return 0;
 }
 

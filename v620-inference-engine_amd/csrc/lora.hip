@@ -401,106 +401,146 @@ __global__ __launch_bounds__(256) void lora_transpose_kernel(LoraTransposeArgs a
     }
 }
 
-constexpr int OUTER_COLS = 512, OUTER_TOKENS = 2048;  // of a block: columns, tokens whose ids it looks at
+constexpr int OUTER_COLS = 512;     // columns of a block
+constexpr int OUTER_TOKENS = 1024;  // tokens whose ids it looks at at once
 
 // G[r][c] = scaling sum_t u[t][r] m[t][c] over the tokens of one adapter in one
 // part of the batch: 128 columns a wave, 16 RF ranks. The tokens are listed in
 // LDS in order. The sum runs over tokens, whose values lie a row apart: a lane
 // loads 8 columns of 8 tokens and turns them in registers (v_perm) into 8
 // operands of one column each, so the wide rows come in 16-byte loads and
-// never pass through LDS. u goes in as three bf16 parts (exact), fp16 rows as
-// two (exact; fp16 products of unscaled sums would overflow).
+// never pass through LDS. u goes in as three bf16 parts (exact) or two fp16 ones
+// (to 2^-23) of u times a power of two per rank, which follows the largest u so
+// far (fp16 of u itself would overflow). 4096 tokens of 4096 and 12288 columns, 16
+// ranks: %s; alike with two steps on their way, with u turned once for the four waves,
+// or a block for all adapters of a part.
 template <class T16, int RF>
 __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
     constexpr bool HALF = __is_same(T16, F16);
-    __shared__ int s_tok[OUTER_TOKENS];
+    constexpr int PARTS = HALF ? 2 : 3;
+    __shared__ uint32_t s_tok[OUTER_TOKENS];
     __shared__ int s_count[4];
-    const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
+    const int tid = int(threadIdx.x), lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int c = lane % 16, g = lane / 16;
     const int part = int(blockIdx.z), l = int(blockIdx.y) % a.L, r0 = int(blockIdx.y) / a.L * (16 * RF);
     const bool second = int(blockIdx.x) >= a.m[0].blocks();
     const LoraOuterSide &m = a.m[second];
     const int c0 = (int(blockIdx.x) - (second ? a.m[0].blocks() : 0)) * OUTER_COLS + wave * 128;
-
-    int n = 0;
-    const int from = part * a.per, to = min(a.T, from + a.per);
-    for (int b = from; b < to; b += 256) {
-        const int t = b + int(threadIdx.x);
-        const bool mine = t < to && a.ids[t] == l;
-        const unsigned long long which = __ballot(mine);
-        if (lane == 0) s_count[wave] = __popcll(which);
-        __syncthreads();
-        int before = n;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            before += w < wave ? s_count[w] : 0;
-            n += s_count[w];
-        }
-        if (mine) s_tok[before + __popcll(which & ((1ull << lane) - 1ull))] = t;
-        __syncthreads();
-    }
-    if (a.parts > 1 && blockIdx.x == 0 && r0 == 0 && threadIdx.x == 0) a.count[part * a.L + l] = n;
-    if (n == 0 && a.parts > 1) return;  // (the joining launch goes by the count)
-    if (c0 >= m.C) return;              // (no barrier below)
-
+    const int from = part * a.per, end = min(a.T, from + a.per);
     const uint16_t *col = m.m + min(c0 + 8 * c, m.C - 8);
-    const int steps = (n + 31) / 32;
+    const uint32_t ldm = uint32_t(m.ldm), R = uint32_t(a.R);
+
     f32x4 acc[RF][8];
 #pragma unroll
     for (int f = 0; f < RF; ++f)
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    uint4 next[8];
-    float nu[RF][8];
-    auto load = [&](int s) {
+    int shift[RF];  // fp16: the power of two of rank r0 + 16 f + c
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int p = 32 * s + 8 * g + e;
-            const int64_t t = s_tok[min(p, n - 1)];
-            const bool in = p < n;
-            next[e] = in ? *reinterpret_cast<const uint4 *>(col + t * m.ldm) : make_uint4(0, 0, 0, 0);
+    for (int f = 0; f < RF; ++f) shift[f] = HALF ? 141 : 0;
+    // row i of a piece's sums is rank 4 g + i, whose power of two lane 4 g + i has
+    auto rescale = [&](int f, int by) {
 #pragma unroll
-            for (int f = 0; f < RF; ++f) nu[f][e] = in ? m.u[t * a.R + min(r0 + 16 * f + c, a.R - 1)] : 0.f;
+        for (int i = 0; i < 4; ++i) {
+            const int d = __shfl(by, 4 * g + i);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[f][j][i] = __builtin_ldexpf(acc[f][j][i], d);
         }
     };
-    if (steps > 0) load(0);
-    for (int s = 0; s < steps; ++s) {
-        uint32_t d[8][4];
-        uint4 part[RF][3];
+
+    int total = 0;
+    for (int b0 = from; b0 < end; b0 += OUTER_TOKENS) {
+        int n = 0;
+        const int b1 = min(end, b0 + OUTER_TOKENS);
+        for (int b = b0; b < b1; b += 256) {
+            const int t = b + tid;
+            const bool mine = t < b1 && a.ids[t] == l;
+            const unsigned long long which = __ballot(mine);
+            if (lane == 0) s_count[wave] = __popcll(which);
+            __syncthreads();
+            int before = n;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[e][0] = next[e].x, d[e][1] = next[e].y, d[e][2] = next[e].z, d[e][3] = next[e].w;
+            for (int w = 0; w < 4; ++w) {
+                before += w < wave ? s_count[w] : 0;
+                n += s_count[w];
+            }
+            if (mine) s_tok[before + __popcll(which & ((1ull << lane) - 1ull))] = uint32_t(t);
+            __syncthreads();
+        }
+        total += n;
+        const int steps = c0 < m.C ? (n + 31) / 32 : 0;
+        uint4 next[8];
+        float nu[RF][8];
+        auto load = [&](int s) {
+            uint32_t t[8];
 #pragma unroll
-        for (int f = 0; f < RF; ++f) split8<BF16, 3>(nu[f], part[f]);
-        if (s + 1 < steps) load(s + 1);
+            for (int e = 0; e < 8; ++e) t[e] = s_tok[min(32 * s + 8 * g + e, n - 1)];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            uint32_t w[4];  // column j of the 8 tokens
+            for (int e = 0; e < 8; ++e) {
+                next[e] = *reinterpret_cast<const uint4 *>(col + uint64_t(t[e]) * ldm);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                w[e] = __builtin_amdgcn_perm(d[2 * e + 1][j / 2], d[2 * e][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
-            if constexpr (HALF) {
-                float v[8];
+                for (int f = 0; f < RF; ++f) nu[f][e] = m.u[t[e] * R + uint32_t(min(r0 + 16 * f + c, a.R - 1))];
+            }
+            // (behind the list: nothing, whatever the repeated row holds)
+            if (32 * s + 32 > n) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) unpack2<F16>(w[e], v[2 * e], v[2 * e + 1]);
-                uint4 h[2];
-                split8<BF16, 2>(v, h);
+                for (int e = 0; e < 8; ++e) {
+                    if (32 * s + 8 * g + e < n) continue;
+                    next[e] = make_uint4(0, 0, 0, 0);
 #pragma unroll
-                for (int f = 0; f < RF; ++f) {
-#pragma unroll
-                    for (int p = 0; p < 3; ++p) acc[f][j] = mfma16<BF16>(part[f][p], h[0], acc[f][j]);
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) acc[f][j] = mfma16<BF16>(part[f][p], h[1], acc[f][j]);
+                    for (int f = 0; f < RF; ++f) nu[f][e] = 0.f;
                 }
-            } else {
+            }
+        };
+        if (steps > 0) load(0);
+        for (int s = 0; s < steps; ++s) {
+            uint32_t d[8][4];
+            uint4 q[RF][PARTS];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e][0] = next[e].x, d[e][1] = next[e].y, d[e][2] = next[e].z, d[e][3] = next[e].w;
+#pragma unroll
+            for (int f = 0; f < RF; ++f) {
+                if constexpr (HALF) {
+                    float top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(nu[f][e]));
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const int size = int((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 126;  // top below 2^size
+                    if (__ballot(size + shift[f] > 15)) {
+                        // (to 2^8: room for values 128 times as large before the next time)
+                        const int by = size + shift[f] > 15 ? 8 - size - shift[f] : 0;
+                        shift[f] += by;
+                        rescale(f, by);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) nu[f][e] = __builtin_ldexpf(nu[f][e], shift[f]);
+                }
+                split8<T16, PARTS>(nu[f], q[f]);
+            }
+            if (s + 1 < steps) load(s + 1);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint32_t w[4];  // column j of the 8 tokens
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    w[e] = __builtin_amdgcn_perm(d[2 * e + 1][j / 2], d[2 * e][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
                 const uint4 h = make_uint4(w[0], w[1], w[2], w[3]);
 #pragma unroll
                 for (int f = 0; f < RF; ++f)
 #pragma unroll
-                    for (int p = 0; p < 3; ++p) acc[f][j] = mfma16<BF16>(part[f][p], h, acc[f][j]);
+                    for (int p = 0; p < PARTS; ++p) acc[f][j] = mfma16<T16>(q[f][p], h, acc[f][j]);
             }
         }
+        __syncthreads();  // (the list is read)
     }
+    if (a.parts > 1 && blockIdx.x == 0 && r0 == 0 && tid == 0) a.count[part * a.L + l] = total;
+    if (total == 0 && a.parts > 1) return;  // (the joining launch goes by the count)
 
+    if constexpr (HALF) {
+#pragma unroll
+        for (int f = 0; f < RF; ++f) rescale(f, -shift[f]);
+    }
     if (c0 + 8 * c >= m.C) return;
     const float scale = a.scaling ? a.scaling[l] : 1.f;
     float *out = m.out + (int64_t(part) * a.L + l) * a.R * m.C;
@@ -518,7 +558,8 @@ __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
                 float *p = out + int64_t(r + i) * m.C + c0 + 8 * c;
 #pragma unroll
                 for (int j = 0; j < 8; j += 4)
-                    *reinterpret_cast<f32x4 *>(p + j) = f32x4{acc[f][j][i], acc[f][j + 1][i], acc[f][j + 2][i], acc[f][j + 3][i]} * scale;
+                    *reinterpret_cast<f32x4 *>(p + j) =
+                        f32x4{acc[f][j][i], acc[f][j + 1][i], acc[f][j + 2][i], acc[f][j + 3][i]} * scale;
             }
         }
     }
@@ -533,24 +574,41 @@ __global__ __launch_bounds__(256) void lora_outer_join_kernel(LoraOuterArgs a, f
     float *out = second ? dB : dA;
     const LoraOuterSide &m = a.m[second];
     const int64_t at = second ? i - n0 : i, each = int64_t(a.R) * m.C;
+    // (which parts have any, before the rows of those are asked for)
+    const int lane = int(threadIdx.x) % WAVE;
+    unsigned long long which = __ballot(lane < a.parts && a.count[min(lane, a.parts - 1) * a.L + l] > 0);
     if (!out || at >= each) return;
+    const float *p = m.out + l * each + at;
+    const int64_t step = a.L * each;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < a.parts; ++p)
-        if (a.count[p * a.L + l])
-            sum += *reinterpret_cast<const f32x4 *>(m.out + (int64_t(p) * a.L + l) * each + at);
+    while (which) {
+        f32x4 v[4];
+        int n = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (!which) continue;
+            v[u] = *reinterpret_cast<const f32x4 *>(p + step * __builtin_ctzll(which));
+            which &= which - 1;
+            ++n;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (u < n) sum += v[u];
+    }
     *reinterpret_cast<f32x4 *>(out + l * each + at) = sum;
 }
 
-// Parts of the batch whose sums over tokens run side by side: until about 2048
-// blocks are there (a block whose adapter has no token in its part ends at
-// once), of at most OUTER_TOKENS tokens each.
+// Parts of the batch whose sums over tokens run side by side, at most
+// MAX_PARTS: until about 2048 blocks are there (one whose adapter has no token in
+// its part ends at once), of 128 tokens or more. Every part has room for every
+// adapter's sums: with the number of blocks that is bounded, 64 MB or so.
+constexpr int MAX_PARTS = 64;
 static int outer_ranks(int R) { return R <= 16 ? 16 : 32; }
 static int outer_parts(int T, int K, int N, int R, int L) {
     const int ranks = outer_ranks(R);
     const int64_t blocks = int64_t((K + OUTER_COLS - 1) / OUTER_COLS + (N + OUTER_COLS - 1) / OUTER_COLS) *
                            ((R + ranks - 1) / ranks) * L;
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>((2048 + blocks - 1) / blocks, (T + 127) / 128));
-    return int(std::max<int64_t>(want, (T + OUTER_TOKENS - 1) / OUTER_TOKENS));
+    return int(std::max<int64_t>(1, std::min<int64_t>({(2048 + blocks - 1) / blocks, (T + 127) / 128, MAX_PARTS})));
 }
 
 // Workspace of the gradients: B and A transposed, dv, and the parts of dA and
