@@ -695,11 +695,11 @@ int qw_lora(const void *x, int ldx, int f16, const void *A, const void *B, const
     if (int r = check_wide_rows(fn, "out", out, y_type, ldo, T, N)) return r;
     if (int r = check_in_place(fn, "out", out, ldo, y, ldy, T)) return r;
     qwq4::launch_lora_shrink(qwq4::LoraShrinkArgs{static_cast<const uint16_t *>(x), ldx,
-                                                  static_cast<const uint16_t *>(A), ids, T, K, R, L, v, f16 != 0},
+                                                  static_cast<const uint16_t *>(A), ids, T, K, R, L, v, f16 != 0, false},
                              st(stream));
     qwq4::launch_lora_expand(qwq4::LoraExpandArgs{v, static_cast<const uint16_t *>(B), ids, scaling, T, N, R, L,
                                                   f16 != 0, y, ldy, out, ldo, y_type, false},
-                             st(stream));
+                             qwq4::LoraJoinArgs{}, st(stream));
     return launched(fn);
 }
 

@@ -16,6 +16,7 @@
 // or three (fp32 outputs) 16-bit parts whose sum it is, to 2^-17 or exactly:
 // with ranks of tens the added products cost less than the rows' traffic.
 #include <algorithm>
+#include <type_traits>
 
 #include "q4_kernels.hpp"
 #include "row_io.cuh"
@@ -49,6 +50,21 @@ __device__ __forceinline__ void load8(const float *p, float (&f)[8]) {
     const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
     f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w;
     f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+}
+
+// 8 columns of 8 rows of 16-bit elements, a row in each register group, as a column in each.
+__device__ __forceinline__ void turn8(const uint4 (&row)[8], uint4 (&column)[8]) {
+    uint32_t d[8][4];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d[e][0] = row[e].x, d[e][1] = row[e].y, d[e][2] = row[e].z, d[e][3] = row[e].w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            w[e] = __builtin_amdgcn_perm(d[2 * e + 1][j / 2], d[2 * e][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+        column[j] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
 }
 
 // The adapters among a wave's tokens (lane i: token i's, or -1), every `of`-th
@@ -103,11 +119,49 @@ struct Turned {
     }
 };
 
+// The same for 16 columns of 64 rows of weights that lie with the ranks inside
+// ([K][R]): read as they lie, and turned by LDS's transposing reads (four rows of 16
+// elements to 16 lanes, each of which gets a column). Against a transposed copy in
+// the workspace: gradients of 601 tokens of rank 64 30 us for 36, of 4096 of rank 32 58 for
+// 65; of rank 128, whose rows' pieces of 32 bytes cost the loads more, 179 for 172.
+struct TurnedColumns {
+    uint4 w[2];
+    // at: the weights of step k's first row and the first of its ranks; the first n of the 64 rows exist, and ranks of
+    // them (a multiple of 8; behind them the last ones again, whose sums nothing takes)
+    __device__ __forceinline__ void load(const uint16_t *at, int R, int ranks, int n) {
+        const int lane = int(threadIdx.x) % WAVE, r = min(lane % 2 * 8, ranks - 8);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int k = 32 * i + lane / 2;
+            w[i] = k < n ? *reinterpret_cast<const uint4 *>(at + k * R + r) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void turn(uint4 *lds) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        const int lane = int(threadIdx.x) % WAVE, c = lane % 16, g = lane / 16;
+        Turned::wave_lds_order();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) lds[WAVE * i + lane] = w[i];
+        Turned::wave_lds_order();
+        short *row = reinterpret_cast<short *>(lds) + (8 * g + c / 4) * 16 + c % 4 * 4;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            auto four = [&](int k) {
+                return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                     (__attribute__((address_space(3))) s16x4 *)(row + k * 16)));
+            };
+            const uint2 a = four(32 * h), b = four(32 * h + 4);
+            w[h] = make_uint4(a.x, a.y, b.x, b.y);
+        }
+    }
+};
+
 // v[t][r] = sum_k A[id_t][r][k] x[t][k] for 16 tokens and 16 RF ranks by a block
 // whose 16 waves take a run of 64-wide steps of K each and join their sums in
 // LDS, in order: a row's bits depend on neither the batch nor its place in it.
-// Every wave has the next U steps of rows and weights on their way.
-template <class T16, int RF>
+// Every wave has the next U steps of rows and weights on their way. INSIDE: the
+// ranks lie inside, A is [K][R].
+template <class T16, int RF, bool INSIDE>
 __global__ __launch_bounds__(1024) void lora_shrink_kernel(LoraShrinkArgs a) {
     constexpr int NW = 16, U = RF == 1 ? 2 : 1;
     __shared__ uint4 s_turn[NW][2][128];  // (4 KB a wave, and then the waves' sums)
@@ -127,12 +181,13 @@ __global__ __launch_bounds__(1024) void lora_shrink_kernel(LoraShrinkArgs a) {
 #pragma unroll
         for (int f = 0; f < RF; ++f)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) w[f][i] = uint32_t(min(r0 + 16 * f + 8 * i + lane / 8, a.R - 1)) * uint32_t(a.K);
+            for (int i = 0; i < 2 && !INSIDE; ++i) w[f][i] = uint32_t(min(r0 + 16 * f + 8 * i + lane / 8, a.R - 1)) * uint32_t(a.K);
         f32x4 acc[RF];
 #pragma unroll
         for (int f = 0; f < RF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
         struct Steps {
-            Turned x[U], w[U][RF];
+            Turned x[U];
+            std::conditional_t<INSIDE, TurnedColumns, Turned> w[U][RF];
         } next;
         auto load = [&](int s0) {
 #pragma unroll
@@ -140,7 +195,12 @@ __global__ __launch_bounds__(1024) void lora_shrink_kernel(LoraShrinkArgs a) {
                 const int k = (s0 + u) * 64, n = s0 + u < end ? a.K - k : 0;
                 next.x[u].load([&](int i) { return x[i] + k; }, n);
 #pragma unroll
-                for (int f = 0; f < RF; ++f) next.w[u][f].load([&](int i) { return A + (w[f][i] + uint32_t(k)); }, n);
+                for (int f = 0; f < RF; ++f) {
+                    if constexpr (INSIDE) {
+                        const int r = min(r0 + 16 * f, a.R - 8);
+                        next.w[u][f].load(A + (uint32_t(k) * uint32_t(a.R) + uint32_t(r)), a.R, a.R - r, n);
+                    } else next.w[u][f].load([&](int i) { return A + (w[f][i] + uint32_t(k)); }, n);
+                }
             }
         };
         load(wave * per);
@@ -180,8 +240,9 @@ void launch_lora_shrink(const LoraShrinkArgs &a, hipStream_t s) {
     const int side = std::max(1, std::min({256 / tiles, 16, a.L, a.T}));
     auto run = [&](auto t16, auto rf) {
         constexpr int RF = decltype(rf)::value;
-        lora_shrink_kernel<decltype(t16), RF>
-            <<<dim3(unsigned(tiles), unsigned(side), unsigned((a.R + 16 * RF - 1) / (16 * RF))), 1024, 0, s>>>(a);
+        const dim3 grid{unsigned(tiles), unsigned(side), unsigned((a.R + 16 * RF - 1) / (16 * RF))};
+        if (a.inside) lora_shrink_kernel<decltype(t16), RF, true><<<grid, 1024, 0, s>>>(a);
+        else lora_shrink_kernel<decltype(t16), RF, false><<<grid, 1024, 0, s>>>(a);
     };
     auto by_rank = [&](auto t16) {
         if (a.R <= 16 || tiles * side < 128) run(t16, Int<1>{});
@@ -192,24 +253,65 @@ void launch_lora_shrink(const LoraShrinkArgs &a, hipStream_t s) {
     else by_rank(BF16{});
 }
 
+// out[l] = the parts of adapter l that have tokens, in order (none: zeros).
+__device__ __forceinline__ void join_parts(const LoraJoinArgs &a, int block) {
+    const int blocks = a.blocks(int(blockDim.x)), l = block / blocks;
+    if (l >= a.L) return;
+    const int64_t i = (int64_t(block % blocks) * int(blockDim.x) + int(threadIdx.x)) * 4;
+    const bool second = i >= a.n[0];
+    float *out = a.out[second];
+    const int64_t at = second ? i - a.n[0] : i, each = a.n[second];
+    // (which parts have any, before the rows of those are asked for)
+    const int lane = int(threadIdx.x) % WAVE;
+    unsigned long long which = __ballot(lane < a.parts && a.count[min(lane, a.parts - 1) * a.L + l] > 0);
+    if (at >= each) return;
+    const float *p = a.part[second] + l * each + at;
+    const int64_t step = a.L * each;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    while (which) {
+        f32x4 v[4];
+        int n = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (!which) continue;
+            v[u] = *reinterpret_cast<const f32x4 *>(p + step * __builtin_ctzll(which));
+            which &= which - 1;
+            ++n;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (u < n) sum += v[u];
+    }
+    *reinterpret_cast<f32x4 *>(out + l * each + at) = sum;
+}
+
 // ------------------------------------------------------------ expand
 // out[t][n] = y[t][n] + scaling[id_t] sum_r B[id_t][n][r] v[t][r]: 16 NT tokens by
 // 128 columns a wave, 16 tokens at a time (NT = a.tiles, at most 4). The columns
 // are dealt to 8 MFMAs so that a lane holds 8 neighbouring ones of four tokens
 // and 16 lanes a row's 128: rows are read and written in 256-byte runs (four lanes
-// to a token's 64 columns: 47 us where this takes @@, 4096 x 12288 in bf16), past
+// to a token's 64 columns: 47 us where this takes 43, 4096 x 12288 in bf16), past
 // the caches (kept in them: 5 us more). K of the MFMA runs over the R values of
 // each of v's parts in turn. fp16 parts are of v times a power of two per token,
 // so that none of them overflows or loses bits to the range. Bound by memory.
 // ONE: one step of the MFMA covers all parts, and its weights stay in registers.
 // Else they lie in LDS, a wave's 128 rows of B as one run of memory (read for
-// every tile in the MFMA's order, they touch a line per lane: 4096 x 12288 of rank 64
-// 172 us where this takes @@); 16-byte piece p of them at place p ^ (row / 8 & 7):
-// without bank conflicts.
-template <class T16, int YT, bool ONE>
-__global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
+// every tile in the MFMA's order, they touch a line per lane: a call of rank 64, 4096
+// x 12288, 172 us where this takes 102); 16-byte piece p of them at place p ^ (row / 8 & 7):
+// without bank conflicts. COLUMNS: the columns lie inside, B is [R][N]: a lane reads
+// its 8 columns of 8 ranks and turns them in registers; and the blocks behind the
+// expanding ones join the parts of the weights' gradients (as much work as in a
+// launch of its own, but without that launch's 3 us or so).
+template <class T16, int YT, bool ONE, bool COLUMNS>
+__global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a, LoraJoinArgs join) {
     constexpr bool HALF = __is_same(T16, F16);
     constexpr int PARTS = YT == 0 ? 3 : 2;
+    if constexpr (COLUMNS) {
+        if (int(blockIdx.z) >= a.side) {
+            join_parts(join, ((int(blockIdx.z) - a.side) * int(gridDim.y) + int(blockIdx.y)) * int(gridDim.x) + int(blockIdx.x));
+            return;
+        }
+    }
     extern __shared__ uint4 s_weights[];  // ONE: none; [waves][128 R / 8]
     const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
     const int c = lane % 16, g = lane / 16;
@@ -232,9 +334,17 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
         }
     }
     uint4 *lds = s_weights + wave * 128 * octets;
-    each_adapter(id, int(blockIdx.z), int(gridDim.z), [&](int l, unsigned long long mine) {
+    each_adapter(id, int(blockIdx.z), a.side, [&](int l, unsigned long long mine) {
         const float scale = a.scaling ? a.scaling[l] : 1.f;
-        const uint16_t *B = a.B + (int64_t(l) * a.N + n0) * a.R;  // the wave's rows, min(128, N - n0) of them
+        // the wave's rows, min(128, N - n0) of them, or its columns
+        const uint16_t *B = a.B + int64_t(l) * a.N * a.R + (COLUMNS ? min(at, a.N - 8) : n0 * a.R);
+        // COLUMNS: octet o of the lane's columns' ranks
+        auto octet = [&](int o, uint4 (&w)[8]) {
+            uint4 rank[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) rank[j] = *reinterpret_cast<const uint4 *>(B + uint32_t(8 * o + j) * uint32_t(a.N));
+            turn8(rank, w);
+        };
         // the tokens of tile i that are this adapter's, and their rows
         auto tokens = [&](int i) { return i < NT ? uint32_t(mine >> (16 * i)) & 0xffffu : 0u; };
         auto rows = [&](int i, RowPiece<YT> (&y)[4]) {
@@ -255,9 +365,21 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
         uint4 wf[8];
         if constexpr (ONE) {
             int p;
-            const uint16_t *w = B + min(8 * c, a.N - 8 - n0) * a.R + 8 * place(0, p);
+            const int ro = place(0, p);
+            if constexpr (COLUMNS) octet(ro, wf);
+            else {
+                const uint16_t *w = B + min(8 * c, a.N - 8 - n0) * a.R + 8 * ro;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) wf[j] = *reinterpret_cast<const uint4 *>(w + j * a.R);
+                for (int j = 0; j < 8; ++j) wf[j] = *reinterpret_cast<const uint4 *>(w + j * a.R);
+            }
+        } else if constexpr (COLUMNS) {
+            Turned::wave_lds_order();
+            for (int o = g; o < octets; o += 4) {
+                octet(o, wf);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) lds[((8 * c + j) * octets + o) ^ (c & 7)] = wf[j];
+            }
+            Turned::wave_lds_order();
         } else {
             const int n = min(128, a.N - n0) * octets;
             const uint32_t inverse = (65536u + uint32_t(octets) - 1) / uint32_t(octets);  // (exact below 4096)
@@ -341,8 +463,9 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a) {
     });
 }
 
-void launch_lora_expand(LoraExpandArgs a, hipStream_t s) {
-    auto run = [&](auto t16, auto yt) {
+void launch_lora_expand(LoraExpandArgs a, const LoraJoinArgs &join, hipStream_t s) {
+    auto run = [&](auto t16, auto yt, auto columns) {
+        constexpr bool COLUMNS = decltype(columns)::value;
         constexpr int YT = decltype(yt)::value;
         const bool one = (YT == 0 ? 3 : 2) * a.R <= 32;
         const int waves = !one && a.R > 64 ? 2 : 4;  // (at most 64 KB of weights a block)
@@ -351,56 +474,24 @@ void launch_lora_expand(LoraExpandArgs a, hipStream_t s) {
         const int tiles = (a.T + 15) / 16, cols = (a.N + 128 * waves - 1) / (128 * waves);
         a.tiles = tiles * cols >= 2048 ? 4 : tiles * cols >= 1024 ? 2 : 1;
         const int groups = (tiles + a.tiles - 1) / a.tiles;
-        const int side = std::max(1, std::min({1024 / (groups * cols), 16 * a.tiles, a.L, a.T}));
-        const dim3 grid{unsigned(cols), unsigned(groups), unsigned(side)};
+        a.side = std::max(1, std::min({1024 / (groups * cols), 16 * a.tiles, a.L, a.T}));
         const unsigned threads = unsigned(waves * WAVE);
-        if (one) lora_expand_kernel<decltype(t16), YT, true><<<grid, threads, 0, s>>>(a);
-        else
-            lora_expand_kernel<decltype(t16), YT, false><<<grid, threads, size_t(waves) * 256 * size_t(a.R), s>>>(a);
+        const int joining = join.L ? (join.L * join.blocks(int(threads)) + groups * cols - 1) / (groups * cols) : 0;
+        const dim3 grid{unsigned(cols), unsigned(groups), unsigned(a.side + joining)};
+        const size_t lds = one ? 0 : size_t(waves) * 256 * size_t(a.R);
+        if (one) lora_expand_kernel<decltype(t16), YT, true, COLUMNS><<<grid, threads, lds, s>>>(a, join);
+        else lora_expand_kernel<decltype(t16), YT, false, COLUMNS><<<grid, threads, lds, s>>>(a, join);
     };
     auto by_16 = [&](auto yt) {
-        if (a.f16) run(F16{}, yt);
-        else run(BF16{}, yt);
+        if (a.f16) run(F16{}, yt, Int<0>{});
+        else run(BF16{}, yt, Int<0>{});
     };
-    if (a.y_type == 2 && a.grad) by_16(Int<GRAD_F16>{});
-    else by_type(a.y_type, by_16);
+    if (!a.columns) by_type(a.y_type, by_16);
+    else if (a.f16) run(F16{}, Int<GRAD_F16>{}, Int<1>{});
+    else run(BF16{}, Int<1>{}, Int<1>{});
 }
 
 // ------------------------------------------------------------ gradients
-// out[l][c][r] = in[l][r][c] of 16-bit elements, 64 x 64 a block; two such
-// problems in one launch. Rows and columns are multiples of 8.
-__global__ __launch_bounds__(256) void lora_transpose_kernel(LoraTransposeArgs a0, LoraTransposeArgs a1) {
-    __shared__ __align__(16) uint16_t s[64][72];
-    int b = int(blockIdx.x);
-    const int n0 = a0.blocks();
-    const LoraTransposeArgs a = b < n0 ? a0 : a1;
-    if (b >= n0) b -= n0;
-    const int rt = (a.rows + 63) / 64, ct = (a.cols + 63) / 64;
-    const int64_t l = b / (rt * ct), base = l * a.rows * a.cols;
-    const int r0 = b % (rt * ct) / ct * 64, c0 = b % ct * 64;
-    const int q = int(threadIdx.x) % 8 * 8, p = int(threadIdx.x) / 8;  // 8 elements of row p (+ 32)
-#pragma unroll
-    for (int i = 0; i < 64; i += 32) {
-        if (r0 + p + i < a.rows && c0 + q < a.cols) {
-            const Halves<8> e = __builtin_bit_cast(
-                Halves<8>, *reinterpret_cast<const uint4 *>(a.in + base + int64_t(r0 + p + i) * a.cols + c0 + q));
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s[p + i][q + j] = e.h[j];
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 64; i += 32) {
-        if (c0 + p + i < a.cols && r0 + q < a.rows) {
-            Halves<8> e;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) e.h[j] = s[q + j][p + i];
-            *reinterpret_cast<uint4 *>(a.out + base + int64_t(c0 + p + i) * a.rows + r0 + q) =
-                __builtin_bit_cast(uint4, e);
-        }
-    }
-}
-
 constexpr int OUTER_COLS = 512;     // columns of a block
 constexpr int OUTER_TOKENS = 1024;  // tokens whose ids it looks at at once
 
@@ -412,7 +503,7 @@ constexpr int OUTER_TOKENS = 1024;  // tokens whose ids it looks at at once
 // never pass through LDS. u goes in as three bf16 parts (exact) or two fp16 ones
 // (to 2^-23) of u times a power of two per rank, which follows the largest u so
 // far (fp16 of u itself would overflow). 4096 tokens of 4096 and 12288 columns, 16
-// ranks: %s; alike with two steps on their way, with u turned once for the four waves,
+// ranks: 31 us, 4.3 TB/s; alike with two steps on their way, with u turned once for the four waves,
 // or a block for all adapters of a part.
 template <class T16, int RF>
 __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
@@ -494,10 +585,8 @@ __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
         };
         if (steps > 0) load(0);
         for (int s = 0; s < steps; ++s) {
-            uint32_t d[8][4];
-            uint4 q[RF][PARTS];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) d[e][0] = next[e].x, d[e][1] = next[e].y, d[e][2] = next[e].z, d[e][3] = next[e].w;
+            uint4 column[8], q[RF][PARTS];
+            turn8(next, column);
 #pragma unroll
             for (int f = 0; f < RF; ++f) {
                 if constexpr (HALF) {
@@ -521,15 +610,10 @@ __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
             if (s + 1 < steps) load(s + 1);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                uint32_t w[4];  // column j of the 8 tokens
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    w[e] = __builtin_amdgcn_perm(d[2 * e + 1][j / 2], d[2 * e][j / 2], j % 2 ? 0x07060302u : 0x05040100u);
-                const uint4 h = make_uint4(w[0], w[1], w[2], w[3]);
 #pragma unroll
                 for (int f = 0; f < RF; ++f)
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p) acc[f][j] = mfma16<T16>(q[f][p], h, acc[f][j]);
+                    for (int p = 0; p < PARTS; ++p) acc[f][j] = mfma16<T16>(q[f][p], column[j], acc[f][j]);
             }
         }
         __syncthreads();  // (the list is read)
@@ -565,38 +649,7 @@ __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
     }
 }
 
-// out[l] = the parts of adapter l that have tokens, in order (none: zeros).
-__global__ __launch_bounds__(256) void lora_outer_join_kernel(LoraOuterArgs a, float *dA, float *dB) {
-    const int l = int(blockIdx.y);
-    const int64_t i = (int64_t(blockIdx.x) * 256 + int(threadIdx.x)) * 4;
-    const int64_t n0 = dA ? int64_t(a.R) * a.m[0].C : 0;
-    const bool second = i >= n0;
-    float *out = second ? dB : dA;
-    const LoraOuterSide &m = a.m[second];
-    const int64_t at = second ? i - n0 : i, each = int64_t(a.R) * m.C;
-    // (which parts have any, before the rows of those are asked for)
-    const int lane = int(threadIdx.x) % WAVE;
-    unsigned long long which = __ballot(lane < a.parts && a.count[min(lane, a.parts - 1) * a.L + l] > 0);
-    if (!out || at >= each) return;
-    const float *p = m.out + l * each + at;
-    const int64_t step = a.L * each;
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    while (which) {
-        f32x4 v[4];
-        int n = 0;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            if (!which) continue;
-            v[u] = *reinterpret_cast<const f32x4 *>(p + step * __builtin_ctzll(which));
-            which &= which - 1;
-            ++n;
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (u < n) sum += v[u];
-    }
-    *reinterpret_cast<f32x4 *>(out + l * each + at) = sum;
-}
+__global__ __launch_bounds__(256) void lora_outer_join_kernel(LoraJoinArgs a) { join_parts(a, int(blockIdx.x)); }
 
 // Parts of the batch whose sums over tokens run side by side, at most
 // MAX_PARTS: until about 2048 blocks are there (one whose adapter has no token in
@@ -611,10 +664,10 @@ static int outer_parts(int T, int K, int N, int R, int L) {
     return int(std::max<int64_t>(1, std::min<int64_t>({(2048 + blocks - 1) / blocks, (T + 127) / 128, MAX_PARTS})));
 }
 
-// Workspace of the gradients: B and A transposed, dv, and the parts of dA and
-// dB with their counts, each at a multiple of 256 bytes.
+// Workspace of the gradients: dv, and the parts of dA and dB with their counts,
+// each at a multiple of 256 bytes.
 struct LoraSpace {
-    size_t bt, at, dv, pa, pb, count, bytes;
+    size_t dv, pa, pb, count, bytes;
     LoraSpace(int T, int K, int N, int R, int L, int parts) {
         size_t end = 0;
         auto take = [&](size_t n) {
@@ -623,8 +676,6 @@ struct LoraSpace {
             return at0;
         };
         const size_t rk = size_t(L) * R * K, rn = size_t(L) * R * N;
-        bt = take(rn * 2);
-        at = take(rk * 2);
         dv = take(size_t(T) * R * 4);
         pa = take(parts > 1 ? rk * 4 * parts : 0);
         pb = take(parts > 1 ? rn * 4 * parts : 0);
@@ -637,8 +688,9 @@ size_t lora_backward_workspace_bytes(int T, int K, int N, int R, int L) {
     return LoraSpace(T, K, N, R, L, outer_parts(T, K, N, R, L)).bytes;
 }
 
-static void launch_lora_outer(const LoraGradArgs &a, char *base, const LoraSpace &at, int parts, const float *dv,
-                              hipStream_t s) {
+// What is left to join: nothing (L = 0) where the batch is one part.
+static LoraJoinArgs launch_lora_outer(const LoraGradArgs &a, char *base, const LoraSpace &at, int parts,
+                                      const float *dv, hipStream_t s) {
     float *pa = parts > 1 ? reinterpret_cast<float *>(base + at.pa) : a.dA;
     float *pb = parts > 1 ? reinterpret_cast<float *>(base + at.pb) : a.dB;
     LoraOuterArgs o{};
@@ -662,29 +714,25 @@ static void launch_lora_outer(const LoraGradArgs &a, char *base, const LoraSpace
     };
     if (a.f16) run(F16{});
     else run(BF16{});
-    if (parts > 1) {
-        const int64_t n = int64_t(a.R) * ((a.dA ? a.K : 0) + int64_t(a.dB ? a.N : 0)) / 4;
-        lora_outer_join_kernel<<<dim3(unsigned((n + 255) / 256), unsigned(a.L)), 256, 0, s>>>(o, a.dA, a.dB);
-    }
+    if (parts == 1) return LoraJoinArgs{};
+    return LoraJoinArgs{{pa, pb}, {a.dA, a.dB}, {a.dA ? int64_t(a.R) * a.K : 0, a.dB ? int64_t(a.R) * a.N : 0}, o.count,
+                        a.L, parts};
 }
 
 void launch_lora_backward(const LoraGradArgs &a, void *ws, hipStream_t s) {
     const int parts = outer_parts(a.T, a.K, a.N, a.R, a.L);
     const LoraSpace at(a.T, a.K, a.N, a.R, a.L, parts);
     char *base = static_cast<char *>(ws);
-    uint16_t *bt = reinterpret_cast<uint16_t *>(base + at.bt), *att = reinterpret_cast<uint16_t *>(base + at.at);
     float *dv = reinterpret_cast<float *>(base + at.dv);
-    const bool need_dv = a.dx || a.dA;
-    if (need_dv) {
-        const LoraTransposeArgs tb{a.B, bt, a.L, a.N, a.R}, ta{a.A, att, a.dx ? a.L : 0, a.R, a.K};
-        lora_transpose_kernel<<<unsigned(tb.blocks() + ta.blocks()), 256, 0, s>>>(tb, ta);
-        launch_lora_shrink(LoraShrinkArgs{a.dy, a.lddy, bt, a.ids, a.T, a.N, a.R, a.L, dv, a.f16}, s);
-    }
-    if (a.dA || a.dB) launch_lora_outer(a, base, at, parts, dv, s);
+    if (a.dx || a.dA)
+        launch_lora_shrink(LoraShrinkArgs{a.dy, a.lddy, a.B, a.ids, a.T, a.N, a.R, a.L, dv, a.f16, true}, s);
+    LoraJoinArgs join{};
+    if (a.dA || a.dB) join = launch_lora_outer(a, base, at, parts, dv, s);
     if (a.dx)
-        launch_lora_expand(LoraExpandArgs{dv, att, a.ids, a.scaling, a.T, a.K, a.R, a.L, a.f16, a.dx, a.lddx, a.dx_out,
+        launch_lora_expand(LoraExpandArgs{dv, a.A, a.ids, a.scaling, a.T, a.K, a.R, a.L, a.f16, a.dx, a.lddx, a.dx_out,
                                           a.lddxo, a.f16 ? 2 : 1, true},
-                           s);
+                           join, s);
+    else if (join.L) lora_outer_join_kernel<<<unsigned(join.L * join.blocks(256)), 256, 0, s>>>(join);
 }
 
 }  // namespace qwq4

@@ -380,6 +380,7 @@ struct LoraShrinkArgs {
     int T, K, R, L;
     float *v;
     bool f16;
+    bool inside;  // the ranks lie inside: A is [L][K][R]
 };
 void launch_lora_shrink(const LoraShrinkArgs &a, hipStream_t s);
 struct LoraExpandArgs {
@@ -394,16 +395,22 @@ struct LoraExpandArgs {
     void *out;
     int64_t ldo;
     int y_type;
-    bool grad;      // fp16 overflows to infinities (else saturates)
-    int tiles = 1;  // of 16 tokens, of a block: set by the launch
+    bool columns;   // gradients: B is [L][R][N], y and out of B's type, fp16 overflows to infinities (else saturates)
+    // set by the launch:
+    int tiles = 1;  // of 16 tokens, of a block
+    int side = 1;   // blocks that share the adapters of a block's tokens
 };
-void launch_lora_expand(LoraExpandArgs a, hipStream_t s);
-struct LoraTransposeArgs {
-    const uint16_t *in;  // [L][rows][cols]
-    uint16_t *out;
-    int L, rows, cols;
-    __host__ __device__ int blocks() const { return L * ((rows + 63) / 64) * ((cols + 63) / 64); }
+// The parts of an adapter's sums and what they add up to.
+struct LoraJoinArgs {
+    const float *part[2];  // dA's, dB's [parts][L][n]
+    float *out[2];         // [L][n]
+    int64_t n[2];          // 0: not wanted; multiples of 64
+    const int *count;      // [parts][L] tokens: parts of none are not read
+    int L, parts;          // L = 0: nothing to join
+    // blocks that an adapter takes
+    __host__ __device__ int blocks(int threads) const { return int((n[0] + n[1] + 4 * threads - 1) / (4 * threads)); }
 };
+void launch_lora_expand(LoraExpandArgs a, const LoraJoinArgs &join, hipStream_t s);
 // One of the two products over tokens: rows m [T][C], factors u [T][R].
 struct LoraOuterSide {
     const uint16_t *m;
