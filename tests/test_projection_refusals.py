@@ -108,7 +108,7 @@ def test_workspace_sizes(lib):
     assert lib.qw_logprobs_workspace_size(0, 100, 1) == 0 == lib.qw_logprobs_workspace_size(4096, 151936, 20)
     assert lib.qw_logprobs_workspace_size(1, 151936, 20) > lib.qw_logprobs_workspace_size(1, 151936, 0) > 0
     assert lib.qw_lora_backward_workspace_size(0, 64, 64, 16, 1) == 0
-    assert lib.qw_lora_backward_workspace_size(1, 64, 32, 16, 2) >= 2 * 16 * (64 + 32) * 2 + 16 * 4
+    assert lib.qw_lora_backward_workspace_size(1, 64, 32, 16, 2) >= 16 * 4  # (dv)
 
 
 def test_python_checks():

@@ -201,13 +201,19 @@ def tile_experts(W, S, Z, rows, K):
 T_F32, T_BF16, T_F16 = 0, 1, 2
 
 
+_codes = {}  # (filled by the first _tcode: this file loads without torch)
+
+
 def _tcode(t):
     """QW_T_* code of a tensor's dtype (float32, bfloat16, float16)."""
-    import torch
-    codes = {torch.float32: T_F32, torch.bfloat16: T_BF16, torch.float16: T_F16}
-    if t.dtype not in codes:
-        raise TypeError(f"unsupported element type {t.dtype}")
-    return codes[t.dtype]
+    code = _codes.get(t.dtype)
+    if code is None:
+        import torch
+        _codes.update({torch.float32: T_F32, torch.bfloat16: T_BF16, torch.float16: T_F16})
+        code = _codes.get(t.dtype)
+        if code is None:
+            raise TypeError(f"unsupported element type {t.dtype}")
+    return code
 
 
 def _tdtype(code):
@@ -533,12 +539,13 @@ def _here(fn, *ts):
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()
+        if at < 0:
             raise RuntimeError(f"{fn}: all tensors must be on the GPU")
         if dev is None:
             dev = torch.cuda.current_device()
-        if t.get_device() != dev:
-            raise RuntimeError(f"{fn}: a tensor is on GPU {t.get_device()}, the current one is {dev}")
+        if at != dev:
+            raise RuntimeError(f"{fn}: a tensor is on GPU {at}, the current one is {dev}")
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     return raw(dev) if raw is not None else torch.cuda.current_stream(dev).cuda_stream
 
@@ -849,7 +856,6 @@ def moe_unpermute_backward(dout, yp, tok_slot, tok_w=None, dyp=None, dw=None, ne
 # ------------------------------------------------------ around a projection
 def _norm_rows(fn, x, w, residual, residual_out):
     """(T, H, arguments of the C call up to eps, residual_out)"""
-    import torch
     _no_autograd(fn, x, w, residual)
     ldx = _matrix(fn, "x", x, None, None)
     T, H = x.shape
@@ -861,7 +867,7 @@ def _norm_rows(fn, x, w, residual, residual_out):
         return T, H, (_ptr(x), _tcode(x), ldx, None, 0, 0, None, 0, _ptr(w), _tcode(w)), None
     ldr = _matrix(fn, "residual", residual, T, H)
     if residual_out is None:
-        residual_out = torch.empty((T, H), dtype=residual.dtype, device=x.device)
+        residual_out = residual.new_empty((T, H))
     ldro = _matrix(fn, "residual_out", residual_out, T, H, residual.dtype)
     return T, H, (_ptr(x), _tcode(x), ldx, _ptr(residual), _tcode(residual), ldr, _ptr(residual_out), ldro, _ptr(w),
                   _tcode(w)), residual_out
@@ -887,9 +893,9 @@ def rms_norm_i8(x, w, eps=1e-6, residual=None, q=None, scale=None, residual_out=
     fn = "rms_norm_i8"
     T, H, args, residual_out = _norm_rows(fn, x, w, residual, residual_out)
     if q is None:
-        q = torch.empty((T, H), dtype=torch.int8, device=x.device)
+        q = x.new_empty((T, H), dtype=torch.int8)
     if scale is None:
-        scale = torch.empty(T, dtype=torch.float32, device=x.device)
+        scale = x.new_empty(T, dtype=torch.float32)
     ldq = _matrix(fn, "q", q, T, H, torch.int8)
     _whole(fn, "scale", scale, (T,), torch.float32)
     stream = _here(fn, x, w, residual, residual_out, q, scale)
@@ -915,16 +921,16 @@ def rms_norm_backward(dy, h, w, eps=1e-6, dres=None, dx=None, dw=None, need_dw=T
         raise ValueError(f"{fn}: w is {tuple(w.shape)}, not ({H},), or not contiguous")
     lddr = _matrix(fn, "dres", dres, T, H, h.dtype) if dres is not None else 0
     if dx is None:
-        dx = torch.empty((T, H), dtype=h.dtype, device=h.device)
+        dx = h.new_empty((T, H))
     lddx = _matrix(fn, "dx", dx, T, H, h.dtype)
     if not need_dw:
         dw = None
     else:
         if dw is None:
-            dw = torch.empty(H, dtype=torch.float32, device=h.device)
+            dw = h.new_empty(H, dtype=torch.float32)
         _whole(fn, "dw", dw, (H,), torch.float32)
         if workspace is None:
-            workspace = torch.empty(rms_norm_backward_workspace_size(T, H), dtype=torch.uint8, device=h.device)
+            workspace = h.new_empty(rms_norm_backward_workspace_size(T, H), dtype=torch.uint8)
     stream = _here(fn, dy, h, w, dres, dx, dw, workspace)
     _check(lib().qw_rms_norm_backward(_ptr(dy), _tcode(dy), lddy, _ptr(h), _tcode(h), ldh, _ptr(w), _tcode(w), eps,
                                       _ptr(dres), lddr, T, H, _ptr(dx), lddx, _ptr(dw), _ptr(workspace),
@@ -969,7 +975,7 @@ def lora(x, A, B, ids, y, scaling=None, out=None, v=None):
         out = y
     ldo = _matrix(fn, "out", out, T, N, y.dtype)
     if v is None:
-        v = torch.empty((T, R), dtype=torch.float32, device=x.device)
+        v = x.new_empty((T, R), dtype=torch.float32)
     else:
         _whole(fn, "v", v, (T, R), torch.float32)
     stream = _here(fn, x, A, B, ids, y, scaling, out, v)
@@ -1002,14 +1008,14 @@ def lora_backward(dy, x, A, B, ids, v, scaling=None, dx=None, dx_out=None, dA=No
     elif dx_out is not None:
         raise ValueError(f"{fn}: dx_out without dx")
     if need_weights:
-        dA = torch.empty((L, R, K), dtype=torch.float32, device=x.device) if dA is None else dA
-        dB = torch.empty((L, N, R), dtype=torch.float32, device=x.device) if dB is None else dB
+        dA = x.new_empty((L, R, K), dtype=torch.float32) if dA is None else dA
+        dB = x.new_empty((L, N, R), dtype=torch.float32) if dB is None else dB
         _whole(fn, "dA", dA, (L, R, K), torch.float32)
         _whole(fn, "dB", dB, (L, N, R), torch.float32)
     else:
         dA = dB = None
     if workspace is None:
-        workspace = torch.empty(lora_backward_workspace_size(T, K, N, R, L), dtype=torch.uint8, device=x.device)
+        workspace = x.new_empty(lora_backward_workspace_size(T, K, N, R, L), dtype=torch.uint8)
     stream = _here(fn, dy, x, A, B, ids, v, scaling, dx, dx_out, dA, dB, workspace)
     _check(lib().qw_lora_backward(_ptr(dy), lddy, _ptr(x), ldx, f16, _ptr(A), _ptr(B), _ptr(ids), _ptr(v), _ptr(scaling),
                                   T, K, N, R, L, _ptr(dx), lddx, _ptr(dx_out), lddxo, _ptr(dA), _ptr(dB),
@@ -1037,14 +1043,14 @@ def logprobs(logits, tokens, top=0, workspace=None):
         raise ValueError(f"{fn}: top = {top} (0..64, at most V = {V})")
     code = _tcode(logits)
     # (one buffer for the fp32 outputs: an allocation each would cost more than the call)
-    own = torch.empty(T * (3 + top), dtype=torch.float32, device=logits.device)
+    own = logits.new_empty(T * (3 + top), dtype=torch.float32)
     logp, entropy, lse, top_logp = own.split_with_sizes((T, T, T, T * top))
-    top_ids = torch.empty((T, top), dtype=torch.int32, device=logits.device) if top else None
+    top_ids = tokens.new_empty((T, top)) if top else None
     top_logp = top_logp.view(T, top) if top else None
     if workspace is None:
         need = logprobs_workspace_size(T, V, top)
         if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+            workspace = logits.new_empty(need, dtype=torch.uint8)
     stream = _here(fn, logits, tokens, own, workspace)
     _check(lib().qw_logprobs(_ptr(logits), code, ld, _ptr(tokens), T, V, top, _ptr(logp), _ptr(entropy), _ptr(lse),
                              _ptr(top_ids), _ptr(top_logp), _ptr(workspace), _space(fn, workspace), stream),
@@ -1064,7 +1070,7 @@ def logprobs_backward(logits, tokens, lse, entropy, dlogp=None, dentropy=None, d
         if t is not None:
             _whole(fn, name, t, (T,), torch.float32)
     if dlogits is None:
-        dlogits = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
+        dlogits = logits.new_empty((T, V))
     ldd = _matrix(fn, "dlogits", dlogits, T, V, logits.dtype)
     stream = _here(fn, logits, tokens, lse, entropy, dlogp, dentropy, dlogits)
     _check(lib().qw_logprobs_backward(_ptr(logits), _tcode(logits), ld, _ptr(tokens), _ptr(lse), _ptr(entropy),
