@@ -539,13 +539,12 @@ def _here(fn, *ts):
     for t in ts:
         if t is None:
             continue
-        at = t.get_device()
-        if at < 0:
+        if not t.is_cuda:
             raise RuntimeError(f"{fn}: all tensors must be on the GPU")
         if dev is None:
             dev = torch.cuda.current_device()
-        if at != dev:
-            raise RuntimeError(f"{fn}: a tensor is on GPU {at}, the current one is {dev}")
+        if t.get_device() != dev:
+            raise RuntimeError(f"{fn}: a tensor is on GPU {t.get_device()}, the current one is {dev}")
     raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     return raw(dev) if raw is not None else torch.cuda.current_stream(dev).cuda_stream
 
