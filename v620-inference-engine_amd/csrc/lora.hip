@@ -95,22 +95,32 @@ __device__ __forceinline__ int adapter_of(const int32_t *ids, int t, int T, int 
 // 7) of its row: without bank conflicts both ways.
 struct Turned {
     uint4 w[2];
-    // row(r): the row's pointer; the first n of the 64 elements exist
-    template <class Row>
-    __device__ __forceinline__ void load(Row row, int n) {
-        const int lane = int(threadIdx.x) % WAVE, k = lane % 8 * 8;
+    // the lane's places, in bytes behind the first element of `rows` (or the last one again) from `row0` on
+    __device__ static __forceinline__ void places(uint32_t (&at)[2], int row0, int rows, uint32_t stride) {
+        const int lane = int(threadIdx.x) % WAVE;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) at[i] = (uint32_t(min(row0 + 8 * i + lane / 8, rows - 1)) * stride + lane % 8 * 8) * 2;
+    }
+    // from: the same in every lane (places of 32 bits beside it: half the registers of pointers); the first n of the 64
+    // elements exist, and of the rows those in `rows` are asked for
+    __device__ __forceinline__ void load(const uint16_t *from, const uint32_t (&at)[2], int n, uint32_t rows = ~0u) {
+        const int lane = int(threadIdx.x) % WAVE;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            w[i] = k < n ? *reinterpret_cast<const uint4 *>(row(i) + k) : make_uint4(0, 0, 0, 0);
+            w[i] = lane % 8 * 8 < n && ((rows >> (8 * i + lane / 8)) & 1) ? *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(from) + at[i])
+                      : make_uint4(0, 0, 0, 0);
     }
-    __device__ __forceinline__ void turn(uint4 *lds) {
-        const int lane = int(threadIdx.x) % WAVE, r = lane / 8, c = lane % 16, g = lane / 16;
+    __device__ __forceinline__ void put(uint4 *lds) const {
+        const int lane = int(threadIdx.x) % WAVE, r = lane / 8;
         wave_lds_order();
 #pragma unroll
         for (int i = 0; i < 2; ++i) lds[(8 * i + r) * 8 + (lane % 8 ^ r)] = w[i];
         wave_lds_order();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) w[h] = lds[c * 8 + ((4 * h + g) ^ (c & 7))];
+    }
+    // the operand of the first or second 32 elements
+    __device__ static __forceinline__ uint4 operand(const uint4 *lds, int h) {
+        const int lane = int(threadIdx.x) % WAVE, c = lane % 16, g = lane / 16;
+        return lds[c * 8 + ((4 * h + g) ^ (c & 7))];
     }
     // (a wave's LDS accesses complete in order; the compiler must keep them so)
     __device__ static __forceinline__ void wave_lds_order() {
@@ -126,44 +136,52 @@ struct Turned {
 // 65; of rank 128, whose rows' pieces of 32 bytes cost the loads more, 179 for 172.
 struct TurnedColumns {
     uint4 w[2];
-    // at: the weights of step k's first row and the first of its ranks; the first n of the 64 rows exist, and ranks of
-    // them (a multiple of 8; behind them the last ones again, whose sums nothing takes)
-    __device__ __forceinline__ void load(const uint16_t *at, int R, int ranks, int n) {
-        const int lane = int(threadIdx.x) % WAVE, r = min(lane % 2 * 8, ranks - 8);
+    // the lane's places in bytes, the ranks from r0 on (behind the last one the last ones again, whose sums nothing takes)
+    __device__ static __forceinline__ void places(uint32_t (&at)[2], int r0, int R) {
+        const int lane = int(threadIdx.x) % WAVE;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int k = 32 * i + lane / 2;
-            w[i] = k < n ? *reinterpret_cast<const uint4 *>(at + k * R + r) : make_uint4(0, 0, 0, 0);
-        }
+        for (int i = 0; i < 2; ++i) at[i] = uint32_t((32 * i + lane / 2) * R + min(r0 + lane % 2 * 8, R - 8)) * 2;
     }
-    __device__ __forceinline__ void turn(uint4 *lds) {
-        typedef short s16x4 __attribute__((ext_vector_type(4)));
-        const int lane = int(threadIdx.x) % WAVE, c = lane % 16, g = lane / 16;
+    // the first n of the 64 rows exist
+    __device__ __forceinline__ void load(const uint16_t *from, const uint32_t (&at)[2], int n) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            w[i] = 32 * i + int(threadIdx.x) % WAVE / 2 < n
+                       ? *reinterpret_cast<const uint4 *>(reinterpret_cast<const char *>(from) + at[i])
+                       : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void put(uint4 *lds) const {
+        const int lane = int(threadIdx.x) % WAVE;
         Turned::wave_lds_order();
 #pragma unroll
         for (int i = 0; i < 2; ++i) lds[WAVE * i + lane] = w[i];
         Turned::wave_lds_order();
-        short *row = reinterpret_cast<short *>(lds) + (8 * g + c / 4) * 16 + c % 4 * 4;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            auto four = [&](int k) {
-                return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                     (__attribute__((address_space(3))) s16x4 *)(row + k * 16)));
-            };
-            const uint2 a = four(32 * h), b = four(32 * h + 4);
-            w[h] = make_uint4(a.x, a.y, b.x, b.y);
-        }
+    }
+    __device__ static __forceinline__ uint4 operand(uint4 *lds, int h) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        const int lane = int(threadIdx.x) % WAVE, c = lane % 16, g = lane / 16;
+        short *row = reinterpret_cast<short *>(lds) + (32 * h + 8 * g + c / 4) * 16 + c % 4 * 4;
+        auto four = [&](int k) {
+            return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                 (__attribute__((address_space(3))) s16x4 *)(row + k * 16)));
+        };
+        const uint2 a = four(0), b = four(4);
+        return make_uint4(a.x, a.y, b.x, b.y);
     }
 };
 
 // v[t][r] = sum_k A[id_t][r][k] x[t][k] for 16 tokens and 16 RF ranks by a block
 // whose 16 waves take a run of 64-wide steps of K each and join their sums in
 // LDS, in order: a row's bits depend on neither the batch nor its place in it.
-// Every wave has the next U steps of rows and weights on their way. INSIDE: the
-// ranks lie inside, A is [K][R].
+// Every wave has U steps of rows and weights on their way: a step's registers are
+// loaded again as soon as it lies in LDS (three steps of 16 ranks or two of 64: no
+// faster, or spilled: 110 us for 102 with 4096 x 12288 of rank 64). Rows of other
+// adapters are not read. A CU takes in rows and weights at 30 to 40 bytes a cycle,
+// which bounds it: 4096 rows of 4096 in 11 us (3.1 TB/s of rows, as much again of
+// weights out of L2), of 12288 in 29 (3.5). INSIDE: the ranks lie inside, A is [K][R].
 template <class T16, int RF, bool INSIDE>
 __global__ __launch_bounds__(1024) void lora_shrink_kernel(LoraShrinkArgs a) {
-    constexpr int NW = 16, U = RF == 1 ? 2 : 1;
+    constexpr int NW = 16, U = RF <= 2 ? 2 : 1;
     __shared__ uint4 s_turn[NW][2][128];  // (4 KB a wave, and then the waves' sums)
     f32x4(*s_part)[RF][WAVE] = reinterpret_cast<f32x4(*)[RF][WAVE]>(s_turn);
     static_assert(sizeof(f32x4) * NW * RF * WAVE <= sizeof(s_turn), "the sums fit");
@@ -172,49 +190,46 @@ __global__ __launch_bounds__(1024) void lora_shrink_kernel(LoraShrinkArgs a) {
     const int r0 = int(blockIdx.z) * (16 * RF);
     const int id = lane < 16 ? adapter_of(a.ids, t0 + lane, a.T, a.L) : -1;
     const int steps = (a.K + 63) / 64, per = (steps + NW - 1) / NW, end = min(steps, (wave + 1) * per);
-    const uint16_t *x[2];
+    const uint16_t *x = a.x + t0 * a.ldx;
+    uint32_t xat[2], wat[RF][2];  // (16 strides are below 2^31 bytes, as R K is)
+    Turned::places(xat, 0, a.T - t0, uint32_t(a.ldx));
 #pragma unroll
-    for (int i = 0; i < 2; ++i) x[i] = a.x + int64_t(min(t0 + 8 * i + lane / 8, a.T - 1)) * a.ldx;
+    for (int f = 0; f < RF; ++f) {
+        if constexpr (INSIDE) TurnedColumns::places(wat[f], r0 + 16 * f, a.R);
+        else Turned::places(wat[f], r0 + 16 * f, a.R, uint32_t(a.K));
+    }
     each_adapter(id, int(blockIdx.y), int(gridDim.y), [&](int l, unsigned long long mine) {
         const uint16_t *A = a.A + int64_t(l) * a.R * a.K;
-        uint32_t w[RF][2];  // (R K is below 2^28)
-#pragma unroll
-        for (int f = 0; f < RF; ++f)
-#pragma unroll
-            for (int i = 0; i < 2 && !INSIDE; ++i) w[f][i] = uint32_t(min(r0 + 16 * f + 8 * i + lane / 8, a.R - 1)) * uint32_t(a.K);
         f32x4 acc[RF];
 #pragma unroll
         for (int f = 0; f < RF; ++f) acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-        struct Steps {
-            Turned x[U];
-            std::conditional_t<INSIDE, TurnedColumns, Turned> w[U][RF];
-        } next;
-        auto load = [&](int s0) {
+        Turned nx[U];
+        std::conditional_t<INSIDE, TurnedColumns, Turned> nw[U][RF];
+        auto load = [&](int u, int step) {
+            if (step >= end) return;
+            const int k = step * 64, n = a.K - k;
+            nx[u].load(x + k, xat, n, uint32_t(mine));
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int k = (s0 + u) * 64, n = s0 + u < end ? a.K - k : 0;
-                next.x[u].load([&](int i) { return x[i] + k; }, n);
-#pragma unroll
-                for (int f = 0; f < RF; ++f) {
-                    if constexpr (INSIDE) {
-                        const int r = min(r0 + 16 * f, a.R - 8);
-                        next.w[u][f].load(A + (uint32_t(k) * uint32_t(a.R) + uint32_t(r)), a.R, a.R - r, n);
-                    } else next.w[u][f].load([&](int i) { return A + (w[f][i] + uint32_t(k)); }, n);
-                }
-            }
+            for (int f = 0; f < RF; ++f) nw[u][f].load(A + (INSIDE ? int64_t(k) * a.R : k), wat[f], n);
         };
-        load(wave * per);
-        for (int s0 = wave * per; s0 < end; s0 += U) {
-            Steps now = next;
-            if (s0 + U < end) load(s0 + U);
+        const int first = wave * per;
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(u, first + u);
+        for (int s0 = first; s0 < end; s0 += U) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                now.x[u].turn(s_turn[wave][0]);
+                if (s0 + u >= end) continue;
+                nx[u].put(s_turn[wave][0]);
+                uint4 xf[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) xf[h] = Turned::operand(s_turn[wave][0], h);
 #pragma unroll
                 for (int f = 0; f < RF; ++f) {
-                    now.w[u][f].turn(s_turn[wave][1]);
+                    nw[u][f].put(s_turn[wave][1]);
+                    if (f + 1 == RF) load(u, s0 + u + U);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) acc[f] = mfma16<T16>(now.w[u][f].w[h], now.x[u].w[h], acc[f]);
+                    for (int h = 0; h < 2; ++h)
+                        acc[f] = mfma16<T16>(nw[u][f].operand(s_turn[wave][1], h), xf[h], acc[f]);
                 }
             }
         }
