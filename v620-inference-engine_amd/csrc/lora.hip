@@ -484,10 +484,12 @@ void launch_lora_expand(LoraExpandArgs a, const LoraJoinArgs &join, hipStream_t 
         constexpr int YT = decltype(yt)::value;
         const bool one = (YT == 0 ? 3 : 2) * a.R <= 32;
         const int waves = !one && a.R > 64 ? 2 : 4;  // (at most 64 KB of weights a block)
-        // Tiles of a block: the weights are read once for all of them, but first of all the chip is to be filled; then
-        // the adapters of a block's tokens side by side.
+        // Tiles of a block: the weights are read once for all of them, but first of all the chip is to be filled (one
+        // tile for two: 2048 x 4096 of rank 16 19.5 us for 16.8). Two serve small ranks up to the largest calls (four: 4096 x
+        // 4096 of rank 32 34.8 us for 33.2; 16384 x 12288 of rank 16 187 for 191), four the large ranks (two: 4096 x
+        // 12288 of rank 128 235 us for 218). Then the adapters of a block's tokens side by side.
         const int tiles = (a.T + 15) / 16, cols = (a.N + 128 * waves - 1) / (128 * waves);
-        a.tiles = tiles * cols >= 2048 ? 4 : tiles * cols >= 1024 ? 2 : 1;
+        a.tiles = tiles * cols >= (a.R < 64 ? 16384 : 2048) ? 4 : tiles * cols >= 1024 ? 2 : 1;
         const int groups = (tiles + a.tiles - 1) / a.tiles;
         a.side = std::max(1, std::min({1024 / (groups * cols), 16 * a.tiles, a.L, a.T}));
         const unsigned threads = unsigned(waves * WAVE);
