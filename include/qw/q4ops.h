@@ -444,8 +444,8 @@ int qw_moe_unpermute_backward(const void *dout, int dout_type, int ldd, const vo
  * Root-mean-square norm of rows x [T][H], with the residual's addition:
  *   h = x + residual (fp32),  y = h w / sqrt(mean(h^2) + eps)
  * residual [T][H] of x's type or fp32, or NULL (h = x); res_out [T][H] of its
- * type gets h, rounded (with a residual only; it may be the residual itself, at
- * the same stride). y is normalised from h as added, before that rounding.
+ * type gets h, rounded (with a residual only; it may be the residual itself, or x
+ * where that is of its type, at the same stride). y is normalised from h as added, before that rounding.
  * x and y of any QW_T_* type, w [H] of x's type or fp32; y may be x where type and
  * stride are the same. fp16 outputs saturate at +-65504. Sums in fp32: rows with values
  * past 1e19 overflow them and give zeros. Any H from 1 to 2^28, any stride >= H and
@@ -458,7 +458,7 @@ int qw_rms_norm(const void *x, int x_type, int ldx, const void *residual, int re
  *   u = h w,  c = max_j |u_j| / 127,  q = rint(u (1 / c)),  scale = c / sqrt(mean(h^2) + eps)
  * (q is what qw_quant_tokens_i8 gives for the rows u in fp32: c is 1 for a row of
  * zeros and at least 2^-126; an infinity or a NaN in u gives a NaN scale and q of
- * zeros). q [T][H] of stride ldq >= H, scale fp32 [T]. */
+ * zeros). q [T][H] of stride ldq >= H, not on x or a residual; scale fp32 [T]. */
 int qw_rms_norm_i8(const void *x, int x_type, int ldx, const void *residual, int res_type, int ldr, void *res_out,
                    int ldro, const void *w, int w_type, float eps, int T, int H, int8_t *q, int ldq, float *scale,
                    void *stream);

@@ -17,7 +17,7 @@ def norm(x=P, xt=1, ldx=64, r=Q, rt=1, ldr=64, ro=Q, ldro=64, w=P, wt=0, eps=1e-
     return "qw_rms_norm", (x, xt, ldx, r, rt, ldr, ro, ldro, w, wt, eps, T, H, y, yt, ldy, None)
 
 
-def norm_i8(x=P, xt=1, ldx=64, r=None, rt=0, ldr=0, ro=None, ldro=0, w=P, wt=0, eps=1e-6, T=4, H=64, q=P, ldq=64, s=P):
+def norm_i8(x=P, xt=1, ldx=64, r=None, rt=0, ldr=0, ro=None, ldro=0, w=P, wt=0, eps=1e-6, T=4, H=64, q=Q, ldq=64, s=P):
     return "qw_rms_norm_i8", (x, xt, ldx, r, rt, ldr, ro, ldro, w, wt, eps, T, H, q, ldq, s, None)
 
 
@@ -56,6 +56,8 @@ CALLS = {
     "norm eps negative": norm(eps=-1.0), "norm eps nan": norm(eps=NAN), "norm eps infinite": norm(eps=float("inf")),
     "i8 null q": norm_i8(q=None), "i8 null scale": norm_i8(s=None), "i8 ldq": norm_i8(ldq=63), "i8 no rows": norm_i8(T=0),
     "i8 x type": norm_i8(xt=5), "i8 scale odd": norm_i8(s=TWO), "i8 residual without res_out": norm_i8(r=P, rt=1, ldr=64),
+    "i8 q on x": norm_i8(q=P), "i8 q on the residual": norm_i8(r=Q, rt=1, ldr=64, ro=Q, ldro=64),
+    "norm res_out on x, other type": norm(ro=P, rt=0, y=EIGHT), "norm res_out on x, other stride": norm(ro=P, ldro=72, ldr=72, y=EIGHT),
     "grad null dy": norm_grad(dy=None), "grad null h": norm_grad(h=None), "grad null w": norm_grad(w=None),
     "grad null dx": norm_grad(dx=None), "grad no rows": norm_grad(T=0), "grad rows too long": norm_grad(H=16385),
     "grad h type": norm_grad(ht=2), "grad w type": norm_grad(wt=2), "grad dy type": norm_grad(dt=7),

@@ -595,6 +595,8 @@ static int check_norm(const char *fn, const qwq4::NormArgs &a) {
     REQUIRE(a.res_type == QW_T_F32 || a.res_type == a.x_type, "%s: res_type = %d (fp32 or x's type)", fn, a.res_type);
     if (int r = check_plain_rows(fn, "residual", a.res, a.res_type, int(a.ldr), a.T, a.H)) return r;
     if (int r = check_plain_rows(fn, "res_out", a.res_out, a.res_type, int(a.ldro), a.T, a.H)) return r;
+    REQUIRE(a.res_out != a.x || (a.res_type == a.x_type && (a.T == 1 || a.ldro == a.ldx)),
+            "%s: res_out lies on x with another type or stride", fn);
     return check_in_place(fn, "res_out", a.res_out, int(a.ldro), a.res, int(a.ldr), a.T);
 }
 
@@ -620,6 +622,7 @@ int qw_rms_norm_i8(const void *x, int x_type, int ldx, const void *residual, int
     const qwq4::NormArgs a{x,      x_type, ldx, residual, res_type, ldr, res_out, ldro, w,
                            w_type, q,      0,   ldq,      scale,    T,   H,       eps};
     if (int r = check_norm(fn, a)) return r;
+    REQUIRE(q != x && q != residual && q != res_out, "%s: q lies on x or the residual", fn);
     REQUIRE((T == 1 || ldq >= H) && aligned(scale, 4), "%s: ldq %d < H = %d, or scale misaligned", fn, ldq, H);
     qwq4::launch_rms_norm(a, st(stream));
     return launched(fn);
