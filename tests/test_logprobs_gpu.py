@@ -183,3 +183,20 @@ def test_offsets_past_32_bits(gpu):
     d = qwq4.logprobs_backward(logits, tok, got[2], got[1], dlogp, dlogp, dlogits=logits.clone())
     want, bound = ref.logprobs_grad(logits[-3:], tok[-3:], got[2][-3:], got[1][-3:], dlogp[-3:], dlogp[-3:])
     assert_close(d[-3:], want, bound)
+
+
+@pytest.mark.parametrize("top", [31, 32, 33, 63, 64])
+@pytest.mark.parametrize("T,V", [(1, 151936), (9, 20011), (70, 9001), (600, 2500)])
+@pytest.mark.parametrize("kind", ["peaks", "wide"])
+def test_many_alternatives(gpu, T, V, top, kind):
+    """Where the groups that bound the alternatives change."""
+    print(f"logprobs T={T} V={V} top={top} {kind}", flush=True)
+    logits, tokens, _ = make(T + top, T, V, "bf16", gpu, kind=kind)
+    check(logits, tokens, top, qwq4.logprobs(logits, tokens, top=top))
+
+
+@pytest.mark.parametrize("kind,top", [("peaks", 20), ("peaks", 64), ("ties", 3)])
+def test_very_long_rows(gpu, kind, top):
+    """Several steps to each largest value that is kept."""
+    logits, tokens, _ = make(top, 1, 17_500_001, "f32", gpu, kind=kind)
+    check(logits, tokens, top, qwq4.logprobs(logits, tokens, top=top))

@@ -214,155 +214,28 @@ __device__ __forceinline__ void rank_keys(const TopKey *keys, int n, int k, Put 
     for (int e = n + int(threadIdx.x); e < k; e += int(blockDim.x)) put(e, TopKey(0));
 }
 
-// A part of a row by four waves with 2 pieces a lane: all of it in registers.
-// The k-th of a wave's lanes' largest has k values at or ahead of it, and so
-// has the farthest of the four waves': only values not behind that can be
-// among the part's first k. They go to a list in LDS (k and a few, and never
-// more than the part has) and are ranked.
-constexpr int MAX_SPLITS = 64;  // parts of a row at most
-constexpr int FEW_PIECES = 4 * WAVE * 2;
-template <int TY, bool TOP>
-__global__ __launch_bounds__(256) void logprobs_few_kernel(LogprobArgs a) {
-    constexpr int Z = TY == 0 ? 4 : 2;
-    __shared__ float s_st[4][3];
-    __shared__ TopKey s_last;
-    __shared__ int s_n;
-    __shared__ TopKey s_best[TOP ? 4 : 1][WAVE];
-    __shared__ TopKey s_keys[TOP ? 8 * FEW_PIECES + WAVE : 1];  // (and the row's head and tail)
-    const int tid = int(threadIdx.x), lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-    const int64_t t = int64_t(blockIdx.x) / a.splits;
-    const int split = int(blockIdx.x) % a.splits;
-    const char *row = static_cast<const char *>(a.logits) + t * a.ld * Z;
-    const RowCut cut(row, Z, a.V);
-    const char *body = row + int64_t(cut.head) * Z;
-    if (tid == 0) {
-        s_last = 0;
-        s_n = 0;
-    }
-    const int p0 = split * FEW_PIECES + tid;
-    Raw8<TY> raw[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-        if (p0 + 256 * u < cut.pieces) raw[u].load(body + int64_t(p0 + 256 * u) * (8 * Z));
-    // (single elements before and behind the pieces: one each by the first lanes)
-    const int alone = tid < cut.head ? tid : 8 * cut.pieces + tid;
-    const bool has_alone = split == 0 && tid < cut.head + cut.tail;
-    const float extra = has_alone ? logit_at<TY>(row, alone) : neg_inf();
-    float v[2][8], largest = extra;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const bool in = p0 + 256 * u < cut.pieces;
-        raw[u].values(v[u]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[u][j] = in ? v[u][j] : neg_inf();
-            largest = fmaxf(largest, v[u][j]);
-        }
-    }
-    SoftStats st;
-    st.clear();
-    const float ref = st.raise(largest);
-    st.add(v, ref);
-    st.add(extra, ref);
-    st = wave_join(st);
-    if (lane == 0) {
-        s_st[wave][0] = st.m;
-        s_st[wave][1] = st.s;
-        s_st[wave][2] = st.u;
-    }
-    // f(value, index) for all that the lane holds, single elements behind the row's before it
-    auto each = [&](auto f) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int p = p0 + 256 * u;
-            if (p < cut.pieces) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) f(v[u][j], cut.head + 8 * p + j);
-            }
-        }
-        if (has_alone) f(extra, alone);
-    };
-    TopKey best = 0;
-    if constexpr (TOP) {
-        float w = neg_inf();
-        int i = INT_MAX;
-        each([&](float x, int at) {
-            const bool first = ahead(x, at, w, i);
-            w = first ? x : w;
-            i = first ? at : i;
-        });
-        best = top_key(w, i);
-        s_best[wave][lane] = best;
-    }
-    __syncthreads();
-    st = SoftStats{s_st[0][0], s_st[0][1], s_st[0][2]};
-#pragma unroll
-    for (int w = 1; w < 4; ++w) st.join(SoftStats{s_st[w][0], s_st[w][1], s_st[w][2]});
-    const int64_t part = t * a.splits + split;
-    if constexpr (TOP) {
-        int rank = 0;
-#pragma unroll 16
-        for (int l = 0; l < WAVE; ++l) rank += int(s_best[wave][l] > best);
-        if (rank == a.top - 1) atomicMax(&s_last, best);
-        __syncthreads();
-        const TopKey last = max(s_last, TopKey(1));
-        const float last_v = key_value(last);
-        const int last_i = key_index(last);
-        const bool any = last == 1;  // (the part has fewer than k values: all of them)
-        auto kept = [&](float x, int at) { return (x > last_v) | ((x == last_v) & (at <= last_i)) | (any & (x == x)); };
-        int mine = 0;
-        if (best >= last) each([&](float x, int at) { mine += int(kept(x, at)); });
-        int before = mine;
-#pragma unroll
-        for (int o = 1; o < WAVE; o <<= 1) {
-            const int u = __shfl_up(before, o);
-            if (lane >= o) before += u;
-        }
-        int base = 0;
-        if (lane == WAVE - 1) base = atomicAdd(&s_n, before);
-        before += __builtin_amdgcn_readlane(base, WAVE - 1) - mine;
-        if (mine > 0) each([&](float x, int at) {
-            if (kept(x, at)) s_keys[before++] = top_key(x, at);
-        });
-        __syncthreads();
-        float lse = 0.f;
-        __shared__ float s_lse;
-        if (a.splits == 1) {
-            if (tid == 0) s_lse = finish_row<TY>(a, t, row, st);
-            __syncthreads();
-            lse = s_lse;
-        }
-        rank_keys(s_keys, s_n, a.top, [&](int r, TopKey k) {
-            if (a.splits == 1) put_top(a, t, r, k, lse);
-            else a.part_key[part * a.top + r] = k;
-        });
-    } else if (a.splits == 1 && tid == 0) {
-        finish_row<TY>(a, t, row, st);
-    }
-    if (a.splits > 1 && tid == 0) {
-        a.part_st[3 * part] = st.m;
-        a.part_st[3 * part + 1] = st.s;
-        a.part_st[3 * part + 2] = st.u;
-    }
-}
-
 // Part `split` of row t by a block of four waves, each taking every fourth
 // step of 64 U pieces. TOP: the largest value of each lane's step is left in LDS
-// on the way. The lanes make 64 groups (a lane of each wave); the k-th of the
-// groups' largest has k values at or above it, and only steps whose largest is
-// not below it are read a second time: of a row of 151936 and k = 5, some 6 of
-// 4736, from which some 5 values go to the list that is ranked. (A sorted list per
-// wave kept up to date on the way: 5 alternatives 45 us more in 4096 rows, 20
-// alternatives 130.) Where more than the list takes are left (rows with thousands of
-// equal values, fewer than k unmasked ones), the part is read again into sorted lists.
+// on the way. The lanes make 64 groups (a lane of each wave; 256, the lanes alone, for
+// k > 32: of 64 groups as many as k are hardly a bound, 4096 rows of 151936 and k = 64
+// 387 us for 248); the k-th of the groups' largest has k values at or above it, and
+// only steps whose largest is not below it are read a second time: of such a row and
+// k = 5, some 6 of 4736, from which some 5 values go to the list that is ranked. (A
+// sorted list per wave kept up to date on the way: 5 alternatives 45 us more in 4096
+// rows, 20 alternatives 130. Each lane reading its own steps again, one after the
+// other: 13 and 38 more, and 200 rows 41 us for 25.) Where more than the list takes
+// are left (rows with thousands of equal values, fewer than k unmasked ones), the
+// part is read again into sorted lists. Bound by memory: 4096 rows 224 us, 5.6 TB/s.
+constexpr int MAX_SPLITS = 64;  // parts of a row at most
 constexpr int TOP_SLOTS = 32, TOP_LIST = 512;
 template <int TY, bool TOP, int U>
 __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     constexpr int Z = TY == 0 ? 4 : 2;
     extern __shared__ float s_max[];  // TOP: [slots][256]
-    __shared__ int s_n;
+    __shared__ int s_n, s_again;
+    __shared__ uint16_t s_slots[TOP ? TOP_LIST : 1];
     __shared__ float s_st[4][3], s_bound, s_lse;
-    __shared__ float s_lane[TOP ? 256 : 1];
+    __shared__ __align__(16) float s_lane[TOP ? 256 : 1];
     __shared__ TopKey s_keys[TOP ? TOP_LIST : 1];
     const int tid = int(threadIdx.x), lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int64_t t = int64_t(blockIdx.x) / a.splits;
@@ -372,7 +245,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     const char *body = row + int64_t(cut.head) * Z;
     const int steps = (cut.pieces + WAVE * U - 1) / (WAVE * U);
     const int per = (steps + a.splits - 1) / a.splits, first = split * per, end = min(steps, first + per);
-    if (TOP && tid == 0) s_n = 0;
+    if (TOP && tid == 0) s_n = s_again = 0;
     // (single elements before and behind the pieces: one each by the first lanes)
     const int alone = tid < cut.head ? tid : 8 * cut.pieces + tid;
     const bool has_alone = split == 0 && tid < cut.head + cut.tail;
@@ -454,7 +327,19 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     }
     if constexpr (!TOP) return;
 
-    if (wave == 0) {
+    if (a.top > WAVE / 2) {
+        const float own = s_lane[tid];
+        int rank = 0;
+#pragma unroll 4
+        for (int l = 0; l < 256; l += 4) {
+            const float4 other = *reinterpret_cast<const float4 *>(&s_lane[l]);
+            rank += int((other.x > own) | ((other.x == own) & (l < tid)));
+            rank += int((other.y > own) | ((other.y == own) & (l + 1 < tid)));
+            rank += int((other.z > own) | ((other.z == own) & (l + 2 < tid)));
+            rank += int((other.w > own) | ((other.w == own) & (l + 3 < tid)));
+        }
+        if (rank == a.top - 1) s_bound = own;
+    } else if (wave == 0) {
         const float own = fmaxf(fmaxf(s_lane[lane], s_lane[lane + 64]), fmaxf(s_lane[lane + 128], s_lane[lane + 192]));
         int rank = 0;
 #pragma unroll 16
@@ -472,32 +357,30 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
         if (n < TOP_LIST) s_keys[n] = top_key(x, at);
     };
     if (has_alone) keep(extra, alone);
+    // (listed before they are read again, a piece a thread: all of them are asked for at once)
+#pragma unroll 4
     for (int k = 0; k < slot; ++k) {
         if (!(s_max[k * 256 + tid] >= bound)) continue;
-        for (int c = 0; c < a.slot_steps; ++c) {
-            const int again = first + wave + 4 * (k * a.slot_steps + c);
-            if (again >= end) break;
-            load(again, raw);
+        const int i = atomicAdd(&s_again, 1);
+        if (i < TOP_LIST) s_slots[i] = uint16_t(k * 256 + tid);
+    }
+    __syncthreads();
+    const int each = a.slot_steps * U;  // pieces of a slot
+    for (int i = tid; i < min(s_again, TOP_LIST) * each; i += 256) {
+        const int at = s_slots[i / each], c = i % each / U, u = i % U;
+        const int again = first + at % 256 / WAVE + 4 * (at / 256 * a.slot_steps + c);
+        const int p = (again * U + u) * WAVE + at % WAVE;
+        if (again >= end || p >= cut.pieces) continue;
+        Raw8<TY> piece;
+        piece.load(body + int64_t(p) * (8 * Z));
+        float v[8];
+        piece.values(v);
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int p = (again * U + u) * WAVE + lane;
-                float v[8];
-                raw[u].values(v);
-                if (p < cut.pieces) {
-#pragma unroll 1
-                    for (int j = 0; j < 8; ++j) {
-                        float x = v[0];
-#pragma unroll
-                        for (int i = 1; i < 8; ++i) x = j == i ? v[i] : x;
-                        keep(x, cut.head + 8 * p + j);
-                    }
-                }
-            }
-        }
+        for (int j = 0; j < 8; ++j) keep(v[j], cut.head + 8 * p + j);
     }
     __syncthreads();
     int n = s_n;
-    if (n > TOP_LIST) {
+    if (max(n, s_again) > TOP_LIST) {
         TopList list;
         list.clear(a.top);
         auto take = [&](float w, int i, bool have) {
@@ -545,7 +428,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
 // The parts of a row joined, in order, by a block. With j the least such that
 // the parts' first j keys are k or more, the ceil(k / j)-th of the parts' j-th
 // keys has k keys at or ahead of it: what is behind it is left out, and the rest
-// ranked. (Of 38 parts of 20 keys each some 40 are left, and 450 if only the
+// ranked. (Of 19 parts of 20 keys each some 30 are left, and most if only the
 // parts' last keys are gone by.)
 template <int TY>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
@@ -593,18 +476,14 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
     rank_keys(s_keys, s_n, a.top, [&](int rank, TopKey key) { put_top(a, t, rank, key, lse); });
 }
 
-// Few rows: a part of a row is what four waves hold at once (a row of 151936
-// in 38 parts). Else a block takes a row, or a part of it while there are too few
-// blocks for the chip, with at least a step for each wave.
-static int logprob_few_parts(int T, int V) {
-    const int parts = std::max(1, (V / 8 + FEW_PIECES - 1) / FEW_PIECES);
-    return T < 64 && parts <= MAX_SPLITS ? parts : 0;
-}
+// A block takes a row, or a part of it while there are too few blocks for the
+// chip, with at least a step for each wave: two blocks a CU (eight: every block
+// has a tail in which it looks for its alternatives, and there are rows to join:
+// 1000 rows of 50257 and 5 alternatives 34 us for 25, of 151936 68 for 63).
 constexpr int LOGPROB_U = 4;
 static int logprob_splits(int T, int V) {
-    if (const int few = logprob_few_parts(T, V)) return few;
     const int steps = std::max(1, V / (8 * WAVE * LOGPROB_U));
-    return std::max(1, std::min({(2048 + T - 1) / T, (steps + 3) / 4, MAX_SPLITS}));
+    return std::max(1, std::min({(512 + T - 1) / T, (steps + 3) / 4, MAX_SPLITS}));
 }
 
 size_t logprobs_workspace_bytes(int T, int V, int top) {
@@ -619,18 +498,13 @@ void launch_logprobs(LogprobArgs a, void *ws, hipStream_t s) {
     a.part_st = reinterpret_cast<float *>(a.part_key + parts * size_t(a.top));
     by_type(a.type, [&](auto ty) {
         constexpr int TY = decltype(ty)::value;
-        if (logprob_few_parts(a.T, a.V)) {
-            if (a.top) logprobs_few_kernel<TY, true><<<unsigned(parts), 256, 0, s>>>(a);
-            else logprobs_few_kernel<TY, false><<<unsigned(parts), 256, 0, s>>>(a);
-        } else {
-            // (a wave's steps at most; a row's cut can only make them fewer)
-            const int steps = (a.V / 8 + WAVE * LOGPROB_U - 1) / (WAVE * LOGPROB_U);
-            const int wave = ((steps + a.splits - 1) / a.splits + 3) / 4;
-            a.slot_steps = std::max(1, (wave + TOP_SLOTS - 1) / TOP_SLOTS);
-            const size_t lds = size_t((wave + a.slot_steps - 1) / a.slot_steps) * 1024;
-            if (a.top) logprobs_kernel<TY, true, LOGPROB_U><<<unsigned(parts), 256, lds, s>>>(a);
-            else logprobs_kernel<TY, false, LOGPROB_U><<<unsigned(parts), 256, 0, s>>>(a);
-        }
+        // (a wave's steps at most; a row's cut can only make them fewer)
+        const int steps = (a.V / 8 + WAVE * LOGPROB_U - 1) / (WAVE * LOGPROB_U);
+        const int wave = ((steps + a.splits - 1) / a.splits + 3) / 4;
+        a.slot_steps = std::max(1, (wave + TOP_SLOTS - 1) / TOP_SLOTS);
+        const size_t lds = size_t((wave + a.slot_steps - 1) / a.slot_steps) * 1024;
+        if (a.top) logprobs_kernel<TY, true, LOGPROB_U><<<unsigned(parts), 256, lds, s>>>(a);
+        else logprobs_kernel<TY, false, LOGPROB_U><<<unsigned(parts), 256, 0, s>>>(a);
         if (a.splits > 1) logprobs_join_kernel<TY><<<unsigned(a.T), 256, 0, s>>>(a);
     });
 }
