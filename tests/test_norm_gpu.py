@@ -229,3 +229,12 @@ def test_offsets_past_32_bits(gpu):
     del y
     dx, _ = qwq4.rms_norm_backward(xs, xs, w, EPS)
     assert torch.equal(dx[-3:], qwq4.rms_norm_backward(xs[-3:], xs[-3:], w, EPS)[0])
+
+
+@pytest.mark.parametrize("T,H", [(40001, 64), (20000, 100), (9001, 129), (9000, 256), (4100, 384), (3001, 1000), (1500, 1032),
+                                 (2100, 2048), (700, 2047), (600, 5120), (300, 12288)])
+@pytest.mark.parametrize("dy,h,dres", [("bf16", "bf16", True), ("f16", "f32", False), ("f32", "f32", False)])
+def test_many_rows(gpu, T, H, dy, h, dres):
+    """Every way of sharing rows among lanes, waves and blocks with more rows than are taken at once."""
+    test_norm_backward(gpu, T, H, dy, h, dres)
+    test_norm(gpu, T, H, dy, "f32" if h == "f32" else None, dy)

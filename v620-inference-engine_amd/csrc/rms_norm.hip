@@ -56,9 +56,11 @@ __device__ __forceinline__ void any_store(void *y, int type, int64_t row, int j,
     else part_store<2, VEC>(y, row, j, n, v);
 }
 
-__device__ __forceinline__ float wave_add(float v) {
+// the sum over groups of G lanes
+template <int G>
+__device__ __forceinline__ float group_add(float v) {
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    for (int o = G / 2; o >= 1; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
 
@@ -74,7 +76,7 @@ __device__ __forceinline__ void load_h(const NormArgs &a, int64_t x0, int64_t r0
     }
 }
 
-// A row by G threads (64: a wave, four rows a block; 256: the block), 8
+// A row by G threads (16: a wave takes four; 64: a wave; 256: the block), 8
 // elements per thread and turn. C > 0: the row is held in C turns' registers
 // and read once; C = 0: any length, read twice (the second time from the
 // caches; the residual is written then, since it may lie on its input).
@@ -83,7 +85,7 @@ template <int XT, int RT, int WT, bool I8, bool VEC, int G, int C>
 __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
     const int li = int(threadIdx.x) % G, H = a.H;
     const int64_t t = int64_t(blockIdx.x) * (256 / G) + int(threadIdx.x) / G;
-    if (t >= a.T) return;  // (whole waves, where G = 64: they meet no barrier)
+    if (t >= a.T) return;  // (whole groups, where G < 256: they meet no barrier)
     const int64_t x0 = t * a.ldx, r0 = t * a.ldr, o0 = t * a.ldro, y0 = t * a.ldy;
     float h[C > 0 ? C : 1][8], w[C > 0 ? C : 1][8];
     float sum = 0.f;
@@ -122,10 +124,10 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a) {
             count(h[0], w[0]);
         }
     }
-    sum = wave_add(sum);
+    sum = group_add<G < WAVE ? G : WAVE>(sum);
     if constexpr (I8) {
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) top = max(top, uint32_t(__shfl_xor(int(top), o)));
+        for (int o = (G < WAVE ? G : WAVE) / 2; o >= 1; o >>= 1) top = max(top, uint32_t(__shfl_xor(int(top), o)));
     }
     if constexpr (G == 256) {
         __shared__ float s_sum[4];
@@ -195,8 +197,13 @@ static void launch_norm(const NormArgs &a, hipStream_t s) {
         rms_norm_kernel<XT, RT, WT, I8, decltype(vec)::value, G, decltype(c)::value>
             <<<unsigned((a.T + ROWS - 1) / ROWS), 256, 0, s>>>(a);
     };
+    // (16.8 million elements in bf16 with a residual: rows of 64 by waves 100 us, by 16 lanes 29; of 520 by blocks 37, by
+    // waves 28)
     auto by_length = [&](auto vec) {
-        if (a.H <= 512) run(vec, Int<64>{}, Int<1>{});
+        if (a.H <= 128) run(vec, Int<16>{}, Int<1>{});
+        else if (a.H <= 256) run(vec, Int<16>{}, Int<2>{});
+        else if (a.H <= 512) run(vec, Int<64>{}, Int<1>{});
+        else if (a.H <= 1024) run(vec, Int<64>{}, Int<2>{});
         else if (a.H <= 2048) run(vec, Int<256>{}, Int<1>{});
         else if (a.H <= 4096) run(vec, Int<256>{}, Int<2>{});
         else if (a.H <= 8192) run(vec, Int<256>{}, Int<4>{});
@@ -248,15 +255,18 @@ struct Part<TY, false> {
     }
 };
 
-// A block of TH threads takes rows blockIdx.x, blockIdx.x + gridDim.x, .., 8
-// elements per thread and C turns each, with the next row on its way while the
-// current one's sums are made, and keeps its columns' part of dw in registers;
-// the blocks' parts are added in order by a second launch. Bound by memory.
-template <int DT, int HT, int WT, bool VEC, int TH, int C>
+// A row by G of the block's TH threads (16, 64: groups of a wave, which meet no
+// barrier but the last; TH: the block), 8 elements per thread and C turns each. A
+// group takes every (groups of the grid)-th row, with the next one on its way
+// while the current one's sums are made, and keeps its columns' part of dw in
+// registers; the block adds its groups' parts and a second launch the blocks', in
+// order. Bound by memory.
+template <int DT, int HT, int WT, bool VEC, int G, int TH, int C>
 __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
-    constexpr int NW = TH / WAVE;
+    constexpr int NW = TH / WAVE, GROUPS = TH / G;
+    constexpr bool BLOCK = G == TH;
     __shared__ float s_sum[2][2][NW];
-    const int tid = int(threadIdx.x), H = a.H;
+    const int tid = int(threadIdx.x), li = BLOCK ? tid : tid % G, H = a.H;
     struct Row {
         Part<HT, VEC> h[C], res[C];
         Part<DT, VEC> d[C];
@@ -266,7 +276,7 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
     auto load = [&](int64_t t) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int j = (tid + c * TH) * 8;
+            const int j = (li + c * G) * 8;
             if (j >= H) continue;
             next.h[c].load(a.h, t * a.ldh, j, H);
             next.d[c].load(a.dy, t * a.lddy, j, H);
@@ -275,20 +285,21 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
     };
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-        const int j = (tid + c * TH) * 8;
+        const int j = (li + c * G) * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) dw[c][e] = 0.f;
         if (j < H) wp[c].load(a.w, 0, j, H);
     }
-    if (int64_t(blockIdx.x) < a.T) load(blockIdx.x);
+    const int64_t t0 = int64_t(blockIdx.x) * GROUPS + (BLOCK ? 0 : tid / G), step = int64_t(gridDim.x) * GROUPS;
+    if (t0 < a.T) load(t0);
     int p = 0;
-    for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x, p ^= 1) {
+    for (int64_t t = t0; t < a.T; t += step, p ^= 1) {
         const Row row = next;
-        if (t + gridDim.x < a.T) load(t + gridDim.x);
+        if (t + step < a.T) load(t + step);
         float h[C][8], g[C][8], sum = 0.f, dot = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            if ((tid + c * TH) * 8 >= H) continue;
+            if ((li + c * G) * 8 >= H) continue;
             float w[8];
             row.h[c].values(h[c]);
             row.d[c].values(g[c]);
@@ -300,25 +311,27 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
             }
         }
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) {
+        for (int o = (BLOCK ? WAVE : G) / 2; o >= 1; o >>= 1) {
             sum += __shfl_xor(sum, o);
             dot += __shfl_xor(dot, o);
         }
-        if (tid % WAVE == 0) {
-            s_sum[p][0][tid / WAVE] = sum;
-            s_sum[p][1][tid / WAVE] = dot;
-        }
-        __syncthreads();  // (one per row: the next row's sums go to the other pair of lists)
-        sum = dot = 0.f;
+        if constexpr (BLOCK) {
+            if (tid % WAVE == 0) {
+                s_sum[p][0][tid / WAVE] = sum;
+                s_sum[p][1][tid / WAVE] = dot;
+            }
+            __syncthreads();  // (one per row: the next row's sums go to the other pair of lists)
+            sum = dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            sum += s_sum[p][0][i];
-            dot += s_sum[p][1][i];
+            for (int i = 0; i < NW; ++i) {
+                sum += s_sum[p][0][i];
+                dot += s_sum[p][1][i];
+            }
         }
         const float r = 1.f / sqrtf(sum / float(H) + a.eps), k = r * r * (dot / float(H));
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int j = (tid + c * TH) * 8;
+            const int j = (li + c * G) * 8;
             if (j >= H) continue;
             float o[8], w[8];
             wp[c].values(w);
@@ -337,12 +350,32 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
         }
     }
     if (!a.dw) return;
+    float *part = a.part + int64_t(blockIdx.x) * H;
+    if constexpr (BLOCK) {
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int j = (tid + c * TH) * 8;
+        for (int c = 0; c < C; ++c) {
+            const int j = (li + c * G) * 8;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (j + e < H) a.part[int64_t(blockIdx.x) * H + j + e] = dw[c][e];
+            for (int e = 0; e < 8; ++e)
+                if (j + e < H) part[j + e] = dw[c][e];
+        }
+    } else {
+        __shared__ float s_dw[NW][C * G * 8];
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+#pragma unroll
+                for (int o = G; o < WAVE; o <<= 1) dw[c][e] += __shfl_xor(dw[c][e], o);
+                if (tid % WAVE < G) s_dw[tid / WAVE][(li + c * G) * 8 + e] = dw[c][e];
+            }
+        __syncthreads();
+        for (int j = tid; j < H; j += TH) {
+            float sum = s_dw[0][j];
+#pragma unroll
+            for (int i = 1; i < NW; ++i) sum += s_dw[i][j];
+            part[j] = sum;
+        }
     }
 }
 
@@ -368,25 +401,35 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float *__restri
     }
 }
 
-// Blocks of the gradients' launch: as many parts of dw are written and read.
-static int norm_grad_blocks(int T) { return std::min(T, 512); }
+// Blocks of the gradients' launch, of T groups: as many parts of dw are written
+// and read (rows of 8192 in 512 parts 37 us for 29, of 16384 52 for 37).
+static int norm_grad_blocks(int T, int H) { return std::min(T, H > 4096 ? 256 : 512); }
 
-size_t rms_norm_backward_workspace_bytes(int T, int H) { return size_t(norm_grad_blocks(T)) * size_t(H) * 4; }
+size_t rms_norm_backward_workspace_bytes(int T, int H) { return size_t(norm_grad_blocks(T, H)) * size_t(H) * 4; }
 
 template <int DT, int HT, int WT>
 static void launch_norm_grad(const NormGradArgs &a, hipStream_t s) {
-    const int blocks = norm_grad_blocks(a.T);
-    auto run = [&](auto vec, auto th, auto c) {
-        constexpr int TH = decltype(th)::value;
-        rms_norm_backward_kernel<DT, HT, WT, decltype(vec)::value, TH, decltype(c)::value>
+    int blocks = 0;
+    auto run = [&](auto vec, auto g, auto th, auto c) {
+        constexpr int G = decltype(g)::value, TH = decltype(th)::value;
+        blocks = norm_grad_blocks((a.T + TH / G - 1) / (TH / G), a.H);
+        rms_norm_backward_kernel<DT, HT, WT, decltype(vec)::value, G, TH, decltype(c)::value>
             <<<unsigned(blocks), TH, 0, s>>>(a);
     };
+    // Short rows by parts of a wave: no barrier, and every thread has work (16.8 million elements in bf16, a block or a
+    // wave a row, and as here: rows of 64 545 us and 46, of 256 140 and 24, of 1024 49 and 23).
     auto by_length = [&](auto vec) {
-        if (a.H <= 512) run(vec, Int<64>{}, Int<1>{});
-        else if (a.H <= 2048) run(vec, Int<256>{}, Int<1>{});
-        else if (a.H <= 4096) run(vec, Int<256>{}, Int<2>{});
-        else if (a.H <= 8192) run(vec, Int<1024>{}, Int<1>{});
-        else run(vec, Int<1024>{}, Int<2>{});
+        if (a.H <= 128) run(vec, Int<16>{}, Int<256>{}, Int<1>{});
+        else if (a.H <= 256) run(vec, Int<16>{}, Int<256>{}, Int<2>{});
+        else if (a.H <= 512) run(vec, Int<64>{}, Int<256>{}, Int<1>{});
+        else if (a.H <= 1024) run(vec, Int<64>{}, Int<256>{}, Int<2>{});
+        else if (a.H <= 2048) {
+            // (rows of 2048 of 16 bits 29 us in blocks, 24 in waves; fp32 and single elements would spill)
+            if constexpr (HT != 0 && decltype(vec)::value) run(vec, Int<64>{}, Int<256>{}, Int<4>{});
+            else run(vec, Int<256>{}, Int<256>{}, Int<1>{});
+        } else if (a.H <= 4096) run(vec, Int<256>{}, Int<256>{}, Int<2>{});
+        else if (a.H <= 8192) run(vec, Int<512>{}, Int<512>{}, Int<2>{});
+        else run(vec, Int<1024>{}, Int<1024>{}, Int<2>{});
     };
     const int64_t one = a.T == 1 ? 0 : 1;  // (a single row's stride does not matter)
     if (a.H % 8 == 0 && rows_aligned(a.dy, DT, one * a.lddy, 8) && rows_aligned(a.h, HT, one * a.ldh, 8) &&
