@@ -202,3 +202,24 @@ def test_fp16_gradient_overflows(gpu):
     v = torch.zeros(T, R, device=gpu)
     dx, dA, _ = qwq4.lora_backward(dy, x, A * 100, B * 100, ids, v, dx=torch.zeros_like(x))
     assert torch.isinf(dx[1]).any() and (dx[0] == 0).all() and torch.isfinite(dA).all()
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("R", [16, 40, 64, 128])
+def test_rows_do_not_depend_on_a_long_batch(gpu, t, R):
+    """Long batches share weights among waves, several tiles to a block; short ones do not: the same bits, forward and
+    back, in any order of the tokens."""
+    T, K, N, L = 2100, 520, 1032, 2
+    x, A, B, ids, scaling, g = make(R, T, K, N, R, L, t, gpu)
+    dy, dx = (torch.randn(T, n, generator=g).to(x.dtype).to(gpu) for n in (N, K))
+    for y in ("f32", t):
+        ys = torch.randn(T, N, generator=g).to(TYPES[y]).to(gpu)
+        v = torch.zeros(T, R, device=gpu)
+        whole = qwq4.lora(x, A, B, ids, ys, scaling=scaling, out=torch.empty_like(ys), v=v)
+        back = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling, dx=dx, dx_out=torch.empty_like(dx), need_weights=False)[0]
+        for at in ([5], list(range(60, 97)), list(range(400, 527)), torch.randperm(T, generator=g).tolist()):
+            i = torch.tensor(at, device=gpu)
+            w = torch.zeros(len(at), R, device=gpu)
+            assert torch.equal(qwq4.lora(x[i], A, B, ids[i], ys[i], scaling=scaling, v=w), whole[i])
+            assert torch.equal(w, v[i])
+            assert torch.equal(qwq4.lora_backward(dy[i], x[i], A, B, ids[i], w, scaling=scaling, dx=dx[i])[0], back[i])

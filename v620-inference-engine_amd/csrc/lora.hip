@@ -270,9 +270,9 @@ void launch_lora_shrink(const LoraShrinkArgs &a, hipStream_t s) {
 
 // out[l] = the parts of adapter l that have tokens, in order (none: zeros).
 __device__ __forceinline__ void join_parts(const LoraJoinArgs &a, int block) {
-    const int blocks = a.blocks(int(blockDim.x)), l = block / blocks;
+    const int blocks = a.blocks(), l = block / blocks;
     if (l >= a.L) return;
-    const int64_t i = (int64_t(block % blocks) * int(blockDim.x) + int(threadIdx.x)) * 4;
+    const int64_t i = (int64_t(block % blocks) * 256 + int(threadIdx.x)) * 4;
     const bool second = i >= a.n[0];
     float *out = a.out[second];
     const int64_t at = second ? i - a.n[0] : i, each = a.n[second];
@@ -301,22 +301,23 @@ __device__ __forceinline__ void join_parts(const LoraJoinArgs &a, int block) {
 }
 
 // ------------------------------------------------------------ expand
-// out[t][n] = y[t][n] + scaling[id_t] sum_r B[id_t][n][r] v[t][r]: 16 NT tokens by
-// 128 columns a wave, 16 tokens at a time (NT = a.tiles, at most 4). The columns
-// are dealt to 8 MFMAs so that a lane holds 8 neighbouring ones of four tokens
-// and 16 lanes a row's 128: rows are read and written in 256-byte runs (four lanes
-// to a token's 64 columns: 47 us where this takes 43, 4096 x 12288 in bf16), past
-// the caches (kept in them: 5 us more). K of the MFMA runs over the R values of
-// each of v's parts in turn. fp16 parts are of v times a power of two per token,
-// so that none of them overflows or loses bits to the range. Bound by memory.
-// ONE: one step of the MFMA covers all parts, and its weights stay in registers.
-// Else they lie in LDS, a wave's 128 rows of B as one run of memory (read for
-// every tile in the MFMA's order, they touch a line per lane: a call of rank 64, 4096
-// x 12288, 172 us where this takes 102); 16-byte piece p of them at place p ^ (row / 8 & 7):
-// without bank conflicts. COLUMNS: the columns lie inside, B is [R][N]: a lane reads
-// its 8 columns of 8 ranks and turns them in registers; and the blocks behind the
-// expanding ones join the parts of the weights' gradients (as much work as in a
-// launch of its own, but without that launch's 3 us or so).
+// out[t][n] = y[t][n] + scaling[id_t] sum_r B[id_t][n][r] v[t][r]: 16 tokens by 128
+// columns a wave at a time. The columns are dealt to 8 MFMAs so that a lane holds 8
+// neighbouring ones of four tokens and 16 lanes a row's 128: rows are read and
+// written in 256-byte runs (four lanes to a token's 64 columns: 47 us where this
+// takes 43, 4096 x 12288 in bf16), past the caches (kept in them: 5 us more). K of the
+// MFMA runs over the R values of each of v's parts in turn. fp16 parts are of v
+// times a power of two per token, so that none of them overflows or loses bits to the
+// range. Bound by memory.
+// ONE: one step of the MFMA covers all parts; its weights stay in registers, and a
+// wave takes NT = a.tiles (at most 4) tiles of 16 tokens one after the other.
+// Else the rows of B lie in LDS, 16-byte piece p of a row at place p ^ (row / 8 & 7):
+// without bank conflicts. The block's four waves take a tile each of the same 128
+// columns (NT = 4), or 128 columns each of one tile (NT = 1).
+// COLUMNS: the columns lie inside, B is [R][N]: a lane reads its 8 columns of 8 ranks
+// and turns them in registers; and the blocks behind the expanding ones join the
+// parts of the weights' gradients (as much work as in a launch of its own, but
+// without that launch's 3 us or so).
 template <class T16, int YT, bool ONE, bool COLUMNS>
 __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a, LoraJoinArgs join) {
     constexpr bool HALF = __is_same(T16, F16);
@@ -327,19 +328,20 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a, Lora
             return;
         }
     }
-    extern __shared__ uint4 s_weights[];  // ONE: none; [waves][128 R / 8]
+    extern __shared__ uint4 s_weights[];  // ONE: none; [columns R / 8]
     const int lane = int(threadIdx.x) % WAVE, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / WAVE);
     const int c = lane % 16, g = lane / 16;
     const int NT = a.tiles, t0 = int(blockIdx.y) * (16 * NT);
-    const int n0 = (int(blockIdx.x) * (int(blockDim.x) / WAVE) + wave) * 128;
-    if (n0 >= a.N) return;  // (no barrier below)
+    const bool share = !ONE && NT == 4;
+    const int n0 = (share ? int(blockIdx.x) : int(blockIdx.x) * 4 + wave) * 128;
+    if (ONE && n0 >= a.N) return;  // (no barrier below)
     const int at = n0 + 8 * c;    // the lane's columns
     const bool in = at < a.N;     // (N is a multiple of 8)
     const int id = lane < 16 * NT ? adapter_of(a.ids, t0 + lane, a.T, a.L) : -1;
     const int octets = a.R / 8, steps = ONE ? 1 : (PARTS * octets + 3) / 4;
     if (a.out != a.y && blockIdx.z == 0) {  // (rows without an adapter)
         const unsigned long long none = ~__ballot(id >= 0);
-        for (int i = 0; i < 16 * NT; i += 4) {
+        for (int i = share ? 4 * wave : 0; i < 16 * NT; i += share ? 16 : 4) {
             const int t = t0 + i + g;
             if (t < a.T && in && ((none >> (i + g)) & 1)) {
                 RowPiece<YT> y;
@@ -348,7 +350,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a, Lora
             }
         }
     }
-    uint4 *lds = s_weights + wave * 128 * octets;
+    uint4 *lds = s_weights + (share ? 0 : wave * 128 * octets);
     each_adapter(id, int(blockIdx.z), a.side, [&](int l, unsigned long long mine) {
         const float scale = a.scaling ? a.scaling[l] : 1.f;
         // the wave's rows, min(128, N - n0) of them, or its columns
@@ -370,7 +372,7 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a, Lora
                 if (in && ((here >> e) & 1)) y[e].load_stream(a.y, row + e * a.ldy);
         };
         RowPiece<YT> next[4];
-        rows(0, next);
+        rows(share ? wave : 0, next);
         // place o of v's parts and what it is: octet ro of part p (none from PARTS on)
         auto place = [&](int q, int &p) {
             const int o = 4 * q + g;
@@ -388,30 +390,23 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a, Lora
                 for (int j = 0; j < 8; ++j) wf[j] = *reinterpret_cast<const uint4 *>(w + j * a.R);
             }
         } else if constexpr (COLUMNS) {
-            Turned::wave_lds_order();
-            for (int o = g; o < octets; o += 4) {
+            for (int o = (share ? 4 * wave : 0) + g; o < octets; o += share ? 16 : 4) {
                 octet(o, wf);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) lds[((8 * c + j) * octets + o) ^ (c & 7)] = wf[j];
             }
-            Turned::wave_lds_order();
+            __syncthreads();
         } else {
             const int n = min(128, a.N - n0) * octets;
             const uint32_t inverse = (65536u + uint32_t(octets) - 1) / uint32_t(octets);  // (exact below 4096)
-            Turned::wave_lds_order();
 #pragma unroll 4
-            for (int i = lane; i < n; i += WAVE)
+            for (int i = share ? int(threadIdx.x) : lane; i < n; i += share ? 4 * WAVE : WAVE)
                 lds[i ^ int(((uint32_t(i) * inverse >> 16) >> 3) & 7)] = reinterpret_cast<const uint4 *>(B)[i];
-            Turned::wave_lds_order();
+            __syncthreads();
         }
-#pragma unroll 1
-        for (int i = 0; i < NT; ++i) {
-            RowPiece<YT> y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = next[e];
-            rows(i + 1, next);
+        auto tile = [&](int i, const RowPiece<YT> (&y)[4]) {
             const uint32_t here = tokens(i);
-            if (!here) continue;
+            if (!here) return;
             const bool own = (here >> c) & 1;  // (token c's values of v are this lane's operand)
             const float *v = a.v + int64_t(t0 + 16 * i + c) * a.R;
             int shift = 0;
@@ -471,9 +466,23 @@ __global__ __launch_bounds__(256) void lora_expand_kernel(LoraExpandArgs a, Lora
                     if constexpr (HALF) d = __builtin_ldexpf(d, back);
                     f[j] += d;
                 }
-                y[e].template set<YT == GRAD_F16>(f);
-                y[e].store_stream(a.out, row + e * a.ldo);
+                RowPiece<YT> o;
+                o.template set<YT == GRAD_F16>(f);
+                o.store_stream(a.out, row + e * a.ldo);
             }
+        };
+        if constexpr (ONE) {
+#pragma unroll 1
+            for (int i = 0; i < NT; ++i) {
+                RowPiece<YT> y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = next[e];
+                rows(i + 1, next);
+                tile(i, y);
+            }
+        } else {
+            tile(share ? wave : 0, next);
+            __syncthreads();  // (the weights are read)
         }
     });
 }
@@ -483,21 +492,22 @@ void launch_lora_expand(LoraExpandArgs a, const LoraJoinArgs &join, hipStream_t 
         constexpr bool COLUMNS = decltype(columns)::value;
         constexpr int YT = decltype(yt)::value;
         const bool one = (YT == 0 ? 3 : 2) * a.R <= 32;
-        const int waves = !one && a.R > 64 ? 2 : 4;  // (at most 64 KB of weights a block)
-        // Tiles of a block: the weights are read once for all of them, but first of all the chip is to be filled (one
-        // tile for two: 2048 x 4096 of rank 16 19.5 us for 16.8). Two serve small ranks up to the largest calls (four: 4096 x
-        // 4096 of rank 32 34.8 us for 33.2; 16384 x 12288 of rank 16 187 for 191), four the large ranks (two: 4096 x
-        // 12288 of rank 128 235 us for 218). Then the adapters of a block's tokens side by side.
-        const int tiles = (a.T + 15) / 16, cols = (a.N + 128 * waves - 1) / (128 * waves);
-        a.tiles = tiles * cols >= (a.R < 64 ? 16384 : 2048) ? 4 : tiles * cols >= 1024 ? 2 : 1;
+        // ONE: the weights are read once for all tiles of a block, but first of all the chip is to be filled (one tile
+        // for two: 2048 x 4096 of rank 16 19.5 us for 16.8); two serve up to the largest calls (four: 4096 x 12288 of
+        // rank 16 55.4 us for 54.0, 16384 x 12288 187 for 191). Then the adapters of a block's tokens side by side.
+        // Else the waves share the columns' weights (with columns of their own a CU holds a third as many waves: 4096 x
+        // 4096 of rank 128 85 us for 53, 4096 x 12288 of rank 64 90 for 77), but where 64 tokens may be of many adapters
+        // (shared: 64 tokens of 64, 4096 columns of rank 64 22.5 us for 19.8; 1024 mixed ones of 64, rank 32 81 for 56).
+        const bool share = !one && (a.T >= 64 * a.L || a.R > 64);  // (at most 64 KB of weights a block)
+        const int wide = share ? 128 : 512, tiles = (a.T + 15) / 16, cols = (a.N + wide - 1) / wide;
+        a.tiles = share || (one && tiles * cols >= 16384) ? 4 : one && tiles * cols >= 1024 ? 2 : 1;
         const int groups = (tiles + a.tiles - 1) / a.tiles;
         a.side = std::max(1, std::min({1024 / (groups * cols), 16 * a.tiles, a.L, a.T}));
-        const unsigned threads = unsigned(waves * WAVE);
-        const int joining = join.L ? (join.L * join.blocks(int(threads)) + groups * cols - 1) / (groups * cols) : 0;
+        const int joining = join.L ? (join.L * join.blocks() + groups * cols - 1) / (groups * cols) : 0;
         const dim3 grid{unsigned(cols), unsigned(groups), unsigned(a.side + joining)};
-        const size_t lds = one ? 0 : size_t(waves) * 256 * size_t(a.R);
-        if (one) lora_expand_kernel<decltype(t16), YT, true, COLUMNS><<<grid, threads, lds, s>>>(a, join);
-        else lora_expand_kernel<decltype(t16), YT, false, COLUMNS><<<grid, threads, lds, s>>>(a, join);
+        const size_t lds = one ? 0 : size_t(share ? 256 : 1024) * size_t(a.R);
+        if (one) lora_expand_kernel<decltype(t16), YT, true, COLUMNS><<<grid, 256, lds, s>>>(a, join);
+        else lora_expand_kernel<decltype(t16), YT, false, COLUMNS><<<grid, 256, lds, s>>>(a, join);
     };
     auto by_16 = [&](auto yt) {
         if (a.f16) run(F16{}, yt, Int<0>{});
@@ -749,7 +759,7 @@ void launch_lora_backward(const LoraGradArgs &a, void *ws, hipStream_t s) {
         launch_lora_expand(LoraExpandArgs{dv, a.A, a.ids, a.scaling, a.T, a.K, a.R, a.L, a.f16, a.dx, a.lddx, a.dx_out,
                                           a.lddxo, a.f16 ? 2 : 1, true},
                            join, s);
-    else if (join.L) lora_outer_join_kernel<<<unsigned(join.L * join.blocks(256)), 256, 0, s>>>(join);
+    else if (join.L) lora_outer_join_kernel<<<unsigned(join.L * join.blocks()), 256, 0, s>>>(join);
 }
 
 }  // namespace qwq4

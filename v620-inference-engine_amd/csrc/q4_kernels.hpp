@@ -407,8 +407,7 @@ struct LoraJoinArgs {
     int64_t n[2];          // 0: not wanted; multiples of 64
     const int *count;      // [parts][L] tokens: parts of none are not read
     int L, parts;          // L = 0: nothing to join
-    // blocks that an adapter takes
-    __host__ __device__ int blocks(int threads) const { return int((n[0] + n[1] + 4 * threads - 1) / (4 * threads)); }
+    __host__ __device__ int blocks() const { return int((n[0] + n[1] + 1023) / 1024); }  // of 256 threads, an adapter's
 };
 void launch_lora_expand(LoraExpandArgs a, const LoraJoinArgs &join, hipStream_t s);
 // One of the two products over tokens: rows m [T][C], factors u [T][R].
