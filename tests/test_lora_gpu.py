@@ -223,3 +223,23 @@ def test_rows_do_not_depend_on_a_long_batch(gpu, t, R):
             assert torch.equal(qwq4.lora(x[i], A, B, ids[i], ys[i], scaling=scaling, v=w), whole[i])
             assert torch.equal(w, v[i])
             assert torch.equal(qwq4.lora_backward(dy[i], x[i], A, B, ids[i], w, scaling=scaling, dx=dx[i])[0], back[i])
+
+
+def test_offsets_past_32_bits(gpu):
+    """Rows 2^23 elements apart: the last ones lie behind 2^32 elements. The same bits as side by side."""
+    T, K, N, R, L, ld = 530, 64, 72, 16, 2, 1 << 23
+    x, A, B, ids, scaling, g = make(20, T, K, N, R, L, "bf16", gpu)
+    flat = torch.empty(T * ld, dtype=x.dtype, device=gpu)  # (9 GB: every row holds x, y, out, dy, dx and dx_out)
+    far = lambda at, n: flat.as_strided((T, n), (ld, 1), at)  # noqa: E731
+    ys, dy, dx = (torch.randn(T, n, generator=g).to(x.dtype).to(gpu) for n in (N, N, K))
+    views = [far(1024 * i, t.shape[1]) for i, t in enumerate((x, ys, ys, dy, dx, dx))]
+    for view, t in zip(views, (x, ys, ys, dy, dx, dx)):
+        view.copy_(t)
+    fx, fy, fout, fdy, fdx, fdxo = views
+    v, w = torch.zeros(T, R, device=gpu), torch.zeros(T, R, device=gpu)
+    want = qwq4.lora(x, A, B, ids, ys, scaling=scaling, out=torch.empty_like(ys), v=v)
+    qwq4.lora(fx, A, B, ids, fy, scaling=scaling, out=fout, v=w)
+    assert torch.equal(fout, want) and torch.equal(v, w)
+    want = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling, dx=dx, dx_out=torch.empty_like(dx))
+    got = qwq4.lora_backward(fdy, fx, A, B, ids, w, scaling=scaling, dx=fdx, dx_out=fdxo)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
