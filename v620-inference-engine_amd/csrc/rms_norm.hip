@@ -269,7 +269,7 @@ struct Part<TY, false> {
 };
 
 // A row by G of the block's TH threads (16, 64: groups of a wave, which meet no
-// barrier but the last; TH: the block), 8 elements per thread and C turns each. A
+// barrier but the last; more: of waves), 8 elements per thread and C turns each. A
 // group takes every (groups of the grid)-th row, with the next one on its way
 // while the current one's sums are made, and keeps its columns' part of dw in
 // registers; the block adds its groups' parts and a second launch the blocks', in
@@ -277,9 +277,10 @@ struct Part<TY, false> {
 template <int DT, int HT, int WT, bool VEC, int G, int TH, int C>
 __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
     constexpr int NW = TH / WAVE, GROUPS = TH / G;
-    constexpr bool BLOCK = G == TH;
+    constexpr bool BLOCK = G > WAVE;  // (groups of waves: all of a block's take their rows together)
     __shared__ float s_sum[2][2][NW];
-    const int tid = int(threadIdx.x), li = BLOCK ? tid : tid % G, H = a.H;
+    const int tid = int(threadIdx.x), H = a.H;
+    const int group = GROUPS == 1 ? 0 : BLOCK ? __builtin_amdgcn_readfirstlane(tid / G) : tid / G, li = tid - group * G;
     struct Row {
         Part<HT, VEC> h[C], res[C];
         Part<DT, VEC> d[C];
@@ -303,10 +304,11 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
         for (int e = 0; e < 8; ++e) dw[c][e] = 0.f;
         if (j < H) wp[c].load(a.w, 0, j, H);
     }
-    const int64_t t0 = int64_t(blockIdx.x) * GROUPS + (BLOCK ? 0 : tid / G), step = int64_t(gridDim.x) * GROUPS;
+    const int64_t t0 = int64_t(blockIdx.x) * GROUPS + group, step = int64_t(gridDim.x) * GROUPS;
     if (t0 < a.T) load(t0);
     int p = 0;
-    for (int64_t t = t0; t < a.T; t += step, p ^= 1) {
+    for (int64_t t = t0; t - (BLOCK ? group : 0) < a.T; t += step, p ^= 1) {
+        const bool live = !BLOCK || GROUPS == 1 || t < a.T;
         const Row row = next;
         if (t + step < a.T) load(t + step);
         float h[C][8], g[C][8], sum = 0.f, dot = 0.f;
@@ -336,16 +338,16 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
             __syncthreads();  // (one per row: the next row's sums go to the other pair of lists)
             sum = dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < NW; ++i) {
-                sum += s_sum[p][0][i];
-                dot += s_sum[p][1][i];
+            for (int i = 0; i < G / WAVE; ++i) {
+                sum += s_sum[p][0][group * (G / WAVE) + i];
+                dot += s_sum[p][1][group * (G / WAVE) + i];
             }
         }
         const float r = 1.f / sqrtf(sum / float(H) + a.eps), k = r * r * (dot / float(H));
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int j = (li + c * G) * 8;
-            if (j >= H) continue;
+            if (j >= H || !live) continue;
             float o[8], w[8];
             wp[c].values(w);
 #pragma unroll
@@ -364,7 +366,7 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
     }
     if (!a.dw) return;
     float *part = a.part + int64_t(blockIdx.x) * H;
-    if constexpr (BLOCK) {
+    if constexpr (G == TH) {
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             const int j = (li + c * G) * 8;
@@ -373,20 +375,21 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
                 if (j + e < H) part[j + e] = dw[c][e];
         }
     } else {
-        __shared__ float s_dw[NW][C * G * 8];
+        constexpr int SETS = BLOCK ? GROUPS : NW;  // (a wave's groups first)
+        __shared__ float s_dw[SETS][C * G * 8];
 #pragma unroll
         for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
 #pragma unroll
                 for (int o = G; o < WAVE; o <<= 1) dw[c][e] += __shfl_xor(dw[c][e], o);
-                if (tid % WAVE < G) s_dw[tid / WAVE][(li + c * G) * 8 + e] = dw[c][e];
+                if (BLOCK || tid % WAVE < G) s_dw[tid / (BLOCK ? G : WAVE)][(li + c * G) * 8 + e] = dw[c][e];
             }
         __syncthreads();
         for (int j = tid; j < H; j += TH) {
             float sum = s_dw[0][j];
 #pragma unroll
-            for (int i = 1; i < NW; ++i) sum += s_dw[i][j];
+            for (int i = 1; i < SETS; ++i) sum += s_dw[i][j];
             part[j] = sum;
         }
     }
@@ -415,8 +418,9 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float *__restri
 }
 
 // Blocks of the gradients' launch, of T groups: as many parts of dw are written
-// and read (rows of 8192 in 512 parts 37 us for 29, of 16384 52 for 37).
-static int norm_grad_blocks(int T, int H) { return std::min(T, H > 4096 ? 256 : 512); }
+// and read (4096 rows of 4096 in 512 parts 32.5 us for 29.6, 1024 of 16384 52 for
+// 37). Two blocks a CU only where waves take rows of up to 2048, 32 KB of LDS a block.
+static int norm_grad_blocks(int T, int H) { return std::min(T, H <= 1024 || H > 2048 ? 256 : 512); }
 
 size_t rms_norm_backward_workspace_bytes(int T, int H) { return size_t(norm_grad_blocks(T, H)) * size_t(H) * 4; }
 
@@ -430,20 +434,24 @@ static void launch_norm_grad(const NormGradArgs &a, hipStream_t s) {
             <<<unsigned(blocks), TH, 0, s>>>(a);
     };
     // Short rows by parts of a wave: no barrier, and every thread has work (16.8 million elements in bf16, a block or a
-    // wave a row, and as here: rows of 64 545 us and 46, of 256 140 and 24, of 1024 49 and 23).
+    // wave a row, and as here: rows of 64 545 us and 42, of 256 140 and 22, of 1024 49 and 22). Rows of 16 bits by as few
+    // waves as registers allow: of 2048 29 us in blocks, 24 in waves; of 2560 32 and 26; of 16384 37 and 34. (fp32, and rows
+    // that start anywhere, which wait as fp32, would spill.)
     auto by_length = [&](auto vec) {
-        if (a.H <= 128) run(vec, Int<16>{}, Int<256>{}, Int<1>{});
-        else if (a.H <= 256) run(vec, Int<16>{}, Int<256>{}, Int<2>{});
-        else if (a.H <= 512) run(vec, Int<64>{}, Int<256>{}, Int<1>{});
-        else if (a.H <= 1024) run(vec, Int<64>{}, Int<256>{}, Int<2>{});
-        else if (a.H <= 2048) {
-            // (rows of 2048 of 16 bits 29 us in blocks, 24 in waves; fp32 would spill)
-            if constexpr (HT != 0 && decltype(vec)::value) run(vec, Int<64>{}, Int<256>{}, Int<4>{});
-            else run(vec, Int<256>{}, Int<256>{}, Int<1>{});
-        } else if (a.H <= 4096) run(vec, Int<256>{}, Int<256>{}, Int<2>{});
-        else if (a.H <= 8192) run(vec, Int<512>{}, Int<512>{}, Int<2>{});
-        else if constexpr (HT != 0 && decltype(vec)::value) run(vec, Int<512>{}, Int<512>{}, Int<4>{});  // (16384: 37 and 34)
-        else run(vec, Int<1024>{}, Int<1024>{}, Int<2>{});
+        constexpr bool HALF = HT != 0 && decltype(vec)::value;
+        if (a.H <= 128) return run(vec, Int<16>{}, Int<512>{}, Int<1>{});
+        if (a.H <= 256) return run(vec, Int<16>{}, Int<512>{}, Int<2>{});
+        if (a.H <= 512) return run(vec, Int<64>{}, Int<512>{}, Int<1>{});
+        if (a.H <= 1024) return run(vec, Int<64>{}, Int<512>{}, Int<2>{});
+        if constexpr (HALF) {
+            if (a.H <= 2048) return run(vec, Int<64>{}, Int<256>{}, Int<4>{});
+            if (a.H <= 128 * 24) return run(vec, Int<128>{}, Int<512>{}, Int<3>{});
+        }
+        if (a.H <= 2048) return run(vec, Int<128>{}, Int<512>{}, Int<2>{});
+        if (a.H <= 4096) return run(vec, Int<256>{}, Int<512>{}, Int<2>{});
+        if (a.H <= 8192) return run(vec, Int<512>{}, Int<512>{}, Int<2>{});
+        if constexpr (HALF) return run(vec, Int<512>{}, Int<512>{}, Int<4>{});
+        else return run(vec, Int<1024>{}, Int<1024>{}, Int<2>{});
     };
     const int64_t one = a.T == 1 ? 0 : 1;  // (a single row's stride does not matter)
     if (a.H % 8 == 0 && rows_aligned(a.dy, DT, one * a.lddy, 8) && rows_aligned(a.h, HT, one * a.ldh, 8) &&
