@@ -144,11 +144,6 @@ struct RowPiece {
             w[0] = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
         }
     }
-    __device__ __forceinline__ void store(void *p, int64_t i) const {
-        char *at = static_cast<char *>(p) + i * (YT == 0 ? 4 : 2);
-        reinterpret_cast<uint4 *>(at)[0] = w[0];
-        if constexpr (YT == 0) reinterpret_cast<uint4 *>(at)[1] = w[1];
-    }
     __device__ __forceinline__ void values(float (&v)[8]) const {
         if constexpr (YT == 0) {
             const f32x4 a = __builtin_bit_cast(f32x4, w[0]), b = __builtin_bit_cast(f32x4, w[1]);
