@@ -515,6 +515,8 @@ int qw_lora_backward(const void *dy, int lddy, const void *x, int ldx, int f16, 
  * element) say of tokens int32 [T], all fp32 [T]:
  *   lse = log sum_j exp(l_j),  logp = l[token] - lse (0 for a token outside 0 .. V - 1),
  *   entropy = -sum_j p_j log p_j
+ * (log probabilities are taken from the differences to the row's largest logit, before lse
+ * is rounded: a row of -1e9 throughout has logp = -log V)
  * and, with top > 0, the top (at most 64 and V) largest logits' indices
  * top_ids int32 [T][top] and log probabilities top_logp fp32 [T][top], largest
  * first, ties by the lowest index. A logit of -infinity is masked: it has p = 0

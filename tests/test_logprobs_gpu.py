@@ -200,3 +200,54 @@ def test_very_long_rows(gpu, kind, top):
     """Several steps to each largest value that is kept."""
     logits, tokens, _ = make(top, 1, 17_500_001, "f32", gpu, kind=kind)
     check(logits, tokens, top, qwq4.logprobs(logits, tokens, top=top))
+
+
+# ------------------------------------------- logits far from zero
+def apart(logits, tokens, top):
+    """(logp, entropy, top logp) in 64 bits with bounds that know the logits' differences only: every sum's relative error
+    (as in the other cases' bounds), and roundings of l - m, of log S and of their difference. No bound grows with lse."""
+    l, tok = f64(logits), tokens.cpu().long()
+    V = l.shape[1]
+    d = l - l.amax(-1, keepdim=True)
+    e = torch.exp(d)
+    s = e.sum(-1)
+    d0 = torch.where(e > 0, d, 0.0)
+    mean1 = (e * d0.abs()).sum(-1) / s
+    log_s = torch.log(s)
+    off = 2 * ref.U * (V / 64 + 80 + 3 * mean1) + 4 * ref.U * log_s.abs()
+
+    def at(i):
+        dv = d.gather(1, i)
+        return dv - log_s[:, None], off[:, None] + 2 * ref.U * dv.abs() + 2 * ref.U * (dv - log_s[:, None]).abs()
+
+    asked = (tok >= 0) & (tok < V)
+    lp, b = at(tok.clamp(0, V - 1)[:, None])
+    logp = torch.where(asked, lp[:, 0], 0.0), torch.where(asked, b[:, 0], 0.0)
+    order = torch.sort(-l, dim=1, stable=True).indices[:, :top]
+    return logp, at(order), order
+
+
+SHIFTS = [(1e3, "f32"), (1e5, "f32"), (-3e6, "f32"), (-1e3, "bf16"), (3e4, "f16"), (4096.0, "same"), (-1e9, "same"),
+          (torch.finfo(torch.float32).min, "same")]
+
+
+def shifted(seed, T, V, shift, t, gpu, pad=0, off=0):
+    logits, tokens, g = make(seed, T, V, "f32" if t == "same" else t, gpu, pad, off)
+    if t == "same":
+        logits[:] = shift
+    else:
+        logits.copy_(logits.float() + shift)
+    return logits, tokens, g
+
+
+@pytest.mark.parametrize("shift,t", SHIFTS)
+@pytest.mark.parametrize("T,V", [(1, 1000), (3, 151936), (2100, 300)])
+def test_shifted_rows(gpu, T, V, shift, t):
+    """Rows far from zero, constant finite ones among them (logp is -log V there): as exact as rows next to it."""
+    print(f"logprobs shifted by {shift} T={T} V={V} {t}", flush=True)
+    logits, tokens, _ = shifted(T, T, V, shift, t, gpu)
+    got = qwq4.logprobs(logits, tokens, top=7)
+    (logp, blp), (tops, btop), order = apart(logits, tokens, 7)
+    assert torch.equal(got[3].cpu().long(), order)
+    assert_close(got[0], logp, blp, "logp")
+    assert_close(got[4], tops, btop, "top")

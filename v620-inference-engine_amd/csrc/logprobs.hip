@@ -6,8 +6,8 @@
 //
 // One pass over the row: each lane keeps the largest value m so far,
 // S = sum exp(l - m) and U = sum exp(l - m) (l - m), rescaled when m grows;
-// then lse = m + log S and H = log S - U / S. A masked logit (-infinity) adds
-// nothing to either sum. A row that masks everything has lse and logp of
+// then lse = m + log S, logp = (l_tok - m) - log S and H = log S - U / S. A masked logit
+// (-infinity) adds nothing to either sum. A row that masks everything has lse and logp of
 // -infinity and entropy 0; one with a NaN or +infinity gives NaN.
 #include <algorithm>
 #include <climits>
@@ -179,24 +179,30 @@ __device__ __forceinline__ float logit_at(const void *row, int64_t j) {
     return v[0];
 }
 
+// The log probability of value v is (v - m) - log S: both differences are small and
+// exact to their own last bit, where lse = m + log S is rounded to a step of m (a row
+// whose values are all -1e9 would have lost log S).
+struct RowLog {
+    float m, log_s;  // -infinity both: nothing but masked values; log_s NaN: a NaN or +infinity among the values
+    __device__ __forceinline__ float of(float v) const { return log_s == neg_inf() ? log_s : (v - m) - log_s; }
+};
+
 // What a row's sums say, by one thread.
 template <int TY>
-__device__ __forceinline__ float finish_row(const LogprobArgs &a, int64_t t, const void *row, SoftStats st) {
+__device__ __forceinline__ RowLog finish_row(const LogprobArgs &a, int64_t t, const void *row, SoftStats st) {
     const bool none = st.m == neg_inf() && st.s == 0.f;  // (nothing but masked values)
-    const float log_s = logf(st.s), lse = none ? neg_inf() : st.m + log_s;
+    const RowLog r{st.m, logf(st.s)};
     const int tok = a.tokens[t];
-    float lp = 0.f;
-    if (tok >= 0 && tok < a.V) lp = none ? neg_inf() : logit_at<TY>(row, tok) - lse;
-    a.logp[t] = lp;
-    a.entropy[t] = none ? 0.f : log_s - st.u / st.s;
-    a.lse[t] = lse;
-    return lse;
+    a.logp[t] = tok >= 0 && tok < a.V ? r.of(logit_at<TY>(row, tok)) : 0.f;
+    a.entropy[t] = none ? 0.f : r.log_s - st.u / st.s;
+    a.lse[t] = none ? neg_inf() : r.m + r.log_s;
+    return r;
 }
 
-__device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t t, int rank, TopKey key, float lse) {
-    const bool bad = lse != lse;
+__device__ __forceinline__ void put_top(const LogprobArgs &a, int64_t t, int rank, TopKey key, RowLog r) {
+    const bool bad = r.log_s != r.log_s;
     a.top_i[t * a.top + rank] = bad ? -1 : key_index(key);
-    a.top_v[t * a.top + rank] = bad ? lse : lse == neg_inf() ? lse : key_value(key) - lse;
+    a.top_v[t * a.top + rank] = bad ? r.log_s : r.of(key_value(key));
 }
 
 // put(rank, key) for the first k of n keys in LDS, none alike (0 for the places
@@ -234,7 +240,8 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
     extern __shared__ float s_max[];  // TOP: [slots][256]
     __shared__ int s_n, s_again;
     __shared__ uint16_t s_slots[TOP ? TOP_LIST : 1];
-    __shared__ float s_st[4][3], s_bound, s_lse;
+    __shared__ float s_st[4][3], s_bound;
+    __shared__ RowLog s_log;
     __shared__ __align__(16) float s_lane[TOP ? 256 : 1];
     __shared__ TopKey s_keys[TOP ? TOP_LIST : 1];
     const int tid = int(threadIdx.x), lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
@@ -316,7 +323,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
         for (int w = 1; w < 4; ++w) st.join(SoftStats{s_st[w][0], s_st[w][1], s_st[w][2]});
         if (tid == (TOP ? 3 * WAVE : 0)) {
             if (a.splits == 1) {
-                s_lse = finish_row<TY>(a, t, row, st);
+                s_log = finish_row<TY>(a, t, row, st);
             } else {
                 float *p = a.part_st + 3 * (t * a.splits + split);
                 p[0] = st.m;
@@ -417,10 +424,10 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobArgs a) {
         __syncthreads();
         n = s_n;
     }
-    const float lse = a.splits == 1 ? s_lse : 0.f;
+    const RowLog log = a.splits == 1 ? s_log : RowLog{0.f, 0.f};
     const int64_t part = t * a.splits + split;
     rank_keys(s_keys, n, a.top, [&](int rank, TopKey key) {
-        if (a.splits == 1) put_top(a, t, rank, key, lse);
+        if (a.splits == 1) put_top(a, t, rank, key, log);
         else a.part_key[part * a.top + rank] = key;
     });
 }
@@ -434,7 +441,7 @@ template <int TY>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
     __shared__ TopKey s_last, s_keys[MAX_SPLITS * WAVE];
     __shared__ int s_n;
-    __shared__ float s_lse;
+    __shared__ RowLog s_log;
     const int tid = int(threadIdx.x), n = a.splits * a.top;
     const int64_t t = blockIdx.x;
     const TopKey *parts = a.part_key + t * n;
@@ -462,7 +469,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
         }
         st = wave_join(st);
         constexpr int Z = TY == 0 ? 4 : 2;
-        if (lane == 0) s_lse = finish_row<TY>(a, t, static_cast<const char *>(a.logits) + t * a.ld * Z, st);
+        if (lane == 0) s_log = finish_row<TY>(a, t, static_cast<const char *>(a.logits) + t * a.ld * Z, st);
     }
     if (!a.top) return;
     __syncthreads();
@@ -472,8 +479,8 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LogprobArgs a) {
         if (key >= last) s_keys[atomicAdd(&s_n, 1)] = key;
     }
     __syncthreads();
-    const float lse = s_lse;
-    rank_keys(s_keys, s_n, a.top, [&](int rank, TopKey key) { put_top(a, t, rank, key, lse); });
+    const RowLog log = s_log;
+    rank_keys(s_keys, s_n, a.top, [&](int rank, TopKey key) { put_top(a, t, rank, key, log); });
 }
 
 // A block takes a row, or a part of it while there are too few blocks for the
