@@ -533,7 +533,9 @@ int qw_logprobs(const void *logits, int type, int ld, const int32_t *tokens, int
  *   dl_j = dlogp ([j = token] - p_j) - dentropy p_j (log p_j + entropy)
  * of the logits' type, in dlogits [T][V] of stride ldd (it may be the logits, at
  * the same stride). dlogp, dentropy fp32 [T], either may be NULL (none; entropy is
- * read with dentropy only); a token outside 0 .. V - 1 has no dlogp. Masked logits and rows of
+ * read with dentropy only); a token outside 0 .. V - 1 has no dlogp. Where the rounding of
+ * lse would show in p (|lse| above 64 for fp32 logits, 1024 for 16-bit ones), the row is
+ * read twice and p put right by up to a step of lse. Masked logits and rows of
  * only such get 0; fp16 beyond +-65504 becomes infinite. */
 int qw_logprobs_backward(const void *logits, int type, int ld, const int32_t *tokens, const float *lse,
                          const float *entropy, const float *dlogp, const float *dentropy, int T, int V, void *dlogits,

@@ -251,3 +251,50 @@ def test_shifted_rows(gpu, T, V, shift, t):
     assert torch.equal(got[3].cpu().long(), order)
     assert_close(got[0], logp, blp, "logp")
     assert_close(got[4], tops, btop, "top")
+
+
+@pytest.mark.parametrize("shift,t", SHIFTS)
+@pytest.mark.parametrize("T,V,pad,off", [(1, 1000, 0, 0), (3, 70001, 3, 1), (601, 2048, 0, 0), (2, 20000, 8, 0)])
+def test_backward_of_shifted_rows(gpu, T, V, pad, off, shift, t):
+    """The gradient by the definition, not by a rounded lse: in rows of their own, of another alignment, in place."""
+    print(f"logprobs_backward shifted by {shift} T={T} V={V} {t}", flush=True)
+    logits, tokens, g = shifted(T + V, T, V, shift, t, gpu, pad, off)
+    _, ent, lse, _, _ = qwq4.logprobs(logits, tokens)
+    dlogp, dent = torch.randn(T, generator=g).to(gpu), torch.randn(T, generator=g).to(gpu)
+    l, tok = f64(logits), tokens.cpu().long()
+    d = l - l.amax(-1, keepdim=True)
+    lp = d - torch.log(torch.exp(d).sum(-1, keepdim=True))
+    p, h = torch.exp(lp), -(torch.exp(lp) * lp).sum(-1, keepdim=True)
+    asked = (tok >= 0) & (tok < V)
+    gl, gh = torch.where(asked, f64(dlogp), 0.0)[:, None], f64(dent)[:, None]
+    want = -p * (gl + gh * (lp + h))
+    want.scatter_add_(1, tok.clamp(0, V - 1)[:, None], gl)
+    # p: its argument's roundings, and the row's sum, whose relative error shows in it; where the sum is not made anew
+    # (lse up to 64 for fp32 rows, 1024 for 16-bit ones), half a step of lse. The entropy is the forward's.
+    mean1 = (p * (d - 0).abs()).sum(-1, keepdim=True)
+    off_lp = 2 * ref.U * (V / 64 + 80 + 3 * mean1) + ref.U * (16 + 4 * lp.abs()) + (2.0**-19 if t in ("f32", "same") else 2.0**-15)
+    off_h = (ref.logprobs(logits, tokens)[1][1])[:, None]
+    size = gl.abs() + gh.abs() * (lp.abs() + h.abs())
+    bound = p * (size * off_lp + gh.abs() * (off_lp + off_h)) + 2 * ref.U * want.abs()
+    other = torch.empty(T, V + 1, dtype=logits.dtype, device=gpu)[:, :V]
+    for out in (None, other):
+        assert_close(qwq4.logprobs_backward(logits, tokens, lse, ent, dlogp, dent, dlogits=out), want, bound)
+    assert_close(qwq4.logprobs_backward(logits, tokens, lse, ent, dlogp, dent, dlogits=logits), want, bound, "in place")
+
+
+@pytest.mark.parametrize("shift", [0.0, 100.0, -3e4])
+def test_backward_of_a_shard(gpu, shift):
+    """A shard of the vocabulary with the lse and the entropy of the whole row: the probabilities are the whole row's."""
+    T, V, own = 5, 4000, 1000
+    logits, tokens, g = shifted(3, T, V, shift, "f32", gpu)
+    _, ent, lse, _, _ = qwq4.logprobs(logits, tokens)
+    dlogp, dent = torch.randn(T, generator=g).to(gpu), torch.randn(T, generator=g).to(gpu)
+    for r in range(V // own):
+        part, tok = logits[:, r * own:(r + 1) * own], tokens - r * own
+        d = qwq4.logprobs_backward(part, tok, lse, ent, dlogp, dent)
+        want, bound = ref.logprobs_grad(part, tok, lse, ent, dlogp, dent)
+        # (a shard that holds nearly everything may have half a step of lse put right: its p moves by as much)
+        p = torch.exp(f64(part) - f64(lse)[:, None])
+        lp = (f64(part) - f64(lse)[:, None]).abs()
+        size = p * (f64(dlogp).abs()[:, None] + f64(dent).abs()[:, None] * (1 + lp + f64(ent)[:, None]))
+        assert_close(d, want, bound + 2 * size * 2 * ref.U * f64(lse).abs()[:, None], f"shard {r}")

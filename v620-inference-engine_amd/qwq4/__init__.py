@@ -1059,7 +1059,8 @@ def logprobs(logits, tokens, top=0, workspace=None):
 
 def logprobs_backward(logits, tokens, lse, entropy, dlogp=None, dentropy=None, dlogits=None):
     """The gradient of logprobs' logp and entropy (dlogp, dentropy fp32 [T], either None: none) in the logits' type,
-    from lse and entropy as logprobs gave them. dlogits may be the logits. float16 beyond +-65504 becomes infinite."""
+    from lse and entropy as logprobs gave them (p is put right where lse is too large for its rounding not to show).
+    dlogits may be the logits. float16 beyond +-65504 becomes infinite."""
     import torch
     fn = "logprobs_backward"
     ld = _matrix(fn, "logits", logits, None, None)
