@@ -503,7 +503,8 @@ int qw_lora(const void *x, int ldx, int f16, const void *A, const void *B, const
  * be dx (the same stride); both NULL: not wanted. dA fp32 [L][R][K] and dB fp32
  * [L][N][R] are written whole (zeros for an adapter without tokens) and may be
  * NULL each, x is read for dA only and v for dB only. fp16 dx_out beyond +-65504
- * becomes infinite. Sums over tokens have a fixed order. Limits as qw_lora's.
+ * becomes infinite. Sums over tokens have a fixed order; an infinity or a NaN of a token's row
+ * shows in its columns of its adapter's gradients only (as either). Limits as qw_lora's.
  * workspace: qw_lora_backward_workspace_size bytes, 256-byte aligned. */
 size_t qw_lora_backward_workspace_size(int T, int K, int N, int R, int L);
 int qw_lora_backward(const void *dy, int lddy, const void *x, int ldx, int f16, const void *A, const void *B,

@@ -243,3 +243,69 @@ def test_offsets_past_32_bits(gpu):
     want = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling, dx=dx, dx_out=torch.empty_like(dx))
     got = qwq4.lora_backward(fdy, fx, A, B, ids, w, scaling=scaling, dx=fdx, dx_out=fdxo)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def two_kinds(T, K, N, R, L, t, gpu, small, large):
+    """Every other token's rows scaled by `small`, the others' by `large` and zero in the first 16 columns of x and dy:
+    there the weights' gradients are sums of the small tokens' products alone."""
+    x, A, B, ids, scaling, g = make(30, T, K, N, R, L, t, gpu, "one")
+    dy = torch.randn(T, N, generator=g).to(x.dtype).to(gpu)
+    big = (torch.arange(T, device=gpu) % 2 == 0)[:, None]
+    by = torch.where(big, large, small)
+    x, dy = (x.float() * by).to(x.dtype), (dy.float() * by).to(x.dtype)
+    x[::2, :16] = 0
+    dy[::2, :16] = 0
+    return x, A, B, ids, scaling, dy
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("T,R", [(60, 16), (700, 16), (300, 64)])
+@pytest.mark.parametrize("small,large", [(2.0**-8, 2.0**4), (2.0**-12, 2.0**12)])
+def test_small_tokens_beside_large_ones(gpu, t, T, R, small, large):
+    """Factors far below the largest of their rank: the sums that only they reach are as exact as any."""
+    K, N, L = 136, 264, 2
+    x, A, B, ids, scaling, dy = two_kinds(T, K, N, R, L, t, gpu, small, large)
+    v = torch.zeros(T, R, device=gpu)
+    qwq4.lora(x, A, B, ids, torch.zeros(T, N, device=gpu), v=v)
+    _, dA, dB = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling)
+    _, wA, bA, wB, bB = ref.lora_grad(dy, x, A, B, ids, v, scaling)
+    assert_close(dA, wA, bA, "dA")
+    assert_close(dB, wB, bB, "dB")
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("T", [300, 2500])
+def test_growing_tokens(gpu, t, T):
+    """Factors that grow a hundredfold and more every 64 tokens of an adapter, and shrink again."""
+    K, N, R, L = 72, 136, 24, 2
+    x, A, B, ids, scaling, g = make(31, T, K, N, R, L, t, gpu)
+    dy = torch.randn(T, N, generator=g).to(x.dtype).to(gpu)
+    by = torch.tensor([2.0**-9, 2.0**-2, 2.0**6, 2.0**9, 1.0], device=gpu)[torch.arange(T, device=gpu) // 128 % 5][:, None]
+    x, dy = (x.float() * by).to(x.dtype), (dy.float() * by).to(x.dtype)
+    v = torch.zeros(T, R, device=gpu)
+    qwq4.lora(x, A, B, ids, torch.zeros(T, N, device=gpu), v=v)
+    _, dA, dB = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling)
+    _, wA, bA, wB, bB = ref.lora_grad(dy, x, A, B, ids, v, scaling)
+    assert_close(dA, wA, bA, "dA")
+    assert_close(dB, wB, bB, "dB")
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_infinite_rows_in_the_weights_gradients(gpu, t):
+    """An infinity or a NaN of a token's row reaches its column of its adapter only, and shows there."""
+    T, K, N, R, L = 70, 64, 136, 16, 2
+    x, A, B, ids, scaling, g = make(32, T, K, N, R, L, t, gpu)
+    ids[:] = torch.arange(T) % 2
+    dy, v = torch.randn(T, N, generator=g).to(x.dtype).to(gpu), torch.randn(T, R, generator=g).to(gpu)
+    _, cA, cB = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling)
+    x2, dy2 = x.clone(), dy.clone()
+    x2[4, 5], x2[6, 9] = float("inf"), float("nan")
+    _, dA, _ = qwq4.lora_backward(dy, x2, A, B, ids, v, scaling=scaling)
+    assert not torch.isfinite(dA[0, :, 5]).any() and torch.isnan(dA[0, :, 9]).all()
+    dA[0, :, 5], dA[0, :, 9] = cA[0, :, 5], cA[0, :, 9]
+    assert torch.equal(dA, cA)
+    dy2[4, 5], dy2[6, 9] = float("-inf"), float("nan")
+    _, _, dB = qwq4.lora_backward(dy2, x, A, B, ids, v, scaling=scaling)
+    assert not torch.isfinite(dB[0, 5]).any() and torch.isnan(dB[0, 9]).all()
+    dB[0, 5], dB[0, 9] = cB[0, 5], cB[0, 9]
+    assert torch.equal(dB, cB)

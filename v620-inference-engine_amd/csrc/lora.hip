@@ -522,20 +522,41 @@ void launch_lora_expand(LoraExpandArgs a, const LoraJoinArgs &join, hipStream_t 
 constexpr int OUTER_COLS = 512;     // columns of a block
 constexpr int OUTER_TOKENS = 1024;  // tokens whose ids it looks at at once
 
+// 8 fp16 values as two bf16 operands: their first 8 bits, and the last 3, which are left behind them exactly.
+__device__ __forceinline__ void halves_of_f16(const uint4 &w, uint4 &high, uint4 &low) {
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t top[2], rest[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float f = f16_bits_to_f32(uint16_t(in[i] >> (16 * e)));
+            top[e] = __builtin_bit_cast(uint32_t, f) & 0xffff0000u;
+            rest[e] = __builtin_bit_cast(uint32_t, f - __builtin_bit_cast(float, top[e]));
+        }
+        h[i] = __builtin_amdgcn_perm(top[1], top[0], 0x07060302u);
+        l[i] = __builtin_amdgcn_perm(rest[1], rest[0], 0x07060302u);
+    }
+    high = make_uint4(h[0], h[1], h[2], h[3]);
+    low = make_uint4(l[0], l[1], l[2], l[3]);
+}
+
 // G[r][c] = scaling sum_t u[t][r] m[t][c] over the tokens of one adapter in one
 // part of the batch: 128 columns a wave, 16 RF ranks. The tokens are listed in
 // LDS in order. The sum runs over tokens, whose values lie a row apart: a lane
 // loads 8 columns of 8 tokens and turns them in registers (v_perm) into 8
 // operands of one column each, so the wide rows come in 16-byte loads and
-// never pass through LDS. u goes in as three bf16 parts (exact) or two fp16 ones
-// (to 2^-23) of u times a power of two per rank, which follows the largest u so
-// far (fp16 of u itself would overflow). 4096 tokens of 4096 and 12288 columns, 16
-// ranks: 31 us, 4.3 TB/s; alike with two steps on their way, with u turned once for the four waves,
-// or a block for all adapters of a part.
-template <class T16, int RF>
+// never pass through LDS. u goes in as three bf16 parts whose sum it is. fp16 rows go
+// in as two bf16 parts, also exactly, so that small factors keep their bits beside
+// large ones, which fp16 has no range for: as two fp16 parts of u times a power of two
+// per rank, a factor of 2e-8 of the largest was off by 1%. (u's third part times the
+// rows' second one is left out: below 2^-25 of the product. A whole call with 4096 fp16
+// tokens of rank 16, 4096 and 12288 columns: 81 us for 76 with two fp16 parts.) 4096 tokens of 4096 and
+// 12288 columns, 16 ranks: 31 us, 4.3 TB/s; alike with two steps on their way, with u
+// turned once for the four waves, or a block for all adapters of a part.
+template <bool HALF, int RF>
 __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
-    constexpr bool HALF = __is_same(T16, F16);
-    constexpr int PARTS = HALF ? 2 : 3;
     __shared__ uint32_t s_tok[OUTER_TOKENS];
     __shared__ int s_count[4];
     const int tid = int(threadIdx.x), lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
@@ -553,18 +574,6 @@ __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
     for (int f = 0; f < RF; ++f)
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[f][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int shift[RF];  // fp16: the power of two of rank r0 + 16 f + c
-#pragma unroll
-    for (int f = 0; f < RF; ++f) shift[f] = HALF ? 141 : 0;
-    // row i of a piece's sums is rank 4 g + i, whose power of two lane 4 g + i has
-    auto rescale = [&](int f, int by) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = __shfl(by, 4 * g + i);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) acc[f][j][i] = __builtin_ldexpf(acc[f][j][i], d);
-        }
-    };
 
     int total = 0;
     for (int b0 = from; b0 < end; b0 += OUTER_TOKENS) {
@@ -612,35 +621,24 @@ __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
         };
         if (steps > 0) load(0);
         for (int s = 0; s < steps; ++s) {
-            uint4 column[8], q[RF][PARTS];
+            uint4 column[8], q[RF][3];
             turn8(next, column);
 #pragma unroll
-            for (int f = 0; f < RF; ++f) {
-                if constexpr (HALF) {
-                    float top = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(nu[f][e]));
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    const int size = int((__builtin_bit_cast(uint32_t, top) >> 23) & 255u) - 126;  // top below 2^size
-                    if (__ballot(size + shift[f] > 15)) {
-                        // (to 2^8: room for values 128 times as large before the next time)
-                        const int by = size + shift[f] > 15 ? 8 - size - shift[f] : 0;
-                        shift[f] += by;
-                        rescale(f, by);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) nu[f][e] = __builtin_ldexpf(nu[f][e], shift[f]);
-                }
-                split8<T16, PARTS>(nu[f], q[f]);
-            }
+            for (int f = 0; f < RF; ++f) split8<BF16, 3>(nu[f], q[f]);
             if (s + 1 < steps) load(s + 1);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
+                uint4 high = column[j], low;
+                if constexpr (HALF) halves_of_f16(column[j], high, low);
 #pragma unroll
-                for (int f = 0; f < RF; ++f)
+                for (int f = 0; f < RF; ++f) {
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p) acc[f][j] = mfma16<T16>(q[f][p], column[j], acc[f][j]);
+                    for (int p = 0; p < 3; ++p) acc[f][j] = mfma16<BF16>(q[f][p], high, acc[f][j]);
+                    if constexpr (HALF) {
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) acc[f][j] = mfma16<BF16>(q[f][p], low, acc[f][j]);
+                    }
+                }
             }
         }
         __syncthreads();  // (the list is read)
@@ -648,10 +646,6 @@ __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
     if (a.parts > 1 && blockIdx.x == 0 && r0 == 0 && tid == 0) a.count[part * a.L + l] = total;
     if (total == 0 && a.parts > 1) return;  // (the joining launch goes by the count)
 
-    if constexpr (HALF) {
-#pragma unroll
-        for (int f = 0; f < RF; ++f) rescale(f, -shift[f]);
-    }
     if (c0 + 8 * c >= m.C) return;
     const float scale = a.scaling ? a.scaling[l] : 1.f;
     float *out = m.out + (int64_t(part) * a.L + l) * a.R * m.C;
@@ -735,12 +729,12 @@ static LoraJoinArgs launch_lora_outer(const LoraGradArgs &a, char *base, const L
     const int ranks = outer_ranks(a.R);
     const dim3 grid(unsigned(o.m[0].blocks() + o.m[1].blocks()), unsigned((a.R + ranks - 1) / ranks * a.L),
                     unsigned(parts));
-    auto run = [&](auto t16) {
-        if (ranks == 16) lora_outer_kernel<decltype(t16), 1><<<grid, 256, 0, s>>>(o);
-        else lora_outer_kernel<decltype(t16), 2><<<grid, 256, 0, s>>>(o);
+    auto run = [&](auto half) {
+        if (ranks == 16) lora_outer_kernel<decltype(half)::value, 1><<<grid, 256, 0, s>>>(o);
+        else lora_outer_kernel<decltype(half)::value, 2><<<grid, 256, 0, s>>>(o);
     };
-    if (a.f16) run(F16{});
-    else run(BF16{});
+    if (a.f16) run(std::true_type{});
+    else run(std::false_type{});
     if (parts == 1) return LoraJoinArgs{};
     return LoraJoinArgs{{pa, pb}, {a.dA, a.dB}, {a.dA ? int64_t(a.R) * a.K : 0, a.dB ? int64_t(a.R) * a.N : 0}, o.count,
                         a.L, parts};
