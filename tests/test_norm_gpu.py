@@ -238,3 +238,51 @@ def test_many_rows(gpu, T, H, dy, h, dres):
     """Every way of sharing rows among lanes, waves and blocks with more rows than are taken at once."""
     test_norm_backward(gpu, T, H, dy, h, dres)
     test_norm(gpu, T, H, dy, "f32" if h == "f32" else None, dy)
+
+
+@pytest.mark.parametrize("x", sorted(TYPES))
+@pytest.mark.parametrize("H", [8, 16, 1000, 1008, 1001, 2560, 9000])
+def test_i8_of_every_type(gpu, x, H):
+    """Every combination of types that the 8-bit call takes: the bits of q, the scale and the residual, against the
+    host's arithmetic in fp32."""
+    xs = rows(H, 5, H, x, gpu)
+    for w in {x, "f32"}:
+        ws = rows(5, 1, H, w, gpu)[0]
+        for res in {None, x, "f32"}:
+            rs = rows(H + 1, 5, H, res, gpu) if res else None
+            q, scale, *more = qwq4.rms_norm_i8(xs, ws, EPS, residual=rs)
+            h = xs.float().cpu().numpy() + (rs.float().cpu().numpy() if res else np.float32(0))
+            u = h * ws.float().cpu().numpy()
+            step = np.maximum(np.abs(u).max(1) / np.float32(127), np.float32(2.0**-126))
+            assert u.dtype == step.dtype == np.float32
+            assert np.array_equal(q.cpu().numpy(), np.rint(u * (np.float32(1) / step)[:, None]).astype(np.int8)), (w, res)
+            r = ref.norm(xs, ws, EPS, rs)[1][:, 0]
+            want = torch.from_numpy(step.astype(np.float64)) * r
+            assert_close(scale, want, want.abs() * ref.U * (ref.norm_chain(H) / 2 + 8), f"scale {w} {res}")
+            if res:
+                assert torch.equal(more[0].cpu(), torch.from_numpy(h).to(TYPES[res])), (w, res)
+
+
+@pytest.mark.parametrize("H", [64, 520, 1160, 2048, 2047, 2560, 4100, 9000, 16384])
+@pytest.mark.parametrize("dy,h", [("bf16", "bf16"), ("f16", "f16"), ("bf16", "f32"), ("f32", "f32")])
+def test_bits_do_not_depend_on_the_place(gpu, H, dy, h):
+    """Rows side by side on 16 bytes, rows at odd elements and strides, and a single row out of them: the same bits,
+    forward and back."""
+    T = 7
+    for off, pad in ((0, 8), (1, 0), (3, 5)):
+        d, hs, rs = rows(1, T, H, dy, gpu, pad, off), rows(2, T, H, h, gpu, pad, off), rows(3, T, H, h, gpu, pad, off)
+        w = rows(4, 1, H, dy, gpu)[0]
+        out = like(T, H, hs.dtype, gpu, pad + 1)[0]
+        dx, dw = qwq4.rms_norm_backward(d.contiguous(), hs.contiguous(), w, EPS, dres=rs.contiguous())
+        dx2, dw2 = qwq4.rms_norm_backward(d, hs, w, EPS, dres=rs, dx=out)
+        assert torch.equal(dx, dx2) and torch.equal(dw, dw2), (off, pad)
+        for t in (0, T - 1):
+            one, _ = qwq4.rms_norm_backward(d[t:t + 1], hs[t:t + 1], w, EPS, dres=rs[t:t + 1])
+            assert torch.equal(one, dx[t:t + 1]), (off, pad, t)
+        ws = w if dy == h else w.float()
+        y, r = qwq4.rms_norm(hs.contiguous(), ws, EPS, residual=rs.contiguous())
+        y2, r2 = qwq4.rms_norm(hs, ws, EPS, residual=rs, y=like(T, H, hs.dtype, gpu, pad + 1)[0])
+        assert torch.equal(y, y2) and torch.equal(r, r2), (off, pad)
+        q, s, _ = qwq4.rms_norm_i8(hs.contiguous(), ws, EPS, residual=rs.contiguous())
+        q2, s2, _ = qwq4.rms_norm_i8(hs, ws, EPS, residual=rs, q=torch.empty(T, H + 3, dtype=torch.int8, device=gpu)[:, :H])
+        assert torch.equal(q, q2) and torch.equal(s, s2), (off, pad)

@@ -251,27 +251,62 @@ void launch_rms_norm(const NormArgs &a, hipStream_t s) {
 }
 
 // ------------------------------------------------------------ gradients
-// 8 elements of a row on their way: as they lie, or (rows that start anywhere) values.
-template <int TY, bool VEC>
+// 8 elements of a row on their way, as they lie (unpacked, those of rows that start
+// anywhere would take twice the registers: 1024 bf16 rows of 16380 120 us for 38). The
+// last piece of such a row is its last 8 elements in one access, moved to their places, with zeros
+// behind them, when the values are asked for. SHORT: a row may have fewer than 8.
+template <int TY, bool VEC, bool SHORT>
 struct Part {
     RowPiece<TY> w;
-    __device__ __forceinline__ void load(const void *x, int64_t row, int j, int) { w.load(x, row + j); }
-    __device__ __forceinline__ void values(float (&v)[8]) const { w.values(v); }
-};
-template <int TY>
-struct Part<TY, false> {
-    float f[8];
-    __device__ __forceinline__ void load(const void *x, int64_t row, int j, int n) { part_load<TY, false>(x, row, j, n, f); }
-    __device__ __forceinline__ void values(float (&v)[8]) const {
+    using E = std::conditional_t<TY == 0, uint32_t, uint16_t>;
+    struct Eight {
+        E e[8];
+    };
+    __device__ __forceinline__ void load(const void *x, int64_t row, int j, int n) {
+        if constexpr (VEC) {
+            w.load(x, row + j);
+            return;
+        }
+        const E *p = static_cast<const E *>(x) + row;
+        if (SHORT && n < 8) {
+            Eight one;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = f[e];
+            for (int e = 0; e < 8; ++e) one.e[e] = p[min(e, n - 1)];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e >= n) one.e[e] = 0;
+            w = __builtin_bit_cast(RowPiece<TY>, one);
+        } else {
+            __builtin_memcpy(&w, p + min(j, n - 8), sizeof(w));
+        }
+    }
+    template <class T>
+    __device__ __forceinline__ static void to_places(T (&v)[8], int j, int n) {
+        if (VEC || j + 8 <= n || (SHORT && n < 8)) return;
+        const int by = j + 8 - n;
+#pragma unroll
+        for (int s = 4; s >= 1; s >>= 1) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = !(by & s) ? v[e] : e + s < 8 ? v[(e + s) % 8] : T(0);
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[8], int j, int n) const {
+        w.values(v);
+        to_places(v, j, n);
+    }
+    // the elements at their places for good: w.values has them (for what is read once and used for every row)
+    __device__ __forceinline__ void settle(int j, int n) {
+        if constexpr (VEC) return;
+        Eight v = __builtin_bit_cast(Eight, w);
+        to_places(v.e, j, n);
+        w = __builtin_bit_cast(RowPiece<TY>, v);
     }
 };
 
 // A row by G of the block's TH threads (16, 64: groups of a wave, which meet no
 // barrier but the last; more: of waves), 8 elements per thread and C turns each. A
 // group takes every (groups of the grid)-th row, with the next one on its way
-// while the current one's sums are made, and keeps its columns' part of dw in
+// while the current one's sums are made (but in blocks of 1024), and keeps its columns' part of dw in
 // registers; the block adds its groups' parts and a second launch the blocks', in
 // order. Bound by memory.
 template <int DT, int HT, int WT, bool VEC, int G, int TH, int C>
@@ -281,11 +316,13 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
     __shared__ float s_sum[2][2][NW];
     const int tid = int(threadIdx.x), H = a.H;
     const int group = GROUPS == 1 ? 0 : BLOCK ? __builtin_amdgcn_readfirstlane(tid / G) : tid / G, li = tid - group * G;
+    // (with the next row on its way a block of 1024 spills 57 to 113 registers: 512 fp32 rows of 16384 70 us for 45)
+    constexpr bool SHORT = G == 16, AHEAD = G < 1024;
     struct Row {
-        Part<HT, VEC> h[C], res[C];
-        Part<DT, VEC> d[C];
+        Part<HT, VEC, SHORT> h[C], res[C];
+        Part<DT, VEC, SHORT> d[C];
     } next;
-    Part<WT, VEC> wp[C];
+    Part<WT, VEC, SHORT> wp[C];
     float dw[C][8];
     auto load = [&](int64_t t) {
 #pragma unroll
@@ -302,23 +339,28 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
         const int j = (li + c * G) * 8;
 #pragma unroll
         for (int e = 0; e < 8; ++e) dw[c][e] = 0.f;
-        if (j < H) wp[c].load(a.w, 0, j, H);
+        if (j < H) {
+            wp[c].load(a.w, 0, j, H);
+            wp[c].settle(j, H);
+        }
     }
     const int64_t t0 = int64_t(blockIdx.x) * GROUPS + group, step = int64_t(gridDim.x) * GROUPS;
-    if (t0 < a.T) load(t0);
+    if (AHEAD && t0 < a.T) load(t0);
     int p = 0;
     for (int64_t t = t0; t - (BLOCK ? group : 0) < a.T; t += step, p ^= 1) {
         const bool live = !BLOCK || GROUPS == 1 || t < a.T;
+        if (!AHEAD && t < a.T) load(t);
         const Row row = next;
-        if (t + step < a.T) load(t + step);
+        if (AHEAD && t + step < a.T) load(t + step);
         float h[C][8], g[C][8], sum = 0.f, dot = 0.f;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            if ((li + c * G) * 8 >= H) continue;
+            const int j = (li + c * G) * 8;
+            if (j >= H) continue;
             float w[8];
-            row.h[c].values(h[c]);
-            row.d[c].values(g[c]);
-            wp[c].values(w);
+            row.h[c].values(h[c], j, H);
+            row.d[c].values(g[c], j, H);
+            wp[c].w.values(w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 sum = __builtin_fmaf(h[c][e], h[c][e], sum);
@@ -349,7 +391,7 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
             const int j = (li + c * G) * 8;
             if (j >= H || !live) continue;
             float o[8], w[8];
-            wp[c].values(w);
+            wp[c].w.values(w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 o[e] = r * (g[c][e] * w[e] - h[c][e] * k);
@@ -357,7 +399,7 @@ __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
             }
             if (a.dres) {
                 float res[8];
-                row.res[c].values(res);
+                row.res[c].values(res, j, H);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) o[e] += res[e];
             }
@@ -435,10 +477,10 @@ static void launch_norm_grad(const NormGradArgs &a, hipStream_t s) {
     };
     // Short rows by parts of a wave: no barrier, and every thread has work (16.8 million elements in bf16, a block or a
     // wave a row, and as here: rows of 64 545 us and 42, of 256 140 and 22, of 1024 49 and 22). Rows of 16 bits by as few
-    // waves as registers allow: of 2048 29 us in blocks, 24 in waves; of 2560 32 and 26; of 16384 37 and 34. (fp32, and rows
-    // that start anywhere, which wait as fp32, would spill.)
+    // waves as registers allow: of 2048 29 us in blocks, 24 in waves; of 2560 32 and 26; of 16384 37 and 34. fp32 would
+    // spill so, and does (13 to 51 registers) above 8192. How the rows lie is not asked: their bits would depend on it.
     auto by_length = [&](auto vec) {
-        constexpr bool HALF = HT != 0 && decltype(vec)::value;
+        constexpr bool HALF = HT != 0;
         if (a.H <= 128) return run(vec, Int<16>{}, Int<512>{}, Int<1>{});
         if (a.H <= 256) return run(vec, Int<16>{}, Int<512>{}, Int<2>{});
         if (a.H <= 512) return run(vec, Int<64>{}, Int<512>{}, Int<1>{});
