@@ -309,3 +309,18 @@ def test_infinite_rows_in_the_weights_gradients(gpu, t):
     assert not torch.isfinite(dB[0, 5]).any() and torch.isnan(dB[0, 9]).all()
     dB[0, 5], dB[0, 9] = cB[0, 5], cB[0, 9]
     assert torch.equal(dB, cB)
+
+
+@pytest.mark.parametrize("T", [40, 1000])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_scaling_of_an_adapter_without_tokens(gpu, T, bad):
+    """A free slot's scaling may hold anything: its gradients are zeros, in one part of the batch or several."""
+    K, N, R, L = 64, 72, 16, 3
+    x, A, B, ids, scaling, g = make(33, T, K, N, R, L, "bf16", gpu)
+    ids[ids == 1] = 2
+    dy, v = torch.randn(T, N, generator=g).to(x.dtype).to(gpu), torch.randn(T, R, generator=g).to(gpu)
+    dx = torch.zeros(T, K, dtype=x.dtype, device=gpu)
+    want = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling, dx=dx.clone())
+    scaling[1] = bad
+    got = qwq4.lora_backward(dy, x, A, B, ids, v, scaling=scaling, dx=dx.clone())
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and (got[1][1] == 0).all() and (got[2][1] == 0).all()

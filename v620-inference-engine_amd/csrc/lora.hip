@@ -647,7 +647,7 @@ __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
     if (total == 0 && a.parts > 1) return;  // (the joining launch goes by the count)
 
     if (c0 + 8 * c >= m.C) return;
-    const float scale = a.scaling ? a.scaling[l] : 1.f;
+    const float scale = a.scaling && total ? a.scaling[l] : 1.f;  // (without tokens: zeros, whatever a free slot's is)
     float *out = m.out + (int64_t(part) * a.L + l) * a.R * m.C;
 #pragma unroll
     for (int f = 0; f < RF; ++f) {
