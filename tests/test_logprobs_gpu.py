@@ -298,3 +298,32 @@ def test_backward_of_a_shard(gpu, shift):
         lp = (f64(part) - f64(lse)[:, None]).abs()
         size = p * (f64(dlogp).abs()[:, None] + f64(dent).abs()[:, None] * (1 + lp + f64(ent)[:, None]))
         assert_close(d, want, bound + 2 * size * 2 * ref.U * f64(lse).abs()[:, None], f"shard {r}")
+
+
+def test_outputs_are_tensors_of_their_own(gpu):
+    """What torch asks of a Function's outputs: in-place work on one, with the others' graphs still read; and no output
+    keeps another's memory."""
+    T, V = 6, 300
+    logits, tokens, g = make(8, T, V, "f32", gpu)
+
+    class LogProbs(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, l):
+            logp, entropy, lse, _, _ = qwq4.logprobs(l, tokens)
+            ctx.save_for_backward(l, lse, entropy)
+            return logp, entropy
+
+        @staticmethod
+        def backward(ctx, dlogp, dentropy):
+            l, lse, entropy = ctx.saved_tensors
+            return qwq4.logprobs_backward(l, tokens, lse, entropy, dlogp.contiguous(), dentropy.contiguous())
+
+    leaf = logits.clone().requires_grad_()
+    logp, entropy = LogProbs.apply(leaf)
+    mask = torch.tensor([1.0, 0, 1, 1, 0, 1], device=gpu)
+    logp.mul_(mask)
+    (logp.sum() + 0.5 * entropy.sum()).backward()
+    _, ent, lse, _, _ = got = qwq4.logprobs(logits, tokens, top=3)
+    assert torch.equal(leaf.grad, qwq4.logprobs_backward(logits, tokens, lse, ent, mask, torch.full((T,), 0.5, device=gpu)))
+    assert len({t.untyped_storage().data_ptr() for t in got}) == 5
+    assert all(t._base is None and t.untyped_storage().nbytes() == t.numel() * t.element_size() for t in got)

@@ -1041,19 +1041,19 @@ def logprobs(logits, tokens, top=0, workspace=None):
     if not 0 <= top <= min(64, V):
         raise ValueError(f"{fn}: top = {top} (0..64, at most V = {V})")
     code = _tcode(logits)
-    # (one buffer for the fp32 outputs: an allocation each would cost more than the call)
-    own = logits.new_empty(T * (3 + top), dtype=torch.float32)
-    logp, entropy, lse, top_logp = own.split_with_sizes((T, T, T, T * top))
-    top_ids = tokens.new_empty((T, top)) if top else None
-    top_logp = top_logp.view(T, top) if top else None
+    # (tensors of their own: torch refuses in-place work on several views of one buffer, and each would keep all of it)
+    logp = logits.new_empty(T, dtype=torch.float32)
+    entropy, lse = logp.new_empty(T), logp.new_empty(T)
+    top_ids, top_logp = (tokens.new_empty((T, top)), logp.new_empty((T, top))) if top else (None, None)
+    stream = _here(fn, logits, tokens, workspace)  # (the outputs are where logits is)
     if workspace is None:
-        need = logprobs_workspace_size(T, V, top)
-        if need:
-            workspace = logits.new_empty(need, dtype=torch.uint8)
-    stream = _here(fn, logits, tokens, own, workspace)
-    _check(lib().qw_logprobs(_ptr(logits), code, ld, _ptr(tokens), T, V, top, _ptr(logp), _ptr(entropy), _ptr(lse),
-                             _ptr(top_ids), _ptr(top_logp), _ptr(workspace), _space(fn, workspace), stream),
-           "qw_logprobs")
+        space = lib().qw_logprobs_workspace_size(T, V, top)
+        workspace = logp.new_empty((space + 3) // 4) if space else None
+    else:
+        space = _space(fn, workspace)
+    _check(lib().qw_logprobs(logits.data_ptr(), code, ld, tokens.data_ptr(), T, V, top, logp.data_ptr(),
+                             entropy.data_ptr(), lse.data_ptr(), _ptr(top_ids), _ptr(top_logp), _ptr(workspace), space,
+                             stream), "qw_logprobs")
     return logp, entropy, lse, top_ids, top_logp
 
 
