@@ -523,7 +523,7 @@ int qw_lora_backward(const void *dy, int lddy, const void *x, int ldx, int f16, 
  * first, ties by the lowest index. A logit of -infinity is masked: it has p = 0
  * and adds nothing. A row of only such has lse, logp and top_logp of -infinity and
  * entropy 0. A row with a NaN or +infinity gives NaN, and top_ids of -1.
- * workspace: qw_logprobs_workspace_size bytes (0 from 2048 rows on), 256-byte
+ * workspace: qw_logprobs_workspace_size bytes (0 from 512 rows on), 256-byte
  * aligned. */
 size_t qw_logprobs_workspace_size(int T, int V, int top);
 int qw_logprobs(const void *logits, int type, int ld, const int32_t *tokens, int T, int V, int top, float *logp,
@@ -536,8 +536,8 @@ int qw_logprobs(const void *logits, int type, int ld, const int32_t *tokens, int
  * the same stride). dlogp, dentropy fp32 [T], either may be NULL (none; entropy is
  * read with dentropy only); a token outside 0 .. V - 1 has no dlogp. Where the rounding of
  * lse would show in p (|lse| above 64 for fp32 logits, 1024 for 16-bit ones), the row is
- * read twice and p put right by up to a step of lse. Masked logits and rows of
- * only such get 0; fp16 beyond +-65504 becomes infinite. */
+ * read twice and p put right by up to a step of lse. Masked logits get 0 (the token's own,
+ * if it is masked, dlogp), rows of only such get 0; fp16 beyond +-65504 becomes infinite. */
 int qw_logprobs_backward(const void *logits, int type, int ld, const int32_t *tokens, const float *lse,
                          const float *entropy, const float *dlogp, const float *dentropy, int T, int V, void *dlogits,
                          int ldd, void *stream);

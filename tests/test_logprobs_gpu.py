@@ -327,3 +327,29 @@ def test_outputs_are_tensors_of_their_own(gpu):
     assert torch.equal(leaf.grad, qwq4.logprobs_backward(logits, tokens, lse, ent, mask, torch.full((T,), 0.5, device=gpu)))
     assert len({t.untyped_storage().data_ptr() for t in got}) == 5
     assert all(t._base is None and t.untyped_storage().nbytes() == t.numel() * t.element_size() for t in got)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+def test_gradient_of_a_masked_token(gpu, t):
+    """A masked logit has no gradient, but for a token that is itself masked: its logp is -inf, and its dlogp passes on to
+    its logit as the formula has it (and torch's log_softmax)."""
+    T, V = 5, 203
+    logits, tokens, g = make(12, T, V, t, gpu)
+    tokens = tokens.clamp(0, V - 1)
+    at = torch.arange(T, device=gpu)
+    logits[:, 50:90] = -INF
+    tokens[:3] = 60
+    logp, ent, lse, _, _ = qwq4.logprobs(logits, tokens)
+    assert (logp[:3] == -INF).all() and torch.isfinite(logp[3:]).all()
+    dlogp, dent = torch.randn(T, generator=g).to(gpu), torch.randn(T, generator=g).to(gpu)
+    d = qwq4.logprobs_backward(logits, tokens, lse, ent, dlogp, dent)
+    want, bound = ref.logprobs_grad(logits, tokens, lse, ent, dlogp, dent)
+    assert_close(d, want, bound)
+    assert torch.equal(d[at[:3], 60], dlogp[:3].to(d.dtype))
+    masked = d[:, 50:90].clone()
+    masked[:3, 10] = 0
+    assert (masked == 0).all()
+    l = logits.double().cpu().requires_grad_()
+    torch.log_softmax(l, -1)[torch.arange(T), tokens.cpu().long()].backward(f64(dlogp))
+    d = qwq4.logprobs_backward(logits, tokens, lse, ent, dlogp)
+    assert_close(d, l.grad, ref.logprobs_grad(logits, tokens, lse, ent, dlogp, None)[1] + 2.0**-18 * torch.exp(f64(logits) - f64(lse)[:, None]) * f64(dlogp).abs()[:, None])
