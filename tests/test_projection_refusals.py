@@ -113,6 +113,22 @@ def test_workspace_sizes(lib):
     assert lib.qw_lora_backward_workspace_size(1, 64, 32, 16, 2) >= 16 * 4  # (dv)
 
 
+@pytest.mark.parametrize("K,N,R,L", [(64, 72, 8, 1), (4096, 12288, 16, 4), (4096, 4096, 64, 63), (2560, 4096, 128, 3),
+                                     (512, 512, 32, 1023), (1 << 20, 8, 16, 1), (4096, 4096, 128, 4096)])
+def test_lora_workspace_is_bounded(lib, K, N, R, L):
+    """dv, and sums of parts of the batch below 256 MB with their counts, however long the batch."""
+    for T in (1, 129, 5000, 1 << 20):
+        size = lib.qw_lora_backward_workspace_size(T, K, N, R, L)
+        assert T * R * 4 <= size < T * R * 4 + (256 << 20) + 64 * 4 * min(L, 2048) + 1024
+
+
+def test_logprobs_workspace_of_many_rows(lib):
+    assert lib.qw_logprobs_workspace_size(511, 151936, 20) > 0
+    for T in (512, 513, 2047, 1 << 23):
+        for V in (1, 151936, 1 << 28):
+            assert lib.qw_logprobs_workspace_size(T, V, min(V, 64)) == 0
+
+
 def test_python_checks():
     """What the binding itself refuses, on CPU tensors of shapes that the C call never sees."""
     import torch

@@ -675,7 +675,8 @@ __global__ __launch_bounds__(256) void lora_outer_join_kernel(LoraJoinArgs a) { 
 // Parts of the batch whose sums over tokens run side by side, at most
 // MAX_PARTS: until about 2048 blocks are there (one whose adapter has no token in
 // its part ends at once), of 128 tokens or more. Every part has room for every
-// adapter's sums: with the number of blocks that is bounded, 64 MB or so.
+// adapter's sums, 64 KB a block at most: with fewer than 4096 blocks in several parts,
+// below 256 MB.
 constexpr int MAX_PARTS = 64;
 static int outer_ranks(int R) { return R <= 16 ? 16 : 32; }
 static int outer_parts(int T, int K, int N, int R, int L) {
