@@ -448,7 +448,8 @@ int qw_moe_unpermute_backward(const void *dout, int dout_type, int ldd, const vo
  * where that is of its type, at the same stride). y is normalised from h as added, before that rounding.
  * x and y of any QW_T_* type, w [H] of x's type or fp32; y may be x where type and
  * stride are the same. fp16 outputs saturate at +-65504. Sums in fp32: rows with values
- * past 1e19 overflow them and give zeros. Any H from 1 to 2^28, any stride >= H and
+ * past 1e19 overflow them and give zeros (and with eps = 0, values all below 1e-19 lose
+ * their squares' bits). Any H from 1 to 2^28, any stride >= H and
  * alignment of the elements; rows of a multiple of 8 on 16 bytes are fastest. */
 int qw_rms_norm(const void *x, int x_type, int ldx, const void *residual, int res_type, int ldr, void *res_out,
                 int ldro, const void *w, int w_type, float eps, int T, int H, void *y, int y_type, int ldy,

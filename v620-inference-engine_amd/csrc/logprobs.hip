@@ -21,6 +21,7 @@ constexpr float LOG2E = 1.44269504088896341f;
 // exp(x - y) of sums: below this nothing is left in fp32
 constexpr float NEARLY_NONE = -200.f;
 
+// (the product with log2 e is rounded: 2^-24 |d| of the result beside the exponential's own)
 __device__ __forceinline__ float exp_fast(float d) { return __builtin_amdgcn_exp2f(d * LOG2E); }
 __device__ __forceinline__ float neg_inf() { return -__builtin_huge_valf(); }
 

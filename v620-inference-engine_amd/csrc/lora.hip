@@ -13,8 +13,12 @@
 // a batch of single tokens reads each adapter's weights where it has to
 // anyway. All products run on the 16-bit MFMA with sums in fp32. v is kept in
 // fp32; where it meets 16-bit weights again it goes in as two (16-bit outputs)
-// or three (fp32 outputs) 16-bit parts whose sum it is, to 2^-17 or exactly:
-// with ranks of tens the added products cost less than the rows' traffic.
+// or three (fp32 outputs) 16-bit parts: with ranks of tens the added products cost
+// less than the rows' traffic. In bf16 their sum is v to 2^-17 or exactly. In fp16,
+// scaled by the token's largest, it is to 2^-22 or exactly down to 2^-15 of that, and
+// below to 2^-39 of it. The fewer bits of 16-bit outputs are a choice: 2^-17 stands
+// beside the output's own 2^-8, and a third part would not fit the one step of the
+// MFMA that covers two of rank 16.
 #include <algorithm>
 #include <type_traits>
 
