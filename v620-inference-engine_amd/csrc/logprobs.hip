@@ -558,15 +558,16 @@ struct LogprobRow {
 
 // A row in parts of 256 threads with pieces of 8 (V8) or single elements; U
 // pieces per thread requested together. Bound by memory: the logits read, the
-// gradient written (in the same place, if the caller likes): 601 bf16 rows of 151936 68
+// gradient written (in the same place, if the caller likes): 601 bf16 rows of 151936 65
 // us. A row far from zero is read twice, by one block alone, since the gradient may lie on
-// it (601 such rows 176 us, one 57 us for 4.5). The bounds on registers keep as many waves
-// a CU as rows next to zero alone would have (without them 601 fp16 rows 67 us for 64).
+// it (601 such rows 173 us, one 52 us for 4.5; 2100 fp32 rows of 32000 167 us for 101, and
+// 376 where that block was each row's first and came to two of the XCDs).
 template <int TY, bool V8>
-__global__ __launch_bounds__(256, TY == 0 ? 6 : 8) void logprobs_backward_kernel(LogprobGradArgs a, int parts) {
+__global__ __launch_bounds__(256) void logprobs_backward_kernel(LogprobGradArgs a, int parts) {
     constexpr int Z = TY == 0 ? 4 : 2, U = 4, OT = TY == 2 ? GRAD_F16 : TY;
     const int64_t t = int64_t(blockIdx.x) / parts;
-    const int part = int(blockIdx.x) % parts, tid = int(threadIdx.x);
+    int part = int(blockIdx.x) % parts;
+    const int tid = int(threadIdx.x);
     LogprobRow r(a, t);
     const char *in = static_cast<const char *>(a.logits) + t * a.ld * Z;
     char *out = static_cast<char *>(a.dlogits) + t * a.ldd * Z;
@@ -581,29 +582,33 @@ __global__ __launch_bounds__(256, TY == 0 ? 6 : 8) void logprobs_backward_kernel
     int64_t p0 = int64_t(part) * (256 * U) + tid;
     if constexpr (V8) load(p0);  // (asked for beside lse: behind it, 601 rows of 151936 80 us for 66)
     const bool far = fabsf(r.lse) > FAR_ROW<TY> && fabsf(r.lse) < __builtin_huge_valf();
-    const bool alone = part == 0 && tid < cut.head + cut.tail;
+    const bool alone = tid < cut.head + cut.tail;
     const int at = tid < cut.head ? tid : 8 * cut.pieces + tid;  // the thread's single element
     if (far) {
-        if (part) return;
+        if (part != (t + t / 8) % parts) return;  // (another part from row to row: all XCDs have a share)
+        part = 0;
+        parts = 1;
         __shared__ float s_sum[4];
         float sum = alone ? exp_fast(logit_at<TY>(in, at) - r.lse) : 0.f;
-#pragma unroll 1
-        for (int64_t p = tid; p < cut.pieces; p += 256) {
-            Raw8<TY> piece;
-            piece.load(body + p * (8 * Z));
-            float v[8];
-            piece.values(v);
+        for (int64_t p = tid; p < cut.pieces; p += 256 * U) {
+            load(p);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = exp_fast(v[j] - r.lse);
-            sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            for (int u = 0; u < U; ++u) {
+                if (p + 256 * u >= cut.pieces) continue;
+                float v[8];
+                raw[u].values(v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = exp_fast(v[j] - r.lse);
+                sum += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            }
         }
 #pragma unroll
         for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
         if (tid % WAVE == 0) s_sum[tid / WAVE] = sum;
         __syncthreads();  // (and nothing of the row is overwritten before all of it is read)
         r.put_right((s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]));
-        parts = 1;
-        if constexpr (V8) load(p0);  // (again: no registers held over the sum)
+        p0 = tid;
+        if constexpr (V8) load(p0);
     }
     auto single = [&](int i) {
         float v[1] = {r.value(logit_at<TY>(in, i), i)};
@@ -625,7 +630,7 @@ __global__ __launch_bounds__(256, TY == 0 ? 6 : 8) void logprobs_backward_kernel
             p0 += int64_t(parts) * (256 * U);
             load(p0);
         }
-        if (alone) single(at);
+        if (alone && part == 0) single(at);
     } else {
         for (int64_t i = int64_t(part) * 256 + tid; i < a.V; i += int64_t(parts) * 256) single(int(i));
     }
