@@ -556,9 +556,9 @@ __device__ __forceinline__ void halves_of_f16(const uint4 &w, uint4 &high, uint4
 // large ones, which fp16 has no range for: as two fp16 parts of u times a power of two
 // per rank, a factor of 2e-8 of the largest was off by 1%. (u's third part times the
 // rows' second one is left out: below 2^-25 of the product. A whole call with 4096 fp16
-// tokens of rank 16, 4096 and 12288 columns: 81 us for 76 with two fp16 parts.) 4096 tokens of 4096 and
-// 12288 columns, 16 ranks: 31 us, 4.3 TB/s; alike with two steps on their way, with u
-// turned once for the four waves, or a block for all adapters of a part.
+// tokens of rank 16, 4096 and 12288 columns: 81 us for 76 with two fp16 parts.) 4096
+// tokens of 4096 and 12288 columns, 16 ranks: 31 us, 4.3 TB/s; alike with two steps on
+// their way, with u turned once for the four waves, or a block for all adapters of a part.
 template <bool HALF, int RF>
 __global__ __launch_bounds__(256) void lora_outer_kernel(LoraOuterArgs a) {
     __shared__ uint32_t s_tok[OUTER_TOKENS];

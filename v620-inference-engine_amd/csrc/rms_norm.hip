@@ -253,8 +253,8 @@ void launch_rms_norm(const NormArgs &a, hipStream_t s) {
 // ------------------------------------------------------------ gradients
 // 8 elements of a row on their way, as they lie (unpacked, those of rows that start
 // anywhere would take twice the registers: 1024 bf16 rows of 16380 120 us for 38). The
-// last piece of such a row is its last 8 elements in one access, moved to their places, with zeros
-// behind them, when the values are asked for. SHORT: a row may have fewer than 8.
+// last piece of such a row is its last 8 elements in one access, moved to their places,
+// with zeros behind them, when the values are asked for. SHORT: a row may have fewer than 8.
 template <int TY, bool VEC, bool SHORT>
 struct Part {
     RowPiece<TY> w;
@@ -306,9 +306,9 @@ struct Part {
 // A row by G of the block's TH threads (16, 64: groups of a wave, which meet no
 // barrier but the last; more: of waves), 8 elements per thread and C turns each. A
 // group takes every (groups of the grid)-th row, with the next one on its way
-// while the current one's sums are made (but in blocks of 1024), and keeps its columns' part of dw in
-// registers; the block adds its groups' parts and a second launch the blocks', in
-// order. Bound by memory.
+// while the current one's sums are made (but in blocks of 1024), and keeps its
+// columns' part of dw in registers; the block adds its groups' parts and a second
+// launch the blocks', in order. Bound by memory.
 template <int DT, int HT, int WT, bool VEC, int G, int TH, int C>
 __global__ __launch_bounds__(TH) void rms_norm_backward_kernel(NormGradArgs a) {
     constexpr int NW = TH / WAVE, GROUPS = TH / G;
